@@ -377,6 +377,165 @@ int bonsai_p40_chain_plan(const bonsai_p40_chain_step * steps, int n_steps, void
 int bonsai_p40_chain_run(const void * plan, int n_steps, void * workspace, uint32_t * status,
                          bonsai_stream stream);
 
+// ---------------------------------------------------------------------------
+// The token mixers between a layer's projections (no counterpart in the
+// reference header but bonsai_p40_attn and bonsai_p40_gdn_step, whose dense
+// caches and single steps they take the place of).  Each takes one struct,
+// which the call copies: it may be changed or freed when the call returns.
+// Metadata (lengths, positions, slots, page tables) is read on the device, so a
+// captured graph may be replayed after it changed; a value out of range never
+// leaves the buffers named here, and what it stands for is stated.  Element
+// types:
+#define BONSAI_P40_F32 0
+#define BONSAI_P40_F16 1
+#define BONSAI_P40_BF16 2
+// Pages of a key/value cache: page p holds, for each of n_kv_head heads,
+// page_size (a power of two) rows of head_dim elements; element e of slot i of
+// head h at p * page_stride + (h * page_size + i) * head_dim + e (elements;
+// page_stride a multiple of 8, n_kv_head * page_size * head_dim at least).
+// 16-byte aligned; keys and values in buffers of their own.
+
+// RMSNorm of every query and key head, position rotation, and the append of
+// keys and values to the pages, in one launch:
+//   y = x / sqrt(mean(x^2) + eps) * w      (q_norm, k_norm: head_dim weights; NULL: y = x)
+//   a = pos[t] * inv_freq[i] (radians, in fp64), (y_i, y_j) -> (y_i cos a - y_j sin a,
+//   y_j cos a + y_i sin a) for i < n_rot / 2, j = i + n_rot / 2, or with interleaved != 0
+//   the elements 2i and 2i + 1; elements from n_rot on pass.
+// Element e of head h of token t of q at t * q_tok + h * q_head + e * q_el
+// floats (k and v likewise).  Either the elements of a head are consecutive
+// (q_el == 1: rows of a GEMV; a head's queries may be followed by its gates) or the
+// tokens are (q_tok == 1: the feature-major Y of bonsai_p40_gemm, q_el = n_tok).
+// q goes to q_out (q_type: fp32, f16 or bf16), token t at t * q_out_tok, heads
+// one after another; k and v, rounded to kv_type (f16 or bf16), go to slot
+// slots[t] = page * page_size + i.  A slot outside 0 .. n_pages * page_size - 1
+// (-1: padding) is not written.  Slots of one call have to differ: what two
+// tokens leave in one slot is a mix.  Where slots are not written, the pages
+// stay as they were.
+// Errors: 1 if head_dim is not 64, 128 or 256, n_rot is not a multiple of 8 in
+// 0 .. head_dim, a type, page_size (1 .. 65536) or stride is not as stated (n_tok
+// > 1 with neither stride 1, q_out_tok < n_head * head_dim or q_out rows not
+// 16-byte aligned), n_head or n_kv_head is outside 1 .. 16384, a pointer is NULL
+// (pos and inv_freq may be where n_rot == 0) or misaligned; 0 (no-op) if n_tok <= 0.
+typedef struct bonsai_p40_qk_norm_rope_args {
+    const float * q, * k, * v;
+    int64_t q_tok, q_head, q_el, k_tok, k_head, k_el, v_tok, v_head, v_el;
+    int64_t n_tok;
+    int n_head, n_kv_head, head_dim, n_rot, interleaved;
+    float eps;
+    const float * q_norm, * k_norm;
+    const int32_t * pos;                // n_tok
+    const double * inv_freq;            // n_rot / 2
+    const int64_t * slots;              // n_tok
+    void * q_out;
+    int64_t q_out_tok;
+    int q_type, kv_type;
+    void * k_pages, * v_pages;
+    int64_t n_pages, page_stride;
+    int page_size;
+} bonsai_p40_qk_norm_rope_args;
+int bonsai_p40_qk_norm_rope(const bonsai_p40_qk_norm_rope_args * args, bonsai_stream stream);
+
+// Causal attention of the new tokens of n_seq sequences over their pages, in
+// which their own keys and values already are (bonsai_p40_qk_norm_rope):
+//   out_t = sum_{j < p_t} softmax_j(scale q_t . k_j) v_j,   p_t = kv_len - n_new + t + 1
+// for token t of the n_new = starts[s + 1] - starts[s] tokens of sequence s; 0
+// where no key is seen.  n_head is a multiple of n_kv_head; query head h reads
+// key/value head h / (n_head / n_kv_head).  Key j of sequence s is slot j %
+// page_size of page table[s * table_stride + j / page_size].  A page outside
+// 0 .. n_pages - 1 (-1: freed) holds no keys: they are not seen.  kv_len is cut to
+// max_pages * page_size, starts to 0 .. n_tok.  Rows of q and out before starts[0]
+// and from starts[n_seq] on are not touched.  Keys and values that a token does
+// not see never reach its output, whatever they hold.
+// q and out: token t at t * q_tok and t * out_tok, heads one after another, of
+// io_type: kv_type, or fp32, which keeps fp32 accuracy throughout.
+// max_kv: about the largest kv_len (0: unknown); it places the work, results hold for
+// any.  workspace: bonsai_p40_attn_paged_workspace_bytes bytes (of the same
+// args), 16-byte aligned, scratch for the call (stream-ordered; calls that may
+// run at the same time, and graphs that may, need their own); NULL: few long
+// sequences are not spread over the card.  The last bits depend on n_tok, n_seq,
+// max_kv and on whether a workspace is given; the same call gives the same bytes.
+// Errors: 1 if head_dim is not 64, 128 or 256, n_head (up to 65536) is no multiple
+// of n_kv_head, io_type, kv_type, page_size (a power of two, 16 .. 65536) or a
+// stride is not as stated (rows of q and out are 16-byte aligned), scale is not
+// finite and > 0, max_pages * page_size >= 2^31 - 65536, a pointer is NULL or
+// misaligned, the workspace is too small, or there are more than 2^28 / n_head tokens and
+// sequences; 0 (no-op) if n_tok <= 0 or n_seq <= 0.
+typedef struct bonsai_p40_attn_paged_args {
+    const void * q;
+    void * out;
+    int64_t q_tok, out_tok;
+    int64_t n_tok;
+    int n_seq, n_head, n_kv_head, head_dim;
+    int io_type, kv_type;
+    float scale;
+    const void * k_pages, * v_pages;
+    int64_t n_pages, page_stride;
+    int page_size, max_pages;
+    const int32_t * table;              // n_seq rows of max_pages
+    int64_t table_stride;
+    const int32_t * starts;             // n_seq + 1
+    const int32_t * kv_len;             // n_seq
+    int64_t max_kv;
+    void * workspace;
+    int64_t workspace_bytes;
+} bonsai_p40_attn_paged_args;
+int bonsai_p40_attn_paged(const bonsai_p40_attn_paged_args * args, bonsai_stream stream);
+// The pointers of args are not looked at; 0 where the call needs none or args
+// are invalid.
+int64_t bonsai_p40_attn_paged_workspace_bytes(const bonsai_p40_attn_paged_args * args);
+
+// Gated delta rule over the new tokens of n_seq sequences (the linear-attention
+// layers), with a state S of k_dim x v_dim fp32 for each value head.  Token by
+// token, for value head h and its key head:
+//   S <- exp(g_t) S;  u = beta_t (v_t - S^T k_t);  S <- S + k_t u^T;  out_t = scale S^T q_t
+// q and k are first divided by sqrt(sum of squares + l2_eps) where l2_eps > 0, and
+// taken as they are where it is 0.  Value head h reads key head h % n_k_head
+// (tiled != 0) or h / (n_v_head / n_k_head).  Sequence s starts from state[i] and
+// leaves state_out[i], i = slots[s] (NULL: s): [n_states][n_v_head][k_dim][v_dim].
+// state_out may be state.  Slots of one call have to differ; a sequence whose
+// slot is outside 0 .. n_states - 1 is passed over (its rows of out, too).  One
+// without tokens copies its state.  Other states, and rows of out before starts[0] and
+// from starts[n_seq] on, are not touched.
+// q, k, v, out: type fp32, f16 or bf16; token t at t * q_tok (k_tok, v_tok,
+// out_tok) elements, heads one after another: slices of one row may be passed.
+// g and beta: fp32, head h of token t at t * gate_tok + h; a g below -10000 counts as
+// that (exp is 0 there).  All sums, and the products' operands to 22 bits or more, are
+// fp32's.
+// max_new: about the largest number of tokens of a sequence (0: unknown); it picks
+// between token-by-token steps and chunks of 64 tokens, results hold for any.
+// workspace: bonsai_p40_gdn_workspace_bytes bytes (of the same args), 16-byte
+// aligned, scratch for the call (stream-ordered; calls that may run at the
+// same time, and graphs that may, need their own); NULL: token by token.
+// Errors: 1 if k_dim is not 64 or 128, v_dim is not a multiple of 16 up to 256,
+// n_v_head (up to 65536) is no multiple of n_k_head, the type or a stride is not as
+// stated (q_tok, k_tok, v_tok, out_tok and gate_tok at least a row; q and k rows
+// 16-byte aligned), scale or l2_eps is not finite or l2_eps is negative, a
+// pointer is NULL or misaligned, the workspace is too small, or there are more
+// than 2^27 / n_v_head tokens and sequences; 0 (no-op) if n_seq <= 0.
+typedef struct bonsai_p40_gdn_args {
+    const void * q, * k, * v;
+    void * out;
+    int64_t q_tok, k_tok, v_tok, out_tok;
+    const float * g, * beta;
+    int64_t gate_tok;
+    const float * state;
+    float * state_out;
+    int64_t n_states;
+    const int32_t * slots;              // n_seq, or NULL
+    const int32_t * starts;             // n_seq + 1
+    int64_t n_tok;
+    int n_seq, n_k_head, n_v_head, k_dim, v_dim;
+    int type, tiled;
+    float scale, l2_eps;
+    int64_t max_new;
+    void * workspace;
+    int64_t workspace_bytes;
+} bonsai_p40_gdn_args;
+int bonsai_p40_gdn(const bonsai_p40_gdn_args * args, bonsai_stream stream);
+// The pointers of args are not looked at; 0 where the call needs none or args
+// are invalid.
+int64_t bonsai_p40_gdn_workspace_bytes(const bonsai_p40_gdn_args * args);
+
 // Test hook: out[r * (n_in/32) + c] = the int32 chunk dot sum_k (code-1)*q of
 // row r, chunk c, computed by the same device code path as bonsai_p40_gemv
 // (the value of src/pq2_0.h:149-177 before scaling).  Errors as bonsai_p40_gemv.

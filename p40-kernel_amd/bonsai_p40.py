@@ -55,6 +55,11 @@ SIGNATURES = {
                                               _V, _V],
     "bonsai_p40_quantize_pq2_0": [_F32P, _V, _I64, _V],
     "bonsai_p40_dequantize_pq2_0": [_V, _F32P, _I64, _V],
+    "bonsai_p40_qk_norm_rope": [_V, _V],
+    "bonsai_p40_attn_paged": [_V, _V],
+    "bonsai_p40_attn_paged_workspace_bytes": [_V],
+    "bonsai_p40_gdn": [_V, _V],
+    "bonsai_p40_gdn_workspace_bytes": [_V],
     "bonsai_p40_chunk_dots": [_V, _V, _V, _I64, _I64, _V],
     "bonsai_p40_stream_read": [_V, _I64, _V, C.c_int, _V],
     "bonsai_p40_reload_tuning": [],
@@ -66,7 +71,8 @@ SIGNATURES = {
     "bonsai_p40_chain_plan": [_V, C.c_int, _V],
     "bonsai_p40_chain_run": [_V, C.c_int, _V, _V, _V],
 }
-RESTYPES = {"bonsai_p40_chain_plan_bytes": C.c_int64, "bonsai_p40_gemm_workspace_bytes": C.c_int64}
+RESTYPES = {"bonsai_p40_chain_plan_bytes": C.c_int64, "bonsai_p40_gemm_workspace_bytes": C.c_int64,
+            "bonsai_p40_attn_paged_workspace_bytes": C.c_int64, "bonsai_p40_gdn_workspace_bytes": C.c_int64}
 
 _lib = None
 
@@ -411,3 +417,189 @@ class Chain:
 
     def run(self, stream=None) -> None:
         chain_run(self.plan, self.n, self.workspace, self.status, stream=stream)
+
+
+# ------------------------------------------------------------ token mixers
+F32, F16, BF16 = 0, 1, 2
+
+
+def _args_struct(name, **fields):
+    return type(name, (C.Structure,), {"_fields_": [(f, t) for t, names in fields["spec"] for f in names.split()],
+                                       "__doc__": fields["doc"]})
+
+
+QkNormRopeArgs = _args_struct("QkNormRopeArgs", doc="bonsai_p40_qk_norm_rope_args of include/bonsai_p40.h.", spec=[
+    (_V, "q k v"), (_I64, "q_tok q_head q_el k_tok k_head k_el v_tok v_head v_el n_tok"),
+    (C.c_int, "n_head n_kv_head head_dim n_rot interleaved"), (C.c_float, "eps"),
+    (_V, "q_norm k_norm pos inv_freq slots q_out"), (_I64, "q_out_tok"), (C.c_int, "q_type kv_type"),
+    (_V, "k_pages v_pages"), (_I64, "n_pages page_stride"), (C.c_int, "page_size")])
+AttnPagedArgs = _args_struct("AttnPagedArgs", doc="bonsai_p40_attn_paged_args of include/bonsai_p40.h.", spec=[
+    (_V, "q out"), (_I64, "q_tok out_tok n_tok"), (C.c_int, "n_seq n_head n_kv_head head_dim io_type kv_type"),
+    (C.c_float, "scale"), (_V, "k_pages v_pages"), (_I64, "n_pages page_stride"), (C.c_int, "page_size max_pages"),
+    (_V, "table"), (_I64, "table_stride"), (_V, "starts kv_len"), (_I64, "max_kv"), (_V, "workspace"),
+    (_I64, "workspace_bytes")])
+GdnArgs = _args_struct("GdnArgs", doc="bonsai_p40_gdn_args of include/bonsai_p40.h.", spec=[
+    (_V, "q k v out"), (_I64, "q_tok k_tok v_tok out_tok"), (_V, "g beta"), (_I64, "gate_tok"),
+    (_V, "state state_out"), (_I64, "n_states"), (_V, "slots starts"), (_I64, "n_tok"),
+    (C.c_int, "n_seq n_k_head n_v_head k_dim v_dim type tiled"), (C.c_float, "scale l2_eps"), (_I64, "max_new"),
+    (_V, "workspace"), (_I64, "workspace_bytes")])
+
+_TYPES = {}
+
+
+def _type(t) -> int:
+    if not _TYPES:
+        import torch
+        _TYPES.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.int32: "int32",
+                       torch.int64: "int64", torch.float64: "float64"})
+    ty = _TYPES.get(t.dtype)
+    if ty is None or ty.__class__ is str:
+        raise ValueError(f"element type {t.dtype}: fp32, f16 or bf16 is wanted")
+    return ty
+
+
+def _flat(t, name: str, dtype, shape) -> int:
+    """The address of t, which has this type and shape and lies in one piece."""
+    if _TYPES.get(t.dtype) != dtype or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name}: contiguous {'fp32' if dtype == F32 else dtype} {shape} is wanted, "
+                         f"not {t.dtype} {tuple(t.shape)} of strides {t.stride()}")
+    return t.data_ptr()
+
+
+def _rows(t, name: str, shape) -> int:
+    """The token stride of (token, head, element) rows whose heads follow each other."""
+    if t.shape != shape:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, wanted {shape}")
+    n, heads, dim = shape
+    tok, head, el = t.stride()
+    if (el != 1 and dim != 1) or (head != dim and heads != 1):
+        raise ValueError(f"{name}: heads have to follow each other, the strides are {t.stride()}")
+    return tok if n > 1 else max(tok, heads * dim)
+
+
+def _pages(k_pages, v_pages):
+    """(n_pages, n_kv_head, page_size, head_dim) pages of keys and values: shape, page stride and type."""
+    shape, st = k_pages.shape, k_pages.stride()
+    if len(shape) != 4 or v_pages.shape != shape or v_pages.stride() != st or v_pages.dtype != k_pages.dtype:
+        raise ValueError("k_pages and v_pages: alike, (n_pages, n_kv_head, page_size, head_dim)")
+    n, h, p, d = shape
+    if (st[3] != 1 and d != 1) or (st[2] != d and p != 1) or (st[1] != p * d and h != 1):
+        raise ValueError("a page has to lie in one piece")
+    return shape, st[0] if n > 1 else max(st[0], h * p * d), _type(k_pages)
+
+
+def rope_inv_freq(n_rot: int, base: float, device="cuda"):
+    """base^(-2 i / n_rot), i < n_rot / 2, in fp64: the inv_freq of qk_norm_rope."""
+    import torch
+    return base ** (-torch.arange(0, n_rot, 2, dtype=torch.float64, device=device) / n_rot)
+
+
+def _qk_norm_rope_args(q, k, v, q_norm, k_norm, eps, pos, inv_freq, slots, k_pages, v_pages, q_out, interleaved):
+    if q.dim() != 3 or k.dim() != 3:
+        raise ValueError("q, k and v: (n_tok, heads, head_dim) is wanted")
+    n, h, d = shape = q.shape
+    kv = k.shape[1]
+    if not _type(q) == _type(k) == _type(v) == F32:
+        raise ValueError("q, k and v: fp32 is wanted")
+    if k.shape != (n, kv, d) or v.shape != k.shape:
+        raise ValueError(f"k, v: shapes {tuple(k.shape)}, {tuple(v.shape)} beside q's {tuple(shape)}")
+    (pages, page_kv, page_size, page_d), stride, kv_type = _pages(k_pages, v_pages)
+    if page_kv != kv or page_d != d:
+        raise ValueError("the pages have other heads")
+    half = 0 if inv_freq is None else inv_freq.numel()
+    return QkNormRopeArgs(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride(), *k.stride(), *v.stride(), n, h, kv, d, 2 * half,
+        1 if interleaved else 0, eps, None if q_norm is None else _flat(q_norm, "q_norm", F32, (d,)),
+        None if k_norm is None else _flat(k_norm, "k_norm", F32, (d,)),
+        _flat(pos, "pos", "int32", (n,)) if half else None, _flat(inv_freq, "inv_freq", "float64", (half,)) if half else None,
+        _flat(slots, "slots", "int64", (n,)), q_out.data_ptr(), _rows(q_out, "q_out", shape), _type(q_out), kv_type,
+        k_pages.data_ptr(), v_pages.data_ptr(), pages, stride, page_size)
+
+
+def qk_norm_rope(q, k, v, q_norm, k_norm, eps: float, pos, inv_freq, slots, k_pages, v_pages, q_out,
+                 interleaved: bool = False, stream=None) -> None:
+    """RMSNorm of query and key heads (q_norm, k_norm None: none), rotation of
+    their first 2 * len(inv_freq) elements, and the append of keys and values to
+    the pages.  q, k, v: fp32 (n_tok, heads, head_dim) views with the elements of
+    a head or the tokens consecutive (Y.view(heads, head_dim, n_tok).permute(2, 0,
+    1) of a gemm)."""
+    a = _qk_norm_rope_args(q, k, v, q_norm, k_norm, eps, pos, inv_freq, slots, k_pages, v_pages, q_out, interleaved)
+    _check("bonsai_p40_qk_norm_rope", lib().bonsai_p40_qk_norm_rope(C.byref(a), _stream(stream)))
+
+
+def _attn_args(q, k_pages, v_pages, table, starts, kv_len, out, workspace, max_kv, scale):
+    if q.dim() != 3 or table.dim() != 2:
+        raise ValueError("q: (n_tok, heads, head_dim) and table: (n_seq, max_pages) are wanted")
+    n, h, d = shape = q.shape
+    io = _type(q)
+    if _type(out) != io:
+        raise ValueError("out has to have q's type")
+    (pages, kv, page_size, page_d), stride, kv_type = _pages(k_pages, v_pages)
+    if page_d != d:
+        raise ValueError("the pages have another head_dim")
+    n_seq, cols = table.shape
+    row, col = table.stride()
+    if _TYPES.get(table.dtype) != "int32" or (col != 1 and cols > 1):
+        raise ValueError("table: int32 rows are wanted")
+    return AttnPagedArgs(
+        q.data_ptr(), out.data_ptr(), _rows(q, "q", shape), _rows(out, "out", shape), n, n_seq, h, kv, d, io, kv_type,
+        d ** -0.5 if scale is None else scale, k_pages.data_ptr(), v_pages.data_ptr(), pages, stride, page_size, cols,
+        table.data_ptr(), row if n_seq > 1 else cols, _flat(starts, "starts", "int32", (n_seq + 1,)),
+        _flat(kv_len, "kv_len", "int32", (n_seq,)), max_kv, None if workspace is None else workspace.data_ptr(),
+        0 if workspace is None else workspace.numel() * workspace.element_size())
+
+
+def attn_paged_workspace_bytes(q, k_pages, v_pages, table, starts, kv_len, out, max_kv: int = 0, scale=None) -> int:
+    """bonsai_p40_attn_paged_workspace_bytes for these arguments of attn_paged."""
+    a = _attn_args(q, k_pages, v_pages, table, starts, kv_len, out, None, max_kv, scale)
+    return int(lib().bonsai_p40_attn_paged_workspace_bytes(C.byref(a)))
+
+
+def attn_paged(q, k_pages, v_pages, table, starts, kv_len, out, workspace=None, max_kv: int = 0, scale=None,
+               stream=None) -> None:
+    """Causal attention of every sequence's new tokens (rows starts[s] ..
+    starts[s + 1] - 1 of q and out, (n_tok, heads, head_dim)) over its kv_len[s] keys
+    in the pages table[s]; scale None: head_dim^-1/2."""
+    a = _attn_args(q, k_pages, v_pages, table, starts, kv_len, out, workspace, max_kv, scale)
+    _check("bonsai_p40_attn_paged", lib().bonsai_p40_attn_paged(C.byref(a), _stream(stream)))
+
+
+def _gdn_args(q, k, v, g, beta, state, state_out, out, starts, workspace, max_new, slots, scale, l2_eps, tiled):
+    if q.dim() != 3 or v.dim() != 3 or starts.dim() != 1 or state.dim() != 4:
+        raise ValueError("q, k, v: (n_tok, heads, dim), state: (n_states, heads, k_dim, v_dim), starts: (n_seq + 1,)")
+    n, kh, kd = qs = q.shape
+    _, vh, vd = v.shape
+    ty = _type(q)
+    if _type(k) != ty or _type(v) != ty or _type(out) != ty:
+        raise ValueError("q, k, v and out: one type is wanted")
+    if _type(g) != F32 or _type(beta) != F32 or g.shape != (n, vh) or beta.shape != g.shape:
+        raise ValueError(f"g and beta: fp32 ({n}, {vh}) is wanted")
+    (gt, gh), (bt, bh) = g.stride(), beta.stride()
+    if (vh > 1 and not gh == bh == 1) or (n > 1 and gt != bt):
+        raise ValueError("g and beta: one token stride, and the heads of a token consecutive")
+    ss, n_seq = (state.shape[0], vh, kd, vd), starts.shape[0] - 1
+    return GdnArgs(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _rows(q, "q", qs), _rows(k, "k", qs),
+        _rows(v, "v", (n, vh, vd)), _rows(out, "out", (n, vh, vd)), g.data_ptr(), beta.data_ptr(), gt if n > 1 else vh,
+        _flat(state, "state", F32, ss), _flat(state_out, "state_out", F32, ss), ss[0],
+        None if slots is None else _flat(slots, "slots", "int32", (n_seq,)),
+        _flat(starts, "starts", "int32", (n_seq + 1,)), n, n_seq, kh, vh, kd, vd, ty, 1 if tiled else 0,
+        kd ** -0.5 if scale is None else scale, l2_eps, max_new, None if workspace is None else workspace.data_ptr(),
+        0 if workspace is None else workspace.numel() * workspace.element_size())
+
+
+def gdn_workspace_bytes(q, k, v, g, beta, state, state_out, out, starts, max_new: int = 0, slots=None, scale=None,
+                        l2_eps: float = 0.0, tiled: bool = False) -> int:
+    """bonsai_p40_gdn_workspace_bytes for these arguments of gdn."""
+    a = _gdn_args(q, k, v, g, beta, state, state_out, out, starts, None, max_new, slots, scale, l2_eps, tiled)
+    return int(lib().bonsai_p40_gdn_workspace_bytes(C.byref(a)))
+
+
+def gdn(q, k, v, g, beta, state, state_out, out, starts, workspace=None, max_new: int = 0, slots=None, scale=None,
+        l2_eps: float = 0.0, tiled: bool = False, stream=None) -> None:
+    """The gated delta rule over every sequence's tokens (rows starts[s] ..
+    starts[s + 1] - 1): q, k (n_tok, k_heads, k_dim), v, out (n_tok, v_heads, v_dim),
+    g (log decay) and beta (n_tok, v_heads), state (n_states, v_heads, k_dim, v_dim);
+    scale None: k_dim^-1/2."""
+    a = _gdn_args(q, k, v, g, beta, state, state_out, out, starts, workspace, max_new, slots, scale, l2_eps, tiled)
+    _check("bonsai_p40_gdn", lib().bonsai_p40_gdn(C.byref(a), _stream(stream)))

@@ -1,0 +1,662 @@
+// attn_paged.hip -- attention of every sequence's new tokens over its pages
+// (bonsai_p40_attn_paged): one token (decode), a few, or a prompt chunk, ragged,
+// grouped heads, causal.
+//
+//   o_t = sum_{j < p_t} softmax(scale q_t . k_j) v_j,   p_t = kv_len - n_new + t + 1
+//
+// One pass over the keys with the running maximum m and sum l of the softmax
+// (in units of log2, so that exp2 takes them):
+//   m' = max(m, c s),  p = 2^(c s - m'),  l' = l 2^(m - m') + sum p,  O' = O 2^(m - m') + p V.
+//
+// A row of the products is a (token, query head) pair: the heads that share a
+// key/value head share its tiles, so a decode step of 6 heads is 6 rows and a
+// chunk of n tokens 6 n.  Both products run transposed on v_mfma 32x32x16:
+//   S^T (32 keys x 32 rows) = K . Q^T,   O^T (32 d x 32 rows) += V^T . P^T.
+// A lane then holds 16 keys of ONE row, so that maximum, sum and rescaling are a
+// lane's own (one exchange with lane ^ 32), and the P it computes is the operand
+// of the second product as it stands: element j of half h is key 4 h + j % 4 +
+// 8 (j / 4) there, an order of the contraction that V^T is read in too
+// (ds_read_b64_tr_b16 transposes 4 keys x 16 d on the way out of LDS).
+// K and V tiles reach LDS by DMA, 16-byte units XOR-swizzled by the key on the
+// source side so that neither read meets a bank twice.
+//
+// Two shapes of workgroup:
+//   rows: a wave per 32 rows (128 a workgroup), all on the same tiles of 64 keys,
+//     double-buffered: prompts, bound by the matrix cores;
+//   keys: 32 rows, each wave its own tiles of 32 keys, double-buffered, joined in
+//     LDS at the end: decode, bound by the stream of K and V.
+// Either splits the keys over workgroups where there are too few rows to fill the
+// card; attn_join_kernel adds the parts.
+//
+// fp32 queries and output (the activations' type) keep fp32 accuracy: Q and P
+// are split into 2 f16 terms (rows scaled by a power of two, 22 bits) or 3 bf16
+// terms (24 bits) and the products summed in fp32.  16-bit ones round P once to
+// the pages' type, as its relative error is that of the output's own rounding.
+#include "gemv_device.h"
+#include "host_state.h"
+#include "launch_rules.h"
+#include "mixer_device.h"
+
+using namespace mixer;
+
+namespace {
+
+struct AttnArgs {
+    const void * q;
+    void * out;
+    const uint8_t * k, * v;
+    const int32_t * table, * starts, * kv_len;
+    float * part;                       // [split][row][D] then [split][row] (m, l)
+    int64_t q_tok, out_tok;             // elements
+    int64_t page_bytes, head_bytes;
+    int64_t table_stride;
+    int n_tok, n_seq, n_head, n_kv, group;
+    int n_pages, page_log2, cap;        // cap: keys the table can name
+    int chunk, n_split, tiles;
+    float c;                            // scale * log2(e)
+};
+
+template <class T>
+__device__ __forceinline__ v16f mfma(typename T::frag a, typename T::frag b, v16f c);
+template <>
+__device__ __forceinline__ v16f mfma<F16>(v8h a, v8h b, v16f c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ v16f mfma<BF16>(v8b a, v8b b, v16f c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// 4 keys x 16 d per 16 lanes, transposed: lane i gets column i
+__device__ __forceinline__ v2u read_tr(const uint8_t * at) {
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s4 lds_s4;
+    return __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)at));
+}
+
+template <class T, int D, int NT, bool KEYS>
+struct Shape {
+    // waves: with heads of 256, LDS has two buffers of 32 keys for 2 waves, or 64 rows of two terms of Q
+    static constexpr int NW = D == 256 && (KEYS || NT == 3) ? 2 : 4;
+    static constexpr int BM = KEYS ? 32 : 32 * NW;
+    // fp32 queries of 256: the registers hold one term of Q, the others are in LDS
+    static constexpr bool QL = NT > 1 && D == 256;
+    static constexpr int QR = QL ? 1 : NT;                 // terms in registers
+    static constexpr int KT = KEYS || QL ? 32 : 64;        // keys of a staged tile
+    static constexpr int RB = 2 * D;                       // bytes of a key
+    static constexpr int TILE = KT * RB;
+    static constexpr int OROW = D + 4;                     // floats of a row in the join
+    static constexpr int JOIN = NW * 32 * OROW * 4 + NW * 32 * 8;
+    static constexpr int MAIN = KEYS ? NW * 4 * TILE : 4 * TILE;   // two buffers of K and V
+    static constexpr int QT = 2 * 32 * D;                  // bytes of a term of 32 rows
+    static constexpr int ALL = MAIN + (NT - QR) * (KEYS ? QT : NW * QT);
+    static constexpr int LDS = KEYS && JOIN > ALL ? JOIN : ALL;
+};
+
+template <class T, int D, int NT, bool KEYS>
+__global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) attn_kernel(AttnArgs a) {
+    typedef Shape<T, D, NT, KEYS> Z;
+    typedef typename T::elem elem;
+    typedef typename T::frag frag;
+    constexpr int U = D / 8;                               // 16-byte units of a key
+    constexpr int RPI = 64 / U;                            // keys per DMA instruction
+    constexpr int QS = D / 16, DT = D / 32;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[Z::LDS];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 31, half = lane >> 5;
+    // heads vary fastest (a head's tiles meet on the same XCDs), the last tiles,
+    // which see the most keys, start first
+    const int kvh = blockIdx.x % a.n_kv, rest = blockIdx.x / a.n_kv;
+    const int split = rest % a.n_split, tile_no = a.tiles - 1 - rest / a.n_split;
+    const Tile tl = find_tile<Z::BM>(a.starts, a.n_seq, a.n_tok, a.group, tile_no);
+    if (tl.seq < 0) return;
+    const int rows = tl.count * a.group, row0 = tl.index * Z::BM;
+    const int kv = iclamp(sload(a.kv_len, tl.seq), 0, a.cap), before = kv - tl.count;
+    const int last = min(row0 + Z::BM, rows) - 1;
+    const int nk = a.n_pages > 0 ? iclamp(before + last / a.group + 1, 0, kv) : 0;
+    const int k0 = split * a.chunk;
+    const int k1 = split == a.n_split - 1 ? nk : min(nk, k0 + a.chunk);
+    if (split > 0 && k0 >= nk) return;                     // the join counts the parts
+
+    // this lane's row
+    const int wrow = row0 + (KEYS ? 0 : 32 * wave);
+    const int r = wrow + n;
+    const bool live = r < rows;
+    const int tok = live ? r / a.group : 0, head = kvh * a.group + (live ? r - tok * a.group : 0);
+    const int vis = live ? iclamp(before + tok + 1, 0, kv) : 0;
+    const int64_t grow = (int64_t)(tl.first + tok);
+    // the fewest keys any live row of the wave sees; 0 rows: nothing to do but stage
+    const bool work = wrow < rows;
+    const int least = work ? iclamp(before + wrow / a.group + 1, 0, kv) : 0;
+
+    // the keys that all rows of the workgroup see
+    const int first_vis = iclamp(before + row0 / a.group + 1, 0, kv);
+
+    // Q^T, element j of half h: d = 16 step + 8 h + j
+    frag qf[Z::QR][QS];
+    uint8_t * const ql = lds + Z::MAIN + (KEYS ? 0 : wave * (NT - Z::QR) * Z::QT) + 16 * lane;
+    float c = a.c;
+    if constexpr (NT == 1) {
+        const elem * const qp = reinterpret_cast<const elem *>(a.q) + grow * a.q_tok + (int64_t)head * D + 8 * half;
+#pragma unroll
+        for (int s = 0; s < QS; ++s)
+            qf[0][s] = live ? *reinterpret_cast<const frag *>(qp + 16 * s) : frag{};
+    } else {
+        const float * const qp = reinterpret_cast<const float *>(a.q) + grow * a.q_tok + (int64_t)head * D + 8 * half;
+        float up = 1.0f;
+        if constexpr (NT == 2) {
+            // the row's largest element to [1, 2): f16 then holds 22 bits in two terms
+            float big = 0.0f;
+            if (live)
+#pragma unroll
+                for (int s = 0; s < QS; ++s) {
+                    const v4f x = *reinterpret_cast<const v4f *>(qp + 16 * s), y = *reinterpret_cast<const v4f *>(qp + 16 * s + 4);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) big = fmaxf(big, fmaxf(fabsf(x[j]), fabsf(y[j])));
+                }
+            big = fmaxf(big, __shfl_xor(big, 32));
+            const int e = (int)((__builtin_bit_cast(uint32_t, big) >> 23) & 255);
+            if (e > 2 && e < 252) {
+                up = __builtin_bit_cast(float, (uint32_t)(254 - e) << 23);
+                c *= __builtin_bit_cast(float, (uint32_t)e << 23);
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < QS; ++s) {
+            v4f x = {}, y = {};
+            if (live) {
+                x = *reinterpret_cast<const v4f *>(qp + 16 * s);
+                y = *reinterpret_cast<const v4f *>(qp + 16 * s + 4);
+            }
+            frag low[NT];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float f = (j < 4 ? x[j & 3] : y[j & 3]) * up;
+#pragma unroll
+                for (int k = 0; k < NT; ++k) {
+                    const elem e = T::from(f);
+                    if (k < Z::QR) qf[k][s][j] = e;
+                    else low[k][j] = e;
+                    f -= T::to(e);
+                }
+            }
+#pragma unroll
+            for (int k = Z::QR; k < NT; ++k)
+                if (!KEYS || wave == 0) *reinterpret_cast<frag *>(ql + (k - Z::QR) * Z::QT + 1024 * s) = low[k];
+        }
+        if constexpr (Z::QL) __syncthreads();
+    }
+
+    v16f o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[d] = v16f{};
+    float m = -INFINITY, l = 0.0f;
+
+    // ---- staging: 16 keys of K and V a call, all of one page
+    const int64_t trow = (int64_t)tl.seq * a.table_stride;
+    const int drow = lane / U, dunit = lane % U;
+    auto swz_k = [](int key) { return U >= 16 ? key & 15 : (key >> 1) & 7; };
+    auto swz_v = [](int key) { return U >= 32 ? (key & 7) * 4 : U >= 16 ? (key & 3) * 4 : ((key >> 1) & 1) * 4; };
+    // the page of the 16 keys from `key` on; -1: none of them is to be read
+    auto page_of = [&](int key) {
+        if (key >= nk) return -1;
+        const int id = sload(a.table, trow + (key >> a.page_log2));
+        return id >= 0 && id < a.n_pages ? id : -1;
+    };
+    auto stage16 = [&](const uint8_t * base, int id, int key, uint8_t * dst, bool is_v) __attribute__((always_inline)) {
+        const uint8_t * const p = base + (int64_t)max(id, 0) * a.page_bytes + (int64_t)kvh * a.head_bytes +
+                                  (int64_t)(key & ((1 << a.page_log2) - 1)) * Z::RB;
+#pragma unroll
+        for (int i = 0; i < 16 / RPI; ++i) {
+            const int kr = i * RPI + drow;                 // key % 16, and as far as the swizzle looks, key in the tile
+            const int u = dunit ^ (is_v ? swz_v(kr) : swz_k(kr));
+            dma16(p + kr * Z::RB + 16 * u, dst + i * 1024);
+        }
+    };
+    // zero the V rows [from, 16) of a 16-key group: p is 0 there, and 0 times what memory holds may be NaN
+    auto zero16 = [&](uint8_t * dst, int from) {
+        for (int i = from * U + lane; i < 16 * U; i += 64) *reinterpret_cast<v4u *>(dst + 16 * i) = v4u{};
+    };
+
+    // ---- one sub-tile of 32 keys: kb, vb its first keys in LDS, key0 its place
+    // in the sequence, holes: bit g: the 16 keys from 16 g on are absent
+    const int l16 = lane & 15, vkey = 4 * half + (l16 >> 2), vcol = 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1);
+    auto scores = [&](const uint8_t * kb, const uint8_t * ql) __attribute__((always_inline)) {
+        v16f s = {};
+#pragma unroll
+        for (int i = 0; i < QS; ++i) {
+            const frag kf = *reinterpret_cast<const frag *>(kb + n * Z::RB + 16 * ((2 * i + half) ^ swz_k(n)));
+#pragma unroll
+            for (int k = NT - 1; k >= Z::QR; --k)
+                s = mfma<T>(kf, *reinterpret_cast<const frag *>(ql + (k - Z::QR) * Z::QT + 1024 * i), s);
+#pragma unroll
+            for (int k = Z::QR - 1; k >= 0; --k) s = mfma<T>(kf, qf[k][i], s);
+        }
+        return s;
+    };
+    auto softmax = [&](v16f & s, int key0, int holes) __attribute__((always_inline)) {
+        if (key0 + 32 > least || holes) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int j = 8 * (i / 4) + 4 * half + i % 4;
+                if (key0 + j >= vis || (holes >> (j >> 4) & 1)) s[i] = -INFINITY;
+            }
+        }
+        float mx = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const float m2 = fmaxf(m, mx * c);
+        const float ref = m2 == -INFINITY ? 0.0f : m2;
+        const float alpha = __builtin_amdgcn_exp2f(m - ref);
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -ref));
+            sum += s[i];
+        }
+        l = fmaf(l, alpha, sum);
+        m = m2;
+        if (__any(alpha != 1.0f)) {
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
+        }
+    };
+    // where some rows of the wave see a key and others do not, p = 0 does not keep an infinity or NaN of V out
+    // of the others' sums: bit k: key k of the sub-tile has one
+    auto wild = [&](const uint8_t * vb) __attribute__((always_inline)) {
+        typedef unsigned short u2 __attribute__((ext_vector_type(2)));
+        constexpr uint32_t EXP = T::EXP * 0x10001u;
+        u2 top = {0, 0};
+#pragma unroll
+        for (int i = 0; i < U / 2; ++i) {
+            const v4u x = *reinterpret_cast<const v4u *>(vb + n * Z::RB + 16 * (half * (U / 2) + (i + n) % (U / 2)));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) top = __builtin_elementwise_max(top, __builtin_bit_cast(u2, x[j] & EXP));
+        }
+        const uint64_t hit = __ballot(top[0] == T::EXP || top[1] == T::EXP);
+        return (uint32_t)(hit | hit >> 32);
+    };
+    // those keys one by one, for the rows that see them; then their rows of V are zeroed.  mixed is uniform
+    // over the waves that share the tile, and so is what is found
+    auto apart = [&](const v16f & p, uint8_t * vb, int key0) __attribute__((always_inline)) {
+        const uint32_t bad = wild(vb);
+        if (!bad) return;
+        for (uint32_t left = bad; left; left &= left - 1) {
+            const int k = __builtin_ctz(left), at = (k & 3) + 4 * (k >> 3);
+            float x = p[0];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) x = at == i ? p[i] : x;
+            x = __shfl(x, n + 32 * (k >> 2 & 1));
+            if (key0 + k < vis) {
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        float v[4];
+                        load_row<T>(reinterpret_cast<const elem *>(vb + k * Z::RB + 16 * ((4 * d + g) ^ swz_v(k)) + 8 * half), v);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) o[d][4 * g + j] = fmaf(x, v[j], o[d][4 * g + j]);
+                    }
+            }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (!KEYS) __builtin_amdgcn_s_barrier();           // all waves have what they need of these rows
+        asm volatile("" ::: "memory");
+        for (uint32_t left = bad; left; left &= left - 1)
+            for (int i = lane; i < U; i += 64)
+                *reinterpret_cast<v4u *>(vb + __builtin_ctz(left) * Z::RB + 16 * i) = v4u{};
+    };
+    auto values = [&](const v16f & p, const uint8_t * vb) __attribute__((always_inline)) {
+        frag pf[NT][2];
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float f = p[8 * g + j];
+#pragma unroll
+                for (int k = 0; k < NT; ++k) {
+                    const elem e = T::from(f);
+                    pf[k][g][j] = e;
+                    f -= T::to(e);
+                }
+            }
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const uint8_t * const at = vb + (16 * g + vkey) * Z::RB + 8 * (l16 & 1);
+                const int u = 4 * d + vcol;
+                const v2u x = read_tr(at + 16 * (u ^ swz_v(vkey)));
+                const v2u y = read_tr(at + 8 * Z::RB + 16 * (u ^ swz_v(vkey + 8)));
+                const frag vf = __builtin_bit_cast(frag, (v4u){x[0], x[1], y[0], y[1]});
+#pragma unroll
+                for (int k = NT - 1; k >= 0; --k) o[d] = mfma<T>(vf, pf[k][g], o[d]);
+            }
+        }
+    };
+
+    if constexpr (!KEYS) {
+        constexpr int KT = Z::KT;
+        // each wave stages K and V of 16 keys, or of 32 keys waves 0, 1 K and 2, 3 V
+        constexpr bool SPLIT = KT < 16 * Z::NW;
+        const int own = SPLIT ? (wave & 1) * 16 : wave * 16;
+        int holes_next = 0;
+        auto stage = [&](int key, uint8_t * to) __attribute__((always_inline)) {
+            uint8_t * const kd = to + own * Z::RB;
+            const int mine = page_of(key + own);
+            if (!SPLIT || wave < 2) stage16(a.k, mine, key + own, kd, false);
+            if (!SPLIT || wave >= 2) stage16(a.v, mine, key + own, kd + Z::TILE, true);
+            holes_next = 0;
+#pragma unroll
+            for (int g = 0; g < KT / 16; ++g) holes_next |= (page_of(key + 16 * g) < 0 ? 1 : 0) << g;
+        };
+        // the next tile's DMA runs while this one is computed on; that the buffers
+        // differ has to be said, else every read of LDS waits for the DMA
+        auto step = [&](uint8_t * __restrict__ next, uint8_t * __restrict__ cur, const uint8_t * __restrict__ qlow,
+                        int key, int holes) __attribute__((always_inline)) {
+            if (key + KT < k1) stage(key + KT, next);
+            const bool mixed = key + KT > first_vis && nk > max(first_vis, key);
+            if (work || mixed) {
+#pragma unroll 1
+                for (int u = 0; u < KT / 32; ++u) {
+                    v16f s = scores(cur + 32 * u * Z::RB, qlow);
+                    softmax(s, key + 32 * u, holes >> (2 * u) & 3);
+                    if (mixed) apart(s, cur + Z::TILE + 32 * u * Z::RB, key + 32 * u);
+                    values(s, cur + Z::TILE + 32 * u * Z::RB);
+                }
+            }
+        };
+        if (k0 < k1) stage(k0, lds);
+        int b = 0;
+#pragma clang loop unroll(disable)
+        for (int key = k0; key < k1; key += KT, b ^= 1) {
+            const int holes = holes_next;
+            uint8_t * const cur = lds + b * 2 * Z::TILE;
+            pq2::wait_vmcnt<0>();
+            const bool hole = holes >> (own >> 4) & 1;
+            if ((!SPLIT || wave >= 2) && (hole || key + own + 16 > nk))
+                zero16(cur + Z::TILE + own * Z::RB, hole ? 0 : max(nk - key - own, 0));
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();                  // the tile is there, and all have left the other buffer
+            asm volatile("" ::: "memory");
+            step(lds + (b ^ 1) * 2 * Z::TILE, cur, ql, key, holes);
+        }
+    } else {
+        uint8_t * const mine = lds + wave * 4 * Z::TILE;
+        int id0 = -1, id1 = -1;
+        auto stage = [&](int key, uint8_t * to) __attribute__((always_inline)) {
+            id0 = page_of(key);
+            id1 = page_of(key + 16);
+            stage16(a.k, id0, key, to, false);
+            stage16(a.k, id1, key + 16, to + 16 * Z::RB, false);
+            stage16(a.v, id0, key, to + Z::TILE, true);
+            stage16(a.v, id1, key + 16, to + Z::TILE + 16 * Z::RB, true);
+        };
+        auto step = [&](uint8_t * __restrict__ next, uint8_t * __restrict__ cur, const uint8_t * __restrict__ qlow,
+                        int key, int holes) __attribute__((always_inline)) {
+            if (key + 32 * Z::NW < k1) stage(key + 32 * Z::NW, next);
+            v16f s = scores(cur, qlow);
+            softmax(s, key, holes);
+            if (key + 32 > first_vis && nk > max(first_vis, key)) apart(s, cur + Z::TILE, key);
+            values(s, cur + Z::TILE);
+        };
+        int key = k0 + 32 * wave, b = 0;
+        if (key < k1) stage(key, mine);
+#pragma clang loop unroll(disable)
+        for (; key < k1; key += 32 * Z::NW, b ^= 1) {
+            const int holes = (id0 < 0 ? 1 : 0) | (id1 < 0 ? 2 : 0);
+            uint8_t * const cur = mine + b * 2 * Z::TILE;
+            pq2::wait_vmcnt<0>();
+            if (holes || key + 32 > nk) {
+                zero16(cur + Z::TILE, holes & 1 ? 0 : iclamp(nk - key, 0, 16));
+                zero16(cur + Z::TILE + 16 * Z::RB, holes & 2 ? 0 : iclamp(nk - key - 16, 0, 16));
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // also: the other buffer's reads are done
+            step(mine + (b ^ 1) * 2 * Z::TILE, cur, ql, key, holes);
+        }
+    }
+    l += __shfl_xor(l, 32);
+
+    const bool parts = a.n_split > 1;
+    const int64_t all_rows = (int64_t)a.n_tok * a.n_head;
+    if constexpr (!KEYS) {
+        if (!live) return;
+        const int64_t row = grow * a.n_head + head;
+        const float inv = parts ? 1.0f : l != 0.0f ? 1.0f / l : 0.0f;
+        float * const po = a.part + ((int64_t)split * all_rows + row) * D;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                float x[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j] = o[d][4 * g + j] * inv;
+                const int at = 32 * d + 8 * g + 4 * half;
+                if (parts) store_row<F32>(po + at, x);
+                else if constexpr (NT == 1)
+                    store_row<T>(reinterpret_cast<elem *>(a.out) + grow * a.out_tok + (int64_t)head * D + at, x);
+                else store_row<F32>(reinterpret_cast<float *>(a.out) + grow * a.out_tok + (int64_t)head * D + at, x);
+            }
+        if (parts && half == 0)
+            *reinterpret_cast<float2 *>(a.part + (int64_t)a.n_split * all_rows * D + 2 * ((int64_t)split * all_rows + row)) =
+                make_float2(m, l);
+    } else {
+        // join the waves: [wave][row][D] and [wave][row] (m, l)
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        float * const jo = reinterpret_cast<float *>(lds);
+        float2 * const ml = reinterpret_cast<float2 *>(lds + Z::NW * 32 * Z::OROW * 4);
+        if (live) {
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    *reinterpret_cast<v4f *>(jo + (wave * 32 + n) * Z::OROW + 32 * d + 8 * g + 4 * half) =
+                        (v4f){o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+            if (half == 0) ml[wave * 32 + n] = make_float2(m, l);
+        }
+        __syncthreads();
+        constexpr int E = D / 64;
+        for (int i = wave; i <= last - row0; i += Z::NW) {
+            float mm = -INFINITY, ll = 0.0f;
+#pragma unroll
+            for (int k = 0; k < Z::NW; ++k) mm = fmaxf(mm, ml[k * 32 + i].x);
+            const float ref = mm == -INFINITY ? 0.0f : mm;
+            float x[E] = {};
+#pragma unroll
+            for (int k = 0; k < Z::NW; ++k) {
+                const float2 e = ml[k * 32 + i];
+                const float w = __builtin_amdgcn_exp2f(e.x - ref);
+                ll = fmaf(e.y, w, ll);
+#pragma unroll
+                for (int j = 0; j < E; ++j) x[j] = fmaf(jo[(k * 32 + i) * Z::OROW + lane * E + j], w, x[j]);
+            }
+            const int rr = row0 + i, t = rr / a.group, h = kvh * a.group + rr - t * a.group;
+            const int64_t g = tl.first + t, row = g * a.n_head + h;
+            if (parts) {
+                store_row<F32>(a.part + ((int64_t)split * all_rows + row) * D + lane * E, x);
+                if (lane == 0)
+                    *reinterpret_cast<float2 *>(a.part + (int64_t)a.n_split * all_rows * D +
+                                                2 * ((int64_t)split * all_rows + row)) = make_float2(mm, ll);
+            } else {
+                const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;
+#pragma unroll
+                for (int j = 0; j < E; ++j) x[j] *= inv;
+                if constexpr (NT == 1)
+                    store_row<T>(reinterpret_cast<elem *>(a.out) + g * a.out_tok + (int64_t)h * D + lane * E, x);
+                else store_row<F32>(reinterpret_cast<float *>(a.out) + g * a.out_tok + (int64_t)h * D + lane * E, x);
+            }
+        }
+    }
+}
+
+// The parts of every row: a wave per row.  Their number follows from the keys
+// the row's tile saw, as in attn_kernel.
+template <class TO, int D>
+__global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int bm) {
+    constexpr int E = D / 64;
+    const int lane = threadIdx.x & 63;
+    const int64_t all_rows = (int64_t)a.n_tok * a.n_head, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= all_rows) return;
+    const int tok = (int)(row / a.n_head), head = (int)(row - (int64_t)tok * a.n_head);
+    // the sequence of this token
+    int seq = -1, first = 0, count = 0;
+    for (int s0 = 0; s0 < a.n_seq && seq < 0; s0 += 64) {
+        const int s = s0 + lane;
+        int b = 0, e = 0;
+        if (s < a.n_seq) {
+            b = iclamp(a.starts[s], 0, a.n_tok);
+            e = iclamp(a.starts[s + 1], 0, a.n_tok);
+        }
+        const uint64_t hit = __ballot(tok >= b && tok < e);
+        if (hit) {
+            const int k = __builtin_ctzll(hit);
+            seq = s0 + k;
+            first = __builtin_amdgcn_readlane(b, k);
+            count = __builtin_amdgcn_readlane(e, k) - first;
+        }
+    }
+    if (seq < 0) return;                                   // a row behind the last sequence
+    const int kv = iclamp(a.kv_len[seq], 0, a.cap);
+    const int r = (tok - first) * a.group + head % a.group;
+    const int last = min(r / bm * bm + bm, count * a.group) - 1;
+    const int nk = a.n_pages > 0 ? iclamp(kv - count + last / a.group + 1, 0, kv) : 0;
+    const int n = iclamp((nk + a.chunk - 1) / a.chunk, 1, a.n_split);
+    const float2 * const ml = reinterpret_cast<const float2 *>(a.part + (int64_t)a.n_split * all_rows * D) + row;
+    float mm = -INFINITY;
+    for (int i = lane; i < n; i += 64) mm = fmaxf(mm, ml[i * all_rows].x);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) mm = fmaxf(mm, __shfl_xor(mm, d));
+    const float ref = mm == -INFINITY ? 0.0f : mm;
+    float x[E] = {}, l = 0.0f;
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+        const float2 e = ml[i * all_rows];
+        const float w = __builtin_amdgcn_exp2f(e.x - ref);
+        float v[E];
+        load_row<F32>(a.part + (i * all_rows + row) * D + lane * E, v);
+        l = fmaf(e.y, w, l);
+#pragma unroll
+        for (int j = 0; j < E; ++j) x[j] = fmaf(v[j], w, x[j]);
+    }
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+    for (int j = 0; j < E; ++j) x[j] *= inv;
+    store_row<TO>(reinterpret_cast<typename TO::elem *>(a.out) + (int64_t)tok * a.out_tok + (int64_t)head * D + lane * E, x);
+}
+
+template <class T, int D, int NT, bool KEYS>
+int launch(AttnArgs & a, hipStream_t s) {
+    typedef Shape<T, D, NT, KEYS> Z;
+    const int64_t blocks = (int64_t)a.tiles * a.n_split * a.n_kv;
+    hipLaunchKernelGGL((attn_kernel<T, D, NT, KEYS>), dim3((unsigned)blocks), dim3(64 * Z::NW), 0, s, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || a.n_split == 1) return (int)e;
+    const unsigned jb = (unsigned)(((int64_t)a.n_tok * a.n_head + 3) / 4);
+    if constexpr (NT == 1) hipLaunchKernelGGL((attn_join_kernel<T, D>), dim3(jb), dim3(256), 0, s, a, (int)Z::BM);
+    else hipLaunchKernelGGL((attn_join_kernel<F32, D>), dim3(jb), dim3(256), 0, s, a, (int)Z::BM);
+    return (int)hipGetLastError();
+}
+template <class T, int D, int NT>
+int launch_k(bool keys, AttnArgs & a, hipStream_t s) {
+    return keys ? launch<T, D, NT, true>(a, s) : launch<T, D, NT, false>(a, s);
+}
+template <class T, int NT>
+int launch_d(int d, bool keys, AttnArgs & a, hipStream_t s) {
+    return d == 256 ? launch_k<T, 256, NT>(keys, a, s) : d == 128 ? launch_k<T, 128, NT>(keys, a, s)
+                                                                  : launch_k<T, 64, NT>(keys, a, s);
+}
+
+// 1: invalid, 0: nothing to do, -1: to be run
+int check(const bonsai_p40_attn_paged_args * p) {
+    if (!p) return 1;
+    const int d = p->head_dim;
+    if (d != 64 && d != 128 && d != 256) return 1;
+    if (p->n_kv_head < 1 || p->n_head < 1 || p->n_head > 65536 || p->n_head % p->n_kv_head != 0) return 1;
+    if (!is_half(p->kv_type) || (p->io_type != BONSAI_P40_F32 && p->io_type != p->kv_type)) return 1;
+    if (!is_pow2(p->page_size) || p->page_size < 16 || p->page_size > 65536) return 1;
+    if (p->n_pages < 0 || p->n_pages > 0x7fffffff) return 1;
+    if (p->page_stride < (int64_t)p->n_kv_head * p->page_size * d || p->page_stride % 8 != 0) return 1;
+    const int per16 = 16 / type_bytes(p->io_type);
+    if (p->q_tok < (int64_t)p->n_head * d || p->q_tok % per16 != 0) return 1;
+    if (p->out_tok < (int64_t)p->n_head * d || p->out_tok % per16 != 0) return 1;
+    if (!(p->scale > 0.0f) || !(p->scale < INFINITY)) return 1;
+    if (p->max_pages < 0 || p->table_stride < p->max_pages || p->max_kv < 0) return 1;
+    if (p->max_pages * (int64_t)p->page_size > 0x7fff0000) return 1;
+    if (p->n_tok <= 0 || p->n_seq <= 0) return 0;
+    if (p->n_tok > 0x7fffffff / p->n_head || p->n_seq > 0xffffff) return 1;
+    if ((p->n_tok + p->n_seq) * (int64_t)p->n_head > 0x7fffffff / 8) return 1;     // workgroups
+    return -1;
+}
+
+struct Plan {
+    bool keys;
+    int tiles, chunk, n_split;
+};
+Plan plan_of(const bonsai_p40_attn_paged_args * p) {
+    const int group = p->n_head / p->n_kv_head;
+    const int64_t cap = (int64_t)p->max_pages * p->page_size;
+    const int64_t most = p->max_kv > 0 && p->max_kv < cap ? p->max_kv : cap;
+    const int rows = p->head_dim == 256 && p->kv_type == BONSAI_P40_BF16 && p->io_type == BONSAI_P40_F32 ? 64 : 128;
+    const pq2::AttnPlan a = pq2::attn_plan(p->n_tok, p->n_seq, group, p->n_kv_head, p->head_dim, most, rows,
+                                           pq2host::device_info().cus);
+    return {a.keys, (int)a.tiles, (int)a.chunk, (int)a.n_split};
+}
+int64_t part_bytes(const bonsai_p40_attn_paged_args * p, int n_split) {
+    return n_split <= 1 ? 0 : (int64_t)n_split * p->n_tok * p->n_head * (p->head_dim + 2) * 4;
+}
+
+}  // namespace
+
+extern "C" int64_t bonsai_p40_attn_paged_workspace_bytes(const bonsai_p40_attn_paged_args * p) {
+    return check(p) == -1 ? part_bytes(p, plan_of(p).n_split) : 0;
+}
+
+extern "C" int bonsai_p40_attn_paged(const bonsai_p40_attn_paged_args * p, bonsai_stream stream) {
+    const int rc = check(p);
+    if (rc >= 0) return rc;
+    if (pq2host::any_null(p->q, p->out, p->starts, p->kv_len)) return 1;
+    if (p->max_pages > 0 && p->n_pages > 0 && pq2host::any_null(p->k_pages, p->v_pages, p->table)) return 1;
+    if (!aligned(p->q, 16) || !aligned(p->out, 16) || !aligned(p->k_pages, 16) || !aligned(p->v_pages, 16) ||
+        !aligned(p->workspace, 16) || !aligned(p->table, 4) || !aligned(p->starts, 4) || !aligned(p->kv_len, 4))
+        return 1;
+    Plan pl = plan_of(p);
+    if (p->workspace == nullptr) pl.n_split = 1;
+    else if (p->workspace_bytes < part_bytes(p, pl.n_split)) return 1;
+    AttnArgs a;
+    a.q = p->q;
+    a.out = p->out;
+    a.k = reinterpret_cast<const uint8_t *>(p->k_pages);
+    a.v = reinterpret_cast<const uint8_t *>(p->v_pages);
+    a.table = p->table;
+    a.starts = p->starts;
+    a.kv_len = p->kv_len;
+    a.part = reinterpret_cast<float *>(p->workspace);
+    a.q_tok = p->q_tok;
+    a.out_tok = p->out_tok;
+    a.page_bytes = p->page_stride * 2;
+    a.head_bytes = (int64_t)p->page_size * p->head_dim * 2;
+    a.table_stride = p->table_stride;
+    a.n_tok = (int)p->n_tok;
+    a.n_seq = p->n_seq;
+    a.n_head = p->n_head;
+    a.n_kv = p->n_kv_head;
+    a.group = p->n_head / p->n_kv_head;
+    a.n_pages = p->max_pages > 0 ? (int)p->n_pages : 0;
+    a.page_log2 = __builtin_ctz((unsigned)p->page_size);
+    a.cap = p->max_pages * p->page_size;
+    a.chunk = pl.chunk;
+    a.n_split = pl.n_split;
+    a.tiles = pl.tiles;
+    a.c = p->scale * 1.4426950408889634f;
+    const hipStream_t s = (hipStream_t)stream;
+    const bool f32 = p->io_type == BONSAI_P40_F32;
+    if (p->kv_type == BONSAI_P40_F16)
+        return f32 ? launch_d<F16, 2>(p->head_dim, pl.keys, a, s) : launch_d<F16, 1>(p->head_dim, pl.keys, a, s);
+    return f32 ? launch_d<BF16, 3>(p->head_dim, pl.keys, a, s) : launch_d<BF16, 1>(p->head_dim, pl.keys, a, s);
+}

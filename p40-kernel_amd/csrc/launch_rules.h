@@ -190,6 +190,37 @@ inline void prefill_plan(bool wide, bool small, int64_t n_out, int64_t n_tok, in
     }
 }
 
+// Attention over pages (attn_paged.hip): workgroups whose waves split the keys
+// (32 rows, decode) or the rows (64 or 128), the number of row tiles that n_tok tokens
+// of n_seq sequences can have at most, and the keys of one workgroup: n_split
+// workgroups share a tile, the last of them takes what is left.
+struct AttnPlan {
+    bool keys;
+    int64_t tiles, chunk, n_split;
+};
+inline AttnPlan attn_plan(int64_t n_tok, int64_t n_seq, int64_t group, int64_t n_kv, int64_t dim, int64_t max_kv, int64_t rows,
+                          int64_t cus) {
+    AttnPlan p;
+    p.keys = n_tok * group <= 64 * n_seq;
+    const int64_t bm = p.keys ? 32 : rows, step = p.keys ? 128 : 64;
+    const int64_t some = n_seq < n_tok ? n_seq : n_tok;
+    p.tiles = n_tok * group / bm + some;
+    const int64_t blocks = (p.keys ? some : p.tiles) * n_kv;
+    const int64_t slots = cus * (256 / dim);
+    int64_t want = p.keys ? (some == 1 ? slots : 3 * slots) / blocks : blocks < 2 * cus ? (2 * cus + blocks - 1) / blocks : 1;
+    if (want < 1) want = 1;
+    p.chunk = (max_kv + want * step - 1) / (want * step) * step;
+    if (p.chunk < 2 * step) p.chunk = p.keys ? step : 4 * step;
+    p.n_split = max_kv > p.chunk ? (max_kv + p.chunk - 1) / p.chunk : 1;
+    return p;
+}
+
+// The gated delta rule (gdn.hip) in chunks of 64 tokens, or token by token.
+inline bool gdn_chunked(int64_t max_new, int64_t n_seq) {
+    (void)n_seq;
+    return max_new > 16;
+}
+
 }  // namespace pq2
 
 #endif

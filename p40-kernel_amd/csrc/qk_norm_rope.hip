@@ -1,0 +1,224 @@
+// qk_norm_rope.hip -- between the q/k/v projections and attention: RMSNorm of
+// every query and key head, position rotation, and the append of keys and
+// values to the pages of the cache, in one launch (bonsai_p40_qk_norm_rope).
+//
+//   y = x / sqrt(mean(x^2) + eps) * w                       per head row
+//   (y_i, y_j) -> (y_i c - y_j s, y_j c + y_i s),  c, s = cos, sin(pos f_i)
+//
+// It moves bytes and little else: 4 in and 2 or 4 out an element.  A workgroup
+// takes one head row of TT tokens; the angles of those tokens are computed once
+// into LDS.  An angle is pos * f / 2 pi in fp64, reduced to half a turn there:
+// in fp32 a position of 1e6 would leave it 4 bits.
+//   Rows (one per token): a wave reads a token's head row from memory.
+//   Columns (one row per feature, as bonsai_p40_gemm writes): the tile of
+// head_dim features x TT tokens goes through LDS, padded by a word a token so
+// that neither side of the transpose meets a bank twice.
+#include "host_state.h"
+#include "mixer_device.h"
+#include "pq2_device.h"
+
+using namespace mixer;
+
+namespace {
+
+struct QkvArgs {
+    const float * x[3];                 // q, k, v
+    int64_t tok[3], head[3], el[3];     // strides in floats
+    const float * w[3];                 // norm weights or NULL
+    const int32_t * pos;
+    const double * inv_freq;
+    const int64_t * slots;
+    void * q_out;
+    int64_t q_out_tok;
+    void * pages[2];                    // k, v
+    int64_t page_stride, n_slots;
+    float eps;
+    int n_tok, n_head, n_kv, half, interleaved, page_log2, tt, vec;
+};
+
+template <int D, class TQ, class TC>
+__global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkvArgs a) {
+    constexpr int E = D / 64;           // consecutive elements of a lane
+    extern __shared__ __attribute__((aligned(16))) float lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int row = blockIdx.y;
+    const int kind = row < a.n_head ? 0 : row < a.n_head + a.n_kv ? 1 : 2;
+    row -= kind == 0 ? 0 : a.n_head + (kind - 1) * a.n_kv;
+    const int t0 = blockIdx.x * a.tt, nt = min(a.tt, a.n_tok - t0);
+    const float * const x = a.x[kind] + (int64_t)row * a.head[kind];
+    const int64_t ts = a.tok[kind], es = a.el[kind];
+    const bool columns = es != 1;
+    float * const tile = lds;                                            // [tt][D + 1] where columns
+    float2 * const turn = reinterpret_cast<float2 *>(lds + (columns ? a.tt * (D + 1) + (a.tt & 1) : 0));   // [tt][half]
+
+    if (columns) {
+        // 32 tokens of a feature are one run of 128 bytes: half a wave each
+        const int sub = threadIdx.x & 31;
+        if (sub < nt) {
+            const float * const c = x + (int64_t)(t0 + sub) * ts;
+#pragma unroll 8
+            for (int e = threadIdx.x >> 5; e < D; e += 8) tile[sub * (D + 1) + e] = c[(int64_t)e * es];
+        }
+    }
+    if (kind < 2) {
+        for (int i = threadIdx.x; i < nt * a.half; i += 256) {
+            const int t = i / a.half, f = i - t * a.half;
+            const double rev = (double)a.pos[t0 + t] * a.inv_freq[f] * 0.15915494309189535;
+            const float r = (float)(rev - rint(rev));
+            float sn, cs;
+            sincospif(2.0f * r, &sn, &cs);
+            turn[i] = make_float2(cs, sn);
+        }
+    }
+    __syncthreads();
+
+    float w[E];
+#pragma unroll
+    for (int j = 0; j < E; ++j) w[j] = 1.0f;
+    const bool norm = kind < 2 && a.w[kind] != nullptr;
+    if (norm)
+#pragma unroll
+        for (int j = 0; j < E; ++j) w[j] = a.w[kind][lane * E + j];
+
+    for (int t = wave; t < nt; t += 4) {
+        float v[E];
+        if (columns) {
+#pragma unroll
+            for (int j = 0; j < E; ++j) v[j] = tile[t * (D + 1) + lane * E + j];
+        } else {
+            const float * const r = x + (int64_t)(t0 + t) * ts + lane * E;
+            if (a.vec) load_row<F32>(r, v);
+            else
+#pragma unroll
+                for (int j = 0; j < E; ++j) v[j] = r[j];
+        }
+        if (kind < 2) {
+            if (norm) {
+                float ss = 0.0f;
+#pragma unroll
+                for (int j = 0; j < E; ++j) ss = fmaf(v[j], v[j], ss);
+                ss = __builtin_bit_cast(float, __builtin_amdgcn_readlane(
+                         __builtin_bit_cast(int, pq2::wave_sum_to_lane63(ss)), 63));
+                const float s = 1.0f / sqrtf(ss * (1.0f / D) + a.eps);
+#pragma unroll
+                for (int j = 0; j < E; ++j) v[j] = v[j] * s * w[j];
+            }
+            if (a.half > 0) {
+                const float2 * const tr = turn + t * a.half;
+                float o[E];
+                if (a.interleaved) {
+#pragma unroll
+                    for (int j = 0; j < E; ++j) o[j] = E == 1 ? __shfl_xor(v[j], 1) : v[j ^ (E > 1)];
+                } else {
+                    // the partner is half elements away: a whole number of lanes
+                    const int d = a.half / E, src = lane < d ? lane + d : lane - d;
+#pragma unroll
+                    for (int j = 0; j < E; ++j) o[j] = __shfl(v[j], src & 63);
+                }
+#pragma unroll
+                for (int j = 0; j < E; ++j) {
+                    const int e = lane * E + j;
+                    if (e < 2 * a.half) {
+                        const bool second = a.interleaved ? (e & 1) : e >= a.half;
+                        const float2 cs = tr[a.interleaved ? e >> 1 : second ? e - a.half : e];
+                        v[j] = fmaf(second ? o[j] : -o[j], cs.y, v[j] * cs.x);
+                    }
+                }
+            }
+        }
+        if (kind == 0) {
+            typename TQ::elem * const q = reinterpret_cast<typename TQ::elem *>(a.q_out) +
+                                          (int64_t)(t0 + t) * a.q_out_tok + (int64_t)row * D + lane * E;
+            store_row<TQ>(q, v);
+        } else {
+            const int64_t slot = a.slots[t0 + t];
+            if (slot >= 0 && slot < a.n_slots) {
+                const int64_t page = slot >> a.page_log2, off = slot & ((1ll << a.page_log2) - 1);
+                typename TC::elem * const c = reinterpret_cast<typename TC::elem *>(a.pages[kind - 1]) +
+                    page * a.page_stride + (((int64_t)row << a.page_log2) + off) * D + lane * E;
+                store_row<TC>(c, v);
+            }
+        }
+    }
+}
+
+template <int D, class TQ, class TC>
+void launch(const QkvArgs & a, dim3 grid, size_t bytes, hipStream_t s) {
+    hipLaunchKernelGGL((qk_norm_rope_kernel<D, TQ, TC>), grid, dim3(256), bytes, s, a);
+}
+template <int D, class TQ>
+void launch_c(int kv, const QkvArgs & a, dim3 grid, size_t bytes, hipStream_t s) {
+    if (kv == BONSAI_P40_F16) launch<D, TQ, F16>(a, grid, bytes, s);
+    else launch<D, TQ, BF16>(a, grid, bytes, s);
+}
+template <int D>
+void launch_q(int q, int kv, const QkvArgs & a, dim3 grid, size_t bytes, hipStream_t s) {
+    if (q == BONSAI_P40_F32) launch_c<D, F32>(kv, a, grid, bytes, s);
+    else if (q == BONSAI_P40_F16) launch_c<D, F16>(kv, a, grid, bytes, s);
+    else launch_c<D, BF16>(kv, a, grid, bytes, s);
+}
+
+}  // namespace
+
+extern "C" int bonsai_p40_qk_norm_rope(const bonsai_p40_qk_norm_rope_args * p, bonsai_stream stream) {
+    if (!p) return 1;
+    const int d = p->head_dim;
+    if (d != 64 && d != 128 && d != 256) return 1;
+    if (p->n_head < 1 || p->n_kv_head < 1 || p->n_head > 16384 || p->n_kv_head > 16384) return 1;
+    if (p->n_rot < 0 || p->n_rot > d || p->n_rot % 8 != 0) return 1;
+    if (!is_type(p->q_type) || !is_half(p->kv_type) || !is_pow2(p->page_size) || p->page_size > 65536) return 1;
+    if (p->n_pages < 0 || p->n_pages > (1ll << 40) || p->page_stride < (int64_t)p->n_kv_head * p->page_size * d || p->page_stride % 8 != 0) return 1;
+    if (p->q_out_tok < (int64_t)p->n_head * d || p->q_out_tok % (16 / type_bytes(p->q_type)) != 0) return 1;
+    if (p->n_tok <= 0) return 0;
+    if (p->n_tok > 0x7fffffff / 64) return 1;
+    if (pq2host::any_null(p->q, p->k, p->v, p->slots, p->q_out, p->k_pages, p->v_pages)) return 1;
+    if (p->n_rot > 0 && pq2host::any_null(p->pos, p->inv_freq)) return 1;
+    if (!aligned(p->q_out, 16) || !aligned(p->k_pages, 16) || !aligned(p->v_pages, 16)) return 1;
+    if (!aligned(p->q_norm, 4) || !aligned(p->k_norm, 4) || !aligned(p->pos, 4) || !aligned(p->inv_freq, 8) ||
+        !aligned(p->slots, 8))
+        return 1;
+    QkvArgs a;
+    const float * const x[3] = {p->q, p->k, p->v};
+    const int64_t st[3][3] = {{p->q_tok, p->q_head, p->q_el}, {p->k_tok, p->k_head, p->k_el}, {p->v_tok, p->v_head, p->v_el}};
+    bool columns = false;
+    a.vec = 1;
+    for (int i = 0; i < 3; ++i) {
+        if (st[i][2] != 1 && (st[i][0] != 1 && p->n_tok > 1)) return 1;   // features or tokens are consecutive
+        a.x[i] = x[i];
+        a.tok[i] = st[i][0];
+        a.head[i] = st[i][1];
+        a.el[i] = st[i][2];
+        if (!aligned(x[i], 4)) return 1;
+        if (st[i][2] != 1) columns = true;
+        else if (!aligned(x[i], 16) || st[i][0] % 4 != 0 || st[i][1] % 4 != 0) a.vec = 0;
+    }
+    a.w[0] = p->q_norm;
+    a.w[1] = p->k_norm;
+    a.w[2] = nullptr;
+    a.pos = p->pos;
+    a.inv_freq = p->inv_freq;
+    a.slots = p->slots;
+    a.q_out = p->q_out;
+    a.q_out_tok = p->q_out_tok;
+    a.pages[0] = p->k_pages;
+    a.pages[1] = p->v_pages;
+    a.page_stride = p->page_stride;
+    a.page_log2 = __builtin_ctz((unsigned)p->page_size);
+    a.n_slots = p->n_pages << a.page_log2;
+    a.eps = p->eps;
+    a.n_tok = (int)p->n_tok;
+    a.n_head = p->n_head;
+    a.n_kv = p->n_kv_head;
+    a.half = p->n_rot / 2;
+    a.interleaved = p->interleaved != 0;
+    a.tt = columns || p->n_tok > 64 ? 32 : 4;
+    auto lds = [&](int tt) { return (columns ? (size_t)tt * (d + 1) * 4 : 0) + (size_t)tt * a.half * 8; };
+    if (lds(a.tt) > 64 * 1024) a.tt = 16;       // 256 columns, all of them rotated
+    const size_t bytes = lds(a.tt);
+    const dim3 grid((unsigned)((p->n_tok + a.tt - 1) / a.tt), (unsigned)(p->n_head + 2 * p->n_kv_head));
+    const hipStream_t s = (hipStream_t)stream;
+    if (d == 256) launch_q<256>(p->q_type, p->kv_type, a, grid, bytes, s);
+    else if (d == 128) launch_q<128>(p->q_type, p->kv_type, a, grid, bytes, s);
+    else launch_q<64>(p->q_type, p->kv_type, a, grid, bytes, s);
+    return (int)hipGetLastError();
+}
