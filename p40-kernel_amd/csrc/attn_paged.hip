@@ -37,6 +37,8 @@
 #include "launch_rules.h"
 #include "mixer_device.h"
 
+#include <type_traits>
+
 using namespace mixer;
 
 namespace {
@@ -82,12 +84,12 @@ struct Shape {
     // fp32 queries of 256: the registers hold one term of Q, the others are in LDS
     static constexpr bool QL = NT > 1 && D == 256;
     static constexpr int QR = QL ? 1 : NT;                 // terms in registers
-    static constexpr int KT = KEYS || QL ? 32 : 64;        // keys of a staged tile
     static constexpr int RB = 2 * D;                       // bytes of a key
-    static constexpr int TILE = KT * RB;
+    static constexpr int TILE = 32 * RB;                   // of a tile of 32 keys
+    static constexpr int R = QL ? 3 : 4;                   // rows: tiles of K, and of V, in LDS
     static constexpr int OROW = D + 4;                     // floats of a row in the join
     static constexpr int JOIN = NW * 32 * OROW * 4 + NW * 32 * 8;
-    static constexpr int MAIN = KEYS ? NW * 4 * TILE : 4 * TILE;   // two buffers of K and V
+    static constexpr int MAIN = KEYS ? NW * 4 * TILE : 2 * R * TILE;   // keys: two buffers of K and V a wave
     static constexpr int QT = 2 * 32 * D;                  // bytes of a term of 32 rows
     static constexpr int ALL = MAIN + (NT - QR) * (KEYS ? QT : NW * QT);
     static constexpr int LDS = KEYS && JOIN > ALL ? JOIN : ALL;
@@ -105,10 +107,10 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 31, half = lane >> 5;
-    // heads vary fastest (a head's tiles meet on the same XCDs), the last tiles,
-    // which see the most keys, start first
+    // heads vary fastest: a head's tiles meet on the same XCDs, and then in their L2, as those that run at the
+    // same time have the same keys; the last tiles, which see the most, start first
     const int kvh = blockIdx.x % a.n_kv, rest = blockIdx.x / a.n_kv;
-    const int split = rest % a.n_split, tile_no = a.tiles - 1 - rest / a.n_split;
+    const int split = rest / a.tiles, tile_no = a.tiles - 1 - rest % a.tiles;
     const Tile tl = find_tile<Z::BM>(a.starts, a.n_seq, a.n_tok, a.group, tile_no);
     if (tl.seq < 0) return;
     const int rows = tl.count * a.group, row0 = tl.index * Z::BM;
@@ -204,19 +206,19 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
         const int id = sload(a.table, trow + (key >> a.page_log2));
         return id >= 0 && id < a.n_pages ? id : -1;
     };
-    auto stage16 = [&](const uint8_t * base, int id, int key, uint8_t * dst, bool is_v) __attribute__((always_inline)) {
+    // N keys of one page from `key` on to dst; place: that of the first among 16, as far as the swizzle looks
+    auto stage_n = [&](auto count, const uint8_t * base, int id, int key, int place, uint8_t * dst, bool is_v) __attribute__((always_inline)) {
         const uint8_t * const p = base + (int64_t)max(id, 0) * a.page_bytes + (int64_t)kvh * a.head_bytes +
                                   (int64_t)(key & ((1 << a.page_log2) - 1)) * Z::RB;
 #pragma unroll
-        for (int i = 0; i < 16 / RPI; ++i) {
-            const int kr = i * RPI + drow;                 // key % 16, and as far as the swizzle looks, key in the tile
-            const int u = dunit ^ (is_v ? swz_v(kr) : swz_k(kr));
+        for (int i = 0; i < decltype(count)::value / RPI; ++i) {
+            const int kr = i * RPI + drow, u = dunit ^ (is_v ? swz_v(place + kr) : swz_k(place + kr));
             dma16(p + kr * Z::RB + 16 * u, dst + i * 1024);
         }
     };
-    // zero the V rows [from, 16) of a 16-key group: p is 0 there, and 0 times what memory holds may be NaN
-    auto zero16 = [&](uint8_t * dst, int from) {
-        for (int i = from * U + lane; i < 16 * U; i += 64) *reinterpret_cast<v4u *>(dst + 16 * i) = v4u{};
+    // zero the rows [from, to) of V: p is 0 there, and 0 times what memory holds may be NaN
+    auto zero_keys = [&](uint8_t * dst, int from, int to) {
+        for (int i = from * U + lane; i < to * U; i += 64) *reinterpret_cast<v4u *>(dst + 16 * i) = v4u{};
     };
 
     // ---- one sub-tile of 32 keys: kb, vb its first keys in LDS, key0 its place
@@ -235,35 +237,39 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
         }
         return s;
     };
-    auto softmax = [&](v16f & s, int key0, int holes) __attribute__((always_inline)) {
-        if (key0 + 32 > least || holes) {
+    // scores that are not seen to -inf
+    auto mask = [&](v16f & s, int key0, int holes) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int j = 8 * (i / 4) + 4 * half + i % 4;
-                if (key0 + j >= vis || (holes >> (j >> 4) & 1)) s[i] = -INFINITY;
-            }
+        for (int i = 0; i < 16; ++i) {
+            const int j = 8 * (i / 4) + 4 * half + i % 4;
+            if (key0 + j >= vis || (holes >> (j >> 4) & 1)) s[i] = -INFINITY;
         }
+    };
+    // m follows the running maximum with a lag of up to 2^8, which the sums bear: they are rescaled seldom
+    auto maximum = [&](const v16f & s) __attribute__((always_inline)) {
         float mx = s[0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float m2 = fmaxf(m, mx * c);
-        const float ref = m2 == -INFINITY ? 0.0f : m2;
-        const float alpha = __builtin_amdgcn_exp2f(m - ref);
+        mx = fmaxf(mx, __shfl_xor(mx, 32)) * c;
+        if (__any(mx > m + 8.0f)) {
+            const float m2 = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - (m2 == -INFINITY ? 0.0f : m2));
+            m = m2;
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
+        }
+    };
+    auto weights = [&](v16f & s) __attribute__((always_inline)) {
+        const float ref = m == -INFINITY ? 0.0f : m;
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -ref));
             sum += s[i];
         }
-        l = fmaf(l, alpha, sum);
-        m = m2;
-        if (__any(alpha != 1.0f)) {
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
-        }
+        l += sum;
     };
     // where some rows of the wave see a key and others do not, p = 0 does not keep an infinity or NaN of V out
     // of the others' sums: bit k: key k of the sub-tile has one
@@ -340,50 +346,82 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
     };
 
     if constexpr (!KEYS) {
-        constexpr int KT = Z::KT;
-        // each wave stages K and V of 16 keys, or of 32 keys waves 0, 1 K and 2, 3 V
-        constexpr bool SPLIT = KT < 16 * Z::NW;
-        const int own = SPLIT ? (wave & 1) * 16 : wave * 16;
-        int holes_next = 0;
-        auto stage = [&](int key, uint8_t * to) __attribute__((always_inline)) {
-            uint8_t * const kd = to + own * Z::RB;
-            const int mine = page_of(key + own);
-            if (!SPLIT || wave < 2) stage16(a.k, mine, key + own, kd, false);
-            if (!SPLIT || wave >= 2) stage16(a.v, mine, key + own, kd + Z::TILE, true);
-            holes_next = 0;
+        // A tile of 32 keys at a time: while the matrix cores work on the scores of tile j + 1, the weights of
+        // tile j are made, then O takes them.  R tiles of K and R of V are in LDS, the others on their way
+        constexpr int R = Z::R, OWN = 32 / Z::NW, PER = 2 * OWN / RPI;   // keys, and DMA instructions, of a wave a tile
+        const int own = wave * OWN, nt = (k1 - k0 + 31) / 32;
+        uint8_t * const kring = lds, * const vring = lds + R * Z::TILE;
+        uint32_t hq = 0;                                   // holes of the last 16 tiles, 2 bits each
+        int idk = -1, idv = -1;                            // pages of this wave's keys of the next tiles of K and of V
+        auto look = [&](int t) __attribute__((always_inline)) {
+            const int key = k0 + 32 * t, a0 = page_of(key), a1 = page_of(key + 16), at = 2 * (t & 15);
+            hq = (hq & ~(3u << at)) | (uint32_t)((a0 < 0 ? 1 : 0) | (a1 < 0 ? 2 : 0)) << at;
+            idv = idk;
+            idk = own < 16 ? a0 : a1;
+        };
+        auto stage = [&](const uint8_t * base, int id, int t, uint8_t * to, bool is_v) __attribute__((always_inline)) {
+            stage_n(std::integral_constant<int, OWN>{}, base, id, k0 + 32 * t + own, own & 15, to + own * Z::RB, is_v);
+        };
+        // that the buffers differ has to be said, else every read of LDS waits for the DMA
+        auto step = [&](auto edge, uint8_t * __restrict__ kw, uint8_t * __restrict__ vw, const uint8_t * __restrict__ kr,
+                        uint8_t * __restrict__ vr, const uint8_t * __restrict__ qlow, v16f & s, int j) __attribute__((always_inline)) {
+            constexpr bool EDGE = decltype(edge)::value;
+            if (j + R < nt) stage(a.k, idk, j + R, kw, false);
+            if (j + R - 1 < nt) stage(a.v, idv, j + R - 1, vw, true);
+            const int key = k0 + 32 * j, holes = hq >> (2 * (j & 15)) & 3;
+            if (j + R + 1 < nt) look(j + R + 1);
+            else idv = idk;
+            const bool mixed = EDGE && key + 32 > first_vis && nk > max(first_vis, key);
+            if (!work && !mixed) return;
+            if (EDGE || holes) mask(s, key, holes);
+            maximum(s);
+            v16f next = scores(kr, qlow);
+            weights(s);
+            if (EDGE)
+                if (mixed) apart(s, vr, key);
+            values(s, vr);
+            s = next;
+        };
+        if (nt > 0) {
 #pragma unroll
-            for (int g = 0; g < KT / 16; ++g) holes_next |= (page_of(key + 16 * g) < 0 ? 1 : 0) << g;
-        };
-        // the next tile's DMA runs while this one is computed on; that the buffers
-        // differ has to be said, else every read of LDS waits for the DMA
-        auto step = [&](uint8_t * __restrict__ next, uint8_t * __restrict__ cur, const uint8_t * __restrict__ qlow,
-                        int key, int holes) __attribute__((always_inline)) {
-            if (key + KT < k1) stage(key + KT, next);
-            const bool mixed = key + KT > first_vis && nk > max(first_vis, key);
-            if (work || mixed) {
-#pragma unroll 1
-                for (int u = 0; u < KT / 32; ++u) {
-                    v16f s = scores(cur + 32 * u * Z::RB, qlow);
-                    softmax(s, key + 32 * u, holes >> (2 * u) & 3);
-                    if (mixed) apart(s, cur + Z::TILE + 32 * u * Z::RB, key + 32 * u);
-                    values(s, cur + Z::TILE + 32 * u * Z::RB);
+            for (int t = 0; t < R; ++t) {
+                if (t < nt) {
+                    look(t);
+                    stage(a.k, idk, t, kring + t * Z::TILE, false);
+                } else {
+                    idv = idk;
                 }
+                if (t > 0 && t - 1 < nt) stage(a.v, idv, t - 1, vring + (t - 1) * Z::TILE, true);
             }
-        };
-        if (k0 < k1) stage(k0, lds);
-        int b = 0;
-#pragma clang loop unroll(disable)
-        for (int key = k0; key < k1; key += KT, b ^= 1) {
-            const int holes = holes_next;
-            uint8_t * const cur = lds + b * 2 * Z::TILE;
-            pq2::wait_vmcnt<0>();
-            const bool hole = holes >> (own >> 4) & 1;
-            if ((!SPLIT || wave >= 2) && (hole || key + own + 16 > nk))
-                zero16(cur + Z::TILE + own * Z::RB, hole ? 0 : max(nk - key - own, 0));
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();                  // the tile is there, and all have left the other buffer
+            if (R < nt) look(R);
+            else idv = idk;
+            if (nt >= R) pq2::wait_vmcnt<(R - 1) * PER>();
+            else pq2::wait_vmcnt<0>();
+            __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            step(lds + (b ^ 1) * 2 * Z::TILE, cur, ql, key, holes);
+            v16f s = scores(kring, ql);
+            // tiles that every row sees whole, then those at the edge
+            const int plain = max(min(nt, (first_vis - k0) / 32), 0);
+            int slot = 0;
+            auto pass = [&](auto edge, int j) __attribute__((always_inline)) {
+                const int after = slot + 1 == R ? 0 : slot + 1, before = slot == 0 ? R - 1 : slot - 1;
+                if (j - 1 + R < nt) pq2::wait_vmcnt<(R - 2) * PER>();
+                else pq2::wait_vmcnt<0>();
+                const int holes = hq >> (2 * (j & 15)) & 3, key = k0 + 32 * j + own;
+                const bool hole = holes >> (own >> 4) & 1;
+                uint8_t * const vr = vring + slot * Z::TILE;
+                if (hole || key + OWN > nk) zero_keys(vr + own * Z::RB, hole ? 0 : iclamp(nk - key, 0, OWN), OWN);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();              // the tiles are there, and all are done with the last ones
+                asm volatile("" ::: "memory");
+                step(edge, kring + slot * Z::TILE, vring + before * Z::TILE, kring + after * Z::TILE, vr, ql, s, j);
+                slot = after;
+            };
+            int j = 0;
+#pragma clang loop unroll(disable)
+            for (; j < plain; ++j) pass(std::false_type{}, j);
+#pragma clang loop unroll(disable)
+            for (; j < nt; ++j) pass(std::true_type{}, j);
         }
     } else {
         uint8_t * const mine = lds + wave * 4 * Z::TILE;
@@ -391,16 +429,19 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
         auto stage = [&](int key, uint8_t * to) __attribute__((always_inline)) {
             id0 = page_of(key);
             id1 = page_of(key + 16);
-            stage16(a.k, id0, key, to, false);
-            stage16(a.k, id1, key + 16, to + 16 * Z::RB, false);
-            stage16(a.v, id0, key, to + Z::TILE, true);
-            stage16(a.v, id1, key + 16, to + Z::TILE + 16 * Z::RB, true);
+            const std::integral_constant<int, 16> half_tile;
+            stage_n(half_tile, a.k, id0, key, 0, to, false);
+            stage_n(half_tile, a.k, id1, key + 16, 0, to + 16 * Z::RB, false);
+            stage_n(half_tile, a.v, id0, key, 0, to + Z::TILE, true);
+            stage_n(half_tile, a.v, id1, key + 16, 0, to + Z::TILE + 16 * Z::RB, true);
         };
         auto step = [&](uint8_t * __restrict__ next, uint8_t * __restrict__ cur, const uint8_t * __restrict__ qlow,
                         int key, int holes) __attribute__((always_inline)) {
             if (key + 32 * Z::NW < k1) stage(key + 32 * Z::NW, next);
             v16f s = scores(cur, qlow);
-            softmax(s, key, holes);
+            if (key + 32 > least || holes) mask(s, key, holes);
+            maximum(s);
+            weights(s);
             if (key + 32 > first_vis && nk > max(first_vis, key)) apart(s, cur + Z::TILE, key);
             values(s, cur + Z::TILE);
         };
@@ -412,8 +453,8 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
             uint8_t * const cur = mine + b * 2 * Z::TILE;
             pq2::wait_vmcnt<0>();
             if (holes || key + 32 > nk) {
-                zero16(cur + Z::TILE, holes & 1 ? 0 : iclamp(nk - key, 0, 16));
-                zero16(cur + Z::TILE + 16 * Z::RB, holes & 2 ? 0 : iclamp(nk - key - 16, 0, 16));
+                zero_keys(cur + Z::TILE, holes & 1 ? 0 : iclamp(nk - key, 0, 16), 16);
+                zero_keys(cur + Z::TILE, holes & 2 ? 16 : iclamp(nk - key, 16, 32), 32);
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // also: the other buffer's reads are done
             step(mine + (b ^ 1) * 2 * Z::TILE, cur, ql, key, holes);

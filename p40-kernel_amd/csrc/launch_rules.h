@@ -205,12 +205,26 @@ inline AttnPlan attn_plan(int64_t n_tok, int64_t n_seq, int64_t group, int64_t n
     const int64_t bm = p.keys ? 32 : rows, step = p.keys ? 128 : 64;
     const int64_t some = n_seq < n_tok ? n_seq : n_tok;
     p.tiles = n_tok * group / bm + some;
-    const int64_t blocks = (p.keys ? some : p.tiles) * n_kv;
-    const int64_t slots = cus * (256 / dim);
-    int64_t want = p.keys ? (some == 1 ? slots : 3 * slots) / blocks : blocks < 2 * cus ? (2 * cus + blocks - 1) / blocks : 1;
+    int64_t want = 1;
+    if (p.keys) {
+        const int64_t slots = cus * (256 / dim);
+        want = (some == 1 ? slots : 3 * slots) / (some * n_kv);
+    } else {
+        // rounds of workgroups times the keys of one, or the longest; a part of a row is written and read
+        const int64_t slots = cus * (dim == 256 ? 1 : 2), blocks = p.tiles * n_kv;
+        const double key = 0.022 * (double)dim / 256, part = (double)n_tok * group * n_kv * dim * 8 / 4.5e6;
+        const double longest = (double)max_kv, mean = longest - 0.5 * (double)(n_tok / some < max_kv ? n_tok / some : max_kv);
+        double best = 0.0;
+        for (int64_t n = 1; n <= 16 && blocks < 2 * slots; ++n) {
+            const double rounds = (double)((blocks * n + slots - 1) / slots) * mean;
+            const double us = key * (rounds > longest ? rounds : longest) / (double)n + (n > 1 ? 5.0 + part * (double)n : 0.0);
+            if (n == 1 || us < best) best = us, want = n;
+        }
+    }
     if (want < 1) want = 1;
     p.chunk = (max_kv + want * step - 1) / (want * step) * step;
-    if (p.chunk < 2 * step) p.chunk = p.keys ? step : 4 * step;
+    if (p.chunk < step) p.chunk = step;
+    if (p.keys && p.chunk < 2 * step) p.chunk = step;
     p.n_split = max_kv > p.chunk ? (max_kv + p.chunk - 1) / p.chunk : 1;
     return p;
 }
