@@ -116,7 +116,8 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
     const int rows = tl.count * a.group, row0 = tl.index * Z::BM;
     const int kv = iclamp(sload(a.kv_len, tl.seq), 0, a.cap), before = kv - tl.count;
     const int last = min(row0 + Z::BM, rows) - 1;
-    const int nk = a.n_pages > 0 ? iclamp(before + last / a.group + 1, 0, kv) : 0;
+    // (readfirstlane: the same in all lanes, which the compiler does not see through the division)
+    const int nk = a.n_pages > 0 ? __builtin_amdgcn_readfirstlane(iclamp(before + last / a.group + 1, 0, kv)) : 0;
     const int k0 = split * a.chunk;
     const int k1 = split == a.n_split - 1 ? nk : min(nk, k0 + a.chunk);
     if (split > 0 && k0 >= nk) return;                     // the join counts the parts
@@ -130,10 +131,10 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
     const int64_t grow = (int64_t)(tl.first + tok);
     // the fewest keys any live row of the wave sees; 0 rows: nothing to do but stage
     const bool work = wrow < rows;
-    const int least = work ? iclamp(before + wrow / a.group + 1, 0, kv) : 0;
+    const int least = work ? __builtin_amdgcn_readfirstlane(iclamp(before + wrow / a.group + 1, 0, kv)) : 0;
 
     // the keys that all rows of the workgroup see
-    const int first_vis = iclamp(before + row0 / a.group + 1, 0, kv);
+    const int first_vis = __builtin_amdgcn_readfirstlane(iclamp(before + row0 / a.group + 1, 0, kv));
 
     // Q^T, element j of half h: d = 16 step + 8 h + j
     frag qf[Z::QR][QS];
@@ -223,12 +224,23 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
 
     // ---- one sub-tile of 32 keys: kb, vb its first keys in LDS, key0 its place
     // in the sequence, holes: bit g: the 16 keys from 16 g on are absent
+    // the swizzle leaves the address of step i, or of the 32 d of block i, at one address XOR a constant
     const int l16 = lane & 15, vkey = 4 * half + (l16 >> 2), vcol = 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1);
+    uint32_t kat = n * Z::RB + 16 * (half ^ swz_k(n)), vat = vkey * Z::RB + 16 * (vcol ^ swz_v(vkey)) + 8 * (l16 & 1);
+    auto k_frag = [&](const uint8_t * kb, int i) __attribute__((always_inline)) {
+        return *reinterpret_cast<const frag *>(kb + (kat ^ (32 * i)));
+    };
+    // keys 16 g + 4 half + j % 4 + 8 (j / 4) of d = 32 d + lane % 32
+    auto v_frag = [&](const uint8_t * vb, int d, int g) __attribute__((always_inline)) {
+        const uint8_t * const at = vb + (vat ^ (64 * d)) + 16 * g * Z::RB;
+        const v2u x = read_tr(at), y = read_tr(at + 8 * Z::RB);
+        return __builtin_bit_cast(frag, (v4u){x[0], x[1], y[0], y[1]});
+    };
     auto scores = [&](const uint8_t * kb, const uint8_t * ql) __attribute__((always_inline)) {
         v16f s = {};
 #pragma unroll
         for (int i = 0; i < QS; ++i) {
-            const frag kf = *reinterpret_cast<const frag *>(kb + n * Z::RB + 16 * ((2 * i + half) ^ swz_k(n)));
+            const frag kf = k_frag(kb, i);
 #pragma unroll
             for (int k = NT - 1; k >= Z::QR; --k)
                 s = mfma<T>(kf, *reinterpret_cast<const frag *>(ql + (k - Z::QR) * Z::QT + 1024 * i), s);
@@ -245,12 +257,22 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
             if (key0 + j >= vis || (holes >> (j >> 4) & 1)) s[i] = -INFINITY;
         }
     };
-    // m follows the running maximum with a lag of up to 2^8, which the sums bear: they are rescaled seldom
-    auto maximum = [&](const v16f & s) __attribute__((always_inline)) {
+    // a row's largest score, in units of log2: half the keys are in lane ^ 32
+    auto over_halves = [&](float mx) __attribute__((always_inline)) {
+        const uint32_t x = __builtin_bit_cast(uint32_t, mx);
+        const auto both = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+        uint32_t lo = both[0], hi = both[1];
+        asm("" : "+v"(lo), "+v"(hi));                      // they differ, though the operands do not
+        return fmaxf(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi)) * c;
+    };
+    auto largest = [&](const v16f & s) __attribute__((always_inline)) {
         float mx = s[0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32)) * c;
+        return over_halves(mx);
+    };
+    // m follows the running maximum with a lag of up to 2^8, which the sums bear: they are rescaled seldom
+    auto follow = [&](float mx) __attribute__((always_inline)) {
         if (__any(mx > m + 8.0f)) {
             const float m2 = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - (m2 == -INFINITY ? 0.0f : m2));
             m = m2;
@@ -263,13 +285,13 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
     };
     auto weights = [&](v16f & s) __attribute__((always_inline)) {
         const float ref = m == -INFINITY ? 0.0f : m;
-        float sum = 0.0f;
+        float sum[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -ref));
-            sum += s[i];
+            sum[i & 1] += s[i];
         }
-        l += sum;
+        l += sum[0] + sum[1];
     };
     // where some rows of the wave see a key and others do not, p = 0 does not keep an infinity or NaN of V out
     // of the others' sums: bit k: key k of the sub-tile has one
@@ -331,18 +353,13 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
                 }
             }
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
+        for (int g = 0; g < 2; ++g)
 #pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                const uint8_t * const at = vb + (16 * g + vkey) * Z::RB + 8 * (l16 & 1);
-                const int u = 4 * d + vcol;
-                const v2u x = read_tr(at + 16 * (u ^ swz_v(vkey)));
-                const v2u y = read_tr(at + 8 * Z::RB + 16 * (u ^ swz_v(vkey + 8)));
-                const frag vf = __builtin_bit_cast(frag, (v4u){x[0], x[1], y[0], y[1]});
+            for (int d = 0; d < DT; ++d) {
+                const frag vf = v_frag(vb, d, g);
 #pragma unroll
                 for (int k = NT - 1; k >= 0; --k) o[d] = mfma<T>(vf, pf[k][g], o[d]);
             }
-        }
     };
 
     if constexpr (!KEYS) {
@@ -353,53 +370,119 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
         uint8_t * const kring = lds, * const vring = lds + R * Z::TILE;
         uint32_t hq = 0;                                   // holes of the last 16 tiles, 2 bits each
         int idk = -1, idv = -1;                            // pages of this wave's keys of the next tiles of K and of V
-        auto look = [&](int t) __attribute__((always_inline)) {
-            const int key = k0 + 32 * t, a0 = page_of(key), a1 = page_of(key + 16), at = 2 * (t & 15);
-            hq = (hq & ~(3u << at)) | (uint32_t)((a0 < 0 ? 1 : 0) | (a1 < 0 ? 2 : 0)) << at;
+        // the table's entries for tile t are asked for one tile before they are taken
+        int raw0 = 0, raw1 = 0;
+        const int top = max(nk - 1, 0) >> a.page_log2;
+        auto ask = [&](int t) __attribute__((always_inline)) {
+            const int key = k0 + 32 * t;
+            raw0 = sload(a.table, trow + min(key >> a.page_log2, top));
+            raw1 = sload(a.table, trow + min((key + 16) >> a.page_log2, top));
+        };
+        auto take = [&](int t) __attribute__((always_inline)) {
+            const int key = k0 + 32 * t, at = 2 * (t & 15);
+            const bool ok0 = key < nk && (uint32_t)raw0 < (uint32_t)a.n_pages;
+            const bool ok1 = key + 16 < nk && (uint32_t)raw1 < (uint32_t)a.n_pages;
+            hq = (hq & ~(3u << at)) | (uint32_t)((ok0 ? 0 : 1) | (ok1 ? 0 : 2)) << at;
             idv = idk;
-            idk = own < 16 ? a0 : a1;
+            idk = own < 16 ? (ok0 ? raw0 : -1) : (ok1 ? raw1 : -1);
         };
         auto stage = [&](const uint8_t * base, int id, int t, uint8_t * to, bool is_v) __attribute__((always_inline)) {
             stage_n(std::integral_constant<int, OWN>{}, base, id, k0 + 32 * t + own, own & 15, to + own * Z::RB, is_v);
         };
         // that the buffers differ has to be said, else every read of LDS waits for the DMA
         auto step = [&](auto edge, uint8_t * __restrict__ kw, uint8_t * __restrict__ vw, const uint8_t * __restrict__ kr,
-                        uint8_t * __restrict__ vr, const uint8_t * __restrict__ qlow, v16f & s, int j) __attribute__((always_inline)) {
+                        uint8_t * __restrict__ vr, const uint8_t * __restrict__ qlow, v16f & s, float & mx, int j) __attribute__((always_inline)) {
             constexpr bool EDGE = decltype(edge)::value;
+            // fragments are read AHEAD steps before they are used
+            constexpr int AHEAD = Z::QL ? 2 : 4;
+            asm volatile("" : "+v"(kat), "+v"(vat));       // addresses are made at each step: 24 registers are not there
+            frag kf[AHEAD], lf[AHEAD][NT];
+            auto k_read = [&](int i) __attribute__((always_inline)) {
+                kf[i % AHEAD] = k_frag(kr, i);
+#pragma unroll
+                for (int k = Z::QR; k < NT; ++k)
+                    lf[i % AHEAD][k - Z::QR] = *reinterpret_cast<const frag *>(qlow + (k - Z::QR) * Z::QT + 1024 * i);
+            };
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) k_read(i);
+            __builtin_amdgcn_sched_barrier(0);
+            take(j + R);
+            ask(j + R + 1);
             if (j + R < nt) stage(a.k, idk, j + R, kw, false);
             if (j + R - 1 < nt) stage(a.v, idv, j + R - 1, vw, true);
             const int key = k0 + 32 * j, holes = hq >> (2 * (j & 15)) & 3;
-            if (j + R + 1 < nt) look(j + R + 1);
-            else idv = idk;
             const bool mixed = EDGE && key + 32 > first_vis && nk > max(first_vis, key);
             if (!work && !mixed) return;
-            if (EDGE || holes) mask(s, key, holes);
-            maximum(s);
-            v16f next = scores(kr, qlow);
-            weights(s);
-            if (EDGE)
+            if (EDGE || holes) {
+                mask(s, key, holes);
+                mx = largest(s);
+            }
+            follow(mx);
+            // the scores of the next tile, and between their MFMAs the weights of this one (E of a step)
+            constexpr int E = 16 / QS > 0 ? 16 / QS : 1;
+            const float ref = m == -INFINITY ? 0.0f : m;
+            float sum[2] = {0.0f, 0.0f};
+            frag vf[AHEAD], pf[NT][2];
+            v16f next = {};
+            // lgkmcnt(0): with a scalar load under way the waits below could not count
+            __builtin_amdgcn_s_waitcnt(0xC07F);
+#pragma unroll
+            for (int i = 0; i < QS; ++i) {
+#pragma unroll
+                for (int k = NT - 1; k >= Z::QR; --k) next = mfma<T>(kf[i % AHEAD], lf[i % AHEAD][k - Z::QR], next);
+#pragma unroll
+                for (int k = Z::QR - 1; k >= 0; --k) next = mfma<T>(kf[i % AHEAD], qf[k][i], next);
+                if (i + AHEAD < QS) k_read(i + AHEAD);
+                else if (!EDGE) vf[i + AHEAD - QS] = v_frag(vr, (i + AHEAD - QS) % DT, (i + AHEAD - QS) / DT);
+#pragma unroll
+                for (int e = i * E; e < (i + 1) * E; ++e) {
+                    s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, -ref));
+                    sum[e & 1] += s[e];
+                    float f = s[e];
+#pragma unroll
+                    for (int k = 0; k < NT; ++k) {
+                        const elem x = T::from(f);
+                        pf[k][e / 8][e % 8] = x;
+                        f -= T::to(x);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            l += sum[0] + sum[1];
+            if (EDGE) {
                 if (mixed) apart(s, vr, key);
-            values(s, vr);
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) vf[i] = v_frag(vr, i % DT, i / DT);
+            }
+            // O takes them, and between the MFMAs the largest of the next scores are found
+            float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int i = 0; i < 2 * DT; ++i) {
+#pragma unroll
+                for (int k = NT - 1; k >= 0; --k) o[i % DT] = mfma<T>(vf[i % AHEAD], pf[k][i / DT], o[i % DT]);
+                if (i + AHEAD < 2 * DT) vf[i % AHEAD] = v_frag(vr, (i + AHEAD) % DT, (i + AHEAD) / DT);
+#pragma unroll
+                for (int e = i * 8 / DT; e < (i + 1) * 8 / DT; ++e) top[e & 1] = fmaxf(top[e & 1], next[e]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            mx = over_halves(fmaxf(top[0], top[1]));
             s = next;
         };
         if (nt > 0) {
+            ask(0);
 #pragma unroll
             for (int t = 0; t < R; ++t) {
-                if (t < nt) {
-                    look(t);
-                    stage(a.k, idk, t, kring + t * Z::TILE, false);
-                } else {
-                    idv = idk;
-                }
+                take(t);
+                ask(t + 1);
+                if (t < nt) stage(a.k, idk, t, kring + t * Z::TILE, false);
                 if (t > 0 && t - 1 < nt) stage(a.v, idv, t - 1, vring + (t - 1) * Z::TILE, true);
             }
-            if (R < nt) look(R);
-            else idv = idk;
             if (nt >= R) pq2::wait_vmcnt<(R - 1) * PER>();
             else pq2::wait_vmcnt<0>();
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
             v16f s = scores(kring, ql);
+            float mx = largest(s);
             // tiles that every row sees whole, then those at the edge
             const int plain = max(min(nt, (first_vis - k0) / 32), 0);
             int slot = 0;
@@ -414,7 +497,7 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 __builtin_amdgcn_s_barrier();              // the tiles are there, and all are done with the last ones
                 asm volatile("" ::: "memory");
-                step(edge, kring + slot * Z::TILE, vring + before * Z::TILE, kring + after * Z::TILE, vr, ql, s, j);
+                step(edge, kring + slot * Z::TILE, vring + before * Z::TILE, kring + after * Z::TILE, vr, ql, s, mx, j);
                 slot = after;
             };
             int j = 0;
@@ -440,7 +523,7 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
             if (key + 32 * Z::NW < k1) stage(key + 32 * Z::NW, next);
             v16f s = scores(cur, qlow);
             if (key + 32 > least || holes) mask(s, key, holes);
-            maximum(s);
+            follow(largest(s));
             weights(s);
             if (key + 32 > first_vis && nk > max(first_vis, key)) apart(s, cur + Z::TILE, key);
             values(s, cur + Z::TILE);
