@@ -209,12 +209,14 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
     };
     // N keys of one page from `key` on to dst; place: that of the first among 16, as far as the swizzle looks
     auto stage_n = [&](auto count, const uint8_t * base, int id, int key, int place, uint8_t * dst, bool is_v) __attribute__((always_inline)) {
-        const uint8_t * const p = base + (int64_t)max(id, 0) * a.page_bytes + (int64_t)kvh * a.head_bytes +
-                                  (int64_t)(key & ((1 << a.page_log2) - 1)) * Z::RB;
+        // the page's rows of this head, and no others, are in range
+        const auto from = buffer_of(base + (int64_t)max(id, 0) * a.page_bytes + (int64_t)kvh * a.head_bytes,
+                                    Z::RB << a.page_log2);
+        const int first = (key & ((1 << a.page_log2) - 1)) * Z::RB;
 #pragma unroll
         for (int i = 0; i < decltype(count)::value / RPI; ++i) {
             const int kr = i * RPI + drow, u = dunit ^ (is_v ? swz_v(place + kr) : swz_k(place + kr));
-            dma16(p + kr * Z::RB + 16 * u, dst + i * 1024);
+            dma16(from, dst + i * 1024, drow * Z::RB + 16 * u, first + i * 1024);
         }
     };
     // zero the rows [from, to) of V: p is 0 there, and 0 times what memory holds may be NaN

@@ -436,7 +436,8 @@ __global__ void __launch_bounds__(256) gdn_scan_kernel(GdnArgs a) {
     chunks = iclamp(chunks, 0, max(a.chunks - chunk0, 0));   // starts that overlap: what prep made, no more
 
     auto copy = [&](const uint8_t * src, uint8_t * dst, int bytes) __attribute__((always_inline)) {
-        for (int i = wave * 1024; i < bytes; i += 4096) dma16(src + i + 16 * lane, dst + i);
+        const auto from = buffer_of(src, bytes);
+        for (int i = wave * 1024; i < bytes; i += 4096) dma16(from, dst + i, 16 * lane, i);
     };
     auto stage1 = [&](int c) __attribute__((always_inline)) {
         copy(a.ws + ((int64_t)(chunk0 + c) * a.n_kh + hk) * W::HEAD, r1, REG1);

@@ -62,9 +62,15 @@ __device__ __forceinline__ int sload(const int32_t * p, int64_t i) {
     typedef const __attribute__((address_space(4))) int32_t cint;
     return *(cint *)(uintptr_t)(p + i);
 }
-// 16 bytes a lane to LDS: dst is the wave's, lane l lands at dst + 16 l
-__device__ __forceinline__ void dma16(const uint8_t * src, uint8_t * dst) {
-    __builtin_amdgcn_global_load_lds(src, (lds_void *)dst, 16, 0, 0);
+// 16 bytes a lane from a buffer (uniform base, a lane's offset, a constant one) to
+// LDS: dst is the wave's, lane l lands at dst + 16 l.  Through the buffer path, as
+// beside the global one (which counts as a flat access) the compiler's waits for
+// LDS reads no longer count, but wait for all.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const uint8_t * base, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), (short)0, bytes, 0x00020000);
+}
+__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t from, uint8_t * dst, int off, int soff) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_void *)dst, 16, off, soff, 0, 0);
 }
 
 // Which sequence a tile of up to BM rows (per_tok of them a token) belongs to;
