@@ -207,16 +207,26 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
         const int id = sload(a.table, trow + (key >> a.page_log2));
         return id >= 0 && id < a.n_pages ? id : -1;
     };
-    // N keys of one page from `key` on to dst; place: that of the first among 16, as far as the swizzle looks
-    auto stage_n = [&](auto count, const uint8_t * base, int id, int key, int place, uint8_t * dst, bool is_v) __attribute__((always_inline)) {
-        // the page's rows of this head, and no others, are in range
-        const auto from = buffer_of(base + (int64_t)max(id, 0) * a.page_bytes + (int64_t)kvh * a.head_bytes,
-                                    Z::RB << a.page_log2);
-        const int first = (key & ((1 << a.page_log2) - 1)) * Z::RB;
+    // N keys of one page from `key` on to dst; place: that of the first among 16, as far as the swizzle looks.
+    // The page's rows of this head, and no others, are in range
+    const uint8_t * const khead = a.k + (int64_t)kvh * a.head_bytes, * const vhead = a.v + (int64_t)kvh * a.head_bytes;
+    const int in_page = (1 << a.page_log2) - 1, range = Z::RB << a.page_log2;
+    auto stage_n = [&](auto count, const uint8_t * head, int id, int key, int place, uint8_t * dst, bool is_v) __attribute__((always_inline)) {
+        const auto from = buffer_of(head + (int64_t)max(id, 0) * a.page_bytes, range);
+        const int first = (key & in_page) * Z::RB;
+        constexpr int N = decltype(count)::value / RPI;
+        auto lane_off = [&](int i) __attribute__((always_inline)) {
+            const int kr = place + i * RPI + drow;
+            return drow * Z::RB + 16 * (dunit ^ (is_v ? swz_v(kr) : swz_k(kr)));
+        };
 #pragma unroll
-        for (int i = 0; i < decltype(count)::value / RPI; ++i) {
-            const int kr = i * RPI + drow, u = dunit ^ (is_v ? swz_v(place + kr) : swz_k(place + kr));
-            dma16(from, dst + i * 1024, drow * Z::RB + 16 * u, first + i * 1024);
+        for (int i = 0; i < N; i += 4) {
+            dma16_at<0>(from, dst + i * 1024, lane_off(i), first + i * 1024);
+            if constexpr (N > 1) dma16_at<1024>(from, dst + i * 1024, lane_off(i + 1), first + i * 1024);
+            if constexpr (N > 2) {
+                dma16_at<2048>(from, dst + i * 1024, lane_off(i + 2), first + i * 1024);
+                dma16_at<3072>(from, dst + i * 1024, lane_off(i + 3), first + i * 1024);
+            }
         }
     };
     // zero the rows [from, to) of V: p is 0 there, and 0 times what memory holds may be NaN
@@ -228,13 +238,17 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
     // in the sequence, holes: bit g: the 16 keys from 16 g on are absent
     // the swizzle leaves the address of step i, or of the 32 d of block i, at one address XOR a constant
     const int l16 = lane & 15, vkey = 4 * half + (l16 >> 2), vcol = 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1);
-    uint32_t kat = n * Z::RB + 16 * (half ^ swz_k(n)), vat = vkey * Z::RB + 16 * (vcol ^ swz_v(vkey)) + 8 * (l16 & 1);
+    const uint32_t kat = n * Z::RB + 16 * (half ^ swz_k(n));
+    // (V's place, VOFF behind K's, goes into its address: it is more than an instruction's offset holds)
+    constexpr int VOFF = KEYS ? Z::TILE : Z::R * Z::TILE;
+    uint32_t vat = VOFF + vkey * Z::RB + 16 * (vcol ^ swz_v(vkey)) + 8 * (l16 & 1);
+    asm("" : "+v"(vat));
     auto k_frag = [&](const uint8_t * kb, int i) __attribute__((always_inline)) {
         return *reinterpret_cast<const frag *>(kb + (kat ^ (32 * i)));
     };
-    // keys 16 g + 4 half + j % 4 + 8 (j / 4) of d = 32 d + lane % 32
-    auto v_frag = [&](const uint8_t * vb, int d, int g) __attribute__((always_inline)) {
-        const uint8_t * const at = vb + (vat ^ (64 * d)) + 16 * g * Z::RB;
+    // keys 16 g + 4 half + j % 4 + 8 (j / 4) of d = 32 d + lane % 32; kb: as for K
+    auto v_frag = [&](const uint8_t * kb, int d, int g) __attribute__((always_inline)) {
+        const uint8_t * const at = kb + (vat ^ (64 * d)) + 16 * g * Z::RB;
         const v2u x = read_tr(at), y = read_tr(at + 8 * Z::RB);
         return __builtin_bit_cast(frag, (v4u){x[0], x[1], y[0], y[1]});
     };
@@ -340,7 +354,7 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
             for (int i = lane; i < U; i += 64)
                 *reinterpret_cast<v4u *>(vb + __builtin_ctz(left) * Z::RB + 16 * i) = v4u{};
     };
-    auto values = [&](const v16f & p, const uint8_t * vb) __attribute__((always_inline)) {
+    auto values = [&](const v16f & p, const uint8_t * kb) __attribute__((always_inline)) {
         frag pf[NT][2];
 #pragma unroll
         for (int g = 0; g < 2; ++g)
@@ -358,7 +372,7 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
         for (int g = 0; g < 2; ++g)
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                const frag vf = v_frag(vb, d, g);
+                const frag vf = v_frag(kb, d, g);
 #pragma unroll
                 for (int k = NT - 1; k >= 0; --k) o[d] = mfma<T>(vf, pf[k][g], o[d]);
             }
@@ -370,21 +384,22 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
         constexpr int R = Z::R, OWN = 32 / Z::NW, PER = 2 * OWN / RPI;   // keys, and DMA instructions, of a wave a tile
         const int own = wave * OWN, nt = (k1 - k0 + 31) / 32;
         uint8_t * const kring = lds, * const vring = lds + R * Z::TILE;
-        uint32_t hq = 0;                                   // holes of the last 16 tiles, 2 bits each
+        uint32_t hq = 0;                                   // holes, 2 bits a tile, the latest taken lowest
         int idk = -1, idv = -1;                            // pages of this wave's keys of the next tiles of K and of V
         // the table's entries for tile t are asked for one tile before they are taken
         int raw0 = 0, raw1 = 0;
         const int top = max(nk - 1, 0) >> a.page_log2;
+        const int32_t * const row = a.table + trow;
         auto ask = [&](int t) __attribute__((always_inline)) {
             const int key = k0 + 32 * t;
-            raw0 = sload(a.table, trow + min(key >> a.page_log2, top));
-            raw1 = sload(a.table, trow + min((key + 16) >> a.page_log2, top));
+            raw0 = sload(row, min(key >> a.page_log2, top));
+            raw1 = sload(row, min((key + 16) >> a.page_log2, top));
         };
         auto take = [&](int t) __attribute__((always_inline)) {
-            const int key = k0 + 32 * t, at = 2 * (t & 15);
+            const int key = k0 + 32 * t;
             const bool ok0 = key < nk && (uint32_t)raw0 < (uint32_t)a.n_pages;
             const bool ok1 = key + 16 < nk && (uint32_t)raw1 < (uint32_t)a.n_pages;
-            hq = (hq & ~(3u << at)) | (uint32_t)((ok0 ? 0 : 1) | (ok1 ? 0 : 2)) << at;
+            hq = hq << 2 | (ok0 ? 0 : 1) | (ok1 ? 0 : 2);
             idv = idk;
             idk = own < 16 ? (ok0 ? raw0 : -1) : (ok1 ? raw1 : -1);
         };
@@ -392,12 +407,11 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
             stage_n(std::integral_constant<int, OWN>{}, base, id, k0 + 32 * t + own, own & 15, to + own * Z::RB, is_v);
         };
         // that the buffers differ has to be said, else every read of LDS waits for the DMA
-        auto step = [&](auto edge, uint8_t * __restrict__ kw, uint8_t * __restrict__ vw, const uint8_t * __restrict__ kr,
+        auto step = [&](auto edge, auto steady, uint8_t * __restrict__ kw, uint8_t * __restrict__ vw, const uint8_t * __restrict__ kr,
                         uint8_t * __restrict__ vr, const uint8_t * __restrict__ qlow, v16f & s, float & mx, int j) __attribute__((always_inline)) {
             constexpr bool EDGE = decltype(edge)::value;
             // fragments are read AHEAD steps before they are used
             constexpr int AHEAD = Z::QL ? 2 : 4;
-            asm volatile("" : "+v"(kat), "+v"(vat));       // addresses are made at each step: 24 registers are not there
             frag kf[AHEAD], lf[AHEAD][NT];
             auto k_read = [&](int i) __attribute__((always_inline)) {
                 kf[i % AHEAD] = k_frag(kr, i);
@@ -410,9 +424,9 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
             __builtin_amdgcn_sched_barrier(0);
             take(j + R);
             ask(j + R + 1);
-            if (j + R < nt) stage(a.k, idk, j + R, kw, false);
-            if (j + R - 1 < nt) stage(a.v, idv, j + R - 1, vw, true);
-            const int key = k0 + 32 * j, holes = hq >> (2 * (j & 15)) & 3;
+            if (steady || j + R < nt) stage(khead, idk, j + R, kw, false);
+            if (steady || j + R - 1 < nt) stage(vhead, idv, j + R - 1, vw, true);
+            const int key = k0 + 32 * j, holes = hq >> (2 * R) & 3;
             const bool mixed = EDGE && key + 32 > first_vis && nk > max(first_vis, key);
             if (!work && !mixed) return;
             if (EDGE || holes) {
@@ -452,7 +466,7 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
             }
             l += sum[0] + sum[1];
             if (EDGE) {
-                if (mixed) apart(s, vr, key);
+                if (mixed) apart(s, vr + VOFF, key);
 #pragma unroll
                 for (int i = 0; i < AHEAD; ++i) vf[i] = v_frag(vr, i % DT, i / DT);
             }
@@ -476,8 +490,8 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
             for (int t = 0; t < R; ++t) {
                 take(t);
                 ask(t + 1);
-                if (t < nt) stage(a.k, idk, t, kring + t * Z::TILE, false);
-                if (t > 0 && t - 1 < nt) stage(a.v, idv, t - 1, vring + (t - 1) * Z::TILE, true);
+                if (t < nt) stage(khead, idk, t, kring + t * Z::TILE, false);
+                if (t > 0 && t - 1 < nt) stage(vhead, idv, t - 1, vring + (t - 1) * Z::TILE, true);
             }
             if (nt >= R) pq2::wait_vmcnt<(R - 1) * PER>();
             else pq2::wait_vmcnt<0>();
@@ -487,26 +501,36 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
             float mx = largest(s);
             // tiles that every row sees whole, then those at the edge
             const int plain = max(min(nt, (first_vis - k0) / 32), 0);
-            int slot = 0;
-            auto pass = [&](auto edge, int j) __attribute__((always_inline)) {
+            // (steady: every load that a tile can start is there; R of them at a time, with the rings' places
+            // known to the compiler)
+            auto pass = [&](auto edge, auto steady, int slot, int j) __attribute__((always_inline)) {
                 const int after = slot + 1 == R ? 0 : slot + 1, before = slot == 0 ? R - 1 : slot - 1;
-                if (j - 1 + R < nt) pq2::wait_vmcnt<(R - 2) * PER>();
+                if (steady || j - 1 + R < nt) pq2::wait_vmcnt<(R - 2) * PER>();
                 else pq2::wait_vmcnt<0>();
-                const int holes = hq >> (2 * (j & 15)) & 3, key = k0 + 32 * j + own;
+                const int holes = hq >> (2 * R - 2) & 3, key = k0 + 32 * j + own;
                 const bool hole = holes >> (own >> 4) & 1;
-                uint8_t * const vr = vring + slot * Z::TILE;
-                if (hole || key + OWN > nk) zero_keys(vr + own * Z::RB, hole ? 0 : iclamp(nk - key, 0, OWN), OWN);
+                if (hole || (!steady && key + OWN > nk))
+                    zero_keys(vring + slot * Z::TILE + own * Z::RB, hole ? 0 : iclamp(nk - key, 0, OWN), OWN);
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 __builtin_amdgcn_s_barrier();              // the tiles are there, and all are done with the last ones
                 asm volatile("" ::: "memory");
-                step(edge, kring + slot * Z::TILE, vring + before * Z::TILE, kring + after * Z::TILE, vr, ql, s, mx, j);
-                slot = after;
+                step(edge, steady, kring + slot * Z::TILE, vring + before * Z::TILE, kring + after * Z::TILE, lds + slot * Z::TILE,
+                     ql, s, mx, j);
             };
             int j = 0;
+            const int whole = min(plain, nt - R);
 #pragma clang loop unroll(disable)
-            for (; j < plain; ++j) pass(std::false_type{}, j);
+            for (; j + R <= whole; j += R) {
+                pass(std::false_type{}, std::true_type{}, 0, j);
+                pass(std::false_type{}, std::true_type{}, 1, j + 1);
+                pass(std::false_type{}, std::true_type{}, 2, j + 2);
+                if constexpr (R == 4) pass(std::false_type{}, std::true_type{}, 3, j + 3);
+            }
+            int slot = 0;
 #pragma clang loop unroll(disable)
-            for (; j < nt; ++j) pass(std::true_type{}, j);
+            for (; j < plain; ++j, slot = slot + 1 == R ? 0 : slot + 1) pass(std::false_type{}, std::false_type{}, slot, j);
+#pragma clang loop unroll(disable)
+            for (; j < nt; ++j, slot = slot + 1 == R ? 0 : slot + 1) pass(std::true_type{}, std::false_type{}, slot, j);
         }
     } else {
         uint8_t * const mine = lds + wave * 4 * Z::TILE;
@@ -515,10 +539,10 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
             id0 = page_of(key);
             id1 = page_of(key + 16);
             const std::integral_constant<int, 16> half_tile;
-            stage_n(half_tile, a.k, id0, key, 0, to, false);
-            stage_n(half_tile, a.k, id1, key + 16, 0, to + 16 * Z::RB, false);
-            stage_n(half_tile, a.v, id0, key, 0, to + Z::TILE, true);
-            stage_n(half_tile, a.v, id1, key + 16, 0, to + Z::TILE + 16 * Z::RB, true);
+            stage_n(half_tile, khead, id0, key, 0, to, false);
+            stage_n(half_tile, khead, id1, key + 16, 0, to + 16 * Z::RB, false);
+            stage_n(half_tile, vhead, id0, key, 0, to + Z::TILE, true);
+            stage_n(half_tile, vhead, id1, key + 16, 0, to + Z::TILE + 16 * Z::RB, true);
         };
         auto step = [&](uint8_t * __restrict__ next, uint8_t * __restrict__ cur, const uint8_t * __restrict__ qlow,
                         int key, int holes) __attribute__((always_inline)) {
@@ -528,7 +552,7 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
             follow(largest(s));
             weights(s);
             if (key + 32 > first_vis && nk > max(first_vis, key)) apart(s, cur + Z::TILE, key);
-            values(s, cur + Z::TILE);
+            values(s, cur);
         };
         int key = k0 + 32 * wave, b = 0;
         if (key < k1) stage(key, mine);

@@ -72,6 +72,11 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const uint8_t * base
 __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t from, uint8_t * dst, int off, int soff) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_void *)dst, 16, off, soff, 0, 0);
 }
+// BOTH bytes further on either side (the instruction's own offset counts for both)
+template <int BOTH>
+__device__ __forceinline__ void dma16_at(__amdgpu_buffer_rsrc_t from, uint8_t * dst, int off, int soff) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_void *)dst, 16, off, soff, BOTH, 0);
+}
 
 // Which sequence a tile of up to BM rows (per_tok of them a token) belongs to;
 // the tiles of sequence s follow those of s - 1.  starts: n_seq + 1 entries, cut
