@@ -508,8 +508,8 @@ int64_t bonsai_p40_attn_paged_workspace_bytes(const bonsai_p40_attn_paged_args *
 // same time, and graphs that may, need their own); NULL: token by token.
 // Errors: 1 if k_dim is not 64 or 128, v_dim is not a multiple of 16 up to 256,
 // n_v_head (up to 65536) is no multiple of n_k_head, the type or a stride is not as
-// stated (q_tok, k_tok, v_tok, out_tok and gate_tok at least a row; q and k rows
-// 16-byte aligned), scale or l2_eps is not finite or l2_eps is negative, a
+// stated (q_tok, k_tok, v_tok, out_tok and gate_tok at least a row; q, k and v rows
+// 16-byte aligned, v_tok up to 2^22), scale or l2_eps is not finite or l2_eps is negative, a
 // pointer is NULL or misaligned, the workspace is too small, or there are more
 // than 2^27 / n_v_head tokens and sequences; 0 (no-op) if n_seq <= 0.
 typedef struct bonsai_p40_gdn_args {

@@ -30,6 +30,8 @@
 #include "launch_rules.h"
 #include "mixer_device.h"
 
+#include <type_traits>
+
 using namespace mixer;
 
 namespace {
@@ -44,7 +46,7 @@ struct GdnArgs {
     const int32_t * slots, * starts;
     uint8_t * ws;
     int64_t q_tok, k_tok, v_tok, out_tok, gate_tok, n_states;
-    int n_tok, n_seq, n_kh, n_vh, vd, tiled, chunks;
+    int n_tok, n_seq, n_kh, n_vh, vd, tiled, chunks, out16;
     float scale, eps;
 };
 
@@ -159,6 +161,10 @@ __device__ __forceinline__ void split(float x, _Float16 & hi, _Float16 & lo) {
     lo = (_Float16)(x - (float)hi);
 }
 
+// A workgroup per chunk and key head: K K^T and Q K^T once, then T and the masked
+// Q K^T of each of its value heads.  Bound by latencies (9 barriers a value head,
+// a triangular solve in four 16 x 16 blocks), so what counts is that two
+// workgroups share a CU: the C x C matrices take the place of K and Q in LDS.
 template <class T, int K>
 __global__ void __launch_bounds__(256) gdn_prep_kernel(GdnArgs a) {
     typedef typename T::elem elem;
@@ -166,20 +172,20 @@ __global__ void __launch_bounds__(256) gdn_prep_kernel(GdnArgs a) {
     constexpr int P = K + 8;                              // halves of a row: 16 rows of 16 bytes meet all banks
     constexpr int M = 68;                                 // floats of a row of the C x C matrices
     constexpr int SM = K / 32;
-    __shared__ __attribute__((aligned(16))) _Float16 pl[4][C][P];     // K hi, lo, Q hi, lo
-    __shared__ float L[C][M], X[C][M];
+    constexpr int PL = 4 * C * P * 2, LX = 2 * C * M * 4;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[PL > LX ? PL : LX];
+    _Float16 (* const pl)[C][P] = reinterpret_cast<_Float16 (*)[C][P]>(lds);      // K hi, lo, Q hi, lo
+    float (* const L)[M] = reinterpret_cast<float (*)[M]>(lds), (* const X)[M] = L + C;
     __shared__ float tmp[4][16][17];
-    __shared__ double G[C];
-    __shared__ float fk[C], fq[C], bt[C], rt[C], ra[C];
+    __shared__ double G[4][C];
+    __shared__ float fk[C], fq[C], bt[4][C], rt[C], ra[C];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, g = lane >> 4;
-    const int hv = blockIdx.x % a.n_vh, chunk = blockIdx.x / a.n_vh;
+    const int hk = blockIdx.x % a.n_kh, chunk = blockIdx.x / a.n_kh, per = a.n_vh / a.n_kh;
     const Tile tl = find_tile<C>(a.starts, a.n_seq, a.n_tok, 1, chunk);
     if (tl.seq < 0) return;
-    const int hk = key_head(a, hv), t0 = tl.first + tl.index * C, nt = min(C, tl.count - tl.index * C);
-    const bool lead = a.tiled ? hv < a.n_kh : hv % (a.n_vh / a.n_kh) == 0;   // writes the key head's fragments
+    const int t0 = tl.first + tl.index * C, nt = min(C, tl.count - tl.index * C);
     uint8_t * const wk = a.ws + ((int64_t)chunk * a.n_kh + hk) * W::HEAD;
-    uint8_t * const wv = a.ws + (int64_t)a.chunks * a.n_kh * W::HEAD + ((int64_t)chunk * a.n_vh + hv) * W::VHEAD;
 
     // rows of K and Q: 4 threads each
     {
@@ -209,20 +215,10 @@ __global__ void __launch_bounds__(256) gdn_prep_kernel(GdnArgs a) {
             for (int j = 0; j < N; ++j) split(x[j] * down, pl[2 * m][row][part * N + j], pl[2 * m + 1][row][part * N + j]);
         }
     }
-    if (wave == 0) {
-        const float gt = lane < nt ? gate(a.g[(int64_t)(t0 + lane) * a.gate_tok + hv]) : 0.0f;
-        double s = (double)gt;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const double o = __shfl_up(s, d);
-            if (lane >= d) s += o;
-        }
-        G[lane] = s;
-        bt[lane] = lane < nt ? a.beta[(int64_t)(t0 + lane) * a.gate_tok + hv] : 0.0f;
-    }
     __syncthreads();
 
-    // rows 16 wave .. of K K^T and Q K^T, in fp32; then L, and Q K^T with its decay in X
+    // rows 16 wave .. of K K^T and Q K^T (element: column 16 n + l16, row 16 wave + 4 g + r), without the rows' factors
+    v4f kk[4], qk[4];
     {
         v8h ka[SM][2], qa[SM][2];
 #pragma unroll
@@ -232,46 +228,47 @@ __global__ void __launch_bounds__(256) gdn_prep_kernel(GdnArgs a) {
                 ka[s][k] = *reinterpret_cast<const v8h *>(&pl[k][16 * wave + l16][32 * s + 8 * g]);
                 qa[s][k] = *reinterpret_cast<const v8h *>(&pl[2 + k][16 * wave + l16][32 * s + 8 * g]);
             }
-        float top[4] = {};
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-            v4f kk = {}, qk = {};
+            kk[n] = qk[n] = v4f{};
             if (n <= wave) {
 #pragma unroll
                 for (int s = 0; s < SM; ++s) {
                     const v8h bh = *reinterpret_cast<const v8h *>(&pl[0][16 * n + l16][32 * s + 8 * g]);
                     const v8h bl = *reinterpret_cast<const v8h *>(&pl[1][16 * n + l16][32 * s + 8 * g]);
-                    kk = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[s][1], bh, kk, 0, 0, 0);
-                    kk = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[s][0], bl, kk, 0, 0, 0);
-                    kk = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[s][0], bh, kk, 0, 0, 0);
-                    qk = __builtin_amdgcn_mfma_f32_16x16x32_f16(qa[s][1], bh, qk, 0, 0, 0);
-                    qk = __builtin_amdgcn_mfma_f32_16x16x32_f16(qa[s][0], bl, qk, 0, 0, 0);
-                    qk = __builtin_amdgcn_mfma_f32_16x16x32_f16(qa[s][0], bh, qk, 0, 0, 0);
+                    kk[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[s][1], bh, kk[n], 0, 0, 0);
+                    qk[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qa[s][1], bh, qk[n], 0, 0, 0);
+                    kk[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[s][0], bl, kk[n], 0, 0, 0);
+                    qk[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qa[s][0], bl, qk[n], 0, 0, 0);
+                    kk[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[s][0], bh, kk[n], 0, 0, 0);
+                    qk[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qa[s][0], bh, qk[n], 0, 0, 0);
                 }
             }
-            const int j = 16 * n + l16;
-            const double Gj = G[j];
-            const float fj = fk[j];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = 16 * wave + 4 * g + r;
-                const float d = j <= i ? expf((float)(G[i] - Gj)) : 0.0f;
-                L[i][j] = j < i ? bt[i] * (kk[r] * fk[i] * fj) * d : 0.0f;
-                const float x = j <= i ? a.scale * (qk[r] * fq[i] * fj) * d : 0.0f;
-                X[i][j] = x;
-                top[r] = fmaxf(top[r], fabsf(x));
-            }
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-#pragma unroll
-            for (int d = 1; d < 16; d <<= 1) top[r] = fmaxf(top[r], __shfl_xor(top[r], d));
-            if (l16 == 0) ra[16 * wave + 4 * g + r] = pow2(exponent(top[r]));
         }
     }
-    __syncthreads();
+    // the fragments of K, Q (m-tile of 16 tokens, steps of 32 dims) and K^T (m-tile of 16 dims, steps of 32 tokens)
+    for (int f = wave; f < 4 * SM; f += 4) {
+        const int mt = f / SM, ks = f % SM, row = 16 * mt + l16;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            v8h x;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = pl[k][row][32 * ks + (j < 4 ? 4 * g + j : 12 + 4 * g + j)];
+            *reinterpret_cast<v8h *>(wk + (k >> 1) * W::KF + (2 * f + (k & 1)) * 1024 + 16 * lane) = x;
+        }
+    }
+    for (int f = wave; f < K / 8; f += 4) {
+        const int mt = f >> 1, ks = f & 1, dim = 16 * mt + l16;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            v8h x;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = pl[k][32 * ks + (j < 4 ? 4 * g + j : 12 + 4 * g + j)][dim];
+            *reinterpret_cast<v8h *>(wk + 2 * W::KF + (2 * f + k) * 1024 + 16 * lane) = x;
+        }
+    }
 
-    // a fragment of a C x C matrix in LDS: m-tile mt, step ks, as two terms
+    // a C x C matrix in LDS as fragments (m-tile mt, step ks)
     auto put_square = [&](const float (*m)[M], const float * scale, uint8_t * to) {
         for (int f = wave; f < 8; f += 4) {
             const int mt = f >> 1, ks = f & 1, row = 16 * mt + l16;
@@ -288,141 +285,173 @@ __global__ void __launch_bounds__(256) gdn_prep_kernel(GdnArgs a) {
             *reinterpret_cast<v8h *>(to + (2 * f + 1) * 1024 + 16 * lane) = lo;
         }
     };
-    put_square(X, ra, wv + W::TF);
-    if (lead) {
-        // K, Q: m-tile of 16 tokens, steps of 32 dims; K^T: m-tile of 16 dims, steps of 32 tokens
-        for (int f = wave; f < 4 * SM; f += 4) {
-            const int mt = f / SM, ks = f % SM, row = 16 * mt + l16;
+#pragma unroll 1
+    for (int r = 0; r < per; ++r) {
+        auto head = [&](int r) { return a.tiled ? hk + r * a.n_kh : hk * per + r; };
+        const int hv = head(r), q4 = r & 3;
+        uint8_t * const wv = a.ws + (int64_t)a.chunks * a.n_kh * W::HEAD + ((int64_t)chunk * a.n_vh + hv) * W::VHEAD;
+        if (q4 == 0) {
+            // the sums of g of up to 4 heads, a wave each, in fp64
+            if (r + wave < per) {
+                const int h = head(r + wave);
+                double s = lane < nt ? (double)gate(a.g[(int64_t)(t0 + lane) * a.gate_tok + h]) : 0.0;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                v8h x;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = pl[k][row][32 * ks + (j < 4 ? 4 * g + j : 12 + 4 * g + j)];
-                *reinterpret_cast<v8h *>(wk + (k >> 1) * W::KF + (2 * f + (k & 1)) * 1024 + 16 * lane) = x;
+                for (int d = 1; d < 64; d <<= 1) {
+                    const double o = __shfl_up(s, d);
+                    if (lane >= d) s += o;
+                }
+                G[wave][lane] = s;
+                bt[wave][lane] = lane < nt ? a.beta[(int64_t)(t0 + lane) * a.gate_tok + h] : 0.0f;
             }
         }
-        for (int f = wave; f < K / 8; f += 4) {
-            const int mt = f >> 1, ks = f & 1, dim = 16 * mt + l16;
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                v8h x;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = pl[k][32 * ks + (j < 4 ? 4 * g + j : 12 + 4 * g + j)][dim];
-                *reinterpret_cast<v8h *>(wk + 2 * W::KF + (2 * f + k) * 1024 + 16 * lane) = x;
-            }
-        }
-    }
-    __syncthreads();                                      // X is free
+        __syncthreads();                                  // (and: K and Q have been read, or the last head's X)
 
-    // X = (I + L)^-1.  Diagonal blocks of 16: a lane per column, forward substitution
-    {
-        float x[16];
+        // L, and Q K^T with its decay in X
+        float top[4] = {};
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            float s = l16 == i ? 1.0f : 0.0f;
+        for (int n = 0; n < 4; ++n) {
+            const int j = 16 * n + l16;
+            const double Gj = G[q4][j];
+            const float fj = fk[j];
 #pragma unroll
-            for (int l = 0; l < i; ++l) s = fmaf(-L[16 * wave + i][16 * wave + l], x[l], s);
-            x[i] = s;
+            for (int i4 = 0; i4 < 4; ++i4) {
+                const int i = 16 * wave + 4 * g + i4;
+                const float d = j <= i ? expf((float)(G[q4][i] - Gj)) : 0.0f;
+                L[i][j] = j < i ? bt[q4][i] * (kk[n][i4] * fk[i] * fj) * d : 0.0f;
+                const float x = j <= i ? a.scale * (qk[n][i4] * fq[i] * fj) * d : 0.0f;
+                X[i][j] = x;
+                top[i4] = fmaxf(top[i4], fabsf(x));
+            }
         }
-        if (g == 0)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) X[16 * wave + i][16 * wave + l16] = x[i];
-        // what is above the diagonal
-        for (int n = wave + 1; n < 4; ++n)
+        for (int i4 = 0; i4 < 4; ++i4) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) X[16 * wave + 4 * g + r][16 * n + l16] = 0.0f;
-    }
-    __syncthreads();
-    // below it, wave j has block column j: X_ij = -X_ii sum_l L_il X_lj
-    for (int i = wave + 1; i < 4; ++i) {
-        v4f s = {};
-        for (int l = wave; l < i; ++l)
+            for (int d = 1; d < 16; d <<= 1) top[i4] = fmaxf(top[i4], __shfl_xor(top[i4], d));
+            if (l16 == 0) ra[16 * wave + 4 * g + i4] = pow2(exponent(top[i4]));
+        }
+        __syncthreads();
+        put_square(X, ra, wv + W::TF);
+        __syncthreads();                                  // X is free
+
+        // X = (I + L)^-1.  Diagonal blocks of 16: a lane per column, forward substitution
+        {
+            float x[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float s = l16 == i ? 1.0f : 0.0f;
+#pragma unroll
+                for (int l = 0; l < i; ++l) s = fmaf(-L[16 * wave + i][16 * wave + l], x[l], s);
+                x[i] = s;
+            }
+            if (g == 0)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) X[16 * wave + i][16 * wave + l16] = x[i];
+            // what is above the diagonal
+            for (int n = wave + 1; n < 4; ++n)
+#pragma unroll
+                for (int i4 = 0; i4 < 4; ++i4) X[16 * wave + 4 * g + i4][16 * n + l16] = 0.0f;
+        }
+        __syncthreads();
+        // below it, wave j has block column j: X_ij = -X_ii sum_l L_il X_lj
+        for (int i = wave + 1; i < 4; ++i) {
+            v4f s = {};
+            for (int l = wave; l < i; ++l)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    s = __builtin_amdgcn_mfma_f32_16x16x4f32(L[16 * i + l16][16 * l + 4 * k + g],
+                                                             X[16 * l + 4 * k + g][16 * wave + l16], s, 0, 0, 0);
+#pragma unroll
+            for (int i4 = 0; i4 < 4; ++i4) tmp[wave][4 * g + i4][l16] = s[i4];
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // other lanes read it
+            v4f x = {};
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                s = __builtin_amdgcn_mfma_f32_16x16x4f32(L[16 * i + l16][16 * l + 4 * k + g],
-                                                         X[16 * l + 4 * k + g][16 * wave + l16], s, 0, 0, 0);
+                x = __builtin_amdgcn_mfma_f32_16x16x4f32(X[16 * i + l16][16 * i + 4 * k + g], tmp[wave][4 * k + g][l16], x, 0, 0, 0);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) tmp[wave][4 * g + r][l16] = s[r];
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // other lanes read it
-        v4f x = {};
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            x = __builtin_amdgcn_mfma_f32_16x16x4f32(X[16 * i + l16][16 * i + 4 * k + g], tmp[wave][4 * k + g][l16], x, 0, 0, 0);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) X[16 * i + 4 * g + r][16 * wave + l16] = -x[r];
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // other lanes read it
-    }
-    __syncthreads();
-    // T = X diag(beta), and the largest element of its rows
-    {
-        const int row = tid >> 2, part = tid & 3;
-        float big = 0.0f;
-        for (int j = part; j < C; j += 4) {
-            const float x = X[row][j] * bt[j];
-            X[row][j] = x;
-            big = fmaxf(big, fabsf(x));
+            for (int i4 = 0; i4 < 4; ++i4) X[16 * i + 4 * g + i4][16 * wave + l16] = -x[i4];
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
-        big = fmaxf(big, __shfl_xor(big, 1));
-        big = fmaxf(big, __shfl_xor(big, 2));
-        if (part == 0) rt[row] = pow2(exponent(big));
-    }
-    __syncthreads();
-    put_square(X, rt, wv);
-    // factors of the rows
-    if (tid < C) {
-        float * const vec = reinterpret_cast<float *>(wv + 2 * W::TF);
-        const float e = expf((float)G[tid]);
-        vec[tid] = e * fk[tid];
-        vec[C + tid] = e * fq[tid] * a.scale;
-        vec[2 * C + tid] = rt[tid];
-        vec[3 * C + tid] = ra[tid];
-        vec[4 * C + tid] = expf((float)(G[C - 1] - G[tid])) * fk[tid];
-        vec[5 * C + tid] = expf((float)G[C - 1]);
+        __syncthreads();
+        // T = X diag(beta), and the largest element of its rows
+        {
+            const int row = tid >> 2, part = tid & 3;
+            float big = 0.0f;
+            for (int j = part; j < C; j += 4) {
+                const float x = X[row][j] * bt[q4][j];
+                X[row][j] = x;
+                big = fmaxf(big, fabsf(x));
+            }
+            big = fmaxf(big, __shfl_xor(big, 1));
+            big = fmaxf(big, __shfl_xor(big, 2));
+            if (part == 0) rt[row] = pow2(exponent(big));
+        }
+        __syncthreads();
+        put_square(X, rt, wv);
+        // factors of the rows
+        if (tid < C) {
+            float * const vec = reinterpret_cast<float *>(wv + 2 * W::TF);
+            const double Gi = G[q4][tid], Ge = G[q4][C - 1];
+            const float e = expf((float)Gi);
+            vec[tid] = e * fk[tid];
+            vec[C + tid] = e * fq[tid] * a.scale;
+            vec[2 * C + tid] = rt[tid];
+            vec[3 * C + tid] = ra[tid];
+            vec[4 * C + tid] = expf((float)(Ge - Gi)) * fk[tid];
+            vec[5 * C + tid] = expf((float)Ge);
+        }
+        if (q4 == 3) __syncthreads();                     // G and bt are written anew
     }
 }
 
-// right operand from result tiles: columns scaled to about 1; the factor that
-// takes a product back
+// the largest of the 4 lanes that hold a column
+__device__ __forceinline__ float over_column(float x) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    uint32_t a = p[0], b = p[1];
+    asm("" : "+v"(a), "+v"(b));                           // they differ, though the operands do not
+    const uint32_t m = __builtin_bit_cast(uint32_t, fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)));
+    const auto q = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+    uint32_t c = q[0], d = q[1];
+    asm("" : "+v"(c), "+v"(d));
+    return fmaxf(__builtin_bit_cast(float, c), __builtin_bit_cast(float, d));
+}
 template <int N>
-__device__ __forceinline__ float to_right(const v4f (&x)[N], v8h (&hi)[N / 2], v8h (&lo)[N / 2]) {
-    float big = 0.0f;
+__device__ __forceinline__ float largest(const v4f (&x)[N]) {
+    float big[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) big = fmaxf(big, fabsf(x[i][j]));
-    big = fmaxf(big, __shfl_xor(big, 16));
-    big = fmaxf(big, __shfl_xor(big, 32));
-    const int e = exponent(big);
-    const float down = pow2(-e);
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            _Float16 h, l;
-            split(x[i][j] * down, h, l);
-            hi[i / 2][4 * (i & 1) + j] = h;
-            lo[i / 2][4 * (i & 1) + j] = l;
-        }
-    return pow2(e);
+        for (int j = 0; j < 4; ++j) big[j & 1] = fmaxf(big[j & 1], fabsf(x[i][j]));
+    return over_column(fmaxf(big[0], big[1]));
 }
 
-template <class T, int K>
-__global__ void __launch_bounds__(256) gdn_scan_kernel(GdnArgs a) {
+// NW waves of 16 columns each
+template <class T, int K, int NW>
+__global__ void __launch_bounds__(64 * NW) gdn_scan_kernel(GdnArgs a) {
     typedef typename T::elem elem;
     typedef Work<K> W;
     constexpr int KS = K / 32, KT = K / 16;
-    constexpr int REG1 = 2 * W::KF, REG2 = W::KF + W::VHEAD;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[REG1 + REG2];
-    uint8_t * const r1 = lds, * const r2 = lds + REG1;    // K, Q | K^T, T, QK^T, factors
+    typedef elem Unit __attribute__((ext_vector_type(16 / sizeof(elem))));
+    constexpr int REG1 = 2 * W::KF, REG2 = W::KF + W::VHEAD, OWN = C * 16 * sizeof(elem);
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[REG1 + REG2 + NW * OWN];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l16 = lane & 15, g = lane >> 4;
-    const int quads = (a.vd + 63) / 64;
-    const int hv = blockIdx.x / quads % a.n_vh, seq = blockIdx.x / quads / a.n_vh;
-    const int col0 = 64 * (blockIdx.x % quads) + 16 * wave;
+    // a key head's workgroups, which share fragments, on one XCD (workgroups go to the 8 in turn)
+    const int groups = (a.vd + 16 * NW - 1) / (16 * NW), per = a.n_vh / a.n_kh;
+    int hk = blockIdx.x & 7, rest = blockIdx.x >> 3;
+    const int group = rest % groups;
+    rest /= groups;
+    const int head = rest % per;
+    rest /= per;
+    const int eighth = (a.n_kh + 7) / 8, seq = rest / eighth;
+    hk += 8 * (rest % eighth);
+    if (hk >= a.n_kh) return;
+    const int hv = a.tiled ? hk + head * a.n_kh : hk * per + head;
+    const int col0 = 16 * (NW * group + wave);
     const int64_t slot = slot_of(a, seq);
     if (slot < 0) return;
     const bool work = col0 < a.vd;                        // the others stage
-    const int col = work ? col0 + l16 : 0, hk = key_head(a, hv);
+    const int col = work ? col0 + l16 : 0;
     const int first = iclamp(sload(a.starts, seq), 0, a.n_tok);
     const int count = max(iclamp(sload(a.starts, seq + 1), 0, a.n_tok) - first, 0);
     int chunks = (count + C - 1) / C;
@@ -435,17 +464,21 @@ __global__ void __launch_bounds__(256) gdn_scan_kernel(GdnArgs a) {
     chunk0 = __builtin_amdgcn_readfirstlane(chunk0);
     chunks = iclamp(chunks, 0, max(a.chunks - chunk0, 0));   // starts that overlap: what prep made, no more
 
-    auto copy = [&](const uint8_t * src, uint8_t * dst, int bytes) __attribute__((always_inline)) {
-        const auto from = buffer_of(src, bytes);
-        for (int i = wave * 1024; i < bytes; i += 4096) dma16(from, dst + i, 16 * lane, i);
+    // 1 KB an instruction, the waves in turn
+    auto copy = [&](const uint8_t * src, uint8_t * dst, auto bytes) __attribute__((always_inline)) {
+        constexpr int N = decltype(bytes)::value / 1024;
+        const auto from = buffer_of(src, N * 1024);
+#pragma unroll
+        for (int i = 0; i < N; i += NW)
+            if (N % NW == 0 || i + wave < N) dma16(from, dst + (i + wave) * 1024, 16 * lane, (i + wave) * 1024);
     };
-    auto stage1 = [&](int c) __attribute__((always_inline)) {
-        copy(a.ws + ((int64_t)(chunk0 + c) * a.n_kh + hk) * W::HEAD, r1, REG1);
+    auto stage1 = [&](int c, uint8_t * to) __attribute__((always_inline)) {
+        copy(a.ws + ((int64_t)(chunk0 + c) * a.n_kh + hk) * W::HEAD, to, std::integral_constant<int, REG1>{});
     };
-    auto stage2 = [&](int c) __attribute__((always_inline)) {
-        copy(a.ws + ((int64_t)(chunk0 + c) * a.n_kh + hk) * W::HEAD + REG1, r2, W::KF);
+    auto stage2 = [&](int c, uint8_t * to) __attribute__((always_inline)) {
+        copy(a.ws + ((int64_t)(chunk0 + c) * a.n_kh + hk) * W::HEAD + REG1, to, std::integral_constant<int, W::KF>{});
         copy(a.ws + (int64_t)a.chunks * a.n_kh * W::HEAD + ((int64_t)(chunk0 + c) * a.n_vh + hv) * W::VHEAD,
-             r2 + W::KF, W::VHEAD);
+             to + W::KF, std::integral_constant<int, W::VHEAD>{});
     };
     auto sync = [&]() __attribute__((always_inline)) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -458,100 +491,206 @@ __global__ void __launch_bounds__(256) gdn_scan_kernel(GdnArgs a) {
     for (int i = 0; i < KT; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) S[i][j] = work ? a.state[at + (int64_t)(16 * i + j) * a.vd] : 0.0f;
-    const elem * const v = reinterpret_cast<const elem *>(a.v) + (int64_t)hv * a.vd + col;
-    elem * const out = reinterpret_cast<elem *>(a.out) + (int64_t)hv * a.vd + col;
+    uint8_t * const own_lds = lds + REG1 + REG2 + wave * OWN;
 
-    // acc[m] += left fragments (two terms, 1 KB each, [m][s]) . right
-    auto product = [&](const uint8_t * left, int m, int s, int steps, const v8h & hi, const v8h & lo, v4f c) __attribute__((always_inline)) {
-        const v8h ah = *reinterpret_cast<const v8h *>(left + (2 * (m * steps + s)) * 1024 + 16 * lane);
-        const v8h al = *reinterpret_cast<const v8h *>(left + (2 * (m * steps + s) + 1) * 1024 + 16 * lane);
-        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(al, hi, c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, lo, c, 0, 0, 0);
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, hi, c, 0, 0, 0);
+    // Pairs of products (an MFMA waits for the one before it in its own sum): left fragments, two terms of 1 KB
+    // each, read AHEAD pairs before they are used
+    constexpr int AHEAD = 2;
+    struct Left {
+        v8h h[2], l[2];
+    };
+    auto products = [&](auto count, auto place, auto use) __attribute__((always_inline)) {
+        constexpr int N = decltype(count)::value;
+        Left f[AHEAD];
+        auto read = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const uint8_t * const p = place(i, k) + 16 * lane;
+                f[i % AHEAD].h[k] = *reinterpret_cast<const v8h *>(p);
+                f[i % AHEAD].l[k] = *reinterpret_cast<const v8h *>(p + 1024);
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < AHEAD && i < N; ++i) read(i);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            use(i, f[i % AHEAD]);
+            if (i + AHEAD < N) read(i + AHEAD);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    auto mul = [](const Left & f, const v8h & hi, const v8h & lo, v4f & a, v4f & b) __attribute__((always_inline)) {
+        a = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.l[0], hi, a, 0, 0, 0);
+        b = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.l[1], hi, b, 0, 0, 0);
+        a = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h[0], lo, a, 0, 0, 0);
+        b = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h[1], lo, b, 0, 0, 0);
+        a = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h[0], hi, a, 0, 0, 0);
+        b = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h[1], hi, b, 0, 0, 0);
+    };
+    // half of a right fragment (elements 4 k ..) from a result tile, its columns scaled
+    auto to_right = [](const v4f & x, float down, v8h & hi, v8h & lo, int k) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            _Float16 h, l;
+            split(x[j] * down, h, l);
+            hi[4 * k + j] = h;
+            lo[4 * k + j] = l;
+        }
     };
 
-    if (chunks > 0) stage1(0);
-#pragma clang loop unroll(disable)
-    for (int c = 0; c < chunks; ++c) {
-        const int t0 = first + c * C, nt = min(C, count - c * C);
-        sync();                                           // K, Q are there; r2 is free
-        stage2(c);
-        float vt[4][4];
+    // V comes, and the outputs leave, through a place of the wave's own: [row][16 columns], row 4 j + g of 16 being
+    // token 4 g + j, so that the 4 tokens a lane's column is read at with the others' lie in different banks
+    constexpr int EB = sizeof(elem), UNITS = EB, RPI = 64 / UNITS;    // 16-byte units of a row; rows of an instruction
+    auto token = [](int row) { return (row & ~15) + 4 * (row & 3) + (row >> 2 & 3); };
+    const int row0 = lane / UNITS, unit0 = lane % UNITS;
+    auto stage_v = [&](int c, uint8_t * to) __attribute__((always_inline)) {
+        const int nt = min(C, count - c * C);
+        const auto from = buffer_of(reinterpret_cast<const uint8_t *>(a.v) +
+                                    ((int64_t)(first + c * C) * a.v_tok + (int64_t)hv * a.vd + col0) * EB,
+                                    (int)((nt - 1) * a.v_tok + 16) * EB);    // past the last token: zeros
 #pragma unroll
-        for (int m = 0; m < 4; ++m)
+        for (int i = 0; i < C / RPI; ++i)
+            dma16(from, to + 1024 * i, token(RPI * i + row0) * (int)a.v_tok * EB + 16 * unit0, 0);
+    };
+    auto put = [&](const uint8_t * from, int c) __attribute__((always_inline)) {
+        const int nt = min(C, count - c * C);
+        uint8_t * const to = reinterpret_cast<uint8_t *>(a.out) +
+                             ((int64_t)(first + c * C) * a.out_tok + (int64_t)hv * a.vd + col0) * EB;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int t = 16 * m + 4 * g + j;
-                vt[m][j] = work && t < nt ? T::to(v[(int64_t)(t0 + t) * a.v_tok]) : 0.0f;
-            }
-        v8h sh[KS], sl[KS];
-        const float fs = to_right(S, sh, sl);
-        v4f ks[4], qs[4];
+        for (int i = 0; i < C / RPI; ++i) {
+            const int t = token(RPI * i + row0);
+            const v4u x = *reinterpret_cast<const v4u *>(from + 1024 * i + 16 * lane);
+            if (t < nt) {
+                if (a.out16) *reinterpret_cast<v4u *>(to + (int64_t)t * a.out_tok * EB + 16 * unit0) = x;
+                else
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            ks[m] = v4f{};
-            qs[m] = v4f{};
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                ks[m] = product(r1, m, s, KS, sh[s], sl[s], ks[m]);
-                qs[m] = product(r1 + W::KF, m, s, KS, sh[s], sl[s], qs[m]);
+                    for (int j = 0; j < 16 / EB; ++j)
+                        reinterpret_cast<elem *>(to + (int64_t)t * a.out_tok * EB + 16 * unit0)[j] =
+                            __builtin_bit_cast(Unit, x)[j];
             }
         }
-        sync();                                           // the rest is there; r1 is free
-        if (c + 1 < chunks) stage1(c + 1);
+    };
+
+    float big = largest(S), fs = 1.0f;
+    v4f ks[4], qs[4];
+    // K S and Q S, while K^T, T, QK^T, the factors and V arrive
+    auto first_half = [&](const uint8_t * __restrict__ r1, uint8_t * __restrict__ r2, uint8_t * __restrict__ rv, int c) __attribute__((always_inline)) {
+        stage2(c, r2);
+        if (work) {
+            if (c > 0) put(rv, c - 1);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            stage_v(c, rv);
+        }
+        const int e = exponent(big);
+        const float down = pow2(-e);
+        fs = pow2(e);
+        v8h sh[2], sl[2];
+        to_right(S[0], down, sh[0], sl[0], 0);
+        to_right(S[1], down, sh[0], sl[0], 1);
+#pragma unroll
+        for (int m = 0; m < 4; ++m) ks[m] = qs[m] = v4f{};
+        products(std::integral_constant<int, 4 * KS>{},
+                 [&](int i, int k) __attribute__((always_inline)) { return r1 + k * W::KF + 2 * (i % 4 * KS + i / 4) * 1024; },
+                 [&](int i, const Left & f) __attribute__((always_inline)) {
+                     const int s = i / 4, m = i % 4;
+                     mul(f, sh[s & 1], sl[s & 1], ks[m], qs[m]);
+                     // the next step's right operand, between the products
+                     if (m < 2 && s + 1 < KS) to_right(S[2 * s + 2 + m], down, sh[(s + 1) & 1], sl[(s + 1) & 1], m);
+                 });
+    };
+    // U, the outputs and the next S, while the next K and Q arrive
+    auto second_half = [&](const uint8_t * __restrict__ r2, uint8_t * __restrict__ r1, uint8_t * __restrict__ rv, int c) __attribute__((always_inline)) {
+        if (c + 1 < chunks) stage1(c + 1, r1);
         const uint8_t * const tf = r2 + W::KF, * const af = tf + W::TF;
         const float * const vec = reinterpret_cast<const float *>(af + W::TF);
         auto factor = [&](int which, int m) { return *reinterpret_cast<const v4f *>(vec + which * C + 16 * m + 4 * g); };
-        v4f R[4];
+        elem * const own = reinterpret_cast<elem *>(rv) + 16 * g + l16;      // token 16 m + 4 g + j: row 16 m + 4 j + g
+        // products with T and QK^T, two m-tiles at a time; their blocks above the diagonal are 0
+        auto place = [&](const uint8_t * base, int i, int k) __attribute__((always_inline)) {
+            const int m = (i == 0 ? 0 : 2) + k, s = i / 2;
+            return base + 2 * (2 * m + s) * 1024;
+        };
+        v8h rh[2], rl[2];
+        v4f R[4], Um[4], x[4];
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
             const v4f f = factor(0, m);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) R[m][j] = fmaf(-f[j] * fs, ks[m][j], vt[m][j]);
+            for (int j = 0; j < 4; ++j) R[m][j] = fmaf(-f[j] * fs, ks[m][j], T::to(own[(16 * m + 4 * j) * 16]));
+            x[m] = v4f{};
         }
-        v8h rh[2], rl[2];
-        const float fr = to_right(R, rh, rl);
-        v4f Um[4];
+        int e = exponent(largest(R));
+        float down = pow2(-e);
+        const float fr = pow2(e);
+        to_right(R[0], down, rh[0], rl[0], 0);
+        to_right(R[1], down, rh[0], rl[0], 1);
+        auto square = [&](const uint8_t * base, const v4f (&right)[4], float down) __attribute__((always_inline)) {
+            products(std::integral_constant<int, 3>{}, [&](int i, int k) __attribute__((always_inline)) { return place(base, i, k); },
+                     [&](int i, const Left & f) __attribute__((always_inline)) {
+                         const int m = i == 0 ? 0 : 2, s = i / 2;
+                         mul(f, rh[s], rl[s], x[m], x[m + 1]);
+                         if (i < 2) to_right(right[2 + i], down, rh[1], rl[1], i);
+                     });
+        };
+        square(tf, R, down);
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-            v4f x = {};
-#pragma unroll
-            for (int s = 0; s <= m / 2; ++s) x = product(tf, m, s, 2, rh[s], rl[s], x);
             const v4f f = factor(2, m);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) Um[m][j] = x[j] * f[j] * fr;
+            for (int j = 0; j < 4; ++j) Um[m][j] = x[m][j] * f[j] * fr;
+            x[m] = v4f{};
         }
-        const float fu = to_right(Um, rh, rl);
+        e = exponent(largest(Um));
+        down = pow2(-e);
+        const float fu = pow2(e);
+        to_right(Um[0], down, rh[0], rl[0], 0);
+        to_right(Um[1], down, rh[0], rl[0], 1);
+        square(af, Um, down);
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-            v4f x = {};
-#pragma unroll
-            for (int s = 0; s <= m / 2; ++s) x = product(af, m, s, 2, rh[s], rl[s], x);
-            const v4f f = factor(3, m), h = factor(1, m);
+            const v4f f = factor(3, m), h = factor(1, m), w = factor(4, m);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int t = 16 * m + 4 * g + j;
-                const float o = fmaf(x[j], f[j] * fu, h[j] * fs * qs[m][j]);
-                if (work && t < nt) out[(int64_t)(t0 + t) * a.out_tok] = T::from(o);
+                own[(16 * m + 4 * j) * 16] = T::from(fmaf(x[m][j], f[j] * fu, h[j] * fs * qs[m][j]));
+                Um[m][j] *= w[j];
             }
         }
+        e = exponent(largest(Um));
+        down = pow2(-e);
+        const float fw = pow2(e), keep = vec[5 * C];
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            const v4f f = factor(4, m);
+        for (int m = 0; m < 4; ++m) to_right(Um[m], down, rh[m / 2], rl[m / 2], m & 1);
+        float top[2] = {0.0f, 0.0f};
+        v4f y[2];
+        products(std::integral_constant<int, KT>{},
+                 [&](int i, int k) __attribute__((always_inline)) { return r2 + 2 * (2 * (2 * (i / 2) + k) + (i & 1)) * 1024; },
+                 [&](int i, const Left & f) __attribute__((always_inline)) {
+                     if (!(i & 1)) y[0] = y[1] = v4f{};
+                     mul(f, rh[i & 1], rl[i & 1], y[0], y[1]);
+                     if (i & 1)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) Um[m][j] *= f[j];
-        }
-        const float fw = to_right(Um, rh, rl), keep = vec[5 * C];
+                         for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int i = 0; i < KT; ++i) {
-            v4f x = {};
-#pragma unroll
-            for (int s = 0; s < 2; ++s) x = product(r2, i, s, 2, rh[s], rl[s], x);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) S[i][j] = fmaf(x[j], fw, keep * S[i][j]);
-        }
+                             for (int j = 0; j < 4; ++j) {
+                                 const float st = fmaf(y[k][j], fw, keep * S[2 * (i / 2) + k][j]);
+                                 S[2 * (i / 2) + k][j] = st;
+                                 top[k] = fmaxf(top[k], fabsf(st));
+                             }
+                 });
+        big = over_column(fmaxf(top[0], top[1]));
+    };
+
+    if (chunks > 0) stage1(0, lds);
+#pragma clang loop unroll(disable)
+    for (int c = 0; c < chunks; ++c) {
+        sync();                                           // K, Q are there; the others' place is free
+        first_half(lds, lds + REG1, own_lds, c);
+        sync();                                           // the rest is there; K's and Q's place is free
+        second_half(lds + REG1, lds, own_lds, c);
     }
     if (!work) return;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");    // other lanes read what this one wrote
+    if (chunks > 0) put(own_lds, chunks - 1);
 #pragma unroll
     for (int i = 0; i < KT; ++i)
 #pragma unroll
@@ -565,11 +704,15 @@ int launch(const GdnArgs & a, bool chunked, hipStream_t s) {
         hipLaunchKernelGGL((gdn_step_kernel<T, K>), dim3((unsigned)blocks), dim3(128), 0, s, a);
         return (int)hipGetLastError();
     }
-    hipLaunchKernelGGL((gdn_prep_kernel<T, K>), dim3((unsigned)((int64_t)a.chunks * a.n_vh)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((gdn_prep_kernel<T, K>), dim3((unsigned)((int64_t)a.chunks * a.n_kh)), dim3(256), 0, s, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
-    const int64_t blocks = (int64_t)a.n_seq * a.n_vh * ((a.vd + 63) / 64);
-    hipLaunchKernelGGL((gdn_scan_kernel<T, K>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+    // 32 columns a workgroup as long as each has a CU of its own, then 64
+    // (8 key heads at a time, those that there are not return)
+    const int64_t heads = (int64_t)a.n_seq * (a.n_vh / a.n_kh) * ((a.n_kh + 7) / 8 * 8), few = heads * ((a.vd + 31) / 32);
+    if ((int64_t)a.n_seq * a.n_vh * ((a.vd + 31) / 32) <= pq2host::device_info().cus)
+        hipLaunchKernelGGL((gdn_scan_kernel<T, K, 2>), dim3((unsigned)few), dim3(128), 0, s, a);
+    else hipLaunchKernelGGL((gdn_scan_kernel<T, K, 4>), dim3((unsigned)(heads * ((a.vd + 63) / 64))), dim3(256), 0, s, a);
     return (int)hipGetLastError();
 }
 template <class T>
@@ -587,7 +730,7 @@ int check(const bonsai_p40_gdn_args * p) {
     const int64_t kr = (int64_t)p->n_k_head * p->k_dim, vr = (int64_t)p->n_v_head * p->v_dim;
     const int per16 = 16 / type_bytes(p->type);
     if (p->q_tok < kr || p->k_tok < kr || p->q_tok % per16 != 0 || p->k_tok % per16 != 0) return 1;
-    if (p->v_tok < vr || p->out_tok < vr || p->gate_tok < p->n_v_head) return 1;
+    if (p->v_tok < vr || p->v_tok % per16 != 0 || p->v_tok > (1 << 22) || p->out_tok < vr || p->gate_tok < p->n_v_head) return 1;
     if (!(p->scale > -INFINITY && p->scale < INFINITY) || !(p->l2_eps >= 0.0f && p->l2_eps < INFINITY)) return 1;
     if (p->n_seq <= 0) return 0;
     if (p->n_tok > 0x7fffffff || p->n_states > (1ll << 40)) return 1;
@@ -612,8 +755,8 @@ extern "C" int bonsai_p40_gdn(const bonsai_p40_gdn_args * p, bonsai_stream strea
     if (pq2host::any_null(p->starts)) return 1;
     if (p->n_states > 0 && pq2host::any_null(p->state, p->state_out)) return 1;
     if (p->n_tok > 0 && pq2host::any_null(p->q, p->k, p->v, p->out, p->g, p->beta)) return 1;
-    const int e = type_bytes(p->type);
-    if (!aligned(p->q, 16) || !aligned(p->k, 16) || !aligned(p->v, e) || !aligned(p->out, e) || !aligned(p->g, 4) ||
+    const int e = type_bytes(p->type), per16 = 16 / e;
+    if (!aligned(p->q, 16) || !aligned(p->k, 16) || !aligned(p->v, 16) || !aligned(p->out, e) || !aligned(p->g, 4) ||
         !aligned(p->beta, 4) || !aligned(p->state, 4) || !aligned(p->state_out, 4) || !aligned(p->starts, 4) ||
         !aligned(p->slots, 4) || !aligned(p->workspace, 16))
         return 1;
@@ -644,6 +787,7 @@ extern "C" int bonsai_p40_gdn(const bonsai_p40_gdn_args * p, bonsai_stream strea
     a.vd = p->v_dim;
     a.tiled = p->tiled != 0;
     a.chunks = (int)chunks_of(p);
+    a.out16 = aligned(p->out, 16) && p->out_tok % per16 == 0;    // rows of out that take 16 bytes at a time
     a.scale = p->scale;
     a.eps = p->l2_eps;
     const hipStream_t s = (hipStream_t)stream;

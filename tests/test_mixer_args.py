@@ -53,7 +53,8 @@ REFUSED = {
         dict(n_v_head=5), dict(n_v_head=65538), dict(type=3), dict(n_states=-1), dict(n_tok=-1), dict(max_new=-1),
         dict(q_tok=255), dict(k_tok=258), dict(v_tok=511), dict(out_tok=511), dict(gate_tok=3), dict(scale=INF),
         dict(scale=NAN), dict(l2_eps=-1.0), dict(l2_eps=NAN), dict(l2_eps=INF), dict(n_tok=1 << 26), dict(n_seq=1 << 26),
-        dict(q=A + 8), dict(k=A + 4), dict(v=A + 2), dict(out=A + 1), dict(g=A + 2), dict(beta=A + 1), dict(state=A + 2),
+        dict(v_tok=514), dict(v_tok=(1 << 22) + 4),
+        dict(q=A + 8), dict(k=A + 4), dict(v=A + 8), dict(out=A + 1), dict(g=A + 2), dict(beta=A + 1), dict(state=A + 2),
         dict(state_out=A + 3), dict(starts=A + 2), dict(slots=A + 1), dict(workspace=A + 4, workspace_bytes=1 << 30),
         dict(workspace=A, workspace_bytes=1000)]),
 }
