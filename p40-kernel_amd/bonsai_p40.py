@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libbonsai_p40.so")
@@ -111,11 +112,25 @@ def _ptr(t) -> int | None:
     return t.data_ptr()
 
 
+_raw_stream = _device = None     # a device's current stream as a hipStream_t; the current device
+
+
+def _init_streams() -> None:
+    global _raw_stream, _device
+    import torch
+    torch.cuda.current_stream()                           # initialises the device
+    # what torch.cuda.current_stream(dev).cuda_stream comes to, without the objects made on the way (0.2 us, not 2.9)
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+        lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+    _device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def _stream(stream) -> int | None:
     if stream is not None:
         return stream if isinstance(stream, int) else stream.cuda_stream
-    import torch
-    return torch.cuda.current_stream().cuda_stream
+    if _device is None:
+        _init_streams()
+    return _raw_stream(_device())
 
 
 def call(name: str, *args, stream=None) -> int:
@@ -423,9 +438,14 @@ class Chain:
 F32, F16, BF16 = 0, 1, 2
 
 
+_FORMATS = {_V: "P", _I64: "q", C.c_int: "i", C.c_float: "f"}
+
+
 def _args_struct(name, **fields):
-    return type(name, (C.Structure,), {"_fields_": [(f, t) for t, names in fields["spec"] for f in names.split()],
-                                       "__doc__": fields["doc"]})
+    """The ctypes struct, and pack: its bytes from the fields' values in a row (a third of the time)."""
+    types = [(f, t) for t, names in fields["spec"] for f in names.split()]
+    return type(name, (C.Structure,), {"_fields_": types, "__doc__": fields["doc"],
+                                       "pack": struct.Struct("@" + "".join(_FORMATS[t] for _, t in types) + "0q").pack})
 
 
 QkNormRopeArgs = _args_struct("QkNormRopeArgs", doc="bonsai_p40_qk_norm_rope_args of include/bonsai_p40.h.", spec=[
@@ -458,18 +478,18 @@ def _type(t) -> int:
     return ty
 
 
-def _flat(t, name: str, dtype, shape) -> int:
-    """The address of t, which has this type and shape and lies in one piece."""
-    if _TYPES.get(t.dtype) != dtype or t.shape != shape or not t.is_contiguous():
-        raise ValueError(f"{name}: contiguous {'fp32' if dtype == F32 else dtype} {shape} is wanted, "
-                         f"not {t.dtype} {tuple(t.shape)} of strides {t.stride()}")
+def _flat(t, name: str, dtype, shape, dev: int) -> int:
+    """The address of t, which has this type and shape, lies in one piece and on device dev."""
+    if _TYPES.get(t.dtype) != dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != dev:
+        raise ValueError(f"{name}: contiguous {'fp32' if dtype == F32 else dtype} {shape} beside q is wanted, "
+                         f"not {t.dtype} {tuple(t.shape)} of strides {t.stride()} on {t.device}")
     return t.data_ptr()
 
 
-def _rows(t, name: str, shape) -> int:
-    """The token stride of (token, head, element) rows whose heads follow each other."""
-    if t.shape != shape:
-        raise ValueError(f"{name}: shape {tuple(t.shape)}, wanted {shape}")
+def _rows(t, name: str, shape, dev: int) -> int:
+    """The token stride of (token, head, element) rows on device dev whose heads follow each other."""
+    if t.shape != shape or t.get_device() != dev:
+        raise ValueError(f"{name}: shape {tuple(t.shape)} on {t.device}, wanted {shape} beside q")
     n, heads, dim = shape
     tok, head, el = t.stride()
     if (el != 1 and dim != 1) or (head != dim and heads != 1):
@@ -477,11 +497,12 @@ def _rows(t, name: str, shape) -> int:
     return tok if n > 1 else max(tok, heads * dim)
 
 
-def _pages(k_pages, v_pages):
+def _pages(k_pages, v_pages, dev: int):
     """(n_pages, n_kv_head, page_size, head_dim) pages of keys and values: shape, page stride and type."""
     shape, st = k_pages.shape, k_pages.stride()
-    if len(shape) != 4 or v_pages.shape != shape or v_pages.stride() != st or v_pages.dtype != k_pages.dtype:
-        raise ValueError("k_pages and v_pages: alike, (n_pages, n_kv_head, page_size, head_dim)")
+    if (len(shape) != 4 or v_pages.shape != shape or v_pages.stride() != st or v_pages.dtype != k_pages.dtype
+            or k_pages.get_device() != dev or v_pages.get_device() != dev):
+        raise ValueError("k_pages and v_pages: alike, (n_pages, n_kv_head, page_size, head_dim), beside q")
     n, h, p, d = shape
     if (st[3] != 1 and d != 1) or (st[2] != d and p != 1) or (st[1] != p * d and h != 1):
         raise ValueError("a page has to lie in one piece")
@@ -494,6 +515,26 @@ def rope_inv_freq(n_rot: int, base: float, device="cuda"):
     return base ** (-torch.arange(0, n_rot, 2, dtype=torch.float64, device=device) / n_rot)
 
 
+def _scratch(workspace, dev: int):
+    if workspace is None:
+        return 0, 0
+    if workspace.get_device() != dev or not workspace.is_contiguous():
+        raise ValueError("workspace: one piece beside q is wanted")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
+def _stream_of(q, stream) -> int | None:
+    """The stream for a call on q's device, which has to be the current one."""
+    dev = q.get_device()
+    if dev < 0:
+        raise ValueError("tensors on the device are wanted")
+    if _device is None:
+        _init_streams()
+    if dev != _device():
+        raise ValueError(f"the tensors are on {q.device}, the current device is {_device()}")
+    return _raw_stream(dev) if stream is None else _stream(stream)
+
+
 def _qk_norm_rope_args(q, k, v, q_norm, k_norm, eps, pos, inv_freq, slots, k_pages, v_pages, q_out, interleaved):
     if q.dim() != 3 or k.dim() != 3:
         raise ValueError("q, k and v: (n_tok, heads, head_dim) is wanted")
@@ -501,18 +542,19 @@ def _qk_norm_rope_args(q, k, v, q_norm, k_norm, eps, pos, inv_freq, slots, k_pag
     kv = k.shape[1]
     if not _type(q) == _type(k) == _type(v) == F32:
         raise ValueError("q, k and v: fp32 is wanted")
-    if k.shape != (n, kv, d) or v.shape != k.shape:
-        raise ValueError(f"k, v: shapes {tuple(k.shape)}, {tuple(v.shape)} beside q's {tuple(shape)}")
-    (pages, page_kv, page_size, page_d), stride, kv_type = _pages(k_pages, v_pages)
+    dev = q.get_device()
+    if k.shape != (n, kv, d) or v.shape != k.shape or not dev == k.get_device() == v.get_device():
+        raise ValueError(f"k, v: shapes {tuple(k.shape)}, {tuple(v.shape)} beside q's {tuple(shape)}, on one device")
+    (pages, page_kv, page_size, page_d), stride, kv_type = _pages(k_pages, v_pages, dev)
     if page_kv != kv or page_d != d:
         raise ValueError("the pages have other heads")
     half = 0 if inv_freq is None else inv_freq.numel()
-    return QkNormRopeArgs(
+    return QkNormRopeArgs.pack(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride(), *k.stride(), *v.stride(), n, h, kv, d, 2 * half,
-        1 if interleaved else 0, eps, None if q_norm is None else _flat(q_norm, "q_norm", F32, (d,)),
-        None if k_norm is None else _flat(k_norm, "k_norm", F32, (d,)),
-        _flat(pos, "pos", "int32", (n,)) if half else None, _flat(inv_freq, "inv_freq", "float64", (half,)) if half else None,
-        _flat(slots, "slots", "int64", (n,)), q_out.data_ptr(), _rows(q_out, "q_out", shape), _type(q_out), kv_type,
+        1 if interleaved else 0, eps, 0 if q_norm is None else _flat(q_norm, "q_norm", F32, (d,), dev),
+        0 if k_norm is None else _flat(k_norm, "k_norm", F32, (d,), dev),
+        _flat(pos, "pos", "int32", (n,), dev) if half else 0, _flat(inv_freq, "inv_freq", "float64", (half,), dev) if half else 0,
+        _flat(slots, "slots", "int64", (n,), dev), q_out.data_ptr(), _rows(q_out, "q_out", shape, dev), _type(q_out), kv_type,
         k_pages.data_ptr(), v_pages.data_ptr(), pages, stride, page_size)
 
 
@@ -524,7 +566,7 @@ def qk_norm_rope(q, k, v, q_norm, k_norm, eps: float, pos, inv_freq, slots, k_pa
     a head or the tokens consecutive (Y.view(heads, head_dim, n_tok).permute(2, 0,
     1) of a gemm)."""
     a = _qk_norm_rope_args(q, k, v, q_norm, k_norm, eps, pos, inv_freq, slots, k_pages, v_pages, q_out, interleaved)
-    _check("bonsai_p40_qk_norm_rope", lib().bonsai_p40_qk_norm_rope(C.byref(a), _stream(stream)))
+    _check("bonsai_p40_qk_norm_rope", lib().bonsai_p40_qk_norm_rope(a, _stream_of(q, stream)))
 
 
 def _attn_args(q, k_pages, v_pages, table, starts, kv_len, out, workspace, max_kv, scale):
@@ -534,25 +576,25 @@ def _attn_args(q, k_pages, v_pages, table, starts, kv_len, out, workspace, max_k
     io = _type(q)
     if _type(out) != io:
         raise ValueError("out has to have q's type")
-    (pages, kv, page_size, page_d), stride, kv_type = _pages(k_pages, v_pages)
+    dev = q.get_device()
+    (pages, kv, page_size, page_d), stride, kv_type = _pages(k_pages, v_pages, dev)
     if page_d != d:
         raise ValueError("the pages have another head_dim")
     n_seq, cols = table.shape
     row, col = table.stride()
-    if _TYPES.get(table.dtype) != "int32" or (col != 1 and cols > 1):
-        raise ValueError("table: int32 rows are wanted")
-    return AttnPagedArgs(
-        q.data_ptr(), out.data_ptr(), _rows(q, "q", shape), _rows(out, "out", shape), n, n_seq, h, kv, d, io, kv_type,
+    if _TYPES.get(table.dtype) != "int32" or (col != 1 and cols > 1) or table.get_device() != dev:
+        raise ValueError("table: int32 rows beside q are wanted")
+    return AttnPagedArgs.pack(
+        q.data_ptr(), out.data_ptr(), _rows(q, "q", shape, dev), _rows(out, "out", shape, dev), n, n_seq, h, kv, d, io, kv_type,
         d ** -0.5 if scale is None else scale, k_pages.data_ptr(), v_pages.data_ptr(), pages, stride, page_size, cols,
-        table.data_ptr(), row if n_seq > 1 else cols, _flat(starts, "starts", "int32", (n_seq + 1,)),
-        _flat(kv_len, "kv_len", "int32", (n_seq,)), max_kv, None if workspace is None else workspace.data_ptr(),
-        0 if workspace is None else workspace.numel() * workspace.element_size())
+        table.data_ptr(), row if n_seq > 1 else cols, _flat(starts, "starts", "int32", (n_seq + 1,), dev),
+        _flat(kv_len, "kv_len", "int32", (n_seq,), dev), max_kv, *_scratch(workspace, dev))
 
 
 def attn_paged_workspace_bytes(q, k_pages, v_pages, table, starts, kv_len, out, max_kv: int = 0, scale=None) -> int:
     """bonsai_p40_attn_paged_workspace_bytes for these arguments of attn_paged."""
     a = _attn_args(q, k_pages, v_pages, table, starts, kv_len, out, None, max_kv, scale)
-    return int(lib().bonsai_p40_attn_paged_workspace_bytes(C.byref(a)))
+    return int(lib().bonsai_p40_attn_paged_workspace_bytes(a))
 
 
 def attn_paged(q, k_pages, v_pages, table, starts, kv_len, out, workspace=None, max_kv: int = 0, scale=None,
@@ -561,7 +603,7 @@ def attn_paged(q, k_pages, v_pages, table, starts, kv_len, out, workspace=None, 
     starts[s + 1] - 1 of q and out, (n_tok, heads, head_dim)) over its kv_len[s] keys
     in the pages table[s]; scale None: head_dim^-1/2."""
     a = _attn_args(q, k_pages, v_pages, table, starts, kv_len, out, workspace, max_kv, scale)
-    _check("bonsai_p40_attn_paged", lib().bonsai_p40_attn_paged(C.byref(a), _stream(stream)))
+    _check("bonsai_p40_attn_paged", lib().bonsai_p40_attn_paged(a, _stream_of(q, stream)))
 
 
 def _gdn_args(q, k, v, g, beta, state, state_out, out, starts, workspace, max_new, slots, scale, l2_eps, tiled):
@@ -572,27 +614,28 @@ def _gdn_args(q, k, v, g, beta, state, state_out, out, starts, workspace, max_ne
     ty = _type(q)
     if _type(k) != ty or _type(v) != ty or _type(out) != ty:
         raise ValueError("q, k, v and out: one type is wanted")
-    if _type(g) != F32 or _type(beta) != F32 or g.shape != (n, vh) or beta.shape != g.shape:
-        raise ValueError(f"g and beta: fp32 ({n}, {vh}) is wanted")
+    dev = q.get_device()
+    if (_type(g) != F32 or _type(beta) != F32 or g.shape != (n, vh) or beta.shape != g.shape
+            or not dev == g.get_device() == beta.get_device()):
+        raise ValueError(f"g and beta: fp32 ({n}, {vh}) beside q is wanted")
     (gt, gh), (bt, bh) = g.stride(), beta.stride()
     if (vh > 1 and not gh == bh == 1) or (n > 1 and gt != bt):
         raise ValueError("g and beta: one token stride, and the heads of a token consecutive")
     ss, n_seq = (state.shape[0], vh, kd, vd), starts.shape[0] - 1
-    return GdnArgs(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _rows(q, "q", qs), _rows(k, "k", qs),
-        _rows(v, "v", (n, vh, vd)), _rows(out, "out", (n, vh, vd)), g.data_ptr(), beta.data_ptr(), gt if n > 1 else vh,
-        _flat(state, "state", F32, ss), _flat(state_out, "state_out", F32, ss), ss[0],
-        None if slots is None else _flat(slots, "slots", "int32", (n_seq,)),
-        _flat(starts, "starts", "int32", (n_seq + 1,)), n, n_seq, kh, vh, kd, vd, ty, 1 if tiled else 0,
-        kd ** -0.5 if scale is None else scale, l2_eps, max_new, None if workspace is None else workspace.data_ptr(),
-        0 if workspace is None else workspace.numel() * workspace.element_size())
+    return GdnArgs.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _rows(q, "q", qs, dev), _rows(k, "k", qs, dev),
+        _rows(v, "v", (n, vh, vd), dev), _rows(out, "out", (n, vh, vd), dev), g.data_ptr(), beta.data_ptr(), gt if n > 1 else vh,
+        _flat(state, "state", F32, ss, dev), _flat(state_out, "state_out", F32, ss, dev), ss[0],
+        0 if slots is None else _flat(slots, "slots", "int32", (n_seq,), dev),
+        _flat(starts, "starts", "int32", (n_seq + 1,), dev), n, n_seq, kh, vh, kd, vd, ty, 1 if tiled else 0,
+        kd ** -0.5 if scale is None else scale, l2_eps, max_new, *_scratch(workspace, dev))
 
 
 def gdn_workspace_bytes(q, k, v, g, beta, state, state_out, out, starts, max_new: int = 0, slots=None, scale=None,
                         l2_eps: float = 0.0, tiled: bool = False) -> int:
     """bonsai_p40_gdn_workspace_bytes for these arguments of gdn."""
     a = _gdn_args(q, k, v, g, beta, state, state_out, out, starts, None, max_new, slots, scale, l2_eps, tiled)
-    return int(lib().bonsai_p40_gdn_workspace_bytes(C.byref(a)))
+    return int(lib().bonsai_p40_gdn_workspace_bytes(a))
 
 
 def gdn(q, k, v, g, beta, state, state_out, out, starts, workspace=None, max_new: int = 0, slots=None, scale=None,
@@ -602,4 +645,4 @@ def gdn(q, k, v, g, beta, state, state_out, out, starts, workspace=None, max_new
     g (log decay) and beta (n_tok, v_heads), state (n_states, v_heads, k_dim, v_dim);
     scale None: k_dim^-1/2."""
     a = _gdn_args(q, k, v, g, beta, state, state_out, out, starts, workspace, max_new, slots, scale, l2_eps, tiled)
-    _check("bonsai_p40_gdn", lib().bonsai_p40_gdn(C.byref(a), _stream(stream)))
+    _check("bonsai_p40_gdn", lib().bonsai_p40_gdn(a, _stream_of(q, stream)))

@@ -130,6 +130,18 @@ def test_structs_match_the_header(tmp_path):
         assert int(n) == (C.sizeof(structs[s]) if f == "." else getattr(structs[s], f).offset), line
 
 
+def read(cls, packed):
+    assert len(packed) == C.sizeof(cls)
+    return cls.from_buffer_copy(packed)
+
+
+def test_wrappers_want_device_tensors():
+    t = _tensors()
+    with pytest.raises(ValueError):
+        B.qk_norm_rope(*[t[k] for k in ("q", "k", "v", "q_norm", "k_norm", "eps", "pos", "inv_freq", "slots", "k_pages",
+                                        "v_pages", "q_out")])
+
+
 def _tensors():
     z = torch.zeros
     return dict(q=z(5, 4, 64), k=z(5, 2, 64), v=z(5, 2, 64), q_norm=z(64), k_norm=z(64), eps=1e-6, pos=z(5, dtype=torch.int32),
@@ -140,10 +152,10 @@ def _tensors():
 def test_wrapper_checks_rope():
     z = torch.zeros
     ok = _tensors()
-    a = B._qk_norm_rope_args(**ok)
+    a = read(B.QkNormRopeArgs, B._qk_norm_rope_args(**ok))
     assert (a.n_tok, a.n_head, a.n_kv_head, a.head_dim, a.n_rot, a.page_size, a.n_pages) == (5, 4, 2, 64, 32, 16, 3)
     assert (a.q_tok, a.q_head, a.q_el, a.q_out_tok, a.page_stride, a.q_type, a.kv_type) == (256, 64, 1, 256, 2048, B.F16, B.F16)
-    cols = B._qk_norm_rope_args(**{**ok, "q": z(4, 64, 5).permute(2, 0, 1)})
+    cols = read(B.QkNormRopeArgs, B._qk_norm_rope_args(**{**ok, "q": z(4, 64, 5).permute(2, 0, 1)}))
     assert (cols.q_tok, cols.q_head, cols.q_el) == (1, 320, 5)
     for bad in (dict(q=z(5, 4, 64, dtype=torch.float16)), dict(k=z(5, 2, 32)), dict(v=z(4, 2, 64)), dict(q_norm=z(63)),
                 dict(pos=z(5)), dict(pos=z(4, dtype=torch.int32)), dict(inv_freq=z(16)), dict(slots=z(5, dtype=torch.int32)),
@@ -161,7 +173,7 @@ def test_wrapper_checks_attn():
     t = _tensors()
     ok = dict(q=t["q_out"], k_pages=t["k_pages"], v_pages=t["v_pages"], table=z(2, 3, dtype=i32), starts=z(3, dtype=i32),
               kv_len=z(2, dtype=i32), out=z(5, 4, 64, dtype=torch.float16), workspace=None, max_kv=0, scale=None)
-    a = B._attn_args(**ok)
+    a = read(B.AttnPagedArgs, B._attn_args(**ok))
     assert (a.n_tok, a.n_seq, a.n_head, a.n_kv_head, a.head_dim, a.max_pages, a.table_stride, a.scale) == (5, 2, 4, 2, 64, 3, 3, 0.125)
     for bad in (dict(out=z(5, 4, 64)), dict(out=z(5, 4, 63, dtype=torch.float16)), dict(table=z(2, 3)), dict(starts=z(2, dtype=i32)),
                 dict(kv_len=z(3, dtype=i32)), dict(kv_len=z(2, dtype=torch.int64)), dict(table=z(3, 2, dtype=i32).t()),
@@ -176,7 +188,7 @@ def test_wrapper_checks_gdn():
     ok = dict(q=z(5, 2, 64), k=z(5, 2, 64), v=z(5, 4, 32), g=z(5, 4), beta=z(5, 4), state=z(3, 4, 64, 32),
               state_out=z(3, 4, 64, 32), out=z(5, 4, 32), starts=z(4, dtype=i32), workspace=None, max_new=0, slots=None,
               scale=None, l2_eps=0.0, tiled=False)
-    a = B._gdn_args(**ok)
+    a = read(B.GdnArgs, B._gdn_args(**ok))
     assert (a.n_tok, a.n_seq, a.n_k_head, a.n_v_head, a.k_dim, a.v_dim, a.n_states, a.gate_tok) == (5, 3, 2, 4, 64, 32, 3, 4)
     for bad in (dict(k=z(5, 2, 32)), dict(k=z(5, 2, 64, dtype=torch.float16)), dict(v=z(4, 4, 32)), dict(g=z(5, 3)),
                 dict(beta=z(4, 5).t()), dict(beta=z(5, 8)[:, :4]), dict(state=z(3, 4, 32, 64)), dict(state_out=z(2, 4, 64, 32)),
