@@ -111,10 +111,10 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
     // same time have the same keys; the last tiles, which see the most, start first
     const int kvh = blockIdx.x % a.n_kv, rest = blockIdx.x / a.n_kv;
     const int split = rest / a.tiles, tile_no = a.tiles - 1 - rest % a.tiles;
-    const Tile tl = find_tile<Z::BM>(a.starts, a.n_seq, a.n_tok, a.group, tile_no);
+    const Tile tl = find_tile<Z::BM>(a.starts, a.kv_len, a.n_seq, a.n_tok, a.group, tile_no);
     if (tl.seq < 0) return;
     const int rows = tl.count * a.group, row0 = tl.index * Z::BM;
-    const int kv = iclamp(sload(a.kv_len, tl.seq), 0, a.cap), before = kv - tl.count;
+    const int kv = iclamp(tl.extra, 0, a.cap), before = kv - tl.count;
     const int last = min(row0 + Z::BM, rows) - 1;
     // (readfirstlane: the same in all lanes, which the compiler does not see through the division)
     const int nk = a.n_pages > 0 ? __builtin_amdgcn_readfirstlane(iclamp(before + last / a.group + 1, 0, kv)) : 0;
@@ -136,60 +136,64 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
     // the keys that all rows of the workgroup see
     const int first_vis = __builtin_amdgcn_readfirstlane(iclamp(before + row0 / a.group + 1, 0, kv));
 
-    // Q^T, element j of half h: d = 16 step + 8 h + j
+    // Q^T, element j of half h: d = 16 step + 8 h + j (a lane without a row: the tile's first).  fp32 queries
+    // are asked for here, and made into terms when the first tiles are on their way
+    typedef typename std::conditional<NT == 1, frag, v8f>::type raw;
+    typedef typename std::conditional<NT == 1, elem, float>::type qelem;
+    raw qx[QS];
+    {
+        const qelem * const qp = reinterpret_cast<const qelem *>(a.q) + grow * a.q_tok + (int64_t)head * D + 8 * half;
+#pragma unroll
+        for (int s = 0; s < QS; ++s) qx[s] = *reinterpret_cast<const raw *>(qp + 16 * s);
+    }
     frag qf[Z::QR][QS];
     uint8_t * const ql = lds + Z::MAIN + (KEYS ? 0 : wave * (NT - Z::QR) * Z::QT) + 16 * lane;
     float c = a.c;
-    if constexpr (NT == 1) {
-        const elem * const qp = reinterpret_cast<const elem *>(a.q) + grow * a.q_tok + (int64_t)head * D + 8 * half;
+    auto make_q = [&]() __attribute__((always_inline)) {
+        if constexpr (NT == 1) {
 #pragma unroll
-        for (int s = 0; s < QS; ++s)
-            qf[0][s] = live ? *reinterpret_cast<const frag *>(qp + 16 * s) : frag{};
-    } else {
-        const float * const qp = reinterpret_cast<const float *>(a.q) + grow * a.q_tok + (int64_t)head * D + 8 * half;
-        float up = 1.0f;
-        if constexpr (NT == 2) {
-            // the row's largest element to [1, 2): f16 then holds 22 bits in two terms
-            float big = 0.0f;
-            if (live)
+            for (int s = 0; s < QS; ++s) qf[0][s] = qx[s];
+        } else {
+            float up = 1.0f;
+            if constexpr (NT == 2) {
+                // the row's largest element to [1, 2): f16 then holds 22 bits in two terms
+                float big = 0.0f;
 #pragma unroll
-                for (int s = 0; s < QS; ++s) {
-                    const v4f x = *reinterpret_cast<const v4f *>(qp + 16 * s), y = *reinterpret_cast<const v4f *>(qp + 16 * s + 4);
+                for (int s = 0; s < QS; ++s)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) big = fmaxf(big, fmaxf(fabsf(x[j]), fabsf(y[j])));
-                }
-            big = fmaxf(big, __shfl_xor(big, 32));
-            const int e = (int)((__builtin_bit_cast(uint32_t, big) >> 23) & 255);
-            if (e > 2 && e < 252) {
-                up = __builtin_bit_cast(float, (uint32_t)(254 - e) << 23);
-                c *= __builtin_bit_cast(float, (uint32_t)e << 23);
-            }
-        }
-#pragma unroll
-        for (int s = 0; s < QS; ++s) {
-            v4f x = {}, y = {};
-            if (live) {
-                x = *reinterpret_cast<const v4f *>(qp + 16 * s);
-                y = *reinterpret_cast<const v4f *>(qp + 16 * s + 4);
-            }
-            frag low[NT];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float f = (j < 4 ? x[j & 3] : y[j & 3]) * up;
-#pragma unroll
-                for (int k = 0; k < NT; ++k) {
-                    const elem e = T::from(f);
-                    if (k < Z::QR) qf[k][s][j] = e;
-                    else low[k][j] = e;
-                    f -= T::to(e);
+                    for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(qx[s][j]));
+                big = fmaxf(big, __shfl_xor(big, 32));
+                const int e = (int)((__builtin_bit_cast(uint32_t, big) >> 23) & 255);
+                if (e > 2 && e < 252) {
+                    up = __builtin_bit_cast(float, (uint32_t)(254 - e) << 23);
+                    c *= __builtin_bit_cast(float, (uint32_t)e << 23);
                 }
             }
 #pragma unroll
-            for (int k = Z::QR; k < NT; ++k)
-                if (!KEYS || wave == 0) *reinterpret_cast<frag *>(ql + (k - Z::QR) * Z::QT + 1024 * s) = low[k];
+            for (int s = 0; s < QS; ++s) {
+                frag low[NT];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    float f = qx[s][j] * up;
+#pragma unroll
+                    for (int k = 0; k < NT; ++k) {
+                        const elem e = T::from(f);
+                        if (k < Z::QR) qf[k][s][j] = e;
+                        else low[k][j] = e;
+                        f -= T::to(e);
+                    }
+                }
+#pragma unroll
+                for (int k = Z::QR; k < NT; ++k)
+                    if (!KEYS || wave == 0) *reinterpret_cast<frag *>(ql + (k - Z::QR) * Z::QT + 1024 * s) = low[k];
+            }
+            if constexpr (Z::QL && KEYS) {                 // (rows: each wave reads its own)
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+            }
         }
-        if constexpr (Z::QL) __syncthreads();
-    }
+    };
 
     v16f o[DT];
 #pragma unroll
@@ -493,8 +497,10 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
                 if (t < nt) stage(khead, idk, t, kring + t * Z::TILE, false);
                 if (t > 0 && t - 1 < nt) stage(vhead, idv, t - 1, vring + (t - 1) * Z::TILE, true);
             }
+            make_q();
             if (nt >= R) pq2::wait_vmcnt<(R - 1) * PER>();
             else pq2::wait_vmcnt<0>();
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
             v16f s = scores(kring, ql);
@@ -556,6 +562,7 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
         };
         int key = k0 + 32 * wave, b = 0;
         if (key < k1) stage(key, mine);
+        make_q();
 #pragma clang loop unroll(disable)
         for (; key < k1; key += 32 * Z::NW, b ^= 1) {
             const int holes = (id0 < 0 ? 1 : 0) | (id1 < 0 ? 2 : 0);
@@ -645,23 +652,29 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
     }
 }
 
-// The parts of every row: a wave per row.  Their number follows from the keys
-// the row's tile saw, as in attn_kernel.
-template <class TO, int D>
+// The parts of every row, by WR waves.  Their number follows from the keys the
+// row's tile saw, as in attn_kernel; the largest m is looked for among all that
+// there could be while the lengths are on their way.
+template <class TO, int D, int WR>
 __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int bm) {
-    constexpr int E = D / 64;
-    const int lane = threadIdx.x & 63;
-    const int64_t all_rows = (int64_t)a.n_tok * a.n_head, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    constexpr int E = D / 64, AHEAD = 8;
+    __shared__ float sum[4][D + 1];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave % WR;
+    const int64_t all_rows = (int64_t)a.n_tok * a.n_head, row = (int64_t)blockIdx.x * (4 / WR) + wave / WR;
     if (row >= all_rows) return;
     const int tok = (int)(row / a.n_head), head = (int)(row - (int64_t)tok * a.n_head);
+    const float2 * const ml = reinterpret_cast<const float2 *>(a.part + (int64_t)a.n_split * all_rows * D) + row;
+    float own = -INFINITY;
+    if (lane < a.n_split) own = ml[lane * all_rows].x;
     // the sequence of this token
-    int seq = -1, first = 0, count = 0;
+    int seq = -1, first = 0, count = 0, kv = 0;
     for (int s0 = 0; s0 < a.n_seq && seq < 0; s0 += 64) {
         const int s = s0 + lane;
-        int b = 0, e = 0;
+        int b = 0, e = 0, len = 0;
         if (s < a.n_seq) {
             b = iclamp(a.starts[s], 0, a.n_tok);
             e = iclamp(a.starts[s + 1], 0, a.n_tok);
+            len = iclamp(a.kv_len[s], 0, a.cap);
         }
         const uint64_t hit = __ballot(tok >= b && tok < e);
         if (hit) {
@@ -669,30 +682,49 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int bm) {
             seq = s0 + k;
             first = __builtin_amdgcn_readlane(b, k);
             count = __builtin_amdgcn_readlane(e, k) - first;
+            kv = __builtin_amdgcn_readlane(len, k);
         }
     }
     if (seq < 0) return;                                   // a row behind the last sequence
-    const int kv = iclamp(a.kv_len[seq], 0, a.cap);
     const int r = (tok - first) * a.group + head % a.group;
     const int last = min(r / bm * bm + bm, count * a.group) - 1;
     const int nk = a.n_pages > 0 ? iclamp(kv - count + last / a.group + 1, 0, kv) : 0;
     const int n = iclamp((nk + a.chunk - 1) / a.chunk, 1, a.n_split);
-    const float2 * const ml = reinterpret_cast<const float2 *>(a.part + (int64_t)a.n_split * all_rows * D) + row;
-    float mm = -INFINITY;
-    for (int i = lane; i < n; i += 64) mm = fmaxf(mm, ml[i * all_rows].x);
+    float mm = lane < n ? own : -INFINITY;
+    for (int i = 64 + lane; i < n; i += 64) mm = fmaxf(mm, ml[i * all_rows].x);
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) mm = fmaxf(mm, __shfl_xor(mm, d));
     const float ref = mm == -INFINITY ? 0.0f : mm;
     float x[E] = {}, l = 0.0f;
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-        const float2 e = ml[i * all_rows];
-        const float w = __builtin_amdgcn_exp2f(e.x - ref);
-        float v[E];
-        load_row<F32>(a.part + (i * all_rows + row) * D + lane * E, v);
-        l = fmaf(e.y, w, l);
+    for (int i0 = w; i0 < n; i0 += WR * AHEAD) {
+        float v[AHEAD][E];
+        float2 e[AHEAD];
 #pragma unroll
-        for (int j = 0; j < E; ++j) x[j] = fmaf(v[j], w, x[j]);
+        for (int k = 0; k < AHEAD; ++k) {
+            const int64_t i = min(i0 + k * WR, n - 1);
+            e[k] = ml[i * all_rows];
+            load_row<F32>(a.part + (i * all_rows + row) * D + lane * E, v[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k)
+            if (i0 + k * WR < n) {
+                const float wt = __builtin_amdgcn_exp2f(e[k].x - ref);
+                l = fmaf(e[k].y, wt, l);
+#pragma unroll
+                for (int j = 0; j < E; ++j) x[j] = fmaf(v[k][j], wt, x[j]);
+            }
+    }
+    if constexpr (WR > 1) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) sum[wave][lane * E + j] = x[j];
+        if (lane == 0) sum[wave][D] = l;
+        __syncthreads();                                   // (WR = 4: one row a workgroup, all waves are here)
+        if (w) return;
+        for (int k = 1; k < WR; ++k) {
+            l += sum[k][D];
+#pragma unroll
+            for (int j = 0; j < E; ++j) x[j] += sum[k][lane * E + j];
+        }
     }
     const float inv = l != 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
@@ -707,9 +739,10 @@ int launch(AttnArgs & a, hipStream_t s) {
     hipLaunchKernelGGL((attn_kernel<T, D, NT, KEYS>), dim3((unsigned)blocks), dim3(64 * Z::NW), 0, s, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.n_split == 1) return (int)e;
-    const unsigned jb = (unsigned)(((int64_t)a.n_tok * a.n_head + 3) / 4);
-    if constexpr (NT == 1) hipLaunchKernelGGL((attn_join_kernel<T, D>), dim3(jb), dim3(256), 0, s, a, (int)Z::BM);
-    else hipLaunchKernelGGL((attn_join_kernel<F32, D>), dim3(jb), dim3(256), 0, s, a, (int)Z::BM);
+    typedef typename std::conditional<NT == 1, T, F32>::type TO;
+    const int64_t rows = (int64_t)a.n_tok * a.n_head;
+    if (a.n_split > 8) hipLaunchKernelGGL((attn_join_kernel<TO, D, 4>), dim3((unsigned)rows), dim3(256), 0, s, a, (int)Z::BM);
+    else hipLaunchKernelGGL((attn_join_kernel<TO, D, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a, (int)Z::BM);
     return (int)hipGetLastError();
 }
 template <class T, int D, int NT>

@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(256) gdn_prep_kernel(GdnArgs a) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, g = lane >> 4;
     const int hk = blockIdx.x % a.n_kh, chunk = blockIdx.x / a.n_kh, per = a.n_vh / a.n_kh;
-    const Tile tl = find_tile<C>(a.starts, a.n_seq, a.n_tok, 1, chunk);
+    const Tile tl = find_tile<C>(a.starts, nullptr, a.n_seq, a.n_tok, 1, chunk);
     if (tl.seq < 0) return;
     const int t0 = tl.first + tl.index * C, nt = min(C, tl.count - tl.index * C);
     uint8_t * const wk = a.ws + ((int64_t)chunk * a.n_kh + hk) * W::HEAD;

@@ -11,6 +11,7 @@
 namespace mixer {
 
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v8f __attribute__((ext_vector_type(8)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
@@ -83,17 +84,25 @@ __device__ __forceinline__ void dma16_at(__amdgpu_buffer_rsrc_t from, uint8_t * 
 // to 0 .. n_tok.  seq is -1 behind the last tile.  For whole waves.
 struct Tile {
     int seq, index, first, count;       // sequence, its tile, its first token, its tokens
+    int extra;                          // its entry of `more` (NULL: 0), read beside starts
 };
 template <int BM>
-__device__ __forceinline__ Tile find_tile(const int32_t * starts, int n_seq, int n_tok, int per_tok, int tile) {
+__device__ __forceinline__ Tile find_tile(const int32_t * starts, const int32_t * more, int n_seq, int n_tok, int per_tok,
+                                          int tile) {
+    if (n_seq == 1) {                   // no search, two waits less
+        const int b = iclamp(sload(starts, 0), 0, n_tok), n = max(iclamp(sload(starts, 1), 0, n_tok) - b, 0);
+        const int tiles = (int)(((int64_t)n * per_tok + BM - 1) / BM);
+        return Tile{tile < tiles ? 0 : -1, tile, b, n, more ? sload(more, 0) : 0};
+    }
     const int lane = threadIdx.x & 63;
     int base = 0;
     for (int s0 = 0; s0 < n_seq; s0 += 64) {
         const int s = s0 + lane;
-        int b = 0, n = 0;
+        int b = 0, n = 0, x = 0;
         if (s < n_seq) {
             b = iclamp(starts[s], 0, n_tok);
             n = max(iclamp(starts[s + 1], 0, n_tok) - b, 0);
+            if (more) x = more[s];
         }
         const int own = (int)(((int64_t)n * per_tok + BM - 1) / BM);
         int sum = own;
@@ -110,11 +119,12 @@ __device__ __forceinline__ Tile find_tile(const int32_t * starts, int n_seq, int
             t.index = tile - (base + __builtin_amdgcn_readlane(sum - own, l));
             t.first = __builtin_amdgcn_readlane(b, l);
             t.count = __builtin_amdgcn_readlane(n, l);
+            t.extra = __builtin_amdgcn_readlane(x, l);
             return t;
         }
         base += __builtin_amdgcn_readlane(sum, 63);
     }
-    return Tile{-1, 0, 0, 0};
+    return Tile{-1, 0, 0, 0, 0};
 }
 
 inline int type_bytes(int t) { return t == BONSAI_P40_F32 ? 4 : 2; }
