@@ -202,7 +202,7 @@ inline AttnPlan attn_plan(int64_t n_tok, int64_t n_seq, int64_t group, int64_t n
                           int64_t cus) {
     AttnPlan p;
     p.keys = n_tok * group <= 64 * n_seq;
-    const int64_t bm = p.keys ? 32 : rows, step = p.keys ? 128 : 64;
+    const int64_t bm = p.keys ? 32 : rows, step = p.keys && dim < 256 ? 128 : 64;
     const int64_t some = n_seq < n_tok ? n_seq : n_tok;
     p.tiles = n_tok * group / bm + some;
     int64_t want = 1;
@@ -224,7 +224,6 @@ inline AttnPlan attn_plan(int64_t n_tok, int64_t n_seq, int64_t group, int64_t n
     if (want < 1) want = 1;
     p.chunk = (max_kv + want * step - 1) / (want * step) * step;
     if (p.chunk < step) p.chunk = step;
-    if (p.keys && p.chunk < 2 * step) p.chunk = step;
     p.n_split = max_kv > p.chunk ? (max_kv + p.chunk - 1) / p.chunk : 1;
     return p;
 }
