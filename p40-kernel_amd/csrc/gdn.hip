@@ -51,17 +51,20 @@ struct GdnArgs {
 };
 
 // bytes of the workspace: per chunk and key head the fragments of K, Q and K^T,
-// per chunk and value head those of T and the masked QK^T and the row factors
-template <int K>
+// per chunk and value head those of T and the masked QK^T and the row factors.
+// Rows of 16-bit elements are one f16 term as they stand (but for the scaling and
+// what lies 2^14 below a row's largest, which rounds at 2^-25 of it).
+template <class T, int K>
 struct Work {
-    static constexpr int KF = C * K * 4;                  // 4 m-tiles x K/32 steps x 2 terms of 1 KB
+    static constexpr int TERMS = sizeof(typename T::elem) == 4 ? 2 : 1;
+    static constexpr int KF = C * K * 2 * TERMS;          // 4 m-tiles x K/32 steps x terms of 1 KB
     static constexpr int HEAD = 3 * KF;                   // K, Q, K^T
     static constexpr int TF = C * C * 4;
     static constexpr int VEC = 2048;                      // c1, cq, t, a, w: 64 floats each, then e^Gc
     static constexpr int VHEAD = 2 * TF + VEC;
 };
-inline int64_t work_bytes(int64_t chunks, int n_kh, int n_vh, int k_dim) {
-    const int64_t head = 3ll * C * k_dim * 4, vhead = 2ll * C * C * 4 + 2048;
+inline int64_t work_bytes(int64_t chunks, int n_kh, int n_vh, int k_dim, int elem) {
+    const int64_t head = 3ll * C * k_dim * (elem == 4 ? 4 : 2), vhead = 2ll * C * C * 4 + 2048;
     return chunks * (n_kh * head + n_vh * vhead);
 }
 
@@ -161,24 +164,26 @@ __device__ __forceinline__ void split(float x, _Float16 & hi, _Float16 & lo) {
     lo = (_Float16)(x - (float)hi);
 }
 
-// A workgroup per chunk and key head: K K^T and Q K^T once, then T and the masked
-// Q K^T of each of its value heads.  Bound by latencies (9 barriers a value head,
-// a triangular solve in four 16 x 16 blocks), so what counts is that two
-// workgroups share a CU: the C x C matrices take the place of K and Q in LDS.
+// A workgroup per chunk and key head: K K^T and Q K^T once, by 16 rows a wave, then
+// T and the masked Q K^T of its value heads, a wave each for up to 4 at a time: a
+// head alone on 4 waves is a chain of 7 barriers and of a triangular solve that
+// does not fill them.  The heads' C x C matrices take the place of K and Q in
+// LDS, so that two workgroups share a CU.
 template <class T, int K>
 __global__ void __launch_bounds__(256) gdn_prep_kernel(GdnArgs a) {
     typedef typename T::elem elem;
-    typedef Work<K> W;
+    typedef Work<T, K> W;
+    constexpr int TERMS = W::TERMS;
     constexpr int P = K + 8;                              // halves of a row: 16 rows of 16 bytes meet all banks
     constexpr int M = 68;                                 // floats of a row of the C x C matrices
     constexpr int SM = K / 32;
-    constexpr int PL = 4 * C * P * 2, LX = 2 * C * M * 4;
+    constexpr int PL = 2 * TERMS * C * P * 2, LX = 4 * C * M * 4;
     __shared__ __attribute__((aligned(16))) uint8_t lds[PL > LX ? PL : LX];
-    _Float16 (* const pl)[C][P] = reinterpret_cast<_Float16 (*)[C][P]>(lds);      // K hi, lo, Q hi, lo
-    float (* const L)[M] = reinterpret_cast<float (*)[M]>(lds), (* const X)[M] = L + C;
+    _Float16 (* const pl)[C][P] = reinterpret_cast<_Float16 (*)[C][P]>(lds);      // K's terms, Q's terms
+    float (* const mat)[C][M] = reinterpret_cast<float (*)[C][M]>(lds);           // one a value head
     __shared__ float tmp[4][16][17];
     __shared__ double G[4][C];
-    __shared__ float fk[C], fq[C], bt[4][C], rt[C], ra[C];
+    __shared__ float fk[C], fq[C], bt[4][C], ra[4][C], rt[4][C];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, g = lane >> 4;
     const int hk = blockIdx.x % a.n_kh, chunk = blockIdx.x / a.n_kh, per = a.n_vh / a.n_kh;
@@ -191,16 +196,20 @@ __global__ void __launch_bounds__(256) gdn_prep_kernel(GdnArgs a) {
     {
         constexpr int N = K / 4;
         const int row = tid >> 2, part = tid & 3;
+        float x[2][N];
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-            float x[N] = {};
             const elem * const p = reinterpret_cast<const elem *>(m ? a.q : a.k);
-            if (row < nt) load_n<T>(p + (int64_t)(t0 + row) * (m ? a.q_tok : a.k_tok) + (int64_t)hk * K + part * N, x);
+            load_n<T>(p + (int64_t)(t0 + min(row, nt - 1)) * (m ? a.q_tok : a.k_tok) + (int64_t)hk * K + part * N, x[m]);
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
             float ss = 0.0f, big = 0.0f;
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                ss = fmaf(x[j], x[j], ss);
-                big = fmaxf(big, fabsf(x[j]));
+                if (row >= nt) x[m][j] = 0.0f;
+                ss = fmaf(x[m][j], x[m][j], ss);
+                big = fmaxf(big, fabsf(x[m][j]));
             }
             ss += __shfl_xor(ss, 1);
             ss += __shfl_xor(ss, 2);
@@ -212,7 +221,18 @@ __global__ void __launch_bounds__(256) gdn_prep_kernel(GdnArgs a) {
             if (part == 0) (m ? fq : fk)[row] = f;
             const float down = pow2(-e);
 #pragma unroll
-            for (int j = 0; j < N; ++j) split(x[j] * down, pl[2 * m][row][part * N + j], pl[2 * m + 1][row][part * N + j]);
+            for (int j = 0; j < N; j += 8) {
+                v8h hi, lo;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    _Float16 h, l;
+                    split(x[m][j + i] * down, h, l);
+                    hi[i] = h;
+                    lo[i] = l;
+                }
+                *reinterpret_cast<v8h *>(&pl[TERMS * m][row][part * N + j]) = hi;
+                if (TERMS == 2) *reinterpret_cast<v8h *>(&pl[TERMS * m + 1][row][part * N + j]) = lo;
+            }
         }
     }
     __syncthreads();
@@ -220,13 +240,13 @@ __global__ void __launch_bounds__(256) gdn_prep_kernel(GdnArgs a) {
     // rows 16 wave .. of K K^T and Q K^T (element: column 16 n + l16, row 16 wave + 4 g + r), without the rows' factors
     v4f kk[4], qk[4];
     {
-        v8h ka[SM][2], qa[SM][2];
+        v8h ka[SM][TERMS], qa[SM][TERMS];
 #pragma unroll
         for (int s = 0; s < SM; ++s)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
+            for (int k = 0; k < TERMS; ++k) {
                 ka[s][k] = *reinterpret_cast<const v8h *>(&pl[k][16 * wave + l16][32 * s + 8 * g]);
-                qa[s][k] = *reinterpret_cast<const v8h *>(&pl[2 + k][16 * wave + l16][32 * s + 8 * g]);
+                qa[s][k] = *reinterpret_cast<const v8h *>(&pl[TERMS + k][16 * wave + l16][32 * s + 8 * g]);
             }
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
@@ -235,11 +255,13 @@ __global__ void __launch_bounds__(256) gdn_prep_kernel(GdnArgs a) {
 #pragma unroll
                 for (int s = 0; s < SM; ++s) {
                     const v8h bh = *reinterpret_cast<const v8h *>(&pl[0][16 * n + l16][32 * s + 8 * g]);
-                    const v8h bl = *reinterpret_cast<const v8h *>(&pl[1][16 * n + l16][32 * s + 8 * g]);
-                    kk[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[s][1], bh, kk[n], 0, 0, 0);
-                    qk[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qa[s][1], bh, qk[n], 0, 0, 0);
-                    kk[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[s][0], bl, kk[n], 0, 0, 0);
-                    qk[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qa[s][0], bl, qk[n], 0, 0, 0);
+                    if constexpr (TERMS == 2) {
+                        const v8h bl = *reinterpret_cast<const v8h *>(&pl[1][16 * n + l16][32 * s + 8 * g]);
+                        kk[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[s][1], bh, kk[n], 0, 0, 0);
+                        qk[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qa[s][1], bh, qk[n], 0, 0, 0);
+                        kk[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[s][0], bl, kk[n], 0, 0, 0);
+                        qk[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qa[s][0], bl, qk[n], 0, 0, 0);
+                    }
                     kk[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[s][0], bh, kk[n], 0, 0, 0);
                     qk[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qa[s][0], bh, qk[n], 0, 0, 0);
                 }
@@ -247,37 +269,42 @@ __global__ void __launch_bounds__(256) gdn_prep_kernel(GdnArgs a) {
         }
     }
     // the fragments of K, Q (m-tile of 16 tokens, steps of 32 dims) and K^T (m-tile of 16 dims, steps of 32 tokens)
+    typedef _Float16 v4h __attribute__((ext_vector_type(4)));
     for (int f = wave; f < 4 * SM; f += 4) {
         const int mt = f / SM, ks = f % SM, row = 16 * mt + l16;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            v8h x;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = pl[k][row][32 * ks + (j < 4 ? 4 * g + j : 12 + 4 * g + j)];
-            *reinterpret_cast<v8h *>(wk + (k >> 1) * W::KF + (2 * f + (k & 1)) * 1024 + 16 * lane) = x;
+        for (int k = 0; k < 2 * TERMS; ++k) {
+            const v4h x = *reinterpret_cast<const v4h *>(&pl[k][row][32 * ks + 4 * g]);
+            const v4h y = *reinterpret_cast<const v4h *>(&pl[k][row][32 * ks + 16 + 4 * g]);
+            *reinterpret_cast<v8h *>(wk + (k / TERMS) * W::KF + (TERMS * f + k % TERMS) * 1024 + 16 * lane) =
+                __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
         }
     }
     for (int f = wave; f < K / 8; f += 4) {
         const int mt = f >> 1, ks = f & 1, dim = 16 * mt + l16;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
+        for (int k = 0; k < TERMS; ++k) {
             v8h x;
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[j] = pl[k][32 * ks + (j < 4 ? 4 * g + j : 12 + 4 * g + j)][dim];
-            *reinterpret_cast<v8h *>(wk + 2 * W::KF + (2 * f + k) * 1024 + 16 * lane) = x;
+            *reinterpret_cast<v8h *>(wk + 2 * W::KF + (TERMS * f + k) * 1024 + 16 * lane) = x;
         }
     }
 
-    // a C x C matrix in LDS as fragments (m-tile mt, step ks)
-    auto put_square = [&](const float (*m)[M], const float * scale, uint8_t * to) {
-        for (int f = wave; f < 8; f += 4) {
+    // this wave's C x C matrix as fragments (m-tile mt, step ks), its rows divided by scale
+    float (* const X)[M] = mat[wave];
+    auto put_square = [&](const float * scale, uint8_t * to) {
+#pragma unroll 2
+        for (int f = 0; f < 8; ++f) {
             const int mt = f >> 1, ks = f & 1, row = 16 * mt + l16;
             const float down = 1.0f / scale[row];
+            const v4f x = *reinterpret_cast<const v4f *>(&X[row][32 * ks + 4 * g]);
+            const v4f y = *reinterpret_cast<const v4f *>(&X[row][32 * ks + 16 + 4 * g]);
             v8h hi, lo;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 _Float16 h, l;
-                split(m[row][32 * ks + (j < 4 ? 4 * g + j : 12 + 4 * g + j)] * down, h, l);
+                split((j < 4 ? x[j & 3] : y[j & 3]) * down, h, l);
                 hi[j] = h;
                 lo[j] = l;
             }
@@ -285,121 +312,139 @@ __global__ void __launch_bounds__(256) gdn_prep_kernel(GdnArgs a) {
             *reinterpret_cast<v8h *>(to + (2 * f + 1) * 1024 + 16 * lane) = lo;
         }
     };
+    auto in_wave = []() __attribute__((always_inline)) { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };   // other lanes read it
 #pragma unroll 1
-    for (int r = 0; r < per; ++r) {
-        auto head = [&](int r) { return a.tiled ? hk + r * a.n_kh : hk * per + r; };
-        const int hv = head(r), q4 = r & 3;
-        uint8_t * const wv = a.ws + (int64_t)a.chunks * a.n_kh * W::HEAD + ((int64_t)chunk * a.n_vh + hv) * W::VHEAD;
-        if (q4 == 0) {
-            // the sums of g of up to 4 heads, a wave each, in fp64
-            if (r + wave < per) {
-                const int h = head(r + wave);
-                double s = lane < nt ? (double)gate(a.g[(int64_t)(t0 + lane) * a.gate_tok + h]) : 0.0;
+    for (int r0 = 0; r0 < per; r0 += 4) {
+        const int heads = min(4, per - r0);
+        auto head = [&](int r) { return a.tiled ? hk + (r0 + r) * a.n_kh : hk * per + r0 + r; };
+        const bool mine = wave < heads;
+        uint8_t * const wv = a.ws + (int64_t)a.chunks * a.n_kh * W::HEAD +
+                             ((int64_t)chunk * a.n_vh + head(mine ? wave : 0)) * W::VHEAD;
+        if (mine) {
+            // the sums of g, in fp64
+            const int h = head(wave);
+            double s = lane < nt ? (double)gate(a.g[(int64_t)(t0 + lane) * a.gate_tok + h]) : 0.0;
+            const float beta = lane < nt ? a.beta[(int64_t)(t0 + lane) * a.gate_tok + h] : 0.0f;
 #pragma unroll
-                for (int d = 1; d < 64; d <<= 1) {
-                    const double o = __shfl_up(s, d);
-                    if (lane >= d) s += o;
+            for (int d = 1; d < 64; d <<= 1) {
+                const double o = __shfl_up(s, d);
+                if (lane >= d) s += o;
+            }
+            G[wave][lane] = s;
+            bt[wave][lane] = beta;
+        }
+        __syncthreads();                                  // (and: K and Q, or the last heads' matrices, have been read)
+
+        // rows 16 wave .. of every head's matrix: Q K^T with its decay, then L
+        auto rows = [&](auto is_l) __attribute__((always_inline)) {
+            constexpr bool LL = decltype(is_l)::value;
+#pragma unroll 1
+            for (int r = 0; r < heads; ++r) {
+                float top[4] = {};
+                double Gi[4];
+                float fi[4];
+#pragma unroll
+                for (int i4 = 0; i4 < 4; ++i4) {
+                    const int i = 16 * wave + 4 * g + i4;
+                    Gi[i4] = G[r][i];
+                    fi[i4] = LL ? bt[r][i] * fk[i] : a.scale * fq[i];
                 }
-                G[wave][lane] = s;
-                bt[wave][lane] = lane < nt ? a.beta[(int64_t)(t0 + lane) * a.gate_tok + h] : 0.0f;
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    const int j = 16 * n + l16;
+                    const double Gj = G[r][j];
+                    const float fj = fk[j];
+#pragma unroll
+                    for (int i4 = 0; i4 < 4; ++i4) {
+                        const int i = 16 * wave + 4 * g + i4;
+                        const bool in = LL ? j < i : j <= i;
+                        const float d = expf(in ? (float)(Gi[i4] - Gj) : 0.0f);
+                        const float x = in ? (LL ? kk : qk)[n][i4] * fi[i4] * fj * d : 0.0f;
+                        mat[r][i][j] = x;
+                        top[i4] = fmaxf(top[i4], fabsf(x));
+                    }
+                }
+                if (!LL)
+#pragma unroll
+                    for (int i4 = 0; i4 < 4; ++i4) {
+#pragma unroll
+                        for (int d = 1; d < 16; d <<= 1) top[i4] = fmaxf(top[i4], __shfl_xor(top[i4], d));
+                        if (l16 == 0) ra[r][16 * wave + 4 * g + i4] = pow2(exponent(top[i4]));
+                    }
             }
-        }
-        __syncthreads();                                  // (and: K and Q have been read, or the last head's X)
-
-        // L, and Q K^T with its decay in X
-        float top[4] = {};
+        };
+        rows(std::false_type{});
+        __syncthreads();
+        if (mine) put_square(ra[wave], wv + W::TF);
+        __syncthreads();
+        rows(std::true_type{});
+        __syncthreads();
+        if (mine) {
+            // X = (I + L)^-1 in L's place.  Diagonal blocks of 16 (block g: a lane per column): forward substitution
+            {
+                float x[16];
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-            const int j = 16 * n + l16;
-            const double Gj = G[q4][j];
-            const float fj = fk[j];
+                for (int i = 0; i < 16; ++i) {
+                    float s = l16 == i ? 1.0f : 0.0f;
 #pragma unroll
-            for (int i4 = 0; i4 < 4; ++i4) {
-                const int i = 16 * wave + 4 * g + i4;
-                const float d = j <= i ? expf((float)(G[q4][i] - Gj)) : 0.0f;
-                L[i][j] = j < i ? bt[q4][i] * (kk[n][i4] * fk[i] * fj) * d : 0.0f;
-                const float x = j <= i ? a.scale * (qk[n][i4] * fq[i] * fj) * d : 0.0f;
-                X[i][j] = x;
-                top[i4] = fmaxf(top[i4], fabsf(x));
+                    for (int l = 0; l < i; ++l) s = fmaf(-X[16 * g + i][16 * g + l], x[l], s);
+                    x[i] = s;
+                }
+                in_wave();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) X[16 * g + i][16 * g + l16] = x[i];
+                in_wave();
             }
-        }
+            // below it, column by column: X_ij = -X_ii sum_l L_il X_lj.  A column of L is not needed once its X is there
+#pragma unroll 1
+            for (int j = 0; j < 3; ++j)
+#pragma unroll 1
+                for (int i = j + 1; i < 4; ++i) {
+                    v4f s = {};
+                    for (int l = j; l < i; ++l)
 #pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4) {
+                        for (int k = 0; k < 4; ++k)
+                            s = __builtin_amdgcn_mfma_f32_16x16x4f32(X[16 * i + l16][16 * l + 4 * k + g],
+                                                                     X[16 * l + 4 * k + g][16 * j + l16], s, 0, 0, 0);
 #pragma unroll
-            for (int d = 1; d < 16; d <<= 1) top[i4] = fmaxf(top[i4], __shfl_xor(top[i4], d));
-            if (l16 == 0) ra[16 * wave + 4 * g + i4] = pow2(exponent(top[i4]));
-        }
-        __syncthreads();
-        put_square(X, ra, wv + W::TF);
-        __syncthreads();                                  // X is free
-
-        // X = (I + L)^-1.  Diagonal blocks of 16: a lane per column, forward substitution
-        {
-            float x[16];
+                    for (int i4 = 0; i4 < 4; ++i4) tmp[wave][4 * g + i4][l16] = s[i4];
+                    in_wave();
+                    v4f x = {};
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                float s = l16 == i ? 1.0f : 0.0f;
+                    for (int k = 0; k < 4; ++k)
+                        x = __builtin_amdgcn_mfma_f32_16x16x4f32(X[16 * i + l16][16 * i + 4 * k + g],
+                                                                 tmp[wave][4 * k + g][l16], x, 0, 0, 0);
 #pragma unroll
-                for (int l = 0; l < i; ++l) s = fmaf(-L[16 * wave + i][16 * wave + l], x[l], s);
-                x[i] = s;
-            }
-            if (g == 0)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) X[16 * wave + i][16 * wave + l16] = x[i];
-            // what is above the diagonal
-            for (int n = wave + 1; n < 4; ++n)
-#pragma unroll
-                for (int i4 = 0; i4 < 4; ++i4) X[16 * wave + 4 * g + i4][16 * n + l16] = 0.0f;
-        }
-        __syncthreads();
-        // below it, wave j has block column j: X_ij = -X_ii sum_l L_il X_lj
-        for (int i = wave + 1; i < 4; ++i) {
-            v4f s = {};
-            for (int l = wave; l < i; ++l)
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    s = __builtin_amdgcn_mfma_f32_16x16x4f32(L[16 * i + l16][16 * l + 4 * k + g],
-                                                             X[16 * l + 4 * k + g][16 * wave + l16], s, 0, 0, 0);
-#pragma unroll
-            for (int i4 = 0; i4 < 4; ++i4) tmp[wave][4 * g + i4][l16] = s[i4];
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // other lanes read it
-            v4f x = {};
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                x = __builtin_amdgcn_mfma_f32_16x16x4f32(X[16 * i + l16][16 * i + 4 * k + g], tmp[wave][4 * k + g][l16], x, 0, 0, 0);
-#pragma unroll
-            for (int i4 = 0; i4 < 4; ++i4) X[16 * i + 4 * g + i4][16 * wave + l16] = -x[i4];
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        }
-        __syncthreads();
-        // T = X diag(beta), and the largest element of its rows
-        {
-            const int row = tid >> 2, part = tid & 3;
+                    for (int i4 = 0; i4 < 4; ++i4) X[16 * i + 4 * g + i4][16 * j + l16] = -x[i4];
+                    in_wave();
+                }
+            // T = X diag(beta), and the largest element of its rows (a lane each)
             float big = 0.0f;
-            for (int j = part; j < C; j += 4) {
-                const float x = X[row][j] * bt[q4][j];
-                X[row][j] = x;
-                big = fmaxf(big, fabsf(x));
+#pragma unroll 4
+            for (int j = 0; j < C; j += 4) {
+                v4f x = *reinterpret_cast<const v4f *>(&X[lane][j]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    x[k] *= bt[wave][j + k];
+                    big = fmaxf(big, fabsf(x[k]));
+                }
+                *reinterpret_cast<v4f *>(&X[lane][j]) = x;
             }
-            big = fmaxf(big, __shfl_xor(big, 1));
-            big = fmaxf(big, __shfl_xor(big, 2));
-            if (part == 0) rt[row] = pow2(exponent(big));
-        }
-        __syncthreads();
-        put_square(X, rt, wv);
-        // factors of the rows
-        if (tid < C) {
+            rt[wave][lane] = pow2(exponent(big));
+            in_wave();
+            put_square(rt[wave], wv);
+            // factors of the rows
             float * const vec = reinterpret_cast<float *>(wv + 2 * W::TF);
-            const double Gi = G[q4][tid], Ge = G[q4][C - 1];
+            const double Gi = G[wave][lane], Ge = G[wave][C - 1];
             const float e = expf((float)Gi);
-            vec[tid] = e * fk[tid];
-            vec[C + tid] = e * fq[tid] * a.scale;
-            vec[2 * C + tid] = rt[tid];
-            vec[3 * C + tid] = ra[tid];
-            vec[4 * C + tid] = expf((float)(Ge - Gi)) * fk[tid];
-            vec[5 * C + tid] = expf((float)Ge);
+            vec[lane] = e * fk[lane];
+            vec[C + lane] = e * fq[lane] * a.scale;
+            vec[2 * C + lane] = rt[wave][lane];
+            vec[3 * C + lane] = ra[wave][lane];
+            vec[4 * C + lane] = expf((float)(Ge - Gi)) * fk[lane];
+            vec[5 * C + lane] = expf((float)Ge);
         }
-        if (q4 == 3) __syncthreads();                     // G and bt are written anew
+        if (r0 + 4 < per) __syncthreads();                // G, bt and the matrices are written anew
     }
 }
 
@@ -429,7 +474,7 @@ __device__ __forceinline__ float largest(const v4f (&x)[N]) {
 template <class T, int K, int NW>
 __global__ void __launch_bounds__(64 * NW) gdn_scan_kernel(GdnArgs a) {
     typedef typename T::elem elem;
-    typedef Work<K> W;
+    typedef Work<T, K> W;
     constexpr int KS = K / 32, KT = K / 16;
     typedef elem Unit __attribute__((ext_vector_type(16 / sizeof(elem))));
     constexpr int REG1 = 2 * W::KF, REG2 = W::KF + W::VHEAD, OWN = C * 16 * sizeof(elem);
@@ -499,7 +544,8 @@ __global__ void __launch_bounds__(64 * NW) gdn_scan_kernel(GdnArgs a) {
     struct Left {
         v8h h[2], l[2];
     };
-    auto products = [&](auto count, auto place, auto use) __attribute__((always_inline)) {
+    constexpr int TERMS = W::TERMS;
+    auto products = [&](auto count, auto terms, auto place, auto use) __attribute__((always_inline)) {
         constexpr int N = decltype(count)::value;
         Left f[AHEAD];
         auto read = [&](int i) __attribute__((always_inline)) {
@@ -507,7 +553,7 @@ __global__ void __launch_bounds__(64 * NW) gdn_scan_kernel(GdnArgs a) {
             for (int k = 0; k < 2; ++k) {
                 const uint8_t * const p = place(i, k) + 16 * lane;
                 f[i % AHEAD].h[k] = *reinterpret_cast<const v8h *>(p);
-                f[i % AHEAD].l[k] = *reinterpret_cast<const v8h *>(p + 1024);
+                if (decltype(terms)::value == 2) f[i % AHEAD].l[k] = *reinterpret_cast<const v8h *>(p + 1024);
             }
         };
 #pragma unroll
@@ -519,9 +565,13 @@ __global__ void __launch_bounds__(64 * NW) gdn_scan_kernel(GdnArgs a) {
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    auto mul = [](const Left & f, const v8h & hi, const v8h & lo, v4f & a, v4f & b) __attribute__((always_inline)) {
-        a = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.l[0], hi, a, 0, 0, 0);
-        b = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.l[1], hi, b, 0, 0, 0);
+    const std::integral_constant<int, TERMS> own_terms;   // of K and Q
+    const std::integral_constant<int, 2> two;
+    auto mul = [](auto terms, const Left & f, const v8h & hi, const v8h & lo, v4f & a, v4f & b) __attribute__((always_inline)) {
+        if constexpr (decltype(terms)::value == 2) {
+            a = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.l[0], hi, a, 0, 0, 0);
+            b = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.l[1], hi, b, 0, 0, 0);
+        }
         a = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h[0], lo, a, 0, 0, 0);
         b = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h[1], lo, b, 0, 0, 0);
         a = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h[0], hi, a, 0, 0, 0);
@@ -589,11 +639,11 @@ __global__ void __launch_bounds__(64 * NW) gdn_scan_kernel(GdnArgs a) {
         to_right(S[1], down, sh[0], sl[0], 1);
 #pragma unroll
         for (int m = 0; m < 4; ++m) ks[m] = qs[m] = v4f{};
-        products(std::integral_constant<int, 4 * KS>{},
-                 [&](int i, int k) __attribute__((always_inline)) { return r1 + k * W::KF + 2 * (i % 4 * KS + i / 4) * 1024; },
+        products(std::integral_constant<int, 4 * KS>{}, own_terms,
+                 [&](int i, int k) __attribute__((always_inline)) { return r1 + k * W::KF + TERMS * (i % 4 * KS + i / 4) * 1024; },
                  [&](int i, const Left & f) __attribute__((always_inline)) {
                      const int s = i / 4, m = i % 4;
-                     mul(f, sh[s & 1], sl[s & 1], ks[m], qs[m]);
+                     mul(own_terms, f, sh[s & 1], sl[s & 1], ks[m], qs[m]);
                      // the next step's right operand, between the products
                      if (m < 2 && s + 1 < KS) to_right(S[2 * s + 2 + m], down, sh[(s + 1) & 1], sl[(s + 1) & 1], m);
                  });
@@ -625,10 +675,10 @@ __global__ void __launch_bounds__(64 * NW) gdn_scan_kernel(GdnArgs a) {
         to_right(R[0], down, rh[0], rl[0], 0);
         to_right(R[1], down, rh[0], rl[0], 1);
         auto square = [&](const uint8_t * base, const v4f (&right)[4], float down) __attribute__((always_inline)) {
-            products(std::integral_constant<int, 3>{}, [&](int i, int k) __attribute__((always_inline)) { return place(base, i, k); },
+            products(std::integral_constant<int, 3>{}, two, [&](int i, int k) __attribute__((always_inline)) { return place(base, i, k); },
                      [&](int i, const Left & f) __attribute__((always_inline)) {
                          const int m = i == 0 ? 0 : 2, s = i / 2;
-                         mul(f, rh[s], rl[s], x[m], x[m + 1]);
+                         mul(two, f, rh[s], rl[s], x[m], x[m + 1]);
                          if (i < 2) to_right(right[2 + i], down, rh[1], rl[1], i);
                      });
         };
@@ -662,11 +712,11 @@ __global__ void __launch_bounds__(64 * NW) gdn_scan_kernel(GdnArgs a) {
         for (int m = 0; m < 4; ++m) to_right(Um[m], down, rh[m / 2], rl[m / 2], m & 1);
         float top[2] = {0.0f, 0.0f};
         v4f y[2];
-        products(std::integral_constant<int, KT>{},
-                 [&](int i, int k) __attribute__((always_inline)) { return r2 + 2 * (2 * (2 * (i / 2) + k) + (i & 1)) * 1024; },
+        products(std::integral_constant<int, KT>{}, own_terms,
+                 [&](int i, int k) __attribute__((always_inline)) { return r2 + TERMS * (2 * (2 * (i / 2) + k) + (i & 1)) * 1024; },
                  [&](int i, const Left & f) __attribute__((always_inline)) {
                      if (!(i & 1)) y[0] = y[1] = v4f{};
-                     mul(f, rh[i & 1], rl[i & 1], y[0], y[1]);
+                     mul(own_terms, f, rh[i & 1], rl[i & 1], y[0], y[1]);
                      if (i & 1)
 #pragma unroll
                          for (int k = 0; k < 2; ++k)
@@ -707,12 +757,9 @@ int launch(const GdnArgs & a, bool chunked, hipStream_t s) {
     hipLaunchKernelGGL((gdn_prep_kernel<T, K>), dim3((unsigned)((int64_t)a.chunks * a.n_kh)), dim3(256), 0, s, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
-    // 32 columns a workgroup as long as each has a CU of its own, then 64
     // (8 key heads at a time, those that there are not return)
-    const int64_t heads = (int64_t)a.n_seq * (a.n_vh / a.n_kh) * ((a.n_kh + 7) / 8 * 8), few = heads * ((a.vd + 31) / 32);
-    if ((int64_t)a.n_seq * a.n_vh * ((a.vd + 31) / 32) <= pq2host::device_info().cus)
-        hipLaunchKernelGGL((gdn_scan_kernel<T, K, 2>), dim3((unsigned)few), dim3(128), 0, s, a);
-    else hipLaunchKernelGGL((gdn_scan_kernel<T, K, 4>), dim3((unsigned)(heads * ((a.vd + 63) / 64))), dim3(256), 0, s, a);
+    const int64_t heads = (int64_t)a.n_seq * (a.n_vh / a.n_kh) * ((a.n_kh + 7) / 8 * 8);
+    hipLaunchKernelGGL((gdn_scan_kernel<T, K, 4>), dim3((unsigned)(heads * ((a.vd + 63) / 64))), dim3(256), 0, s, a);
     return (int)hipGetLastError();
 }
 template <class T>
@@ -746,7 +793,7 @@ bool chunked(const bonsai_p40_gdn_args * p) {
 }  // namespace
 
 extern "C" int64_t bonsai_p40_gdn_workspace_bytes(const bonsai_p40_gdn_args * p) {
-    return check(p) == -1 && chunked(p) ? work_bytes(chunks_of(p), p->n_k_head, p->n_v_head, p->k_dim) : 0;
+    return check(p) == -1 && chunked(p) ? work_bytes(chunks_of(p), p->n_k_head, p->n_v_head, p->k_dim, type_bytes(p->type)) : 0;
 }
 
 extern "C" int bonsai_p40_gdn(const bonsai_p40_gdn_args * p, bonsai_stream stream) {
@@ -761,7 +808,7 @@ extern "C" int bonsai_p40_gdn(const bonsai_p40_gdn_args * p, bonsai_stream strea
         !aligned(p->slots, 4) || !aligned(p->workspace, 16))
         return 1;
     const bool ch = p->workspace != nullptr && chunked(p);
-    if (ch && p->workspace_bytes < work_bytes(chunks_of(p), p->n_k_head, p->n_v_head, p->k_dim)) return 1;
+    if (ch && p->workspace_bytes < work_bytes(chunks_of(p), p->n_k_head, p->n_v_head, p->k_dim, type_bytes(p->type))) return 1;
     GdnArgs a;
     a.q = p->q;
     a.k = p->k;
