@@ -18,14 +18,16 @@
 //   The outputs are fp32's, so the products are, too: each operand is split into
 // two f16 terms (22 bits; rows of the left, columns of the right operand scaled by
 // powers of two so that f16's range does not matter) and the products hi hi,
-// hi lo and lo hi run on v_mfma_f32_16x16x32_f16, 5 times the rate of fp32's own
-// matrix instructions.  G is summed and subtracted in fp64: after a strong decay
+// hi lo and lo hi run on v_mfma_f32_16x16x32_f16, the three of them at 5 times the
+// rate of fp32's own matrix instructions.  G is summed and subtracted in fp64: after a strong decay
 // the differences of fp32 sums would have no digits left.
 //   In the scan a wave has 16 columns of S, R and U to itself: a result tile
 // (lane: column, 4 rows 4 g .. 4 g + 3) is the next product's right operand as it
 // stands, if the left one lists its contraction as 4 g + j, 16 + 4 g + j (j < 4).
 // So nothing of the chain passes through LDS; that holds the left operands, which
-// prep writes in the order in which the lanes read them (1 KB a fragment).
+// prep writes in the order in which the lanes read them (1 KB a fragment), and what
+// the waves that make the outputs take from the chain's.
+#include "gemv_device.h"
 #include "host_state.h"
 #include "launch_rules.h"
 #include "mixer_device.h"
@@ -59,12 +61,12 @@ struct Work {
     static constexpr int TERMS = sizeof(typename T::elem) == 4 ? 2 : 1;
     static constexpr int KF = C * K * 2 * TERMS;          // 4 m-tiles x K/32 steps x terms of 1 KB
     static constexpr int HEAD = 3 * KF;                   // K, Q, K^T
-    static constexpr int TF = C * C * 4;
+    static constexpr int TF = C * C * 3;                  // 6 of the 8 fragments: 32 x 32 above the diagonal are 0
     static constexpr int VEC = 2048;                      // c1, cq, t, a, w: 64 floats each, then e^Gc
     static constexpr int VHEAD = 2 * TF + VEC;
 };
 inline int64_t work_bytes(int64_t chunks, int n_kh, int n_vh, int k_dim, int elem) {
-    const int64_t head = 3ll * C * k_dim * (elem == 4 ? 4 : 2), vhead = 2ll * C * C * 4 + 2048;
+    const int64_t head = 3ll * C * k_dim * (elem == 4 ? 4 : 2), vhead = 2ll * C * C * 3 + 2048;
     return chunks * (n_kh * head + n_vh * vhead);
 }
 
@@ -295,8 +297,8 @@ __global__ void __launch_bounds__(256) gdn_prep_kernel(GdnArgs a) {
     float (* const X)[M] = mat[wave];
     auto put_square = [&](const float * scale, uint8_t * to) {
 #pragma unroll 2
-        for (int f = 0; f < 8; ++f) {
-            const int mt = f >> 1, ks = f & 1, row = 16 * mt + l16;
+        for (int f = 0; f < 6; ++f) {
+            const int mt = f < 4 ? f : f - 2, ks = f >> 2, row = 16 * mt + l16;
             const float down = 1.0f / scale[row];
             const v4f x = *reinterpret_cast<const v4f *>(&X[row][32 * ks + 4 * g]);
             const v4f y = *reinterpret_cast<const v4f *>(&X[row][32 * ks + 16 + 4 * g]);
@@ -470,19 +472,38 @@ __device__ __forceinline__ float largest(const v4f (&x)[N]) {
     return over_column(fmaxf(big[0], big[1]));
 }
 
-// NW waves of 16 columns each
-template <class T, int K, int NW>
-__global__ void __launch_bounds__(64 * NW) gdn_scan_kernel(GdnArgs a) {
+// 16 PAIRS columns of a value head, 16 for each pair of waves, of which one has
+// the chain, the other the outputs, a phase behind it:
+//   first:  S as operands, K S    | QK^T U of the last chunk, its outputs
+//   second: U                     | Q S
+//   third:  S                     |
+// S as operands and U go from the one to the other through LDS.  A chunk's 180
+// products (16-bit rows: 132) of 16 columns are 2900 clocks of MFMA; what bounds it
+// is the chain of dependent instructions around them (largest of a column, split,
+// convert, rescale).  One wave that does both takes 11000 clocks a chunk, two 8900.
+//   K, Q and K^T of a chunk follow one another through two buffers, each asked for
+// a phase ahead: with a third one PAIRS = 4 would not fit beside fp32's fragments,
+// and it gains nothing (2048 tokens of one sequence, us: 150 against 153).
+//   2 pairs or 4 (half the fragments' bytes through LDS, two waves to a SIMD):
+// gdn_wide.  MI355X, 48 value heads, 128 x 128, fp32, both kernels: 2048 tokens
+// 150 us, 8 sequences of 2048 749 us, that is 1.4 TB/s of K, Q, V and outputs.
+template <class T, int K, int PAIRS>
+__global__ void __launch_bounds__(128 * PAIRS) gdn_scan_kernel(GdnArgs a) {
     typedef typename T::elem elem;
     typedef Work<T, K> W;
-    constexpr int KS = K / 32, KT = K / 16;
     typedef elem Unit __attribute__((ext_vector_type(16 / sizeof(elem))));
-    constexpr int REG1 = 2 * W::KF, REG2 = W::KF + W::VHEAD, OWN = C * 16 * sizeof(elem);
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[REG1 + REG2 + NW * OWN];
+    constexpr int KS = K / 32, KT = K / 16, NW = 2 * PAIRS, TERMS = W::TERMS;
+    constexpr int EB = sizeof(elem), UNITS = EB, RPI = 64 / UNITS;    // 16-byte units of 16 columns; rows of a load
+    // LDS: K, Q and K^T in two buffers in turn, T, QK^T, factors; then for each pair V, U (and outputs), S as operands and its scale
+    constexpr int AT_T = 2 * W::KF, AT_A = AT_T + W::TF, AT_VEC = AT_A + W::TF;
+    constexpr int AT_V = AT_VEC + W::VEC, V_PAIR = C * 16 * EB, AT_U = AT_V + PAIRS * V_PAIR, U_PAIR = C * 16 * 4;
+    constexpr int AT_S = AT_U + PAIRS * U_PAIR, S_PAIR = 2 * KS * 1024 + 256;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[AT_S + PAIRS * S_PAIR];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int l16 = lane & 15, g = lane >> 4;
+    const int l16 = lane & 15, g = lane >> 4, pair = wave % PAIRS;
+    const bool chain = wave < PAIRS;
     // a key head's workgroups, which share fragments, on one XCD (workgroups go to the 8 in turn)
-    const int groups = (a.vd + 16 * NW - 1) / (16 * NW), per = a.n_vh / a.n_kh;
+    const int groups = (a.vd + 16 * PAIRS - 1) / (16 * PAIRS), per = a.n_vh / a.n_kh;
     int hk = blockIdx.x & 7, rest = blockIdx.x >> 3;
     const int group = rest % groups;
     rest /= groups;
@@ -492,10 +513,10 @@ __global__ void __launch_bounds__(64 * NW) gdn_scan_kernel(GdnArgs a) {
     hk += 8 * (rest % eighth);
     if (hk >= a.n_kh) return;
     const int hv = a.tiled ? hk + head * a.n_kh : hk * per + head;
-    const int col0 = 16 * (NW * group + wave);
+    const int col0 = 16 * (PAIRS * group + pair);
     const int64_t slot = slot_of(a, seq);
     if (slot < 0) return;
-    const bool work = col0 < a.vd;                        // the others stage
+    const bool work = col0 < a.vd;                        // the others load
     const int col = work ? col0 + l16 : 0;
     const int first = iclamp(sload(a.starts, seq), 0, a.n_tok);
     const int count = max(iclamp(sload(a.starts, seq + 1), 0, a.n_tok) - first, 0);
@@ -509,73 +530,74 @@ __global__ void __launch_bounds__(64 * NW) gdn_scan_kernel(GdnArgs a) {
     chunk0 = __builtin_amdgcn_readfirstlane(chunk0);
     chunks = iclamp(chunks, 0, max(a.chunks - chunk0, 0));   // starts that overlap: what prep made, no more
 
-    // 1 KB an instruction, the waves in turn
+    // a run of 1 KB pieces for each wave, 4 of them an address
     auto copy = [&](const uint8_t * src, uint8_t * dst, auto bytes) __attribute__((always_inline)) {
-        constexpr int N = decltype(bytes)::value / 1024;
+        constexpr int N = decltype(bytes)::value / 1024, OWN1 = N / NW;
         const auto from = buffer_of(src, N * 1024);
 #pragma unroll
-        for (int i = 0; i < N; i += NW)
-            if (N % NW == 0 || i + wave < N) dma16(from, dst + (i + wave) * 1024, 16 * lane, (i + wave) * 1024);
+        for (int i = 0; i < OWN1; i += 4) {
+            const int at = (wave * OWN1 + i) * 1024;
+            dma16_at<0>(from, dst + at, 16 * lane, at);
+            if (i + 1 < OWN1) dma16_at<1024>(from, dst + at, 16 * lane, at);
+            if (i + 2 < OWN1) dma16_at<2048>(from, dst + at, 16 * lane, at);
+            if (i + 3 < OWN1) dma16_at<3072>(from, dst + at, 16 * lane, at);
+        }
+        if (N % NW != 0 && wave < N % NW) {
+            const int at = (N / NW * NW + wave) * 1024;
+            dma16(from, dst + at, 16 * lane, at);
+        }
     };
-    auto stage1 = [&](int c, uint8_t * to) __attribute__((always_inline)) {
-        copy(a.ws + ((int64_t)(chunk0 + c) * a.n_kh + hk) * W::HEAD, to, std::integral_constant<int, REG1>{});
+    auto key_part = [&](int c) __attribute__((always_inline)) { return a.ws + ((int64_t)(chunk0 + c) * a.n_kh + hk) * W::HEAD; };
+    auto value_part = [&](int c) __attribute__((always_inline)) {
+        return a.ws + (int64_t)a.chunks * a.n_kh * W::HEAD + ((int64_t)(chunk0 + c) * a.n_vh + hv) * W::VHEAD;
     };
-    auto stage2 = [&](int c, uint8_t * to) __attribute__((always_inline)) {
-        copy(a.ws + ((int64_t)(chunk0 + c) * a.n_kh + hk) * W::HEAD + REG1, to, std::integral_constant<int, W::KF>{});
-        copy(a.ws + (int64_t)a.chunks * a.n_kh * W::HEAD + ((int64_t)(chunk0 + c) * a.n_vh + hv) * W::VHEAD,
-             to + W::KF, std::integral_constant<int, W::VHEAD>{});
-    };
-    auto sync = [&]() __attribute__((always_inline)) {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    const std::integral_constant<int, W::KF> kf_bytes;
+    const std::integral_constant<int, W::TF> tf_bytes;
+    // all but the `left` latest loads of every wave are there, and what the waves read of LDS before has been read
+    auto sync = [&](auto left) __attribute__((always_inline)) {
+        pq2::wait_vmcnt<decltype(left)::value>();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    const int64_t at = ((slot * a.n_vh + hv) * K + 4 * g) * a.vd + col;
-    v4f S[KT];
-#pragma unroll
-    for (int i = 0; i < KT; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) S[i][j] = work ? a.state[at + (int64_t)(16 * i + j) * a.vd] : 0.0f;
-    uint8_t * const own_lds = lds + REG1 + REG2 + wave * OWN;
 
-    // Pairs of products (an MFMA waits for the one before it in its own sum): left fragments, two terms of 1 KB
-    // each, read AHEAD pairs before they are used
-    constexpr int AHEAD = 2;
+    // Products, up to 4 sums side by side (an MFMA waits for the one before it in its own): left fragments, of one
+    // or two terms of 1 KB, read a group ahead of their use
     struct Left {
-        v8h h[2], l[2];
-    };
-    constexpr int TERMS = W::TERMS;
-    auto products = [&](auto count, auto terms, auto place, auto use) __attribute__((always_inline)) {
-        constexpr int N = decltype(count)::value;
-        Left f[AHEAD];
-        auto read = [&](int i) __attribute__((always_inline)) {
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const uint8_t * const p = place(i, k) + 16 * lane;
-                f[i % AHEAD].h[k] = *reinterpret_cast<const v8h *>(p);
-                if (decltype(terms)::value == 2) f[i % AHEAD].l[k] = *reinterpret_cast<const v8h *>(p + 1024);
-            }
-        };
-#pragma unroll
-        for (int i = 0; i < AHEAD && i < N; ++i) read(i);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            use(i, f[i % AHEAD]);
-            if (i + AHEAD < N) read(i + AHEAD);
-            __builtin_amdgcn_sched_barrier(0);
-        }
+        v8h h[4], l[4];
     };
     const std::integral_constant<int, TERMS> own_terms;   // of K and Q
     const std::integral_constant<int, 2> two;
-    auto mul = [](auto terms, const Left & f, const v8h & hi, const v8h & lo, v4f & a, v4f & b) __attribute__((always_inline)) {
-        if constexpr (decltype(terms)::value == 2) {
-            a = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.l[0], hi, a, 0, 0, 0);
-            b = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.l[1], hi, b, 0, 0, 0);
+    auto products = [&](auto count, auto terms, auto width, auto place, auto use) __attribute__((always_inline)) {
+        constexpr int N = decltype(count)::value;
+        Left f[2];
+        auto read = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (k < width(i)) {
+                    const uint8_t * const p = place(i, k) + 16 * lane;
+                    f[i & 1].h[k] = *reinterpret_cast<const v8h *>(p);
+                    if (decltype(terms)::value == 2) f[i & 1].l[k] = *reinterpret_cast<const v8h *>(p + 1024);
+                }
+        };
+        read(0);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (i + 1 < N) read(i + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            use(i, f[i & 1]);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        a = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h[0], lo, a, 0, 0, 0);
-        b = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h[1], lo, b, 0, 0, 0);
-        a = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h[0], hi, a, 0, 0, 0);
-        b = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h[1], hi, b, 0, 0, 0);
+    };
+    auto four = [](int) __attribute__((always_inline)) { return 4; };
+    auto mul = [](auto terms, int n, const Left & f, const v8h & hi, const v8h & lo, v4f * const (&to)[4]) __attribute__((always_inline)) {
+        if constexpr (decltype(terms)::value == 2)
+#pragma unroll
+            for (int k = 0; k < n; ++k) *to[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.l[k], hi, *to[k], 0, 0, 0);
+#pragma unroll
+        for (int k = 0; k < n; ++k) *to[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h[k], lo, *to[k], 0, 0, 0);
+#pragma unroll
+        for (int k = 0; k < n; ++k) *to[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h[k], hi, *to[k], 0, 0, 0);
     };
     // half of a right fragment (elements 4 k ..) from a result tile, its columns scaled
     auto to_right = [](const v4f & x, float down, v8h & hi, v8h & lo, int k) __attribute__((always_inline)) {
@@ -587,10 +609,28 @@ __global__ void __launch_bounds__(64 * NW) gdn_scan_kernel(GdnArgs a) {
             lo[4 * k + j] = l;
         }
     };
+    // a C x C matrix times a right operand: step 0 for all m-tiles, step 1 for the lower two
+    v4f x[4];
+    auto square = [&](const uint8_t * base, const v4f (&right)[4], float down) __attribute__((always_inline)) {
+        v8h rh[2], rl[2];
+        to_right(right[0], down, rh[0], rl[0], 0);
+        to_right(right[1], down, rh[0], rl[0], 1);
+#pragma unroll
+        for (int m = 0; m < 4; ++m) x[m] = v4f{};
+        products(std::integral_constant<int, 2>{}, two, [](int i) __attribute__((always_inline)) { return i ? 2 : 4; },
+                 [&](int i, int k) __attribute__((always_inline)) { return base + 2 * (4 * i + k) * 1024; },
+                 [&](int i, const Left & f) __attribute__((always_inline)) {
+                     v4f * const to[4] = {&x[2 * i], &x[2 * i + 1], &x[2], &x[3]};
+                     mul(two, i ? 2 : 4, f, rh[i], rl[i], to);
+                     if (!i) {
+                         to_right(right[2], down, rh[1], rl[1], 0);
+                         to_right(right[3], down, rh[1], rl[1], 1);
+                     }
+                 });
+    };
 
-    // V comes, and the outputs leave, through a place of the wave's own: [row][16 columns], row 4 j + g of 16 being
-    // token 4 g + j, so that the 4 tokens a lane's column is read at with the others' lie in different banks
-    constexpr int EB = sizeof(elem), UNITS = EB, RPI = 64 / UNITS;    // 16-byte units of a row; rows of an instruction
+    // V comes, and the outputs leave, as [row][16 columns], row 4 j + g of 16 being token 4 g + j, so that the 4 tokens
+    // that the lanes read a column at lie in different banks
     auto token = [](int row) { return (row & ~15) + 4 * (row & 3) + (row >> 2 & 3); };
     const int row0 = lane / UNITS, unit0 = lane % UNITS;
     auto stage_v = [&](int c, uint8_t * to) __attribute__((always_inline)) {
@@ -621,126 +661,166 @@ __global__ void __launch_bounds__(64 * NW) gdn_scan_kernel(GdnArgs a) {
         }
     };
 
-    float big = largest(S), fs = 1.0f;
-    v4f ks[4], qs[4];
-    // K S and Q S, while K^T, T, QK^T, the factors and V arrive
-    auto first_half = [&](const uint8_t * __restrict__ r1, uint8_t * __restrict__ r2, uint8_t * __restrict__ rv, int c) __attribute__((always_inline)) {
-        stage2(c, r2);
-        if (work) {
-            if (c > 0) put(rv, c - 1);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            stage_v(c, rv);
+    const int64_t at = ((slot * a.n_vh + hv) * K + 4 * g) * a.vd + col;
+    v4f S[KT];                                            // (chain)
+#pragma unroll
+    for (int i = 0; i < KT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) S[i][j] = work && chain ? a.state[at + (int64_t)(16 * i + j) * a.vd] : 0.0f;
+    float big = chain ? largest(S) : 0.0f, fs = 1.0f, fw = 1.0f, keep = 1.0f;
+    v4f ks[4], cq[4], ca[4];                              // K S or Q S; the outputs' factors
+    v8h rh[2], rl[2];                                     // w U as right operand
+    auto column = [&](uint8_t * base) __attribute__((always_inline)) { return reinterpret_cast<elem *>(base) + 16 * g + l16; };
+
+    auto outputs = [&](const uint8_t * af, uint8_t * u, int c) __attribute__((always_inline)) {
+        v4f Um[4];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) Um[m] = *reinterpret_cast<const v4f *>(u + 1024 * m + 16 * lane);
+        const int e = exponent(largest(Um));
+        square(af, Um, pow2(-e));
+        const float fu = pow2(e);
+        elem * const own = column(u);                     // (U has been read)
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                own[(16 * m + 4 * j) * 16] = T::from(fmaf(x[m][j], ca[m][j] * fu, cq[m][j] * fs * ks[m][j]));
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");    // other lanes read it
+        put(u, c);
+    };
+    auto phase1 = [&](const uint8_t * __restrict__ k, uint8_t * __restrict__ q, uint8_t * __restrict__ t,
+                      uint8_t * __restrict__ vec, uint8_t * __restrict__ v, const uint8_t * __restrict__ af, uint8_t * __restrict__ u,
+                      uint8_t * __restrict__ sf, int c) __attribute__((always_inline)) {
+        copy(key_part(c) + W::KF, q, kf_bytes);
+        copy(value_part(c), t, tf_bytes);
+        copy(value_part(c) + 2 * W::TF, vec, std::integral_constant<int, W::VEC>{});
+        if (work && chain) stage_v(c, v);
+        if (!work) return;
+        if (!chain) {
+            if (c > 0) outputs(af, u, c - 1);
+            return;
         }
         const int e = exponent(big);
         const float down = pow2(-e);
         fs = pow2(e);
+        *reinterpret_cast<float *>(sf + 2 * KS * 1024 + 4 * lane) = fs;
         v8h sh[2], sl[2];
+        auto give = [&](int s) __attribute__((always_inline)) {
+            *reinterpret_cast<v8h *>(sf + 2 * s * 1024 + 16 * lane) = sh[s & 1];
+            *reinterpret_cast<v8h *>(sf + (2 * s + 1) * 1024 + 16 * lane) = sl[s & 1];
+        };
         to_right(S[0], down, sh[0], sl[0], 0);
         to_right(S[1], down, sh[0], sl[0], 1);
+        give(0);
 #pragma unroll
-        for (int m = 0; m < 4; ++m) ks[m] = qs[m] = v4f{};
-        products(std::integral_constant<int, 4 * KS>{}, own_terms,
-                 [&](int i, int k) __attribute__((always_inline)) { return r1 + k * W::KF + TERMS * (i % 4 * KS + i / 4) * 1024; },
+        for (int m = 0; m < 4; ++m) ks[m] = v4f{};
+        products(std::integral_constant<int, KS>{}, own_terms, four,
+                 [&](int i, int m) __attribute__((always_inline)) { return k + TERMS * (m * KS + i) * 1024; },
                  [&](int i, const Left & f) __attribute__((always_inline)) {
-                     const int s = i / 4, m = i % 4;
-                     mul(own_terms, f, sh[s & 1], sl[s & 1], ks[m], qs[m]);
-                     // the next step's right operand, between the products
-                     if (m < 2 && s + 1 < KS) to_right(S[2 * s + 2 + m], down, sh[(s + 1) & 1], sl[(s + 1) & 1], m);
+                     v4f * const to[4] = {&ks[0], &ks[1], &ks[2], &ks[3]};
+                     mul(own_terms, 4, f, sh[i & 1], sl[i & 1], to);
+                     if (i + 1 < KS) {                    // the next step's right operand, between the products
+                         to_right(S[2 * i + 2], down, sh[(i + 1) & 1], sl[(i + 1) & 1], 0);
+                         to_right(S[2 * i + 3], down, sh[(i + 1) & 1], sl[(i + 1) & 1], 1);
+                         give(i + 1);
+                     }
                  });
     };
-    // U, the outputs and the next S, while the next K and Q arrive
-    auto second_half = [&](const uint8_t * __restrict__ r2, uint8_t * __restrict__ r1, uint8_t * __restrict__ rv, int c) __attribute__((always_inline)) {
-        if (c + 1 < chunks) stage1(c + 1, r1);
-        const uint8_t * const tf = r2 + W::KF, * const af = tf + W::TF;
-        const float * const vec = reinterpret_cast<const float *>(af + W::TF);
-        auto factor = [&](int which, int m) { return *reinterpret_cast<const v4f *>(vec + which * C + 16 * m + 4 * g); };
-        elem * const own = reinterpret_cast<elem *>(rv) + 16 * g + l16;      // token 16 m + 4 g + j: row 16 m + 4 j + g
-        // products with T and QK^T, two m-tiles at a time; their blocks above the diagonal are 0
-        auto place = [&](const uint8_t * base, int i, int k) __attribute__((always_inline)) {
-            const int m = (i == 0 ? 0 : 2) + k, s = i / 2;
-            return base + 2 * (2 * m + s) * 1024;
+    auto phase2 = [&](uint8_t * __restrict__ k, const uint8_t * __restrict__ q, const uint8_t * __restrict__ t,
+                      const uint8_t * __restrict__ vec, uint8_t * __restrict__ v, uint8_t * __restrict__ af, uint8_t * __restrict__ u,
+                      const uint8_t * __restrict__ sf, int c) __attribute__((always_inline)) {
+        copy(key_part(c) + 2 * W::KF, k, kf_bytes);
+        copy(value_part(c) + W::TF, af, tf_bytes);        // last: it may be on its way still after the phase
+        if (!work) return;
+        auto factor = [&](int which, int m) {
+            return *reinterpret_cast<const v4f *>(vec + 4 * (which * C + 16 * m + 4 * g));
         };
-        v8h rh[2], rl[2];
-        v4f R[4], Um[4], x[4];
+        if (!chain) {
+            fs = *reinterpret_cast<const float *>(sf + 2 * KS * 1024 + 4 * lane);
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                ks[m] = v4f{};
+                cq[m] = factor(1, m);
+                ca[m] = factor(3, m);
+            }
+            products(std::integral_constant<int, KS>{}, own_terms, four,
+                     [&](int i, int m) __attribute__((always_inline)) { return q + TERMS * (m * KS + i) * 1024; },
+                     [&](int i, const Left & f) __attribute__((always_inline)) {
+                         const v8h sh = *reinterpret_cast<const v8h *>(sf + 2 * i * 1024 + 16 * lane);
+                         const v8h sl = *reinterpret_cast<const v8h *>(sf + (2 * i + 1) * 1024 + 16 * lane);
+                         v4f * const to[4] = {&ks[0], &ks[1], &ks[2], &ks[3]};
+                         mul(own_terms, 4, f, sh, sl, to);
+                     });
+            return;
+        }
+        v4f R[4], Um[4];
+        const elem * const own = column(v);
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
             const v4f f = factor(0, m);
 #pragma unroll
             for (int j = 0; j < 4; ++j) R[m][j] = fmaf(-f[j] * fs, ks[m][j], T::to(own[(16 * m + 4 * j) * 16]));
-            x[m] = v4f{};
         }
         int e = exponent(largest(R));
-        float down = pow2(-e);
         const float fr = pow2(e);
-        to_right(R[0], down, rh[0], rl[0], 0);
-        to_right(R[1], down, rh[0], rl[0], 1);
-        auto square = [&](const uint8_t * base, const v4f (&right)[4], float down) __attribute__((always_inline)) {
-            products(std::integral_constant<int, 3>{}, two, [&](int i, int k) __attribute__((always_inline)) { return place(base, i, k); },
-                     [&](int i, const Left & f) __attribute__((always_inline)) {
-                         const int m = i == 0 ? 0 : 2, s = i / 2;
-                         mul(two, f, rh[s], rl[s], x[m], x[m + 1]);
-                         if (i < 2) to_right(right[2 + i], down, rh[1], rl[1], i);
-                     });
-        };
-        square(tf, R, down);
+        square(t, R, pow2(-e));
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-            const v4f f = factor(2, m);
+            const v4f f = factor(2, m), w = factor(4, m);
 #pragma unroll
             for (int j = 0; j < 4; ++j) Um[m][j] = x[m][j] * f[j] * fr;
-            x[m] = v4f{};
+            *reinterpret_cast<v4f *>(u + 1024 * m + 16 * lane) = Um[m];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) Um[m][j] *= w[j];
         }
         e = exponent(largest(Um));
-        down = pow2(-e);
-        const float fu = pow2(e);
-        to_right(Um[0], down, rh[0], rl[0], 0);
-        to_right(Um[1], down, rh[0], rl[0], 1);
-        square(af, Um, down);
+        fw = pow2(e);
+        keep = *reinterpret_cast<const float *>(vec + 4 * 5 * C);
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            const v4f f = factor(3, m), h = factor(1, m), w = factor(4, m);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                own[(16 * m + 4 * j) * 16] = T::from(fmaf(x[m][j], f[j] * fu, h[j] * fs * qs[m][j]));
-                Um[m][j] *= w[j];
-            }
-        }
-        e = exponent(largest(Um));
-        down = pow2(-e);
-        const float fw = pow2(e), keep = vec[5 * C];
-#pragma unroll
-        for (int m = 0; m < 4; ++m) to_right(Um[m], down, rh[m / 2], rl[m / 2], m & 1);
+        for (int m = 0; m < 4; ++m) to_right(Um[m], pow2(-e), rh[m / 2], rl[m / 2], m & 1);
+    };
+    auto phase3 = [&](const uint8_t * __restrict__ kt, uint8_t * __restrict__ k, int c) __attribute__((always_inline)) {
+        if (c + 1 < chunks) copy(key_part(c + 1), k, kf_bytes);
+        if (!work || !chain) return;
         float top[2] = {0.0f, 0.0f};
-        v4f y[2];
-        products(std::integral_constant<int, KT>{}, own_terms,
-                 [&](int i, int k) __attribute__((always_inline)) { return r2 + TERMS * (2 * (2 * (i / 2) + k) + (i & 1)) * 1024; },
+        v4f y[4];
+        products(std::integral_constant<int, KT / 2>{}, own_terms, four,
+                 [&](int i, int k) __attribute__((always_inline)) { return kt + TERMS * (2 * (4 * (i / 2) + k) + (i & 1)) * 1024; },
                  [&](int i, const Left & f) __attribute__((always_inline)) {
-                     if (!(i & 1)) y[0] = y[1] = v4f{};
-                     mul(own_terms, f, rh[i & 1], rl[i & 1], y[0], y[1]);
+                     if (!(i & 1)) y[0] = y[1] = y[2] = y[3] = v4f{};
+                     v4f * const to[4] = {&y[0], &y[1], &y[2], &y[3]};
+                     mul(own_terms, 4, f, rh[i & 1], rl[i & 1], to);
                      if (i & 1)
 #pragma unroll
-                         for (int k = 0; k < 2; ++k)
+                         for (int k = 0; k < 4; ++k)
 #pragma unroll
                              for (int j = 0; j < 4; ++j) {
-                                 const float st = fmaf(y[k][j], fw, keep * S[2 * (i / 2) + k][j]);
-                                 S[2 * (i / 2) + k][j] = st;
-                                 top[k] = fmaxf(top[k], fabsf(st));
+                                 const float st = fmaf(y[k][j], fw, keep * S[4 * (i / 2) + k][j]);
+                                 S[4 * (i / 2) + k][j] = st;
+                                 top[k & 1] = fmaxf(top[k & 1], fabsf(st));
                              }
                  });
         big = over_column(fmaxf(top[0], top[1]));
     };
 
-    if (chunks > 0) stage1(0, lds);
+    uint8_t * const v = lds + AT_V + pair * V_PAIR, * const u = lds + AT_U + pair * U_PAIR, * const sf = lds + AT_S + pair * S_PAIR;
+    const std::integral_constant<int, 0> none;
+    if (chunks > 0) copy(key_part(0), lds, kf_bytes);
 #pragma clang loop unroll(disable)
     for (int c = 0; c < chunks; ++c) {
-        sync();                                           // K, Q are there; the others' place is free
-        first_half(lds, lds + REG1, own_lds, c);
-        sync();                                           // the rest is there; K's and Q's place is free
-        second_half(lds + REG1, lds, own_lds, c);
+        uint8_t * const one = lds + (c & 1) * W::KF, * const two = lds + (~c & 1) * W::KF;
+        sync(none);                                       // K is in the one, the last chunk's QK^T and U are there
+        phase1(one, two, lds + AT_T, lds + AT_VEC, v, lds + AT_A, u, sf, c);
+        sync(none);                                       // Q is in the two, S there as operands
+        phase2(one, two, lds + AT_T, lds + AT_VEC, v, lds + AT_A, u, sf, c);
+        sync(std::integral_constant<int, W::TF / 1024 / NW>{});    // K^T is in the one, QK^T on its way
+        phase3(one, two, c);
     }
-    if (!work) return;
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");    // other lanes read what this one wrote
-    if (chunks > 0) put(own_lds, chunks - 1);
+    if (chunks > 0) {
+        sync(none);
+        if (work && !chain) outputs(lds + AT_A, u, chunks - 1);
+    }
+    if (!work || !chain) return;
 #pragma unroll
     for (int i = 0; i < KT; ++i)
 #pragma unroll
@@ -759,7 +839,13 @@ int launch(const GdnArgs & a, bool chunked, hipStream_t s) {
     if (e != hipSuccess) return (int)e;
     // (8 key heads at a time, those that there are not return)
     const int64_t heads = (int64_t)a.n_seq * (a.n_vh / a.n_kh) * ((a.n_kh + 7) / 8 * 8);
-    hipLaunchKernelGGL((gdn_scan_kernel<T, K, 4>), dim3((unsigned)(heads * ((a.vd + 63) / 64))), dim3(256), 0, s, a);
+    auto scan = [&](auto pairs) {
+        constexpr int P = decltype(pairs)::value;
+        hipLaunchKernelGGL((gdn_scan_kernel<T, K, P>), dim3((unsigned)(heads * ((a.vd + 16 * P - 1) / (16 * P)))),
+                           dim3(128 * P), 0, s, a);
+    };
+    if (pq2::gdn_wide((int64_t)a.n_seq * a.n_vh, a.vd, pq2host::device_info().cus)) scan(std::integral_constant<int, 4>{});
+    else scan(std::integral_constant<int, 2>{});
     return (int)hipGetLastError();
 }
 template <class T>
@@ -787,7 +873,7 @@ int check(const bonsai_p40_gdn_args * p) {
 int64_t chunks_of(const bonsai_p40_gdn_args * p) { return p->n_tok / C + (p->n_seq < p->n_tok ? p->n_seq : p->n_tok); }
 bool chunked(const bonsai_p40_gdn_args * p) {
     const int64_t most = p->max_new > 0 && p->max_new < p->n_tok ? p->max_new : p->n_tok;
-    return pq2::gdn_chunked(most, p->n_seq);
+    return pq2::gdn_chunked(most);
 }
 
 }  // namespace

@@ -228,11 +228,21 @@ inline AttnPlan attn_plan(int64_t n_tok, int64_t n_seq, int64_t group, int64_t n
     return p;
 }
 
-// The gated delta rule (gdn.hip) in chunks of 64 tokens, or token by token.
-inline bool gdn_chunked(int64_t max_new, int64_t n_seq) {
-    (void)n_seq;
-    return max_new > 16;
-}
+// The gated delta rule (gdn.hip) in chunks of 64 tokens (true), or token by token:
+// a chunk takes the same time however few tokens it has, a token by itself about 1.1
+// us for one sequence, 2 for 8 and 4.3 for 48.  Measured on MI355X (us, by token / in
+// chunks, fp32, 48 heads of 128): 1 sequence of 16 20.4 / 30.2, 24 29.1 / 30.3, 32
+// 37.3 / 30.3; 8 of 16 41.8 / 50.5, 24 56.7 / 50.7; 48 of 8 137 / 203, 16 210 / 204,
+// 24 282 / 206; bf16 1 of 16 22.4 / 27.7, 24 31.7 / 27.6, 48 of 16 183 / 186.
+inline bool gdn_chunked(int64_t max_new) { return max_new > 16; }
+
+// Columns of a value head that a workgroup of the chunked form takes: 32 (2 pairs of
+// waves) while that leaves no workgroup waiting for a CU, else 64 (4 pairs, true),
+// whose waves share SIMDs and fragments.  Measured on MI355X (256 CUs, us, 32 / 64
+// columns, fp32, 48 heads of 128): 1 sequence of 2048 tokens (192 workgroups of 32)
+// 150 / 172, 2 of 1000 (384) 152 / 107, 8 of 2048 1008 / 749; bf16 127 / 149, 130 /
+// 93, 850 / 597.
+inline bool gdn_wide(int64_t heads, int64_t v_dim, int64_t cus) { return heads * ((v_dim + 31) / 32) > cus; }
 
 }  // namespace pq2
 

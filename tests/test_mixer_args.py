@@ -106,10 +106,11 @@ def test_workspace_bytes():
     assert n > 0 and n % (2 * 8 * 130 * 4) == 0
     assert attn() == 0 and attn(**long, head_dim=96) == 0 and attn(**long, max_kv=64) == 0
     assert attn(**{**long, "n_tok": 0}) == 0
-    # a chunk of 64 tokens: K, Q and K^T of a key head and two 64 x 64 matrices of a value head, each as two f16
-    # terms, and 2 KB of factors
+    # a chunk of 64 tokens: K, Q and K^T of a key head and two 64 x 64 matrices (6 of their 8 blocks of 16 x 32) of a
+    # value head, each as two f16 terms, and 2 KB of factors; 16-bit rows are one term
     chunks = 100 // 64 + 2
-    assert gdn() == chunks * (2 * 3 * 64 * 128 * 4 + 4 * (2 * 64 * 64 * 4 + 2048))
+    assert gdn() == chunks * (2 * 3 * 64 * 128 * 4 + 4 * (2 * 64 * 64 * 3 + 2048))
+    assert gdn(type=B.BF16) == chunks * (2 * 3 * 64 * 128 * 2 + 4 * (2 * 64 * 64 * 3 + 2048))
     assert gdn(max_new=1) == 0 and gdn(n_tok=2) == 0 and gdn(v_dim=24) == 0
 
 
