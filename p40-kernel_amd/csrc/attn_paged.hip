@@ -20,11 +20,11 @@
 // K and V tiles reach LDS by DMA, 16-byte units XOR-swizzled by the key on the
 // source side so that neither read meets a bank twice.
 //
-// Two shapes of workgroup:
-//   rows: a wave per 32 rows (128 a workgroup), all on the same tiles of 64 keys,
-//     double-buffered: prompts, bound by the matrix cores;
-//   keys: 32 rows, each wave its own tiles of 32 keys, double-buffered, joined in
-//     LDS at the end: decode, bound by the stream of K and V.
+// Two shapes of workgroup, both on tiles of 32 keys:
+//   rows: a wave per 32 rows (64 or 128 a workgroup), all on the same tiles, which
+//     come through rings of 3 or 4 in LDS: prompts, bound by the matrix cores;
+//   keys: 32 rows, each wave its own tiles, double-buffered, joined in LDS at the
+//     end: decode, bound by the stream of K and V.
 // Either splits the keys over workgroups where there are too few rows to fill the
 // card; attn_join_kernel adds the parts.
 //
@@ -741,7 +741,8 @@ int launch(AttnArgs & a, hipStream_t s) {
     if (e != hipSuccess || a.n_split == 1) return (int)e;
     typedef typename std::conditional<NT == 1, T, F32>::type TO;
     const int64_t rows = (int64_t)a.n_tok * a.n_head;
-    if (a.n_split > 8) hipLaunchKernelGGL((attn_join_kernel<TO, D, 4>), dim3((unsigned)rows), dim3(256), 0, s, a, (int)Z::BM);
+    if (pq2::attn_join_wide(a.n_split))
+        hipLaunchKernelGGL((attn_join_kernel<TO, D, 4>), dim3((unsigned)rows), dim3(256), 0, s, a, (int)Z::BM);
     else hipLaunchKernelGGL((attn_join_kernel<TO, D, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a, (int)Z::BM);
     return (int)hipGetLastError();
 }

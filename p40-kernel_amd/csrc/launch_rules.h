@@ -190,10 +190,29 @@ inline void prefill_plan(bool wide, bool small, int64_t n_out, int64_t n_tok, in
     }
 }
 
+// Tokens of a workgroup of the head norms and rotations (qk_norm_rope.hip): it
+// takes 4 side by side, so many tokens in one are a chain that few workgroups leave
+// exposed, few of them repeat its start, and in columns (a token's features n_tok
+// floats apart) a tile reads runs of 4 tokens.  Measured on MI355X (us, 4 / 16 / 32
+// tokens, 24 + 8 heads of 256): rows, 64 tokens 4.5 4.9 7.6, 96 5.0 5.1 7.7, 256 8.1
+// 6.0 8.3, 2048 39.6 22.4 22.8; columns, 64 4.9 5.2 7.9, 256 15.1 6.2 8.6, 512 - 10.1
+// 10.4, 768 - 15.4 13.1, 1024 - 17.6 19.3, 2048 81 32.0 30.3, 4096 - 60.4 49.9.
+inline int rope_tile(bool columns, int64_t n_tok) { return n_tok <= 64 ? 4 : columns && n_tok > 512 ? 32 : 16; }
+
 // Attention over pages (attn_paged.hip): workgroups whose waves split the keys
 // (32 rows, decode) or the rows (64 or 128), the number of row tiles that n_tok tokens
 // of n_seq sequences can have at most, and the keys of one workgroup: n_split
 // workgroups share a tile, the last of them takes what is left.
+//   The keys are split while one tile of 32 rows holds a sequence's: a second tile
+// reads K and V again.  Measured on MI355X (us, rows / keys split, 24 heads on 4 of
+// 256, fp32 queries, bf16 pages): 1 sequence, 16000 keys, 24 rows 34 / 31, 48 34 / 54,
+// 96 49 / 96; 8 of 2000, 24 39 / 41, 48 45 / 76; 32 of 4000, 24 143 / 137, 48 242 / 261, 96 300 / 395;
+// bf16 queries, 32 of 4000, 24 121 / 116, 48 115 / 191; 32 heads on 8 of 128, 16 of 2000,
+// 16 rows 62 / 47, 32 64 / 58, 64 53 / 99.
+//   Rows: key is the us of one key of a tile on one workgroup, part those of one more
+// part of every row, as fitted to 1 to 2048 tokens of 1000 to 60000 keys.  Up to 64
+// parts: with 16 at most, 8 tokens of 60000 keys took 228 us for 75 (fp32), 16
+// of 16000 74 for 49.
 struct AttnPlan {
     bool keys;
     int64_t tiles, chunk, n_split;
@@ -201,7 +220,7 @@ struct AttnPlan {
 inline AttnPlan attn_plan(int64_t n_tok, int64_t n_seq, int64_t group, int64_t n_kv, int64_t dim, int64_t max_kv, int64_t rows,
                           int64_t cus) {
     AttnPlan p;
-    p.keys = n_tok * group <= 64 * n_seq;
+    p.keys = n_tok * group <= 32 * n_seq;
     const int64_t bm = p.keys ? 32 : rows, step = p.keys && dim < 256 ? 128 : 64;
     const int64_t some = n_seq < n_tok ? n_seq : n_tok;
     p.tiles = n_tok * group / bm + some;
@@ -215,7 +234,7 @@ inline AttnPlan attn_plan(int64_t n_tok, int64_t n_seq, int64_t group, int64_t n
         const double key = 0.022 * (double)dim / 256, part = (double)n_tok * group * n_kv * dim * 8 / 4.5e6;
         const double longest = (double)max_kv, mean = longest - 0.5 * (double)(n_tok / some < max_kv ? n_tok / some : max_kv);
         double best = 0.0;
-        for (int64_t n = 1; n <= 16 && blocks < 2 * slots; ++n) {
+        for (int64_t n = 1; n <= 64 && blocks < 2 * slots; ++n) {
             const double rounds = (double)((blocks * n + slots - 1) / slots) * mean;
             const double us = key * (rounds > longest ? rounds : longest) / (double)n + (n > 1 ? 5.0 + part * (double)n : 0.0);
             if (n == 1 || us < best) best = us, want = n;
@@ -227,6 +246,13 @@ inline AttnPlan attn_plan(int64_t n_tok, int64_t n_seq, int64_t group, int64_t n
     p.n_split = max_kv > p.chunk ? (max_kv + p.chunk - 1) / p.chunk : 1;
     return p;
 }
+
+// Waves that join the parts of a row: 4 (true) or 1, 4 rows to a workgroup.  Many
+// parts are a chain of loads for one wave; few leave the others idle.  Measured on
+// MI355X (us of attention and join, 1 / 4 waves, 24 heads of 256): 1 token of 400 keys (7
+// parts) 14.2 / 14.4, 1000 (16) 16.0 / 14.8, 4000 (63) 23.5 / 16.9; 32 tokens of 60000 (32) 91.5 /
+// 89.2; 16 of 1000 (8) 24.9 / 25.3, 256 of 60000 (9) 454 / 458, of 16000 (4) 139 / 148.
+inline bool attn_join_wide(int64_t n_split) { return n_split > 8; }
 
 // The gated delta rule (gdn.hip) in chunks of 64 tokens (true), or token by token:
 // a chunk takes the same time however few tokens it has, a token by itself about 1.1

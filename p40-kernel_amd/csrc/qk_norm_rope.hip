@@ -6,7 +6,7 @@
 //   (y_i, y_j) -> (y_i c - y_j s, y_j c + y_i s),  c, s = cos, sin(pos f_i)
 //
 // It moves bytes and little else: 4 in and 2 or 4 out an element.  A workgroup
-// takes one head row of TT tokens; the angles of those tokens are computed once
+// takes one head row of TT tokens (4, 16 or 32: rope_tile); the angles of those tokens are computed once
 // into LDS.  An angle is pos * f / 2 pi in fp64, reduced to half a turn there:
 // in fp32 a position of 1e6 would leave it 4 bits.
 //   Rows (one per token): a wave reads a token's head row from memory.
@@ -15,6 +15,7 @@
 // are read 16 bytes a lane, and written with two lanes on a bank.  All of a
 // tile's loads are asked for at once: at 8 a lane it ran at 2.9 TB/s.
 #include "host_state.h"
+#include "launch_rules.h"
 #include "mixer_device.h"
 #include "pq2_device.h"
 
@@ -53,7 +54,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkvArgs a) {
     float2 * const turn = reinterpret_cast<float2 *>(lds + (columns ? a.tt * (D + 4) : 0));   // [tt][half]
 
     if (columns) {
-        // 32 tokens of a feature are one run of 128 bytes: half a wave each
+        // the tokens of a feature are one run of up to 128 bytes: half a wave each
         const int sub = threadIdx.x & 31;
         if (sub < nt) {
             const float * const c = x + (int64_t)(t0 + sub) * ts + (int64_t)(threadIdx.x >> 5) * es;
@@ -233,7 +234,7 @@ extern "C" int bonsai_p40_qk_norm_rope(const bonsai_p40_qk_norm_rope_args * p, b
     a.n_kv = p->n_kv_head;
     a.half = p->n_rot / 2;
     a.interleaved = p->interleaved != 0;
-    a.tt = columns || p->n_tok > 64 ? 32 : 4;
+    a.tt = pq2::rope_tile(columns, p->n_tok);
     auto lds = [&](int tt) { return (columns ? (size_t)tt * (d + 4) * 4 : 0) + (size_t)tt * a.half * 8; };
     if (lds(a.tt) > 64 * 1024) a.tt = 16;       // 256 columns, all of them rotated
     const size_t bytes = lds(a.tt);
