@@ -447,7 +447,8 @@ int bonsai_p40_qk_norm_rope(const bonsai_p40_qk_norm_rope_args * args, bonsai_st
 // and from starts[n_seq] on are not touched.  Keys and values that a token does
 // not see never reach its output, whatever they hold.
 // q and out: token t at t * q_tok and t * out_tok, heads one after another, of
-// io_type: kv_type, or fp32, which keeps fp32 accuracy throughout.
+// io_type: kv_type, or fp32, which keeps fp32 accuracy throughout; out overlaps
+// nothing that is read.
 // max_kv: about the largest kv_len (0: unknown); it places the work, results hold for
 // any.  workspace: bonsai_p40_attn_paged_workspace_bytes bytes (of the same
 // args), 16-byte aligned, scratch for the call (stream-ordered; calls that may
@@ -458,8 +459,8 @@ int bonsai_p40_qk_norm_rope(const bonsai_p40_qk_norm_rope_args * args, bonsai_st
 // of n_kv_head, io_type, kv_type, page_size (a power of two, 16 .. 65536) or a
 // stride is not as stated (rows of q and out are 16-byte aligned), scale is not
 // finite and > 0, max_pages * page_size >= 2^31 - 65536, a pointer is NULL or
-// misaligned, the workspace is too small, or there are more than 2^28 / n_head tokens and
-// sequences; 0 (no-op) if n_tok <= 0 or n_seq <= 0.
+// misaligned, the workspace is too small, or there are 2^24 / n_head tokens and
+// sequences or more; 0 (no-op) if n_tok <= 0 or n_seq <= 0.
 typedef struct bonsai_p40_attn_paged_args {
     const void * q;
     void * out;
@@ -497,7 +498,8 @@ int64_t bonsai_p40_attn_paged_workspace_bytes(const bonsai_p40_attn_paged_args *
 // without tokens copies its state.  Other states, and rows of out before starts[0] and
 // from starts[n_seq] on, are not touched.
 // q, k, v, out: type fp32, f16 or bf16; token t at t * q_tok (k_tok, v_tok,
-// out_tok) elements, heads one after another: slices of one row may be passed.
+// out_tok) elements, heads one after another: slices of one row may be passed;
+// out overlaps nothing that is read.
 // g and beta: fp32, head h of token t at t * gate_tok + h; a g below -10000 counts as
 // that (exp is 0 there).  All sums, and the products' operands to 22 bits or more, are
 // fp32's.
@@ -511,7 +513,7 @@ int64_t bonsai_p40_attn_paged_workspace_bytes(const bonsai_p40_attn_paged_args *
 // stated (q_tok, k_tok, v_tok, out_tok and gate_tok at least a row; q, k and v rows
 // 16-byte aligned, v_tok up to 2^22), scale or l2_eps is not finite or l2_eps is negative, a
 // pointer is NULL or misaligned, the workspace is too small, or there are more
-// than 2^27 / n_v_head tokens and sequences; 0 (no-op) if n_seq <= 0.
+// than 2^27 / n_v_head tokens or 2^20 / n_v_head sequences; 0 (no-op) if n_seq <= 0.
 typedef struct bonsai_p40_gdn_args {
     const void * q, * k, * v;
     void * out;

@@ -774,7 +774,7 @@ int check(const bonsai_p40_attn_paged_args * p) {
     if (p->max_pages * (int64_t)p->page_size > 0x7fff0000) return 1;
     if (p->n_tok <= 0 || p->n_seq <= 0) return 0;
     if (p->n_tok > 0x7fffffff / p->n_head || p->n_seq > 0xffffff) return 1;
-    if ((p->n_tok + p->n_seq) * (int64_t)p->n_head > 0x7fffffff / 8) return 1;     // workgroups
+    if ((p->n_tok + p->n_seq) * (int64_t)p->n_head >= 1 << 24) return 1;    // a grid has fewer than 2^32 threads
     return -1;
 }
 

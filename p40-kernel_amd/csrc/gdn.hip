@@ -504,13 +504,14 @@ __global__ void __launch_bounds__(128 * PAIRS) gdn_scan_kernel(GdnArgs a) {
     const bool chain = wave < PAIRS;
     // a key head's workgroups, which share fragments, on one XCD (workgroups go to the 8 in turn)
     const int groups = (a.vd + 16 * PAIRS - 1) / (16 * PAIRS), per = a.n_vh / a.n_kh;
-    int hk = blockIdx.x & 7, rest = blockIdx.x >> 3;
+    const int at_once = min(a.n_kh, 8);
+    int hk = blockIdx.x % at_once, rest = blockIdx.x / at_once;
     const int group = rest % groups;
     rest /= groups;
     const int head = rest % per;
     rest /= per;
-    const int eighth = (a.n_kh + 7) / 8, seq = rest / eighth;
-    hk += 8 * (rest % eighth);
+    const int times = (a.n_kh + at_once - 1) / at_once, seq = rest / times;
+    hk += at_once * (rest % times);
     if (hk >= a.n_kh) return;
     const int hv = a.tiled ? hk + head * a.n_kh : hk * per + head;
     const int col0 = 16 * (PAIRS * group + pair);
@@ -838,7 +839,7 @@ int launch(const GdnArgs & a, bool chunked, hipStream_t s) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
     // (8 key heads at a time, those that there are not return)
-    const int64_t heads = (int64_t)a.n_seq * (a.n_vh / a.n_kh) * ((a.n_kh + 7) / 8 * 8);
+    const int64_t heads = (int64_t)a.n_seq * (a.n_vh / a.n_kh) * (a.n_kh < 8 ? a.n_kh : (a.n_kh + 7) / 8 * 8);
     auto scan = [&](auto pairs) {
         constexpr int P = decltype(pairs)::value;
         hipLaunchKernelGGL((gdn_scan_kernel<T, K, P>), dim3((unsigned)(heads * ((a.vd + 16 * P - 1) / (16 * P)))),
@@ -867,7 +868,8 @@ int check(const bonsai_p40_gdn_args * p) {
     if (!(p->scale > -INFINITY && p->scale < INFINITY) || !(p->l2_eps >= 0.0f && p->l2_eps < INFINITY)) return 1;
     if (p->n_seq <= 0) return 0;
     if (p->n_tok > 0x7fffffff || p->n_states > (1ll << 40)) return 1;
-    if (p->n_tok + p->n_seq > (1ll << 27) / p->n_v_head) return 1;      // workgroups
+    // a grid has fewer than 2^32 threads: 128 per 32 columns, twice that in chunks, where key heads are rounded up to 8
+    if (p->n_tok > (1ll << 27) / p->n_v_head || p->n_seq >= (1ll << 20) / p->n_v_head) return 1;
     return -1;
 }
 int64_t chunks_of(const bonsai_p40_gdn_args * p) { return p->n_tok / C + (p->n_seq < p->n_tok ? p->n_seq : p->n_tok); }

@@ -128,6 +128,13 @@ def test_rope_far_positions_and_plain_rows():
     run_rope(70, 2, 2, 64, 64, 128, F32, F16, True, odd=True)
 
 
+@pytest.mark.parametrize("d,rot", [(256, 64), (256, 256), (64, 64)])
+def test_rope_every_tile(d, rot):
+    """More tokens than 4 a workgroup pays for, and in columns than 16 (all of 256 rotated: 16 again)."""
+    for columns, n in ((False, 65), (False, 301), (True, 65), (True, 512), (True, 513), (True, 547)):
+        run_rope(n, 2, 1, d, rot, 64, BF16, F16, columns, seed=n)
+
+
 def test_rope_slots_outside_are_not_written():
     pages, page = 4, 16
     slots = torch.tensor([-1, 3, 64, 2 ** 40, 63, -2 ** 40, 0, 17], dtype=torch.int64)
@@ -268,6 +275,14 @@ def test_attn_few_tokens(io):
     for n in (2, 3, 5, 8, 10, 11, 12, 16, 22):
         run_attn([n], [n + 200], 6, 1, 128, 16, BF16, io, seed=n)
         run_attn([n, n + 1], [n, n + 130], 4, 4, 64, 16, BF16, io, seed=n)
+
+
+@pytest.mark.parametrize("t,io", [(F16, F16), (BF16, F32), (F16, F32)])
+def test_attn_few_tokens_of_a_long_context(t, io):
+    """More rows than one tile of the decode shape, over as many workgroups as there are."""
+    run_attn([8], [5000], 12, 2, 256, 64, t, io)
+    run_attn([40], [1500], 8, 4, 64, 16, t, io, seed=1)
+    run_attn([7, 9, 11], [900, 2000, 30], 6, 1, 128, 32, t, io, seed=2)
 
 
 def test_attn_rows_without_keys():
@@ -480,6 +495,34 @@ def test_gdn_lengths_both_ways(new):
     a = run_gdn([new], 1, 2, 128, 64, F32, seed=new)
     b = run_gdn([new], 1, 2, 128, 64, F32, seed=new, work=False)
     assert normwise(a[0], b[0].double().cpu()) <= 2.0 ** -17
+
+
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("kh,vh,kd,vd", [(2, 6, 128, 128), (3, 9, 64, 48), (10, 10, 64, 16), (1, 2, 128, 144)])
+def test_gdn_many_sequences(kh, vh, kd, vd, t):
+    """More workgroups than CUs; key heads that are no multiple of 8; columns that end inside a workgroup's."""
+    run_gdn([(11 * i) % 71 for i in range(45)], kh, vh, kd, vd, t, seed=7, pad=1)
+    run_gdn([70], kh, vh, kd, vd, t, seed=8, tiled=False)
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+def test_gdn_rows_of_out_at_any_element(t):
+    case(f"gdn out strides {t}")
+    n, r = 100, gen(5)
+    q, k, v = (torch.randn(n, 2, 64, generator=r).to(t).cuda() for _ in range(3))
+    g, beta = -torch.rand(n, 2, generator=r).cuda(), torch.rand(n, 2, generator=r).cuda()
+    st = torch.randn(2, 2, 64, 64, generator=r).cuda()
+    for starts in ([0, 1, 3], [0, 30, 99]):
+        res = []
+        for off, width in ((0, 128), (1, 131)):
+            wide = torch.full((n * width + 8,), 5.0, dtype=t, device="cuda")
+            out = wide[off:off + n * width].view(n, width)[:, :128].unflatten(1, (2, 64))
+            args = (q, k, v, g, beta, st, torch.empty_like(st), out, ints(starts))
+            ws = torch.empty(B.gdn_workspace_bytes(*args, l2_eps=1e-6) + 16, dtype=torch.uint8, device="cuda")
+            B.gdn(*args, ws, l2_eps=1e-6)
+            res.append(out.clone())
+            assert bool((wide[off:off + n * width].view(n, width)[:, 128:] == 5).all()) and bool((wide[n * width + off:] == 5).all())
+        assert torch.equal(*res) and bool((res[0][starts[-1]:] == 5).all())
 
 
 def test_gdn_slots():

@@ -45,7 +45,7 @@ REFUSED = {
         dict(n_pages=-1), dict(n_pages=1 << 31), dict(page_stride=4095), dict(page_stride=4100), dict(q_tok=1023),
         dict(q_tok=1028), dict(out_tok=1000), dict(out_tok=1025), dict(scale=0.0), dict(scale=-1.0), dict(scale=INF),
         dict(scale=NAN), dict(max_pages=-1), dict(max_pages=5), dict(max_pages=1 << 27, table_stride=1 << 27),
-        dict(max_kv=-1), dict(n_tok=1 << 28), dict(n_seq=1 << 26), dict(q=A + 8), dict(out=A + 8), dict(k_pages=A + 8),
+        dict(max_kv=-1), dict(n_tok=1 << 28), dict(n_seq=1 << 26), dict(n_tok=1 << 21), dict(n_tok=1 << 20, n_seq=1 << 20), dict(q=A + 8), dict(out=A + 8), dict(k_pages=A + 8),
         dict(v_pages=A + 4), dict(workspace=A + 8, workspace_bytes=1 << 30), dict(table=A + 1), dict(starts=A + 2),
         dict(kv_len=A + 2), dict(workspace=A, workspace_bytes=16, max_pages=1 << 16, table_stride=1 << 16)]),
     "gdn": (B.GdnArgs, GDN, [
@@ -53,7 +53,7 @@ REFUSED = {
         dict(n_v_head=5), dict(n_v_head=65538), dict(type=3), dict(n_states=-1), dict(n_tok=-1), dict(max_new=-1),
         dict(q_tok=255), dict(k_tok=258), dict(v_tok=511), dict(out_tok=511), dict(gate_tok=3), dict(scale=INF),
         dict(scale=NAN), dict(l2_eps=-1.0), dict(l2_eps=NAN), dict(l2_eps=INF), dict(n_tok=1 << 26), dict(n_seq=1 << 26),
-        dict(v_tok=514), dict(v_tok=(1 << 22) + 4),
+        dict(n_seq=1 << 18), dict(v_tok=514), dict(v_tok=(1 << 22) + 4),
         dict(q=A + 8), dict(k=A + 4), dict(v=A + 8), dict(out=A + 1), dict(g=A + 2), dict(beta=A + 1), dict(state=A + 2),
         dict(state_out=A + 3), dict(starts=A + 2), dict(slots=A + 1), dict(workspace=A + 4, workspace_bytes=1 << 30),
         dict(workspace=A, workspace_bytes=1000)]),
