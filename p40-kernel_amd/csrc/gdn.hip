@@ -19,8 +19,8 @@
 // two f16 terms (22 bits; rows of the left, columns of the right operand scaled by
 // powers of two so that f16's range does not matter) and the products hi hi,
 // hi lo and lo hi run on v_mfma_f32_16x16x32_f16, the three of them at 5 times the
-// rate of fp32's own matrix instructions.  G is summed and subtracted in fp64: after a strong decay
-// the differences of fp32 sums would have no digits left.
+// rate of fp32's own matrix instructions.  G is summed in fp64 and kept as two floats: after a strong
+// decay the differences of fp32 sums would have no digits left.
 //   In the scan a wave has 16 columns of S, R and U to itself: a result tile
 // (lane: column, 4 rows 4 g .. 4 g + 3) is the next product's right operand as it
 // stands, if the left one lists its contraction as 4 g + j, 16 + 4 g + j (j < 4).
@@ -166,6 +166,19 @@ __device__ __forceinline__ void split(float x, _Float16 & hi, _Float16 & lo) {
     lo = (_Float16)(x - (float)hi);
 }
 
+// the largest of the 4 lanes that hold a column
+__device__ __forceinline__ float over_column(float x) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    uint32_t a = p[0], b = p[1];
+    asm("" : "+v"(a), "+v"(b));                           // they differ, though the operands do not
+    const uint32_t m = __builtin_bit_cast(uint32_t, fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)));
+    const auto q = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+    uint32_t c = q[0], d = q[1];
+    asm("" : "+v"(c), "+v"(d));
+    return fmaxf(__builtin_bit_cast(float, c), __builtin_bit_cast(float, d));
+}
+
 // A workgroup per chunk and key head: K K^T and Q K^T once, by 16 rows a wave, then
 // T and the masked Q K^T of its value heads, a wave each for up to 4 at a time: a
 // head alone on 4 waves is a chain of 7 barriers and of a triangular solve that
@@ -183,9 +196,7 @@ __global__ void __launch_bounds__(256) gdn_prep_kernel(GdnArgs a) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[PL > LX ? PL : LX];
     _Float16 (* const pl)[C][P] = reinterpret_cast<_Float16 (*)[C][P]>(lds);      // K's terms, Q's terms
     float (* const mat)[C][M] = reinterpret_cast<float (*)[C][M]>(lds);           // one a value head
-    __shared__ float tmp[4][16][17];
-    __shared__ double G[4][C];
-    __shared__ float fk[C], fq[C], bt[4][C], ra[4][C], rt[4][C];
+    __shared__ __attribute__((aligned(16))) float Gh[4][C], Gl[4][C], fk[C], fq[C], bt[4][C];    // log2(e) G as two floats
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, g = lane >> 4;
     const int hk = blockIdx.x % a.n_kh, chunk = blockIdx.x / a.n_kh, per = a.n_vh / a.n_kh;
@@ -193,6 +204,15 @@ __global__ void __launch_bounds__(256) gdn_prep_kernel(GdnArgs a) {
     if (tl.seq < 0) return;
     const int t0 = tl.first + tl.index * C, nt = min(C, tl.count - tl.index * C);
     uint8_t * const wk = a.ws + ((int64_t)chunk * a.n_kh + hk) * W::HEAD;
+    auto head_of = [&](int r) { return a.tiled ? hk + r * a.n_kh : hk * per + r; };
+    // g and beta of this wave's value head (r0 + wave), a token a lane: before the stores, which they would wait for
+    float gate1 = 0.0f, beta1 = 0.0f;
+    auto gates = [&](int r0) __attribute__((always_inline)) {
+        if (r0 + wave >= per || lane >= nt) return;
+        gate1 = a.g[(int64_t)(t0 + lane) * a.gate_tok + head_of(r0 + wave)];
+        beta1 = a.beta[(int64_t)(t0 + lane) * a.gate_tok + head_of(r0 + wave)];
+    };
+    gates(0);
 
     // rows of K and Q: 4 threads each
     {
@@ -293,93 +313,103 @@ __global__ void __launch_bounds__(256) gdn_prep_kernel(GdnArgs a) {
         }
     }
 
-    // this wave's C x C matrix as fragments (m-tile mt, step ks), its rows divided by scale
+    // this wave's C x C matrix, its columns times col, as fragments (m-tile mt, step ks) and a factor of each row
     float (* const X)[M] = mat[wave];
-    auto put_square = [&](const float * scale, uint8_t * to) {
-#pragma unroll 2
-        for (int f = 0; f < 6; ++f) {
-            const int mt = f < 4 ? f : f - 2, ks = f >> 2, row = 16 * mt + l16;
-            const float down = 1.0f / scale[row];
-            const v4f x = *reinterpret_cast<const v4f *>(&X[row][32 * ks + 4 * g]);
-            const v4f y = *reinterpret_cast<const v4f *>(&X[row][32 * ks + 16 + 4 * g]);
-            v8h hi, lo;
+    auto put_square = [&](const float * col, uint8_t * to, float * factor) __attribute__((always_inline)) {
+        float c[2][8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                _Float16 h, l;
-                split((j < 4 ? x[j & 3] : y[j & 3]) * down, h, l);
-                hi[j] = h;
-                lo[j] = l;
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) c[ks][j] = col ? col[32 * ks + (j < 4 ? 4 * g + j : 12 + 4 * g + j)] : 1.0f;
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) {
+            float x[2][8], big = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks <= mt / 2; ++ks) {
+                const v4f y = *reinterpret_cast<const v4f *>(&X[16 * mt + l16][32 * ks + 4 * g]);
+                const v4f z = *reinterpret_cast<const v4f *>(&X[16 * mt + l16][32 * ks + 16 + 4 * g]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    x[ks][j] = (j < 4 ? y[j & 3] : z[j & 3]) * c[ks][j];
+                    big = fmaxf(big, fabsf(x[ks][j]));
+                }
             }
-            *reinterpret_cast<v8h *>(to + (2 * f) * 1024 + 16 * lane) = hi;
-            *reinterpret_cast<v8h *>(to + (2 * f + 1) * 1024 + 16 * lane) = lo;
+            const int e = exponent(over_column(big));
+            if (g == 0) factor[16 * mt + l16] = pow2(e);
+            const float down = pow2(-e);
+#pragma unroll
+            for (int ks = 0; ks <= mt / 2; ++ks) {
+                v8h hi, lo;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    _Float16 h, l;
+                    split(x[ks][j] * down, h, l);
+                    hi[j] = h;
+                    lo[j] = l;
+                }
+                const int f = ks ? mt + 2 : mt;
+                *reinterpret_cast<v8h *>(to + (2 * f) * 1024 + 16 * lane) = hi;
+                *reinterpret_cast<v8h *>(to + (2 * f + 1) * 1024 + 16 * lane) = lo;
+            }
         }
     };
     auto in_wave = []() __attribute__((always_inline)) { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };   // other lanes read it
 #pragma unroll 1
     for (int r0 = 0; r0 < per; r0 += 4) {
         const int heads = min(4, per - r0);
-        auto head = [&](int r) { return a.tiled ? hk + (r0 + r) * a.n_kh : hk * per + r0 + r; };
         const bool mine = wave < heads;
         uint8_t * const wv = a.ws + (int64_t)a.chunks * a.n_kh * W::HEAD +
-                             ((int64_t)chunk * a.n_vh + head(mine ? wave : 0)) * W::VHEAD;
+                             ((int64_t)chunk * a.n_vh + head_of(r0 + (mine ? wave : 0))) * W::VHEAD;
+        float * const vec = reinterpret_cast<float *>(wv + 2 * W::TF);
         if (mine) {
             // the sums of g, in fp64
-            const int h = head(wave);
-            double s = lane < nt ? (double)gate(a.g[(int64_t)(t0 + lane) * a.gate_tok + h]) : 0.0;
-            const float beta = lane < nt ? a.beta[(int64_t)(t0 + lane) * a.gate_tok + h] : 0.0f;
+            double s = lane < nt ? (double)gate(gate1) * 1.4426950408889634 : 0.0;
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) {
                 const double o = __shfl_up(s, d);
                 if (lane >= d) s += o;
             }
-            G[wave][lane] = s;
-            bt[wave][lane] = beta;
+            const float h = (float)s;
+            Gh[wave][lane] = h;
+            Gl[wave][lane] = (float)(s - (double)h);
+            bt[wave][lane] = lane < nt ? beta1 : 0.0f;
         }
+        gates(r0 + 4);
         __syncthreads();                                  // (and: K and Q, or the last heads' matrices, have been read)
 
-        // rows 16 wave .. of every head's matrix: Q K^T with its decay, then L
-        auto rows = [&](auto is_l) __attribute__((always_inline)) {
-            constexpr bool LL = decltype(is_l)::value;
-#pragma unroll 1
-            for (int r = 0; r < heads; ++r) {
-                float top[4] = {};
-                double Gi[4];
-                float fi[4];
+        // rows 16 wave .. of every head's matrices: Q K^T with its decay in LDS, L in registers until that has been read
+        float L[4][4][4];
+        const int row = 16 * wave + 4 * g;
+        const v4f fqi = *reinterpret_cast<const v4f *>(&fq[row]), fki = *reinterpret_cast<const v4f *>(&fk[row]);
 #pragma unroll
-                for (int i4 = 0; i4 < 4; ++i4) {
-                    const int i = 16 * wave + 4 * g + i4;
-                    Gi[i4] = G[r][i];
-                    fi[i4] = LL ? bt[r][i] * fk[i] : a.scale * fq[i];
-                }
+        for (int r = 0; r < 4; ++r)
+            if (r < heads) {
+                const v4f hi = *reinterpret_cast<const v4f *>(&Gh[r][row]), lo = *reinterpret_cast<const v4f *>(&Gl[r][row]);
+                const v4f bi = *reinterpret_cast<const v4f *>(&bt[r][row]);
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    const int j = 16 * n + l16;
-                    const double Gj = G[r][j];
-                    const float fj = fk[j];
+                for (int n = 0; n < 4; ++n)
+                    if (n <= (wave | 1)) {                // (block n = wave + 1 of even waves: the zeros beside the diagonal)
+                        const int j = 16 * n + l16;
+                        const float hj = Gh[r][j], lj = Gl[r][j], fj = fk[j];
 #pragma unroll
-                    for (int i4 = 0; i4 < 4; ++i4) {
-                        const int i = 16 * wave + 4 * g + i4;
-                        const bool in = LL ? j < i : j <= i;
-                        const float d = expf(in ? (float)(Gi[i4] - Gj) : 0.0f);
-                        const float x = in ? (LL ? kk : qk)[n][i4] * fi[i4] * fj * d : 0.0f;
-                        mat[r][i][j] = x;
-                        top[i4] = fmaxf(top[i4], fabsf(x));
-                    }
-                }
-                if (!LL)
-#pragma unroll
-                    for (int i4 = 0; i4 < 4; ++i4) {
-#pragma unroll
-                        for (int d = 1; d < 16; d <<= 1) top[i4] = fmaxf(top[i4], __shfl_xor(top[i4], d));
-                        if (l16 == 0) ra[r][16 * wave + 4 * g + i4] = pow2(exponent(top[i4]));
+                        for (int i4 = 0; i4 < 4; ++i4) {
+                            const float d = __builtin_amdgcn_exp2f((hi[i4] - hj) + (lo[i4] - lj)) * fj;
+                            mat[r][row + i4][j] = j <= row + i4 ? qk[n][i4] * (a.scale * fqi[i4]) * d : 0.0f;
+                            L[r][n][i4] = j < row + i4 ? kk[n][i4] * (bi[i4] * fki[i4]) * d : 0.0f;
+                        }
                     }
             }
-        };
-        rows(std::false_type{});
         __syncthreads();
-        if (mine) put_square(ra[wave], wv + W::TF);
+        if (mine) put_square(nullptr, wv + W::TF, vec + 3 * C);
         __syncthreads();
-        rows(std::true_type{});
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (r < heads)
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+                    if (n <= (wave | 1))
+#pragma unroll
+                        for (int i4 = 0; i4 < 4; ++i4) mat[r][row + i4][16 * n + l16] = L[r][n][i4];
         __syncthreads();
         if (mine) {
             // X = (I + L)^-1 in L's place.  Diagonal blocks of 16 (block g: a lane per column): forward substitution
@@ -397,71 +427,62 @@ __global__ void __launch_bounds__(256) gdn_prep_kernel(GdnArgs a) {
                 for (int i = 0; i < 16; ++i) X[16 * g + i][16 * g + l16] = x[i];
                 in_wave();
             }
-            // below it, column by column: X_ij = -X_ii sum_l L_il X_lj.  A column of L is not needed once its X is there
-#pragma unroll 1
-            for (int j = 0; j < 3; ++j)
-#pragma unroll 1
-                for (int i = j + 1; i < 4; ++i) {
-                    v4f s = {};
-                    for (int l = j; l < i; ++l)
+            // below it, first for the two diagonal blocks of 32, then for the whole: with Y = L_21 X_11, X_21 = -X_22 Y
+            auto mul = [&](int i, int l, int j, v4f & to) __attribute__((always_inline)) {    // blocks of 16: to += (i, l) (l, j)
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            s = __builtin_amdgcn_mfma_f32_16x16x4f32(X[16 * i + l16][16 * l + 4 * k + g],
-                                                                     X[16 * l + 4 * k + g][16 * j + l16], s, 0, 0, 0);
+                for (int k = 0; k < 4; ++k)
+                    to = __builtin_amdgcn_mfma_f32_16x16x4f32(X[16 * i + l16][16 * l + 4 * k + g], X[16 * l + 4 * k + g][16 * j + l16], to, 0, 0, 0);
+            };
+            auto put = [&](int i, int j, const v4f & x, float sign) __attribute__((always_inline)) {
 #pragma unroll
-                    for (int i4 = 0; i4 < 4; ++i4) tmp[wave][4 * g + i4][l16] = s[i4];
-                    in_wave();
-                    v4f x = {};
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        x = __builtin_amdgcn_mfma_f32_16x16x4f32(X[16 * i + l16][16 * i + 4 * k + g],
-                                                                 tmp[wave][4 * k + g][l16], x, 0, 0, 0);
-#pragma unroll
-                    for (int i4 = 0; i4 < 4; ++i4) X[16 * i + 4 * g + i4][16 * j + l16] = -x[i4];
-                    in_wave();
-                }
-            // T = X diag(beta), and the largest element of its rows (a lane each)
-            float big = 0.0f;
-#pragma unroll 4
-            for (int j = 0; j < C; j += 4) {
-                v4f x = *reinterpret_cast<const v4f *>(&X[lane][j]);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    x[k] *= bt[wave][j + k];
-                    big = fmaxf(big, fabsf(x[k]));
-                }
-                *reinterpret_cast<v4f *>(&X[lane][j]) = x;
+                for (int i4 = 0; i4 < 4; ++i4) X[16 * i + 4 * g + i4][16 * j + l16] = sign * x[i4];
+            };
+            {
+                v4f x = {}, y = {};
+                mul(1, 0, 0, x), mul(3, 2, 2, y);
+                in_wave();
+                put(1, 0, x, 1.0f), put(3, 2, y, 1.0f);
+                in_wave();
+                x = y = v4f{};
+                mul(1, 1, 0, x), mul(3, 3, 2, y);
+                in_wave();
+                put(1, 0, x, -1.0f), put(3, 2, y, -1.0f);
+                in_wave();
             }
-            rt[wave][lane] = pow2(exponent(big));
-            in_wave();
-            put_square(rt[wave], wv);
-            // factors of the rows
-            float * const vec = reinterpret_cast<float *>(wv + 2 * W::TF);
-            const double Gi = G[wave][lane], Ge = G[wave][C - 1];
-            const float e = expf((float)Gi);
+            {
+                v4f x[2][2] = {};
+#pragma unroll
+                for (int i = 0; i < 2; ++i) mul(2 + i, 0, 0, x[i][0]), mul(2 + i, 1, 1, x[i][1]);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) mul(2 + i, 1, 0, x[i][0]);
+                in_wave();
+#pragma unroll
+                for (int i = 0; i < 2; ++i) put(2 + i, 0, x[i][0], 1.0f), put(2 + i, 1, x[i][1], 1.0f);
+                in_wave();
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) x[i][j] = v4f{}, mul(2 + i, 2 + i, j, x[i][j]);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) mul(3, 2, j, x[1][j]);
+                in_wave();
+#pragma unroll
+                for (int i = 0; i < 2; ++i) put(2 + i, 0, x[i][0], -1.0f), put(2 + i, 1, x[i][1], -1.0f);
+                in_wave();
+            }
+            put_square(bt[wave], wv, vec + 2 * C);        // T
+            // the other factors of the rows
+            const float hi = Gh[wave][lane], lo = Gl[wave][lane];
+            const float e = __builtin_amdgcn_exp2f(hi + lo);
             vec[lane] = e * fk[lane];
             vec[C + lane] = e * fq[lane] * a.scale;
-            vec[2 * C + lane] = rt[wave][lane];
-            vec[3 * C + lane] = ra[wave][lane];
-            vec[4 * C + lane] = expf((float)(Ge - Gi)) * fk[lane];
-            vec[5 * C + lane] = expf((float)Ge);
+            vec[4 * C + lane] = __builtin_amdgcn_exp2f((Gh[wave][C - 1] - hi) + (Gl[wave][C - 1] - lo)) * fk[lane];
+            vec[5 * C + lane] = __builtin_amdgcn_exp2f(Gh[wave][C - 1] + Gl[wave][C - 1]);
         }
         if (r0 + 4 < per) __syncthreads();                // G, bt and the matrices are written anew
     }
 }
 
-// the largest of the 4 lanes that hold a column
-__device__ __forceinline__ float over_column(float x) {
-    const uint32_t u = __builtin_bit_cast(uint32_t, x);
-    const auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    uint32_t a = p[0], b = p[1];
-    asm("" : "+v"(a), "+v"(b));                           // they differ, though the operands do not
-    const uint32_t m = __builtin_bit_cast(uint32_t, fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)));
-    const auto q = __builtin_amdgcn_permlane32_swap(m, m, false, false);
-    uint32_t c = q[0], d = q[1];
-    asm("" : "+v"(c), "+v"(d));
-    return fmaxf(__builtin_bit_cast(float, c), __builtin_bit_cast(float, d));
-}
 template <int N>
 __device__ __forceinline__ float largest(const v4f (&x)[N]) {
     float big[2] = {0.0f, 0.0f};
