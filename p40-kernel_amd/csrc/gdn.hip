@@ -494,10 +494,10 @@ __device__ __forceinline__ float largest(const v4f (&x)[N]) {
 }
 
 // 16 PAIRS columns of a value head, 16 for each pair of waves, of which one has
-// the chain, the other the outputs, a phase behind it:
-//   first:  S as operands, K S    | QK^T U of the last chunk, its outputs
+// the chain, the other the outputs and the loads:
+//   first:  S as operands, K S    | loads, the last chunk's outputs leave
 //   second: U                     | Q S
-//   third:  S                     |
+//   third:  S                     | QK^T U, the outputs
 // S as operands and U go from the one to the other through LDS.  A chunk's 180
 // products (16-bit rows: 132) of 16 columns are 2900 clocks of MFMA; what bounds it
 // is the chain of dependent instructions around them (largest of a column, split,
@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(128 * PAIRS) gdn_scan_kernel(GdnArgs a) {
     typedef typename T::elem elem;
     typedef Work<T, K> W;
     typedef elem Unit __attribute__((ext_vector_type(16 / sizeof(elem))));
-    constexpr int KS = K / 32, KT = K / 16, NW = 2 * PAIRS, TERMS = W::TERMS;
+    constexpr int KS = K / 32, KT = K / 16, TERMS = W::TERMS;
     constexpr int EB = sizeof(elem), UNITS = EB, RPI = 64 / UNITS;    // 16-byte units of 16 columns; rows of a load
     // LDS: K, Q and K^T in two buffers in turn, T, QK^T, factors; then for each pair V, U (and outputs), S as operands and its scale
     constexpr int AT_T = 2 * W::KF, AT_A = AT_T + W::TF, AT_VEC = AT_A + W::TF;
@@ -552,20 +552,21 @@ __global__ void __launch_bounds__(128 * PAIRS) gdn_scan_kernel(GdnArgs a) {
     chunk0 = __builtin_amdgcn_readfirstlane(chunk0);
     chunks = iclamp(chunks, 0, max(a.chunks - chunk0, 0));   // starts that overlap: what prep made, no more
 
-    // a run of 1 KB pieces for each wave, 4 of them an address
+    // (waves of the outputs) a run of 1 KB pieces for each, 4 of them an address
+    const int loader = wave - PAIRS;
     auto copy = [&](const uint8_t * src, uint8_t * dst, auto bytes) __attribute__((always_inline)) {
-        constexpr int N = decltype(bytes)::value / 1024, OWN1 = N / NW;
+        constexpr int N = decltype(bytes)::value / 1024, OWN1 = N / PAIRS;
         const auto from = buffer_of(src, N * 1024);
 #pragma unroll
         for (int i = 0; i < OWN1; i += 4) {
-            const int at = (wave * OWN1 + i) * 1024;
+            const int at = (loader * OWN1 + i) * 1024;
             dma16_at<0>(from, dst + at, 16 * lane, at);
             if (i + 1 < OWN1) dma16_at<1024>(from, dst + at, 16 * lane, at);
             if (i + 2 < OWN1) dma16_at<2048>(from, dst + at, 16 * lane, at);
             if (i + 3 < OWN1) dma16_at<3072>(from, dst + at, 16 * lane, at);
         }
-        if (N % NW != 0 && wave < N % NW) {
-            const int at = (N / NW * NW + wave) * 1024;
+        if (N % PAIRS != 0 && loader < N % PAIRS) {
+            const int at = (N / PAIRS * PAIRS + loader) * 1024;
             dma16(from, dst + at, 16 * lane, at);
         }
     };
@@ -575,9 +576,9 @@ __global__ void __launch_bounds__(128 * PAIRS) gdn_scan_kernel(GdnArgs a) {
     };
     const std::integral_constant<int, W::KF> kf_bytes;
     const std::integral_constant<int, W::TF> tf_bytes;
-    // all but the `left` latest loads of every wave are there, and what the waves read of LDS before has been read
-    auto sync = [&](auto left) __attribute__((always_inline)) {
-        pq2::wait_vmcnt<decltype(left)::value>();
+    // the loads are there, and what the waves read of LDS before has been read
+    auto sync = [&]() __attribute__((always_inline)) {
+        pq2::wait_vmcnt<0>();
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
@@ -694,7 +695,7 @@ __global__ void __launch_bounds__(128 * PAIRS) gdn_scan_kernel(GdnArgs a) {
     v8h rh[2], rl[2];                                     // w U as right operand
     auto column = [&](uint8_t * base) __attribute__((always_inline)) { return reinterpret_cast<elem *>(base) + 16 * g + l16; };
 
-    auto outputs = [&](const uint8_t * af, uint8_t * u, int c) __attribute__((always_inline)) {
+    auto outputs = [&](const uint8_t * __restrict__ af, uint8_t * __restrict__ u) __attribute__((always_inline)) {
         v4f Um[4];
 #pragma unroll
         for (int m = 0; m < 4; ++m) Um[m] = *reinterpret_cast<const v4f *>(u + 1024 * m + 16 * lane);
@@ -708,20 +709,18 @@ __global__ void __launch_bounds__(128 * PAIRS) gdn_scan_kernel(GdnArgs a) {
             for (int j = 0; j < 4; ++j)
                 own[(16 * m + 4 * j) * 16] = T::from(fmaf(x[m][j], ca[m][j] * fu, cq[m][j] * fs * ks[m][j]));
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");    // other lanes read it
-        put(u, c);
     };
-    auto phase1 = [&](const uint8_t * __restrict__ k, uint8_t * __restrict__ q, uint8_t * __restrict__ t,
-                      uint8_t * __restrict__ vec, uint8_t * __restrict__ v, const uint8_t * __restrict__ af, uint8_t * __restrict__ u,
-                      uint8_t * __restrict__ sf, int c) __attribute__((always_inline)) {
-        copy(key_part(c) + W::KF, q, kf_bytes);
-        copy(value_part(c), t, tf_bytes);
-        copy(value_part(c) + 2 * W::TF, vec, std::integral_constant<int, W::VEC>{});
-        if (work && chain) stage_v(c, v);
-        if (!work) return;
+    auto phase1 = [&](const uint8_t * __restrict__ k, uint8_t * __restrict__ q, uint8_t * __restrict__ t, uint8_t * __restrict__ vec,
+                      uint8_t * __restrict__ v, const uint8_t * __restrict__ u, uint8_t * __restrict__ sf, int c) __attribute__((always_inline)) {
         if (!chain) {
-            if (c > 0) outputs(af, u, c - 1);
+            copy(key_part(c) + W::KF, q, kf_bytes);
+            copy(value_part(c), t, tf_bytes);
+            copy(value_part(c) + 2 * W::TF, vec, std::integral_constant<int, W::VEC>{});
+            if (work) stage_v(c, v);
+            if (work && c > 0) put(u, c - 1);
             return;
         }
+        if (!work) return;
         const int e = exponent(big);
         const float down = pow2(-e);
         fs = pow2(e);
@@ -751,8 +750,10 @@ __global__ void __launch_bounds__(128 * PAIRS) gdn_scan_kernel(GdnArgs a) {
     auto phase2 = [&](uint8_t * __restrict__ k, const uint8_t * __restrict__ q, const uint8_t * __restrict__ t,
                       const uint8_t * __restrict__ vec, uint8_t * __restrict__ v, uint8_t * __restrict__ af, uint8_t * __restrict__ u,
                       const uint8_t * __restrict__ sf, int c) __attribute__((always_inline)) {
-        copy(key_part(c) + 2 * W::KF, k, kf_bytes);
-        copy(value_part(c) + W::TF, af, tf_bytes);        // last: it may be on its way still after the phase
+        if (!chain) {
+            copy(key_part(c) + 2 * W::KF, k, kf_bytes);
+            copy(value_part(c) + W::TF, af, tf_bytes);
+        }
         if (!work) return;
         auto factor = [&](int which, int m) {
             return *reinterpret_cast<const v4f *>(vec + 4 * (which * C + 16 * m + 4 * g));
@@ -801,9 +802,14 @@ __global__ void __launch_bounds__(128 * PAIRS) gdn_scan_kernel(GdnArgs a) {
 #pragma unroll
         for (int m = 0; m < 4; ++m) to_right(Um[m], pow2(-e), rh[m / 2], rl[m / 2], m & 1);
     };
-    auto phase3 = [&](const uint8_t * __restrict__ kt, uint8_t * __restrict__ k, int c) __attribute__((always_inline)) {
-        if (c + 1 < chunks) copy(key_part(c + 1), k, kf_bytes);
-        if (!work || !chain) return;
+    auto phase3 = [&](const uint8_t * __restrict__ kt, uint8_t * __restrict__ k, const uint8_t * __restrict__ af,
+                      uint8_t * __restrict__ u, int c) __attribute__((always_inline)) {
+        if (!chain) {
+            if (c + 1 < chunks) copy(key_part(c + 1), k, kf_bytes);
+            if (work) outputs(af, u);
+            return;
+        }
+        if (!work) return;
         float top[2] = {0.0f, 0.0f};
         v4f y[4];
         products(std::integral_constant<int, KT / 2>{}, own_terms, four,
@@ -826,22 +832,18 @@ __global__ void __launch_bounds__(128 * PAIRS) gdn_scan_kernel(GdnArgs a) {
     };
 
     uint8_t * const v = lds + AT_V + pair * V_PAIR, * const u = lds + AT_U + pair * U_PAIR, * const sf = lds + AT_S + pair * S_PAIR;
-    const std::integral_constant<int, 0> none;
-    if (chunks > 0) copy(key_part(0), lds, kf_bytes);
+    if (chunks > 0 && !chain) copy(key_part(0), lds, kf_bytes);
 #pragma clang loop unroll(disable)
     for (int c = 0; c < chunks; ++c) {
         uint8_t * const one = lds + (c & 1) * W::KF, * const two = lds + (~c & 1) * W::KF;
-        sync(none);                                       // K is in the one, the last chunk's QK^T and U are there
-        phase1(one, two, lds + AT_T, lds + AT_VEC, v, lds + AT_A, u, sf, c);
-        sync(none);                                       // Q is in the two, S there as operands
+        sync();                                           // K is in the one
+        phase1(one, two, lds + AT_T, lds + AT_VEC, v, u, sf, c);
+        sync();                                           // Q is in the two, T, V and S as operands are there
         phase2(one, two, lds + AT_T, lds + AT_VEC, v, lds + AT_A, u, sf, c);
-        sync(std::integral_constant<int, W::TF / 1024 / NW>{});    // K^T is in the one, QK^T on its way
-        phase3(one, two, c);
+        sync();                                           // K^T is in the one, QK^T and U are there
+        phase3(one, two, lds + AT_A, u, c);
     }
-    if (chunks > 0) {
-        sync(none);
-        if (work && !chain) outputs(lds + AT_A, u, chunks - 1);
-    }
+    if (chunks > 0 && work && !chain) put(u, chunks - 1);
     if (!work || !chain) return;
 #pragma unroll
     for (int i = 0; i < KT; ++i)
