@@ -160,10 +160,21 @@ __global__ void __launch_bounds__(128) gdn_step_kernel(GdnArgs a) {
 }
 
 // ---------------------------------------------------------------------- chunks
-// x (about 1 at most) as two f16 terms
-__device__ __forceinline__ void split(float x, _Float16 & hi, _Float16 & lo) {
-    hi = (_Float16)x;
-    lo = (_Float16)(x - (float)hi);
+// elements at .. at + N - 1 of the two f16 terms of x down (about 1 at most)
+template <int N>
+__device__ __forceinline__ void split(const float * x, float down, v8h & hi, v8h & lo, int at) {
+    typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+        uint32_t u = __builtin_bit_cast(uint32_t, v2h{(_Float16)(x[j] * down), (_Float16)(x[j + 1] * down)});
+        asm("" : "+v"(u));                                // or each is converted a second time for its rest
+        const v2h h = __builtin_bit_cast(v2h, u);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            hi[at + j + i] = h[i];
+            lo[at + j + i] = (_Float16)fmaf(x[j + i], down, -(float)h[i]);
+        }
+    }
 }
 
 // the largest of the 4 lanes that hold a column
@@ -181,9 +192,11 @@ __device__ __forceinline__ float over_column(float x) {
 
 // A workgroup per chunk and key head: K K^T and Q K^T once, by 16 rows a wave, then
 // T and the masked Q K^T of its value heads, a wave each for up to 4 at a time: a
-// head alone on 4 waves is a chain of 7 barriers and of a triangular solve that
-// does not fill them.  The heads' C x C matrices take the place of K and Q in
-// LDS, so that two workgroups share a CU.
+// head alone on 4 waves is a chain of barriers and of a triangular solve that does
+// not fill them.  The heads' C x C matrices take the place of K and Q in LDS, one
+// after the other, so that two workgroups share a CU.  2048 tokens, 16 key and 48
+// value heads of 128 (MI355X): 25 us fp32, of which the rows of K and Q take 4, the
+// two squares 5, the inverse 4; 93 MB written.
 template <class T, int K>
 __global__ void __launch_bounds__(256) gdn_prep_kernel(GdnArgs a) {
     typedef typename T::elem elem;
@@ -245,13 +258,7 @@ __global__ void __launch_bounds__(256) gdn_prep_kernel(GdnArgs a) {
 #pragma unroll
             for (int j = 0; j < N; j += 8) {
                 v8h hi, lo;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    _Float16 h, l;
-                    split(x[m][j + i] * down, h, l);
-                    hi[i] = h;
-                    lo[i] = l;
-                }
+                split<8>(&x[m][j], down, hi, lo, 0);
                 *reinterpret_cast<v8h *>(&pl[TERMS * m][row][part * N + j]) = hi;
                 if (TERMS == 2) *reinterpret_cast<v8h *>(&pl[TERMS * m + 1][row][part * N + j]) = lo;
             }
@@ -340,13 +347,7 @@ __global__ void __launch_bounds__(256) gdn_prep_kernel(GdnArgs a) {
 #pragma unroll
             for (int ks = 0; ks <= mt / 2; ++ks) {
                 v8h hi, lo;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    _Float16 h, l;
-                    split(x[ks][j] * down, h, l);
-                    hi[j] = h;
-                    lo[j] = l;
-                }
+                split<8>(x[ks], down, hi, lo, 0);
                 const int f = ks ? mt + 2 : mt;
                 *reinterpret_cast<v8h *>(to + (2 * f) * 1024 + 16 * lane) = hi;
                 *reinterpret_cast<v8h *>(to + (2 * f + 1) * 1024 + 16 * lane) = lo;
@@ -501,13 +502,14 @@ __device__ __forceinline__ float largest(const v4f (&x)[N]) {
 // S as operands and U go from the one to the other through LDS.  A chunk's 180
 // products (16-bit rows: 132) of 16 columns are 2900 clocks of MFMA; what bounds it
 // is the chain of dependent instructions around them (largest of a column, split,
-// convert, rescale).  One wave that does both takes 11000 clocks a chunk, two 8900.
+// convert, rescale) and the LDS reads before them.  One wave that does it all takes
+// 11000 clocks a chunk, the pair 6700, of which U is 2600.
 //   K, Q and K^T of a chunk follow one another through two buffers, each asked for
 // a phase ahead: with a third one PAIRS = 4 would not fit beside fp32's fragments,
-// and it gains nothing (2048 tokens of one sequence, us: 150 against 153).
+// and it gains nothing (2048 tokens of one sequence, both kernels, us: 150 against 153).
 //   2 pairs or 4 (half the fragments' bytes through LDS, two waves to a SIMD):
-// gdn_wide.  MI355X, 48 value heads, 128 x 128, fp32, both kernels: 2048 tokens
-// 150 us, 8 sequences of 2048 749 us, that is 1.4 TB/s of K, Q, V and outputs.
+// gdn_wide.  MI355X, 48 value heads of 128 x 128, fp32, both kernels: 2048 tokens 116
+// us, 8 sequences of 2048 680 us, that is 1.6 TB/s of K, Q, V and outputs.
 template <class T, int K, int PAIRS>
 __global__ void __launch_bounds__(128 * PAIRS) gdn_scan_kernel(GdnArgs a) {
     typedef typename T::elem elem;
@@ -624,13 +626,8 @@ __global__ void __launch_bounds__(128 * PAIRS) gdn_scan_kernel(GdnArgs a) {
     };
     // half of a right fragment (elements 4 k ..) from a result tile, its columns scaled
     auto to_right = [](const v4f & x, float down, v8h & hi, v8h & lo, int k) __attribute__((always_inline)) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            _Float16 h, l;
-            split(x[j] * down, h, l);
-            hi[4 * k + j] = h;
-            lo[4 * k + j] = l;
-        }
+        const float y[4] = {x[0], x[1], x[2], x[3]};
+        split<4>(y, down, hi, lo, 4 * k);
     };
     // a C x C matrix times a right operand: step 0 for all m-tiles, step 1 for the lower two
     v4f x[4];

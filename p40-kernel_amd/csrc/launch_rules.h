@@ -256,18 +256,19 @@ inline bool attn_join_wide(int64_t n_split) { return n_split > 8; }
 
 // The gated delta rule (gdn.hip) in chunks of 64 tokens (true), or token by token:
 // a chunk takes the same time however few tokens it has, a token by itself about 1.1
-// us for one sequence, 2 for 8 and 4.3 for 48.  Measured on MI355X (us, by token / in
-// chunks, fp32, 48 heads of 128): 1 sequence of 16 20.4 / 30.2, 24 29.1 / 30.3, 32
-// 37.3 / 30.3; 8 of 16 41.8 / 50.5, 24 56.7 / 50.7; 48 of 8 137 / 203, 16 210 / 204,
-// 24 282 / 206; bf16 1 of 16 22.4 / 27.7, 24 31.7 / 27.6, 48 of 16 183 / 186.
-inline bool gdn_chunked(int64_t max_new) { return max_new > 16; }
+// us for one sequence, 2 for 8 and 4.5 for 48.  Measured on MI355X (us, by token / in
+// chunks, 48 heads of 128): fp32, 1 sequence of 12 16.3 / 21.2, 16 20.6 / 21.2, 20 24.7 /
+// 21.3; 8 of 12 33.2 / 40.1, 16 41.1 / 40.3, 24 55.4 / 40.5; 48 of 8 137 / 173, 12 172 /
+// 175, 16 208 / 176; bf16, 1 of 12 17.7 / 18.7, 16 22.4 / 18.8; 8 of 12 34.7 / 36.5, 16 42.7 /
+// 36.4; 48 of 10 127 / 159, 12 146 / 160, 16 180 / 160.
+inline bool gdn_chunked(int64_t max_new) { return max_new > 13; }
 
 // Columns of a value head that a workgroup of the chunked form takes: 32 (2 pairs of
 // waves) while that leaves no workgroup waiting for a CU, else 64 (4 pairs, true),
 // whose waves share SIMDs and fragments.  Measured on MI355X (256 CUs, us, 32 / 64
-// columns, fp32, 48 heads of 128): 1 sequence of 2048 tokens (192 workgroups of 32)
-// 150 / 172, 2 of 1000 (384) 152 / 107, 8 of 2048 1008 / 749; bf16 127 / 149, 130 /
-// 93, 850 / 597.
+// columns, 48 heads of 128): fp32, 1 sequence of 2048 tokens (192 workgroups of 32) 124 /
+// 149, 2 of 1000 (384) 126 / 93, 4 of 500 107 / 95, 8 of 2048 953 / 691; bf16 109 / 130, 111
+// / 81, 93 / 82, 786 / 550.
 inline bool gdn_wide(int64_t heads, int64_t v_dim, int64_t cus) { return heads * ((v_dim + 31) / 32) > cus; }
 
 }  // namespace pq2

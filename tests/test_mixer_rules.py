@@ -70,7 +70,7 @@ def test_attn_join(rules, n_split, wide):
     assert rules.attn_join_wide(I64(n_split)) == wide
 
 
-@pytest.mark.parametrize("max_new,chunked", [(1, 0), (16, 0), (17, 1), (1 << 30, 1)])
+@pytest.mark.parametrize("max_new,chunked", [(1, 0), (12, 0), (13, 0), (14, 1), (16, 1), (1 << 30, 1)])
 def test_gdn_form(rules, max_new, chunked):
     assert rules.gdn_chunked(I64(max_new)) == chunked
 
