@@ -2,8 +2,8 @@
 // matmul path, kept so a host written against include/bonsai_p40.h links.
 //   * bonsai_p40_rmsnorm: per-row RMSNorm, y = x * (1/sqrt(mean(x^2)+eps)) * w
 //     (src/ops.h:13-22; the reference device kernel is elementwise_p40.cu:48-88);
-//   * bonsai_p40_gdn_step / bonsai_p40_attn: outside this library's scope,
-//     they return 2 without touching memory;
+//   * bonsai_p40_gdn_step / bonsai_p40_attn: not in this library (attn_paged.hip
+//     and gdn.hip have other interfaces), they return 2 without touching memory;
 // plus bonsai_p40_reload_tuning, which re-reads the library's BONSAI_* tuning
 // variables (read once per process otherwise).
 #include "pq2_device.h"
