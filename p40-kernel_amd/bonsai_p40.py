@@ -478,10 +478,10 @@ def _type(t) -> int:
     return ty
 
 
-def _flat(t, name: str, dtype, shape, dev: int) -> int:
-    """The address of t, which has this type and shape, lies in one piece and on device dev."""
-    if _TYPES.get(t.dtype) != dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != dev:
-        raise ValueError(f"{name}: contiguous {'fp32' if dtype == F32 else dtype} {shape} beside q is wanted, "
+def _flat(t, name: str, dtype, n: int, dev: int) -> int:
+    """The address of t, which has n elements of this type, lies in one piece and on device dev."""
+    if t.numel() != n or _TYPES.get(t.dtype) != dtype or not t.is_contiguous() or t.get_device() != dev:
+        raise ValueError(f"{name}: {n} contiguous {'fp32' if dtype == F32 else dtype} beside q are wanted, "
                          f"not {t.dtype} {tuple(t.shape)} of strides {t.stride()} on {t.device}")
     return t.data_ptr()
 
@@ -489,7 +489,7 @@ def _flat(t, name: str, dtype, shape, dev: int) -> int:
 def _rows(t, name: str, shape, dev: int) -> int:
     """The token stride of (token, head, element) rows on device dev whose heads follow each other."""
     if t.shape != shape or t.get_device() != dev:
-        raise ValueError(f"{name}: shape {tuple(t.shape)} on {t.device}, wanted {shape} beside q")
+        raise ValueError(f"{name}: shape {tuple(t.shape)} on {t.device}, wanted {tuple(shape)} beside q")
     n, heads, dim = shape
     tok, head, el = t.stride()
     if (el != 1 and dim != 1) or (head != dim and heads != 1):
@@ -500,13 +500,14 @@ def _rows(t, name: str, shape, dev: int) -> int:
 def _pages(k_pages, v_pages, dev: int):
     """(n_pages, n_kv_head, page_size, head_dim) pages of keys and values: shape, page stride and type."""
     shape, st = k_pages.shape, k_pages.stride()
-    if (len(shape) != 4 or v_pages.shape != shape or v_pages.stride() != st or v_pages.dtype != k_pages.dtype
-            or k_pages.get_device() != dev or v_pages.get_device() != dev):
+    if (len(st) != 4 or v_pages.shape != shape or v_pages.stride() != st or v_pages.dtype is not k_pages.dtype
+            or not dev == k_pages.get_device() == v_pages.get_device()):
         raise ValueError("k_pages and v_pages: alike, (n_pages, n_kv_head, page_size, head_dim), beside q")
     n, h, p, d = shape
-    if (st[3] != 1 and d != 1) or (st[2] != d and p != 1) or (st[1] != p * d and h != 1):
+    page, head, row, el = st
+    if (el != 1 and d != 1) or (row != d and p != 1) or (head != p * d and h != 1):
         raise ValueError("a page has to lie in one piece")
-    return shape, st[0] if n > 1 else max(st[0], h * p * d), _type(k_pages)
+    return n, h, p, d, page if n > 1 else max(page, h * p * d), _type(k_pages)
 
 
 def rope_inv_freq(n_rot: int, base: float, device="cuda"):
@@ -536,25 +537,27 @@ def _stream_of(q, stream) -> int | None:
 
 
 def _qk_norm_rope_args(q, k, v, q_norm, k_norm, eps, pos, inv_freq, slots, k_pages, v_pages, q_out, interleaved):
-    if q.dim() != 3 or k.dim() != 3:
+    shape, ks, qt = q.shape, k.shape, q.stride()
+    if len(qt) != 3 or len(ks) != 3:
         raise ValueError("q, k and v: (n_tok, heads, head_dim) is wanted")
-    n, h, d = shape = q.shape
-    kv = k.shape[1]
-    if not _type(q) == _type(k) == _type(v) == F32:
+    n, h, d = shape
+    nk, kv, dk = ks
+    ty = q.dtype
+    if _type(q) != F32 or k.dtype is not ty or v.dtype is not ty:
         raise ValueError("q, k and v: fp32 is wanted")
     dev = q.get_device()
-    if k.shape != (n, kv, d) or v.shape != k.shape or not dev == k.get_device() == v.get_device():
-        raise ValueError(f"k, v: shapes {tuple(k.shape)}, {tuple(v.shape)} beside q's {tuple(shape)}, on one device")
-    (pages, page_kv, page_size, page_d), stride, kv_type = _pages(k_pages, v_pages, dev)
+    if nk != n or dk != d or v.shape != ks or not dev == k.get_device() == v.get_device():
+        raise ValueError(f"k, v: shapes {tuple(ks)}, {tuple(v.shape)} beside q's {tuple(shape)}, on one device")
+    pages, page_kv, page_size, page_d, stride, kv_type = _pages(k_pages, v_pages, dev)
     if page_kv != kv or page_d != d:
         raise ValueError("the pages have other heads")
     half = 0 if inv_freq is None else inv_freq.numel()
     return QkNormRopeArgs.pack(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride(), *k.stride(), *v.stride(), n, h, kv, d, 2 * half,
-        1 if interleaved else 0, eps, 0 if q_norm is None else _flat(q_norm, "q_norm", F32, (d,), dev),
-        0 if k_norm is None else _flat(k_norm, "k_norm", F32, (d,), dev),
-        _flat(pos, "pos", "int32", (n,), dev) if half else 0, _flat(inv_freq, "inv_freq", "float64", (half,), dev) if half else 0,
-        _flat(slots, "slots", "int64", (n,), dev), q_out.data_ptr(), _rows(q_out, "q_out", shape, dev), _type(q_out), kv_type,
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), *qt, *k.stride(), *v.stride(), n, h, kv, d, 2 * half,
+        1 if interleaved else 0, eps, 0 if q_norm is None else _flat(q_norm, "q_norm", F32, d, dev),
+        0 if k_norm is None else _flat(k_norm, "k_norm", F32, d, dev),
+        _flat(pos, "pos", "int32", n, dev) if half else 0, _flat(inv_freq, "inv_freq", "float64", half, dev) if half else 0,
+        _flat(slots, "slots", "int64", n, dev), q_out.data_ptr(), _rows(q_out, "q_out", shape, dev), _type(q_out), kv_type,
         k_pages.data_ptr(), v_pages.data_ptr(), pages, stride, page_size)
 
 
@@ -566,29 +569,33 @@ def qk_norm_rope(q, k, v, q_norm, k_norm, eps: float, pos, inv_freq, slots, k_pa
     a head or the tokens consecutive (Y.view(heads, head_dim, n_tok).permute(2, 0,
     1) of a gemm)."""
     a = _qk_norm_rope_args(q, k, v, q_norm, k_norm, eps, pos, inv_freq, slots, k_pages, v_pages, q_out, interleaved)
-    _check("bonsai_p40_qk_norm_rope", lib().bonsai_p40_qk_norm_rope(a, _stream_of(q, stream)))
+    rc = lib().bonsai_p40_qk_norm_rope(a, _stream_of(q, stream))
+    if rc:
+        _check("bonsai_p40_qk_norm_rope", rc)
 
 
 def _attn_args(q, k_pages, v_pages, table, starts, kv_len, out, workspace, max_kv, scale):
-    if q.dim() != 3 or table.dim() != 2:
+    shape, entries, steps = q.shape, table.shape, table.stride()
+    if len(shape) != 3 or len(steps) != 2:
         raise ValueError("q: (n_tok, heads, head_dim) and table: (n_seq, max_pages) are wanted")
-    n, h, d = shape = q.shape
+    n, h, d = shape
     io = _type(q)
-    if _type(out) != io:
+    if out.dtype is not q.dtype:
         raise ValueError("out has to have q's type")
     dev = q.get_device()
-    (pages, kv, page_size, page_d), stride, kv_type = _pages(k_pages, v_pages, dev)
+    pages, kv, page_size, page_d, stride, kv_type = _pages(k_pages, v_pages, dev)
     if page_d != d:
         raise ValueError("the pages have another head_dim")
-    n_seq, cols = table.shape
-    row, col = table.stride()
+    n_seq, cols = entries
+    row, col = steps
     if _TYPES.get(table.dtype) != "int32" or (col != 1 and cols > 1) or table.get_device() != dev:
         raise ValueError("table: int32 rows beside q are wanted")
+    ws, ws_bytes = _scratch(workspace, dev)
     return AttnPagedArgs.pack(
         q.data_ptr(), out.data_ptr(), _rows(q, "q", shape, dev), _rows(out, "out", shape, dev), n, n_seq, h, kv, d, io, kv_type,
         d ** -0.5 if scale is None else scale, k_pages.data_ptr(), v_pages.data_ptr(), pages, stride, page_size, cols,
-        table.data_ptr(), row if n_seq > 1 else cols, _flat(starts, "starts", "int32", (n_seq + 1,), dev),
-        _flat(kv_len, "kv_len", "int32", (n_seq,), dev), max_kv, *_scratch(workspace, dev))
+        table.data_ptr(), row if n_seq > 1 else cols, _flat(starts, "starts", "int32", n_seq + 1, dev),
+        _flat(kv_len, "kv_len", "int32", n_seq, dev), max_kv, ws, ws_bytes)
 
 
 def attn_paged_workspace_bytes(q, k_pages, v_pages, table, starts, kv_len, out, max_kv: int = 0, scale=None) -> int:
@@ -603,32 +610,41 @@ def attn_paged(q, k_pages, v_pages, table, starts, kv_len, out, workspace=None, 
     starts[s + 1] - 1 of q and out, (n_tok, heads, head_dim)) over its kv_len[s] keys
     in the pages table[s]; scale None: head_dim^-1/2."""
     a = _attn_args(q, k_pages, v_pages, table, starts, kv_len, out, workspace, max_kv, scale)
-    _check("bonsai_p40_attn_paged", lib().bonsai_p40_attn_paged(a, _stream_of(q, stream)))
+    rc = lib().bonsai_p40_attn_paged(a, _stream_of(q, stream))
+    if rc:
+        _check("bonsai_p40_attn_paged", rc)
 
 
 def _gdn_args(q, k, v, g, beta, state, state_out, out, starts, workspace, max_new, slots, scale, l2_eps, tiled):
-    if q.dim() != 3 or v.dim() != 3 or starts.dim() != 1 or state.dim() != 4:
-        raise ValueError("q, k, v: (n_tok, heads, dim), state: (n_states, heads, k_dim, v_dim), starts: (n_seq + 1,)")
-    n, kh, kd = qs = q.shape
-    _, vh, vd = v.shape
-    ty = _type(q)
-    if _type(k) != ty or _type(v) != ty or _type(out) != ty:
+    qs, vs, ss, gs = q.shape, v.shape, state.shape, g.stride()
+    if len(qs) != 3 or len(vs) != 3 or starts.dim() != 1 or len(ss) != 4 or len(gs) != 2:
+        raise ValueError("q, k, v: (n_tok, heads, dim), g, beta: (n_tok, v_heads), state: (n_states, v_heads, k_dim, v_dim) and "
+                         "starts: (n_seq + 1,) are wanted")
+    n, kh, kd = qs
+    nv, vh, vd = vs
+    states, sh, sk, sv = ss
+    ty, dt = _type(q), q.dtype
+    if k.dtype is not dt or v.dtype is not dt or out.dtype is not dt:
         raise ValueError("q, k, v and out: one type is wanted")
     dev = q.get_device()
-    if (_type(g) != F32 or _type(beta) != F32 or g.shape != (n, vh) or beta.shape != g.shape
+    if nv != n or sh != vh or sk != kd or sv != vd or state_out.shape != ss:
+        raise ValueError(f"v, state, state_out: shapes {tuple(vs)}, {tuple(ss)}, {tuple(state_out.shape)} beside q's {tuple(qs)}")
+    if (_type(g) != F32 or beta.dtype is not g.dtype or g.shape != (n, vh) or beta.shape != g.shape
             or not dev == g.get_device() == beta.get_device()):
         raise ValueError(f"g and beta: fp32 ({n}, {vh}) beside q is wanted")
-    (gt, gh), (bt, bh) = g.stride(), beta.stride()
+    gt, gh = gs
+    bt, bh = beta.stride()
     if (vh > 1 and not gh == bh == 1) or (n > 1 and gt != bt):
         raise ValueError("g and beta: one token stride, and the heads of a token consecutive")
-    ss, n_seq = (state.shape[0], vh, kd, vd), starts.shape[0] - 1
+    n_seq, all_states = starts.numel() - 1, states * vh * kd * vd
+    ws, ws_bytes = _scratch(workspace, dev)
     return GdnArgs.pack(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _rows(q, "q", qs, dev), _rows(k, "k", qs, dev),
-        _rows(v, "v", (n, vh, vd), dev), _rows(out, "out", (n, vh, vd), dev), g.data_ptr(), beta.data_ptr(), gt if n > 1 else vh,
-        _flat(state, "state", F32, ss, dev), _flat(state_out, "state_out", F32, ss, dev), ss[0],
-        0 if slots is None else _flat(slots, "slots", "int32", (n_seq,), dev),
-        _flat(starts, "starts", "int32", (n_seq + 1,), dev), n, n_seq, kh, vh, kd, vd, ty, 1 if tiled else 0,
-        kd ** -0.5 if scale is None else scale, l2_eps, max_new, *_scratch(workspace, dev))
+        _rows(v, "v", vs, dev), _rows(out, "out", vs, dev), g.data_ptr(), beta.data_ptr(), gt if n > 1 else vh,
+        _flat(state, "state", F32, all_states, dev), _flat(state_out, "state_out", F32, all_states, dev), states,
+        0 if slots is None else _flat(slots, "slots", "int32", n_seq, dev),
+        _flat(starts, "starts", "int32", n_seq + 1, dev), n, n_seq, kh, vh, kd, vd, ty, 1 if tiled else 0,
+        kd ** -0.5 if scale is None else scale, l2_eps, max_new, ws, ws_bytes)
 
 
 def gdn_workspace_bytes(q, k, v, g, beta, state, state_out, out, starts, max_new: int = 0, slots=None, scale=None,
@@ -645,4 +661,6 @@ def gdn(q, k, v, g, beta, state, state_out, out, starts, workspace=None, max_new
     g (log decay) and beta (n_tok, v_heads), state (n_states, v_heads, k_dim, v_dim);
     scale None: k_dim^-1/2."""
     a = _gdn_args(q, k, v, g, beta, state, state_out, out, starts, workspace, max_new, slots, scale, l2_eps, tiled)
-    _check("bonsai_p40_gdn", lib().bonsai_p40_gdn(a, _stream_of(q, stream)))
+    rc = lib().bonsai_p40_gdn(a, _stream_of(q, stream))
+    if rc:
+        _check("bonsai_p40_gdn", rc)
