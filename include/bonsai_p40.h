@@ -503,6 +503,8 @@ int64_t bonsai_p40_attn_paged_workspace_bytes(const bonsai_p40_attn_paged_args *
 // g and beta: fp32, head h of token t at t * gate_tok + h; a g below -10000 counts as
 // that (exp is 0 there).  All sums, and the products' operands to 22 bits or more, are
 // fp32's.
+// A value that is not finite reaches all later outputs of its head and sequence, and
+// in chunks the earlier ones of its chunk, too.
 // max_new: about the largest number of tokens of a sequence (0: unknown); it picks
 // between token-by-token steps and chunks of 64 tokens, results hold for any.
 // workspace: bonsai_p40_gdn_workspace_bytes bytes (of the same args), 16-byte

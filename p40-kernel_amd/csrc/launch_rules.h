@@ -196,7 +196,7 @@ inline void prefill_plan(bool wide, bool small, int64_t n_out, int64_t n_tok, in
 // floats apart) a tile reads runs of 4 tokens.  Measured on MI355X (us, 4 / 16 / 32
 // tokens, 24 + 8 heads of 256): rows, 64 tokens 4.5 4.9 7.6, 96 5.0 5.1 7.7, 256 8.1
 // 6.0 8.3, 2048 39.6 22.4 22.8; columns, 64 4.9 5.2 7.9, 256 15.1 6.2 8.6, 512 - 10.1
-// 10.4, 768 - 15.4 13.1, 1024 - 17.6 19.3, 2048 81 32.0 30.3, 4096 - 60.4 49.9.
+// 10.4, 768 - 15.5 13.2, 1024 - 17.5 16.1, 2048 81 33.7 26.6, 4096 - 61.3 45.9.
 inline int rope_tile(bool columns, int64_t n_tok) { return n_tok <= 64 ? 4 : columns && n_tok > 512 ? 32 : 16; }
 
 // Attention over pages (attn_paged.hip): workgroups whose waves split the keys

@@ -11,8 +11,10 @@
 // in fp32 a position of 1e6 would leave it 4 bits.
 //   Rows (one per token): a wave reads a token's head row from memory.
 //   Columns (one row per feature, as bonsai_p40_gemm writes): the tile of
-// head_dim features x TT tokens goes through LDS, rows padded by 4 words: they
-// are read 16 bytes a lane, and written with two lanes on a bank.  All of a
+// head_dim features x TT tokens goes through LDS, a row's 16-byte units permuted by
+// its token: they are read 16 bytes a lane, and written with two lanes on a bank.
+// (Padded rows would leave room for 3 workgroups a CU of 32 x 256, not 4: 30.1
+// us for 26.6, 2048 tokens of 24 + 4 + 4 heads, which is 4.7 TB/s.)  All of a
 // tile's loads are asked for at once: at 8 a lane it ran at 2.9 TB/s.
 #include "host_state.h"
 #include "launch_rules.h"
@@ -50,20 +52,25 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkvArgs a) {
     const float * const x = a.x[kind] + (int64_t)row * a.head[kind];
     const int64_t ts = a.tok[kind], es = a.el[kind];
     const bool columns = es != 1;
-    float * const tile = lds;                                            // [tt][D + 4] where columns
-    float2 * const turn = reinterpret_cast<float2 *>(lds + (columns ? a.tt * (D + 4) : 0));   // [tt][half]
+    float * const tile = lds;                                            // [tt][D] where columns, element e at e ^ place(t)
+    float2 * const turn = reinterpret_cast<float2 *>(lds + (columns ? a.tt * D : 0));         // [tt][half]
+    auto place = [](int t) { return 4 * (t & 15); };
 
     if (columns) {
         // the tokens of a feature are one run of up to 128 bytes: half a wave each
         const int sub = threadIdx.x & 31;
         if (sub < nt) {
             const float * const c = x + (int64_t)(t0 + sub) * ts + (int64_t)(threadIdx.x >> 5) * es;
-            float * const to = tile + sub * (D + 4) + (threadIdx.x >> 5);
+            float * const to = tile + sub * D;
             float v[D / 8];
 #pragma unroll
             for (int i = 0; i < D / 8; ++i) v[i] = c[(int64_t)(8 * i) * es];
 #pragma unroll
-            for (int i = 0; i < D / 8; ++i) to[8 * i] = v[i];
+            for (int i = 0; i < 8; ++i) {
+                float * const at = to + ((8 * i + (threadIdx.x >> 5)) ^ place(sub));
+#pragma unroll
+                for (int j = 0; j < D / 64; ++j) at[64 * j] = v[8 * j + i];
+            }
         }
     }
     if (kind < 2) {
@@ -88,7 +95,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkvArgs a) {
 
     auto load = [&](int t, float (&v)[E]) {
         if (columns) {
-            load_row<F32>(tile + t * (D + 4) + lane * E, v);
+            load_row<F32>(tile + t * D + ((lane * E) ^ place(t)), v);
         } else {
             const float * const r = x + (int64_t)(t0 + t) * ts + lane * E;
             if (a.vec) load_row<F32>(r, v);
@@ -235,8 +242,9 @@ extern "C" int bonsai_p40_qk_norm_rope(const bonsai_p40_qk_norm_rope_args * p, b
     a.half = p->n_rot / 2;
     a.interleaved = p->interleaved != 0;
     a.tt = pq2::rope_tile(columns, p->n_tok);
-    auto lds = [&](int tt) { return (columns ? (size_t)tt * (d + 4) * 4 : 0) + (size_t)tt * a.half * 8; };
-    if (lds(a.tt) > 64 * 1024) a.tt = 16;       // 256 columns, all of them rotated
+    auto lds = [&](int tt) { return (columns ? (size_t)tt * d * 4 : 0) + (size_t)tt * a.half * 8; };
+    // 3 workgroups to a CU at least: 2048 tokens of 256 columns, us, 16 / 32: 256 of them rotated 38.8 / 42.9, 128 34.9 / 32.1
+    if (lds(a.tt) > 53 * 1024) a.tt = 16;
     const size_t bytes = lds(a.tt);
     const dim3 grid((unsigned)((p->n_tok + a.tt - 1) / a.tt), (unsigned)(p->n_head + 2 * p->n_kv_head));
     const hipStream_t s = (hipStream_t)stream;

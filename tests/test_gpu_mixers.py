@@ -390,6 +390,14 @@ def test_attn_any_hint_and_many_sequences():
     run_attn([i % 4 for i in range(150)], [(7 * i) % 61 for i in range(150)], 2, 1, 64, 16, F16, F32)
 
 
+def test_attn_pages_that_sequences_share():
+    """A common prefix: the same pages in several rows of the table, and twice in one."""
+    table = torch.tensor([[0, 1, 2], [0, 1, 3], [0, 0, 4]], dtype=torch.int32)
+    for new in ([1, 1, 1], [40, 9, 33]):
+        run_attn(new, [48, 41, 48], 4, 2, 64, 16, F16, F16, table=table)
+        run_attn(new, [48, 41, 48], 4, 2, 64, 16, BF16, F32, table=table)
+
+
 def test_attn_offsets_beyond_32_bits():
     """A page stride that puts pages more than 4 GiB apart."""
     case("attn pages beyond 4 GiB")
