@@ -111,6 +111,14 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
     // same time have the same keys; the last tiles, which see the most, start first
     const int kvh = blockIdx.x % a.n_kv, rest = blockIdx.x / a.n_kv;
     const int split = rest / a.tiles, tile_no = a.tiles - 1 - rest % a.tiles;
+    // one sequence: its row of the table is known (and there is one, where there are pages), and the entries of a wave's first keys are asked for beside starts
+    int early0 = -1, early1 = -1;
+    const bool early = KEYS && a.n_seq == 1 && a.cap > 0 && a.n_pages > 0;
+    if (early) {
+        const int key = split * a.chunk + 32 * wave, top = (a.cap >> a.page_log2) - 1;
+        early0 = sload(a.table, min(key >> a.page_log2, top));
+        early1 = sload(a.table, min((key + 16) >> a.page_log2, top));
+    }
     const Tile tl = find_tile<Z::BM>(a.starts, a.kv_len, a.n_seq, a.n_tok, a.group, tile_no);
     if (tl.seq < 0) return;
     const int rows = tl.count * a.group, row0 = tl.index * Z::BM;
@@ -206,9 +214,9 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
     auto swz_k = [](int key) { return U >= 16 ? key & 15 : (key >> 1) & 7; };
     auto swz_v = [](int key) { return U >= 32 ? (key & 7) * 4 : U >= 16 ? (key & 3) * 4 : ((key >> 1) & 1) * 4; };
     // the page of the 16 keys from `key` on; -1: none of them is to be read
-    auto page_of = [&](int key) {
+    auto page_of = [&](int key, bool have, int id) {
         if (key >= nk) return -1;
-        const int id = sload(a.table, trow + (key >> a.page_log2));
+        if (!have) id = sload(a.table, trow + (key >> a.page_log2));
         return id >= 0 && id < a.n_pages ? id : -1;
     };
     // N keys of one page from `key` on to dst; place: that of the first among 16, as far as the swizzle looks.
@@ -541,9 +549,9 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
     } else {
         uint8_t * const mine = lds + wave * 4 * Z::TILE;
         int id0 = -1, id1 = -1;
-        auto stage = [&](int key, uint8_t * to) __attribute__((always_inline)) {
-            id0 = page_of(key);
-            id1 = page_of(key + 16);
+        auto stage = [&](int key, bool have, uint8_t * to) __attribute__((always_inline)) {
+            id0 = page_of(key, have, early0);
+            id1 = page_of(key + 16, have, early1);
             const std::integral_constant<int, 16> half_tile;
             stage_n(half_tile, khead, id0, key, 0, to, false);
             stage_n(half_tile, khead, id1, key + 16, 0, to + 16 * Z::RB, false);
@@ -552,7 +560,7 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
         };
         auto step = [&](uint8_t * __restrict__ next, uint8_t * __restrict__ cur, const uint8_t * __restrict__ qlow,
                         int key, int holes) __attribute__((always_inline)) {
-            if (key + 32 * Z::NW < k1) stage(key + 32 * Z::NW, next);
+            if (key + 32 * Z::NW < k1) stage(key + 32 * Z::NW, false, next);
             v16f s = scores(cur, qlow);
             if (key + 32 > least || holes) mask(s, key, holes);
             follow(largest(s));
@@ -561,7 +569,7 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
             values(s, cur);
         };
         int key = k0 + 32 * wave, b = 0;
-        if (key < k1) stage(key, mine);
+        if (key < k1) stage(key, early, mine);
         make_q();
 #pragma clang loop unroll(disable)
         for (; key < k1; key += 32 * Z::NW, b ^= 1) {
@@ -666,6 +674,18 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int bm) {
     const float2 * const ml = reinterpret_cast<const float2 *>(a.part + (int64_t)a.n_split * all_rows * D) + row;
     float own = -INFINITY;
     if (lane < a.n_split) own = ml[lane * all_rows].x;
+    // (4 waves: the first parts, too; those behind the last are not written, and not used)
+    float v[AHEAD][E];
+    float2 e[AHEAD];
+    auto load = [&](int i0, int n) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            const int64_t i = min(i0 + k * WR, n - 1);
+            e[k] = ml[i * all_rows];
+            load_row<F32>(a.part + (i * all_rows + row) * D + lane * E, v[k]);
+        }
+    };
+    if (WR > 1) load(w, a.n_split);
     // the sequence of this token
     int seq = -1, first = 0, count = 0, kv = 0;
     for (int s0 = 0; s0 < a.n_seq && seq < 0; s0 += 64) {
@@ -697,14 +717,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int bm) {
     const float ref = mm == -INFINITY ? 0.0f : mm;
     float x[E] = {}, l = 0.0f;
     for (int i0 = w; i0 < n; i0 += WR * AHEAD) {
-        float v[AHEAD][E];
-        float2 e[AHEAD];
-#pragma unroll
-        for (int k = 0; k < AHEAD; ++k) {
-            const int64_t i = min(i0 + k * WR, n - 1);
-            e[k] = ml[i * all_rows];
-            load_row<F32>(a.part + (i * all_rows + row) * D + lane * E, v[k]);
-        }
+        if (WR == 1 || i0 != w) load(i0, n);
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k)
             if (i0 + k * WR < n) {

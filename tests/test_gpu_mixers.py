@@ -3,6 +3,7 @@ in 64 bits, at the sizes and masks where they can go wrong.
 
 Tolerances count roundings.  A store to a type t is off by at most
 finfo(t).eps / 2 of the value; fp32 arithmetic by 2^-24 an operation."""
+import ctypes as C
 import math
 
 import pytest
@@ -388,6 +389,22 @@ def test_attn_any_hint_and_many_sequences():
         run_attn([90], [700], 4, 2, 64, 16, F16, F16, max_kv=mk)
     run_attn([1] * 150, [(7 * i) % 61 for i in range(150)], 2, 1, 64, 16, F16, F16)
     run_attn([i % 4 for i in range(150)], [(7 * i) % 61 for i in range(150)], 2, 1, 64, 16, F16, F32)
+
+
+@pytest.mark.parametrize("n_seq,new", [(1, 1), (2, 1), (1, 40)])
+def test_attn_without_pages(n_seq, new):
+    """No pages, or none that the table could name: nothing is seen, and table and pages may be NULL."""
+    case(f"attn no pages {n_seq} {new}")
+    n = n_seq * new
+    for pages, cols in ((0, 3), (4, 0), (0, 0)):
+        q, out = torch.ones(n, 4, 64, dtype=F16, device="cuda"), torch.ones(n, 4, 64, dtype=F16, device="cuda")
+        kp = torch.zeros(pages, 2, 16, 64, dtype=F16, device="cuda")
+        table = torch.zeros(n_seq, cols, dtype=torch.int32, device="cuda")
+        args = B._attn_args(q, kp, kp, table, ints([i * new for i in range(n_seq + 1)]), ints([40] * n_seq), out, None, 40, None)
+        a = B.AttnPagedArgs.from_buffer_copy(args)
+        a.table = a.k_pages = a.v_pages = None
+        assert B.lib().bonsai_p40_attn_paged(C.byref(a), B._stream(None)) == 0
+        assert bool((out == 0).all())
 
 
 def test_attn_pages_that_sequences_share():
