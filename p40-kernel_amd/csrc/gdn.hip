@@ -533,25 +533,53 @@ __global__ void __launch_bounds__(128 * PAIRS) gdn_scan_kernel(GdnArgs a) {
     rest /= groups;
     const int head = rest % per;
     rest /= per;
-    const int times = (a.n_kh + at_once - 1) / at_once, seq = rest / times;
+    const int times = (a.n_kh + at_once - 1) / at_once;
+    int seq = rest / times;
     hk += at_once * (rest % times);
     if (hk >= a.n_kh) return;
     const int hv = a.tiled ? hk + head * a.n_kh : hk * per + head;
     const int col0 = 16 * (PAIRS * group + pair);
+    // the first token and the number of tokens of a sequence; chunks before it
+    int first, count, chunk0 = 0;
+    auto tokens = [&](int q, int & b) __attribute__((always_inline)) {
+        b = iclamp(a.starts[q], 0, a.n_tok);
+        return max(iclamp(a.starts[q + 1], 0, a.n_tok) - b, 0);
+    };
+    if (a.n_seq <= 64) {
+        // the one with the seq-th most chunks (found bit by bit), as a workgroup that starts behind others with many
+        // chunks is what the rest wait for (1 sequence of 1500 tokens behind 5 of 180, both kernels, us: bf16 128 ->
+        // 106, fp32 159 -> 135)
+        int b = 0, n = 0;
+        if (lane < a.n_seq) n = tokens(lane, b);
+        const int own = (n + C - 1) / C;
+        uint64_t left = ~0ull >> (64 - a.n_seq);          // those it can be
+        for (int bit = a.n_seq > 1 ? 31 - __builtin_clz(max(a.chunks, 1)) : -1; bit >= 0; --bit) {
+            const uint64_t more = __ballot(own >> bit & 1) & left;
+            const int those = __builtin_popcountll(more);
+            left = seq < those ? more : left & ~more;
+            seq -= seq < those ? 0 : those;
+        }
+        const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(left >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)left, 0));
+        seq = __builtin_ctzll(__ballot((left >> lane & 1) && before == seq));
+        first = __builtin_amdgcn_readlane(b, seq);
+        count = __builtin_amdgcn_readlane(n, seq);
+        if (lane < seq) chunk0 = own;
+    } else {
+        for (int s = lane; s < seq; s += 64) {
+            int b;
+            chunk0 += (tokens(s, b) + C - 1) / C;
+        }
+        first = iclamp(sload(a.starts, seq), 0, a.n_tok);
+        count = max(iclamp(sload(a.starts, seq + 1), 0, a.n_tok) - first, 0);
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) chunk0 += __shfl_xor(chunk0, d);
+    chunk0 = __builtin_amdgcn_readfirstlane(chunk0);
     const int64_t slot = slot_of(a, seq);
     if (slot < 0) return;
     const bool work = col0 < a.vd;                        // the others load
     const int col = work ? col0 + l16 : 0;
-    const int first = iclamp(sload(a.starts, seq), 0, a.n_tok);
-    const int count = max(iclamp(sload(a.starts, seq + 1), 0, a.n_tok) - first, 0);
     int chunks = (count + C - 1) / C;
-    // the number of the first chunk: those of the sequences before
-    int chunk0 = 0;
-    for (int s = lane; s < seq; s += 64)
-        chunk0 += (max(iclamp(a.starts[s + 1], 0, a.n_tok) - iclamp(a.starts[s], 0, a.n_tok), 0) + C - 1) / C;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) chunk0 += __shfl_xor(chunk0, d);
-    chunk0 = __builtin_amdgcn_readfirstlane(chunk0);
     chunks = iclamp(chunks, 0, max(a.chunks - chunk0, 0));   // starts that overlap: what prep made, no more
 
     // (waves of the outputs) a run of 1 KB pieces for each, 4 of them an address

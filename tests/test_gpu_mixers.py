@@ -530,6 +530,14 @@ def test_gdn_many_sequences(kh, vh, kd, vd, t):
     run_gdn([70], kh, vh, kd, vd, t, seed=8, tiled=False)
 
 
+@pytest.mark.parametrize("n_seq", [2, 63, 64, 65])
+def test_gdn_sequences_in_any_order(n_seq):
+    """The longest go first, whatever their place: lengths up, down, alike and none, with a wave's lanes full and not."""
+    up = [(i * 5) % 40 for i in range(n_seq - 1)] + [300]
+    for new in (up, up[::-1], [20] * n_seq, [0] * (n_seq - 1) + [70]):
+        run_gdn(new, 1, 2, 64, 16, F32, seed=n_seq)
+
+
 @pytest.mark.parametrize("t", [F32, BF16])
 def test_gdn_rows_of_out_at_any_element(t):
     case(f"gdn out strides {t}")
