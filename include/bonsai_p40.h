@@ -443,7 +443,8 @@ int bonsai_p40_qk_norm_rope(const bonsai_p40_qk_norm_rope_args * args, bonsai_st
 // key/value head h / (n_head / n_kv_head).  Key j of sequence s is slot j %
 // page_size of page table[s * table_stride + j / page_size].  A page outside
 // 0 .. n_pages - 1 (-1: freed) holds no keys: they are not seen.  kv_len is cut to
-// max_pages * page_size, starts to 0 .. n_tok.  Rows of q and out before starts[0]
+// max_pages * page_size, starts, which does not fall (rows that two sequences claim
+// are undefined), to 0 .. n_tok.  Rows of q and out before starts[0]
 // and from starts[n_seq] on are not touched.  Keys and values that a token does
 // not see never reach its output, whatever they hold.
 // q and out: token t at t * q_tok and t * out_tok, heads one after another, of
@@ -495,7 +496,8 @@ int64_t bonsai_p40_attn_paged_workspace_bytes(const bonsai_p40_attn_paged_args *
 // leaves state_out[i], i = slots[s] (NULL: s): [n_states][n_v_head][k_dim][v_dim].
 // state_out may be state.  Slots of one call have to differ; a sequence whose
 // slot is outside 0 .. n_states - 1 is passed over (its rows of out, too).  One
-// without tokens copies its state.  Other states, and rows of out before starts[0] and
+// without tokens copies its state.  starts does not fall (what two sequences claim
+// is undefined) and is cut to 0 .. n_tok.  Other states, and rows of out before starts[0] and
 // from starts[n_seq] on, are not touched.
 // q, k, v, out: type fp32, f16 or bf16; token t at t * q_tok (k_tok, v_tok,
 // out_tok) elements, heads one after another: slices of one row may be passed;

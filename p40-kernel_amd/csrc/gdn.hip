@@ -567,7 +567,7 @@ __global__ void __launch_bounds__(128 * PAIRS) gdn_scan_kernel(GdnArgs a) {
     } else {
         for (int s = lane; s < seq; s += 64) {
             int b;
-            chunk0 += (tokens(s, b) + C - 1) / C;
+            chunk0 = min(chunk0 + (tokens(s, b) + C - 1) / C, 1 << 24);    // (more than there are, if starts overlap)
         }
         first = iclamp(sload(a.starts, seq), 0, a.n_tok);
         count = max(iclamp(sload(a.starts, seq + 1), 0, a.n_tok) - first, 0);

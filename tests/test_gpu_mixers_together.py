@@ -290,3 +290,21 @@ def test_room_for_every_length():
     ref, mag, top = attn_ref(qr.cpu(), kp.cpu(), vp.cpu(), s.table.cpu(), [0, 4, 4, 5], [4, 0, 1], D ** -0.5, out.cpu())
     check_attn(out.cpu(), ref, mag, top, BF16, D, 4)
     assert bool((out[5] == 3).all()) and bool((mixed[5] == 3).all()) and bool((state[1] == 0).all())
+
+
+@pytest.mark.parametrize("new", [[20, 20, 20], [1, 1, 1]])
+def test_starts_that_fall_stay_inside(new):
+    """Sequences that overlap, or lie outside: nothing but their rows changes, and what they do not claim is as ever."""
+    case(f"falling starts {new}")
+    n = sum(new)
+    s = Step(new, 200)
+    s.advance(0)
+    for starts in ([0, n, 1, n - 1], [-5, n - 1, n - 1, n - 1], [n - 1, 0, 0, 0], [0, n + 9, n + 9, n + 99], [2 ** 31 - 1, -2 ** 31, 0, 1]):
+        s.starts.copy_(torch.tensor(starts, dtype=torch.int32))
+        s.out.fill_(3.0), s.mixed.fill_(3.0)
+        s.run()
+        torch.cuda.synchronize()
+        ends = [min(max(x, 0), n) for x in starts]
+        rows = {t for a, b in zip(ends, ends[1:]) for t in range(a, b)}
+        rest = [t for t in range(n) if t not in rows]
+        assert bool((s.out[rest] == 3).all()) and bool((s.mixed[rest] == 3).all())
