@@ -236,8 +236,8 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
             dma16_at<0>(from, dst + i * 1024, lane_off(i), first + i * 1024);
             if constexpr (N > 1) dma16_at<1024>(from, dst + i * 1024, lane_off(i + 1), first + i * 1024);
             if constexpr (N > 2) {
-                dma16_at<2048>(from, dst + i * 1024, lane_off(i + 2), first + i * 1024);
-                dma16_at<3072>(from, dst + i * 1024, lane_off(i + 3), first + i * 1024);
+                dma16_at<2 * 1024>(from, dst + i * 1024, lane_off(i + 2), first + i * 1024);
+                dma16_at<3 * 1024>(from, dst + i * 1024, lane_off(i + 3), first + i * 1024);
             }
         }
     };

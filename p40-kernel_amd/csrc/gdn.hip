@@ -592,8 +592,8 @@ __global__ void __launch_bounds__(128 * PAIRS) gdn_scan_kernel(GdnArgs a) {
             const int at = (loader * OWN1 + i) * 1024;
             dma16_at<0>(from, dst + at, 16 * lane, at);
             if (i + 1 < OWN1) dma16_at<1024>(from, dst + at, 16 * lane, at);
-            if (i + 2 < OWN1) dma16_at<2048>(from, dst + at, 16 * lane, at);
-            if (i + 3 < OWN1) dma16_at<3072>(from, dst + at, 16 * lane, at);
+            if (i + 2 < OWN1) dma16_at<2 * 1024>(from, dst + at, 16 * lane, at);
+            if (i + 3 < OWN1) dma16_at<3 * 1024>(from, dst + at, 16 * lane, at);
         }
         if (N % PAIRS != 0 && loader < N % PAIRS) {
             const int at = (N / PAIRS * PAIRS + loader) * 1024;
