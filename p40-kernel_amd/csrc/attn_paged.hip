@@ -29,9 +29,21 @@
 // card; attn_join_kernel adds the parts.
 //
 // fp32 queries and output (the activations' type) keep fp32 accuracy: Q and P
-// are split into 2 f16 terms (rows scaled by a power of two, 22 bits) or 3 bf16
-// terms (24 bits) and the products summed in fp32.  16-bit ones round P once to
-// the pages' type, as its relative error is that of the output's own rounding.
+// are split into 2 f16 terms (22 bits) or 3 bf16 terms (24 bits) and the products
+// summed in fp32.  16-bit ones round P once to the pages' type, as its relative
+// error is that of the output's own rounding.
+//   f16's smallest step is 2^-24, and a row may have one key of nearly all the weight
+// before thousands that share the rest.  So with f16 pages m is kept 11 below, and P
+// is 2^11 at the maximum, up to 2^15 as m follows with a lag of up to 4 (bf16, which
+// has fp32's range: 0 and 8; l, O and the parts scale alike): one term is 11 bits of
+// weights down to 2^-25 of the row's largest, below that off by up to 2^-36 of it.
+// The second term, up to 2^-12 of its weight, is taken 2^11 up, in sums of its own
+// for a tile that O gets 2^-11 of: 22 bits down to 2^-25, 2^-47 below.  In the first
+// one's sums it would have that one's steps: with a key e^12 above 4000 others, of
+// value 0, the result would be off by 1.2e-6 (6e-8 so), e^18 by 3.2e-4 (2e-7).  It
+// costs 128 FMA a tile of heads of 256: fp32 queries, f16 pages, 2048 tokens 117 -> 129
+// us (MI355X), 777 of 16000 keys 560 -> 617, 9 ragged sequences with heads of 128 183 ->
+// 208.  One term, lags of 2, 4 and 8 (13, 11 and 7 below), 2048 tokens: 79.7, 77.6 and 77.4 us.
 #include "gemv_device.h"
 #include "host_state.h"
 #include "launch_rules.h"
@@ -157,6 +169,9 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
     frag qf[Z::QR][QS];
     uint8_t * const ql = lds + Z::MAIN + (KEYS ? 0 : wave * (NT - Z::QR) * Z::QT) + 16 * lane;
     float c = a.c;
+    constexpr bool LOW = NT == 2;                          // P's second term has sums of its own
+    constexpr float UP = std::is_same<T, F16>::value ? 11.0f : 0.0f, LAG = UP > 0.0f ? 4.0f : 8.0f;
+    constexpr float LOW_UP = 2048.0f;
     auto make_q = [&]() __attribute__((always_inline)) {
         if constexpr (NT == 1) {
 #pragma unroll
@@ -299,10 +314,10 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
         for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
         return over_halves(mx);
     };
-    // m follows the running maximum with a lag of up to 2^8, which the sums bear: they are rescaled seldom
+    // m follows UP below the running maximum with a lag, so that the sums are rescaled seldom
     auto follow = [&](float mx) __attribute__((always_inline)) {
-        if (__any(mx > m + 8.0f)) {
-            const float m2 = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - (m2 == -INFINITY ? 0.0f : m2));
+        if (__any(mx > m + (UP + LAG))) {
+            const float m2 = fmaxf(m, mx - UP), alpha = __builtin_amdgcn_exp2f(m - (m2 == -INFINITY ? 0.0f : m2));
             m = m2;
             l *= alpha;
 #pragma unroll
@@ -366,6 +381,11 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
             for (int i = lane; i < U; i += 64)
                 *reinterpret_cast<v4u *>(vb + __builtin_ctz(left) * Z::RB + 16 * i) = v4u{};
     };
+    // elements from .. to of a block of O get those of P's second term
+    auto add_low = [&](const v16f & low, v16f & to, int first, int end) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = first; i < end; ++i) to[i] = fmaf(low[i], 1.0f / LOW_UP, to[i]);
+    };
     auto values = [&](const v16f & p, const uint8_t * kb) __attribute__((always_inline)) {
         frag pf[NT][2];
 #pragma unroll
@@ -377,17 +397,29 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
                 for (int k = 0; k < NT; ++k) {
                     const elem e = T::from(f);
                     pf[k][g][j] = e;
-                    f -= T::to(e);
+                    f = LOW ? (f - T::to(e)) * LOW_UP : f - T::to(e);
                 }
             }
-#pragma unroll
-        for (int g = 0; g < 2; ++g)
+        if constexpr (LOW) {
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                const frag vf = v_frag(kb, d, g);
-#pragma unroll
-                for (int k = NT - 1; k >= 0; --k) o[d] = mfma<T>(vf, pf[k][g], o[d]);
+                const frag v0 = v_frag(kb, d, 0), v1 = v_frag(kb, d, 1);
+                v16f low = mfma<T>(v0, pf[1][0], v16f{});
+                low = mfma<T>(v1, pf[1][1], low);
+                o[d] = mfma<T>(v0, pf[0][0], o[d]);
+                o[d] = mfma<T>(v1, pf[0][1], o[d]);
+                add_low(low, o[d], 0, 16);
             }
+        } else {
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    const frag vf = v_frag(kb, d, g);
+#pragma unroll
+                    for (int k = NT - 1; k >= 0; --k) o[d] = mfma<T>(vf, pf[k][g], o[d]);
+                }
+        }
     };
 
     if constexpr (!KEYS) {
@@ -451,7 +483,13 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
             const float ref = m == -INFINITY ? 0.0f : m;
             float sum[2] = {0.0f, 0.0f};
             frag vf[AHEAD], pf[NT][2];
-            v16f next = {};
+            // (heads of 256: one wave a SIMD, and room for two blocks' sums of the second term; else a block's go to O before the next)
+            constexpr int LB = D == 256 ? 2 : 1;
+            v16f next = {}, low[LB];
+            // the blocks of V in the order of their products: a block's second term follows at once, where it has sums of its own
+            auto v_read = [&](int i) __attribute__((always_inline)) {
+                vf[i % AHEAD] = LOW ? v_frag(vr, i / 2, i % 2) : v_frag(vr, i % DT, i / DT);
+            };
             // lgkmcnt(0): with a scalar load under way the waits below could not count
             __builtin_amdgcn_s_waitcnt(0xC07F);
 #pragma unroll
@@ -461,7 +499,7 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
 #pragma unroll
                 for (int k = Z::QR - 1; k >= 0; --k) next = mfma<T>(kf[i % AHEAD], qf[k][i], next);
                 if (i + AHEAD < QS) k_read(i + AHEAD);
-                else if (!EDGE) vf[i + AHEAD - QS] = v_frag(vr, (i + AHEAD - QS) % DT, (i + AHEAD - QS) / DT);
+                else if (!EDGE) v_read(i + AHEAD - QS);
 #pragma unroll
                 for (int e = i * E; e < (i + 1) * E; ++e) {
                     s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, -ref));
@@ -471,7 +509,7 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
                     for (int k = 0; k < NT; ++k) {
                         const elem x = T::from(f);
                         pf[k][e / 8][e % 8] = x;
-                        f -= T::to(x);
+                        f = LOW ? (f - T::to(x)) * LOW_UP : f - T::to(x);
                     }
                 }
                 __builtin_amdgcn_sched_barrier(0);
@@ -480,19 +518,31 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
             if (EDGE) {
                 if (mixed) apart(s, vr + VOFF, key);
 #pragma unroll
-                for (int i = 0; i < AHEAD; ++i) vf[i] = v_frag(vr, i % DT, i / DT);
+                for (int i = 0; i < AHEAD; ++i) v_read(i);
             }
             // O takes them, and between the MFMAs the largest of the next scores are found
             float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
             for (int i = 0; i < 2 * DT; ++i) {
+                if constexpr (LOW) {
+                    const int d = i / 2, g = i % 2;
+                    if (LB == 1 && g == 0) {
+                        o[d] = mfma<T>(vf[i % AHEAD], pf[0][g], o[d]);
+                        if (d > 0) add_low(low[0], o[d - 1], 0, 16);
+                    }
+                    low[d % LB] = mfma<T>(vf[i % AHEAD], pf[1][g], g ? low[d % LB] : v16f{});
+                    if (LB == 2 || g == 1) o[d] = mfma<T>(vf[i % AHEAD], pf[0][g], o[d]);
+                    if (LB == 2 && d > 0) add_low(low[(d - 1) % LB], o[d - 1], 8 * g, 8 * g + 8);
+                } else {
 #pragma unroll
-                for (int k = NT - 1; k >= 0; --k) o[i % DT] = mfma<T>(vf[i % AHEAD], pf[k][i / DT], o[i % DT]);
-                if (i + AHEAD < 2 * DT) vf[i % AHEAD] = v_frag(vr, (i + AHEAD) % DT, (i + AHEAD) / DT);
+                    for (int k = NT - 1; k >= 0; --k) o[i % DT] = mfma<T>(vf[i % AHEAD], pf[k][i / DT], o[i % DT]);
+                }
+                if (i + AHEAD < 2 * DT) v_read(i + AHEAD);
 #pragma unroll
                 for (int e = i * 8 / DT; e < (i + 1) * 8 / DT; ++e) top[e & 1] = fmaxf(top[e & 1], next[e]);
                 __builtin_amdgcn_sched_barrier(0);
             }
+            if constexpr (LOW) add_low(low[(DT - 1) % LB], o[DT - 1], 0, 16);
             mx = over_halves(fmaxf(top[0], top[1]));
             s = next;
         };
