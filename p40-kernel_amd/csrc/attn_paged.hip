@@ -179,7 +179,8 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
         } else {
             float up = 1.0f;
             if constexpr (NT == 2) {
-                // the row's largest element to [1, 2): f16 then holds 22 bits in two terms
+                // the row's largest element to 2^14 .. 2^15: f16 then holds 22 bits in two terms of elements down to
+                // 2^-18 of it, and is off by up to 2^-40 of it below
                 float big = 0.0f;
 #pragma unroll
                 for (int s = 0; s < QS; ++s)
@@ -187,9 +188,9 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
                     for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(qx[s][j]));
                 big = fmaxf(big, __shfl_xor(big, 32));
                 const int e = (int)((__builtin_bit_cast(uint32_t, big) >> 23) & 255);
-                if (e > 2 && e < 252) {
-                    up = __builtin_bit_cast(float, (uint32_t)(254 - e) << 23);
-                    c *= __builtin_bit_cast(float, (uint32_t)e << 23);
+                if (e > 14 && e < 255) {
+                    up = __builtin_bit_cast(float, (uint32_t)(268 - e) << 23);
+                    c *= __builtin_bit_cast(float, (uint32_t)(e - 14) << 23);
                 }
             }
 #pragma unroll

@@ -96,3 +96,20 @@ def test_attn_the_key_comes_late(gap):
             err = normwise(got, ref)
             print(f"{err:.2e}", flush=True)
             assert err <= sink_limit(io, gap, ref)
+
+
+@pytest.mark.parametrize("n,kv", [(1, 900), (40, 600)])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("high", [2.0 ** 8, 2.0 ** 14])
+def test_attn_query_elements_beside_a_large_one(n, kv, d, high):
+    """Queries with one element far above the others, where every key is 0: the scores come of the others."""
+    for t in (F16, BF16):
+        case(f"large element n={n} d={d} high={high} {t}")
+        g = gen(d)
+        q, k, v = torch.randn(n, 4, d, generator=g), torch.randn(kv, 2, d, generator=g), torch.randn(kv, 2, d, generator=g)
+        q[..., 5] = high
+        k[..., 5] = 0.0
+        got, ref = attend(q, k, v, F32, t)
+        err = normwise(got, ref)
+        print(f"{err:.2e}", flush=True)
+        assert err <= 2.0 ** -18
