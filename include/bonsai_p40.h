@@ -506,8 +506,10 @@ int64_t bonsai_p40_attn_paged_workspace_bytes(const bonsai_p40_attn_paged_args *
 // out_tok) elements, heads one after another: slices of one row may be passed;
 // out overlaps nothing that is read.
 // g and beta: fp32, head h of token t at t * gate_tok + h; a g below -10000 counts as
-// that (exp is 0 there).  All sums, and the products' operands to 22 bits or more, are
-// fp32's.
+// that (exp is 0 there).  All sums are fp32's.  In chunks the operands of the products
+// (rows of keys and queries, columns of the state and of the chunk's values) have 22 bits
+// down to 2^-18 of the largest of their row or column, and are off by up to 2^-40 of that
+// below; token by token they are fp32.
 // A value that is not finite reaches all later outputs of its head and sequence, and
 // in chunks the earlier ones of its chunk, too.
 // max_new: about the largest number of tokens of a sequence (0: unknown); it picks

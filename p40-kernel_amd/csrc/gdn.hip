@@ -16,10 +16,14 @@
 // (T, the masked QK^T, K, Q and K^T) for all chunks at once, gdn_scan_kernel goes
 // through the chunks.
 //   The outputs are fp32's, so the products are, too: each operand is split into
-// two f16 terms (22 bits; rows of the left, columns of the right operand scaled by
-// powers of two so that f16's range does not matter) and the products hi hi,
-// hi lo and lo hi run on v_mfma_f32_16x16x32_f16, the three of them at 5 times the
-// rate of fp32's own matrix instructions.  G is summed in fp64 and kept as two floats: after a strong
+// two f16 terms and the products hi hi, hi lo and lo hi run on v_mfma_f32_16x16x32_f16,
+// the three of them at 5 times the rate of fp32's own matrix instructions.  Rows of the
+// left and columns of the right operand are scaled by powers of two so that their largest
+// is 2^14 to 2^15, near f16's end: the terms hold 22 bits of what is 2^-18 of that
+// and more, and are off by up to 2^-40 of it below.  (With the largest at 1 the 22 bits
+// would end at 2^-4: a token's values 2^10 above the others' cost the tokens before it
+// 3.0e-5 of their rows, for 4.2e-7; 2^20 3.2e-2 for 1.8e-6.)
+//  G is summed in fp64 and kept as two floats: after a strong
 // decay the differences of fp32 sums would have no digits left.
 //   In the scan a wave has 16 columns of S, R and U to itself: a result tile
 // (lane: column, 4 rows 4 g .. 4 g + 3) is the next product's right operand as it
@@ -54,8 +58,8 @@ struct GdnArgs {
 
 // bytes of the workspace: per chunk and key head the fragments of K, Q and K^T,
 // per chunk and value head those of T and the masked QK^T and the row factors.
-// Rows of 16-bit elements are one f16 term as they stand (but for the scaling and
-// what lies 2^14 below a row's largest, which rounds at 2^-25 of it).
+// Rows of 16-bit elements are one f16 term as they stand (but for the scaling, and
+// what lies 2^32 below a row's largest, in bf16, which rounds at 2^-40 of it).
 template <class T, int K>
 struct Work {
     static constexpr int TERMS = sizeof(typename T::elem) == 4 ? 2 : 1;
@@ -80,10 +84,10 @@ __device__ __forceinline__ int64_t slot_of(const GdnArgs & a, int seq) {
     return s >= 0 && s < a.n_states ? s : -1;
 }
 __device__ __forceinline__ float pow2(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }
-// the power of two that takes x to [1, 2), within what fp32 can invert; 0 for 0, infinities and NaN
+// pow2(-e) takes x to 2^14 .. 2^15 (as far as both are normal numbers: from 2^-112 on); for 0, infinities and NaN as for 1
 __device__ __forceinline__ int exponent(float x) {
     const int e = (int)(__builtin_bit_cast(uint32_t, x) >> 23 & 255) - 127;
-    return e < -100 || e > 126 ? 0 : e > 100 ? 100 : e;
+    return (e < -112 || e > 127 ? 0 : e) - 14;
 }
 
 // ------------------------------------------------------------ token by token
@@ -160,7 +164,7 @@ __global__ void __launch_bounds__(128) gdn_step_kernel(GdnArgs a) {
 }
 
 // ---------------------------------------------------------------------- chunks
-// elements at .. at + N - 1 of the two f16 terms of x down (about 1 at most)
+// elements at .. at + N - 1 of the two f16 terms of x down (less than 2^15)
 template <int N>
 __device__ __forceinline__ void split(const float * x, float down, v8h & hi, v8h & lo, int at) {
     typedef _Float16 v2h __attribute__((ext_vector_type(2)));
@@ -732,7 +736,7 @@ __global__ void __launch_bounds__(128 * PAIRS) gdn_scan_kernel(GdnArgs a) {
         for (int m = 0; m < 4; ++m)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                own[(16 * m + 4 * j) * 16] = T::from(fmaf(x[m][j], ca[m][j] * fu, cq[m][j] * fs * ks[m][j]));
+                own[(16 * m + 4 * j) * 16] = T::from(fmaf(x[m][j] * fu, ca[m][j], ks[m][j] * fs * cq[m][j]));
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");    // other lanes read it
     };
     auto phase1 = [&](const uint8_t * __restrict__ k, uint8_t * __restrict__ q, uint8_t * __restrict__ t, uint8_t * __restrict__ vec,
@@ -807,7 +811,7 @@ __global__ void __launch_bounds__(128 * PAIRS) gdn_scan_kernel(GdnArgs a) {
         for (int m = 0; m < 4; ++m) {
             const v4f f = factor(0, m);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) R[m][j] = fmaf(-f[j] * fs, ks[m][j], T::to(own[(16 * m + 4 * j) * 16]));
+            for (int j = 0; j < 4; ++j) R[m][j] = fmaf(-f[j], ks[m][j] * fs, T::to(own[(16 * m + 4 * j) * 16]));
         }
         int e = exponent(largest(R));
         const float fr = pow2(e);
@@ -816,7 +820,7 @@ __global__ void __launch_bounds__(128 * PAIRS) gdn_scan_kernel(GdnArgs a) {
         for (int m = 0; m < 4; ++m) {
             const v4f f = factor(2, m), w = factor(4, m);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) Um[m][j] = x[m][j] * f[j] * fr;
+            for (int j = 0; j < 4; ++j) Um[m][j] = x[m][j] * fr * f[j];
             *reinterpret_cast<v4f *>(u + 1024 * m + 16 * lane) = Um[m];
 #pragma unroll
             for (int j = 0; j < 4; ++j) Um[m][j] *= w[j];

@@ -113,3 +113,118 @@ def test_attn_query_elements_beside_a_large_one(n, kv, d, high):
         err = normwise(got, ref)
         print(f"{err:.2e}", flush=True)
         assert err <= 2.0 ** -18
+
+
+# -------------------------------------------------------------------- gdn
+def delta(q, k, v, g, beta, state, t, eps, work=True, scale=None):
+    """One sequence; ((outputs, state), the same in 64 bits).  Heads as they come."""
+    n, heads, kd = q.shape
+    q, k, v = q.to(t), k.to(t), v.to(t)
+    out = torch.full(v.shape, 7.0, dtype=t, device="cuda")
+    so = torch.zeros_like(state, device="cuda")
+    args = (q.cuda(), k.cuda(), v.cuda(), g.cuda(), beta.cuda(), state.cuda(), so, out, ints([0, n]))
+    kw = dict(l2_eps=eps, scale=scale)
+    ws = torch.full((B.gdn_workspace_bytes(*args, **kw) + 16,), 255, dtype=torch.uint8, device="cuda") if work else None
+    B.gdn(*args, ws, **kw)
+    torch.cuda.synchronize()
+    q, k, v, g, beta = (x.double() for x in (q, k, v, g, beta))
+    if eps > 0:
+        q, k = (x / torch.sqrt((x * x).sum(-1, keepdim=True) + eps) for x in (q, k))
+    S, ref = state[0].double(), []
+    for i in range(n):
+        S = S * g[i].exp()[:, None, None]
+        u = beta[i][:, None] * (v[i] - (k[i][:, :, None] * S).sum(1))
+        S = S + k[i][:, :, None] * u[:, None]
+        ref.append((q[i][:, :, None] * S).sum(1) * (kd ** -0.5 if scale is None else scale))
+    return (out.cpu(), so.cpu()[0]), (torch.stack(ref), S)
+
+
+def check_rows(got, ref, rows, tol, t):
+    """Every (token, head) row by itself, beside the root mean square norm of its head's rows."""
+    err = (got[rows].double() - ref[rows]).norm(dim=-1)
+    norm = ref[rows].norm(dim=-1)
+    rms = norm.square().mean(0, keepdim=True).sqrt()
+    worst = float(((err - (half_step(t) * norm if t != F32 else 0)) / rms).max())
+    print(f"{worst:.2e} of {tol:.2e}", flush=True)
+    assert worst <= tol
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("kd,vd", [(128, 128), (64, 32)])
+@pytest.mark.parametrize("work", [True, False])
+@pytest.mark.parametrize("high", [2.0 ** 10, 2.0 ** 14, 2.0 ** 20])
+def test_gdn_tokens_before_a_large_one(high, work, kd, vd, t):
+    """One token's values far above the others': what comes before it does not lose by it.
+
+    2^-18 as for values of one size, and what 2^-40 of a chunk's largest comes to, with 8 for the sums."""
+    for n, at in ((138, 100), (60, 59), (70, 20)):
+        case(f"gdn before high={high} work={work} {kd}x{vd} {t} n={n} at={at}")
+        r = gen(n)
+        q, k = torch.randn(n, 2, kd, generator=r), torch.randn(n, 2, kd, generator=r)
+        v, state = torch.randn(n, 2, vd, generator=r), torch.randn(1, 2, kd, vd, generator=r) * 0.3
+        v[at] *= high
+        g, beta = -0.3 * torch.rand(n, 2, generator=r), torch.sigmoid(torch.randn(n, 2, generator=r))
+        (out, _), (ref, _) = delta(q, k, v, g, beta, state, t, 1e-6, work)
+        check_rows(out, ref, list(range(at)), 2.0 ** -18 + 8 * 2.0 ** -40 * high, t)
+
+
+@pytest.mark.parametrize("t", [F32, F16])
+@pytest.mark.parametrize("work", [True, False])
+@pytest.mark.parametrize("high", [2.0 ** 10, 2.0 ** 15])
+def test_gdn_tokens_after_a_large_one_that_has_decayed(high, work, t):
+    """Decay of e^-5 a token: 8 tokens later nothing of the large one is left, and nothing lost."""
+    for n, at in ((60, 20), (140, 70)):
+        case(f"gdn after high={high} work={work} {t} n={n} at={at}")
+        r = gen(n)
+        q, k = torch.randn(n, 2, 128, generator=r), torch.randn(n, 2, 128, generator=r)
+        v, state = torch.randn(n, 2, 64, generator=r), torch.randn(1, 2, 128, 64, generator=r) * 0.3
+        v[at] = torch.where(v[at] > 0, 1.0, -1.0) * high
+        g, beta = torch.full((n, 2), -5.0), torch.sigmoid(torch.randn(n, 2, generator=r))
+        (out, S), (ref, final) = delta(q, k, v, g, beta, state, t, 1e-6, work)
+        rows = [i for i in range(n) if i < at or i >= at + 8]
+        tol = 2.0 ** -18 + 8 * 2.0 ** -40 * high
+        check_rows(out, ref, rows, tol, t)
+        assert all(normwise(S[h], final[h]) <= tol for h in range(2))
+
+
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("work", [True, False])
+def test_gdn_elements_of_a_row_beside_a_large_one(work, t):
+    """Queries and keys with an element 2^18 above the others where the state is 0 (and the other side is): the
+    others make the results.  2^-40 2^18 and the sums of 128: below 2^-18."""
+    n = 100
+    case(f"gdn row range work={work} {t}")
+    for large in ("q", "k"):
+        r = gen(3)
+        q, k = torch.randn(n, 2, 128, generator=r), torch.randn(n, 2, 128, generator=r) / 16
+        v, state = torch.randn(n, 2, 64, generator=r), torch.randn(1, 2, 128, 64, generator=r)
+        state[:, :, 0] = 0.0
+        q[..., 0], k[..., 0] = 0.0, 0.0
+        if large == "q":
+            q *= 2.0 ** -6
+            q[..., 0] = 2.0 ** 12
+            beta = torch.sigmoid(torch.randn(n, 2, generator=r))
+        else:
+            k *= 2.0 ** -6
+            k[:1, :, 0] = 2.0 ** 8                         # one key: the others do not meet it
+            beta = torch.sigmoid(torch.randn(n, 2, generator=r))
+            beta[0] = 2.0 ** -40
+        g = -0.01 * torch.rand(n, 2, generator=r)
+        (out, S), (ref, final) = delta(q, k, v, g, beta, state, t, 0.0, work)
+        check_rows(out, ref, list(range(n)), 2.0 ** -18, t)
+        assert all(normwise(S[h], final[h]) <= 2.0 ** -18 for h in range(2))
+
+
+@pytest.mark.parametrize("work", [True, False])
+def test_gdn_large_and_small_rows(work):
+    """Rows of 2^60 and of 2^-60: each by itself, as sums of fp32 have them."""
+    case(f"gdn powers work={work}")
+    for power in (-60, 60):
+        n, r = 80, gen(4)
+        q, k = torch.randn(n, 2, 64, generator=r), torch.randn(n, 2, 64, generator=r)
+        v = torch.randn(n, 2, 32, generator=r) * 2.0 ** power
+        state = torch.randn(1, 2, 64, 32, generator=r) * 2.0 ** power
+        g, beta = -0.3 * torch.rand(n, 2, generator=r), torch.sigmoid(torch.randn(n, 2, generator=r))
+        (out, S), (ref, final) = delta(q, k, v, g, beta, state, F32, 1e-6, work)
+        check_rows(out, ref, list(range(n)), 2.0 ** -18, F32)
+        assert all(normwise(S[h], final[h]) <= 2.0 ** -18 for h in range(2))
