@@ -510,8 +510,9 @@ int64_t bonsai_p40_attn_paged_workspace_bytes(const bonsai_p40_attn_paged_args *
 // (rows of keys and queries, columns of the state and of the chunk's values) have 22 bits
 // down to 2^-18 of the largest of their row or column, and are off by up to 2^-40 of that
 // below; token by token they are fp32.
-// A value that is not finite reaches all later outputs of its head and sequence, and
-// in chunks the earlier ones of its chunk, too.
+// A value that is not finite reaches what it has a part in: one of q its own token, one
+// of v or the state its column from there on, one of k, g (but -inf) or beta its head
+// from there on, of its sequence; and in chunks the earlier tokens of its chunk, too.
 // max_new: about the largest number of tokens of a sequence (0: unknown); it picks
 // between token-by-token steps and chunks of 64 tokens, results hold for any.
 // workspace: bonsai_p40_gdn_workspace_bytes bytes (of the same args), 16-byte

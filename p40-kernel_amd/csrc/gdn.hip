@@ -23,8 +23,8 @@
 // and more, and are off by up to 2^-40 of it below.  (With the largest at 1 the 22 bits
 // would end at 2^-4: a token's values 2^10 above the others' cost the tokens before it
 // 3.0e-5 of their rows, for 4.2e-7; 2^20 3.2e-2 for 1.8e-6.)
-//  G is summed in fp64 and kept as two floats: after a strong
-// decay the differences of fp32 sums would have no digits left.
+//   G is summed in fp64 and kept as two floats: after a strong decay the differences of
+// fp32 sums would have no digits left.
 //   In the scan a wave has 16 columns of S, R and U to itself: a result tile
 // (lane: column, 4 rows 4 g .. 4 g + 3) is the next product's right operand as it
 // stands, if the left one lists its contraction as 4 g + j, 16 + 4 g + j (j < 4).

@@ -228,3 +228,44 @@ def test_gdn_large_and_small_rows(work):
         (out, S), (ref, final) = delta(q, k, v, g, beta, state, F32, 1e-6, work)
         check_rows(out, ref, list(range(n)), 2.0 ** -18, F32)
         assert all(normwise(S[h], final[h]) <= 2.0 ** -18 for h in range(2))
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("name", ["q", "k", "v", "g", "beta", "state"])
+@pytest.mark.parametrize("work", [True, False])
+def test_gdn_values_that_are_not_finite(work, name, value):
+    """They reach their head of their sequence, from their chunk (token by token: from themselves) on, and nothing else."""
+    case(f"gdn {name}={value} work={work}")
+    n, heads, r = 200, 3, gen(5)
+    x = dict(q=torch.randn(2 * n, heads, 64, generator=r), k=torch.randn(2 * n, heads, 64, generator=r),
+             v=torch.randn(2 * n, heads, 32, generator=r), g=-0.1 * torch.rand(2 * n, heads, generator=r),
+             beta=torch.rand(2 * n, heads, generator=r), state=torch.randn(2, heads, 64, 32, generator=r))
+    at = 150                                               # in the third chunk of the first sequence
+
+    def run():
+        out, so = torch.zeros(2 * n, heads, 32, device="cuda"), torch.zeros(2, heads, 64, 32, device="cuda")
+        args = (*(x[i].cuda() for i in ("q", "k", "v", "g", "beta", "state")), so, out, ints([0, n, 2 * n]))
+        ws = torch.empty(B.gdn_workspace_bytes(*args, l2_eps=1e-6) + 16, dtype=torch.uint8, device="cuda") if work else None
+        B.gdn(*args, ws, l2_eps=1e-6)
+        torch.cuda.synchronize()
+        return out.cpu(), so.cpu()
+    out0, so0 = run()
+    if name == "state":
+        x["state"][0, 1, 7] = value                        # (a row: every column has one)
+    elif x[name].dim() == 3:
+        x[name][at, 1, 5 if name in "qk" else slice(None)] = value
+    else:
+        x[name][at, 1] = value
+    out, so = run()
+    # a decay of e^-inf is e^-10000, that is 0: nothing that is not finite comes of it
+    if name == "g" and value < 0:
+        assert bool(torch.isfinite(out).all()) and bool(torch.isfinite(so).all())
+        return
+    assert torch.equal(out[:, [0, 2]], out0[:, [0, 2]]) and torch.equal(out[n:], out0[n:])
+    assert torch.equal(so[1], so0[1]) and torch.equal(so[0, [0, 2]], so0[0, [0, 2]])
+    first = 0 if name == "state" else at // 64 * 64 if work else at
+    assert torch.equal(out[:first, 1], out0[:first, 1])
+    row = 0 if name == "state" else at
+    assert not bool(torch.isfinite(out[row, 1]).any())
+    if name != "q":                                        # (a query is its own token's alone)
+        assert not bool(torch.isfinite(out[row:n, 1]).any()) and not bool(torch.isfinite(so[0, 1]).any(0).any())
