@@ -494,20 +494,21 @@ def _rows(t, name: str, shape, dev: int) -> int:
     tok, head, el = t.stride()
     if (el != 1 and dim != 1) or (head != dim and heads != 1):
         raise ValueError(f"{name}: heads have to follow each other, the strides are {t.stride()}")
-    return tok if n > 1 else max(tok, heads * dim)
+    return tok if n > 1 else heads * dim          # (one token's stride says nothing)
 
 
 def _pages(k_pages, v_pages, dev: int):
     """(n_pages, n_kv_head, page_size, head_dim) pages of keys and values: shape, page stride and type."""
     shape, st = k_pages.shape, k_pages.stride()
-    if (len(st) != 4 or v_pages.shape != shape or v_pages.stride() != st or v_pages.dtype is not k_pages.dtype
-            or not dev == k_pages.get_device() == v_pages.get_device()):
+    vt = v_pages.stride()
+    if (len(st) != 4 or v_pages.shape != shape or v_pages.dtype is not k_pages.dtype
+            or vt != st and any(a != b and m > 1 for a, b, m in zip(vt, st, shape)) or not dev == k_pages.get_device() == v_pages.get_device()):
         raise ValueError("k_pages and v_pages: alike, (n_pages, n_kv_head, page_size, head_dim), beside q")
     n, h, p, d = shape
     page, head, row, el = st
     if (el != 1 and d != 1) or (row != d and p != 1) or (head != p * d and h != 1):
         raise ValueError("a page has to lie in one piece")
-    return n, h, p, d, page if n > 1 else max(page, h * p * d), _type(k_pages)
+    return n, h, p, d, page if n > 1 else h * p * d, _type(k_pages)
 
 
 def rope_inv_freq(n_rot: int, base: float, device="cuda"):
