@@ -452,7 +452,8 @@ int bonsai_p40_qk_norm_rope(const bonsai_p40_qk_norm_rope_args * args, bonsai_st
 // statistics and all sums are fp32.  io_type kv_type rounds each softmax weight once to
 // it before the product with V (with f16 a weight below 2^-25 of its row's largest is
 // off by up to 2^-36 of that one); fp32 keeps 22 bits of it or more (with f16 pages one
-// below 2^-25 is off by up to 2^-47 of the largest).
+// below 2^-25 is off by up to 2^-47 of the largest).  A row all of whose seen scores are
+// -inf is NaN, as 0 / 0 is; with fp32 rows so is one that sees a key that is not finite.
 // max_kv: about the largest kv_len (0: unknown); it places the work, results hold for
 // any.  workspace: bonsai_p40_attn_paged_workspace_bytes bytes (of the same
 // args), 16-byte aligned, scratch for the call (stream-ordered; calls that may

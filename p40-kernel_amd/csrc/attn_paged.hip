@@ -88,6 +88,9 @@ __device__ __forceinline__ v2u read_tr(const uint8_t * at) {
     return __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)at));
 }
 
+// 1 / l; 0 where no key was seen, NaN where the score of every key that was is -inf
+__device__ __forceinline__ float over(float m, float l) { return m == -INFINITY ? 0.0f : l != 0.0f ? 1.0f / l : NAN; }
+
 template <class T, int D, int NT, bool KEYS>
 struct Shape {
     // waves: with heads of 256, LDS has two buffers of 32 keys for 2 waves, or 64 rows of two terms of Q
@@ -315,7 +318,13 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
         for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
         return over_halves(mx);
     };
-    // m follows UP below the running maximum with a lag, so that the sums are rescaled seldom
+    // whether the row sees a key of the sub-tile
+    auto sees = [&](int key0, int holes) __attribute__((always_inline)) {
+        return (key0 < vis && !(holes & 1)) || (key0 + 16 < vis && !(holes & 2));
+    };
+    // m follows UP below the running maximum with a lag, so that the sums are rescaled seldom.  It is -inf while
+    // the row has seen no key, and finite behind that, whatever the scores (LEAST): l = 0 is then 0 / 0
+    constexpr float LEAST = -3e38f;
     auto follow = [&](float mx) __attribute__((always_inline)) {
         if (__any(mx > m + (UP + LAG))) {
             const float m2 = fmaxf(m, mx - UP), alpha = __builtin_amdgcn_exp2f(m - (m2 == -INFINITY ? 0.0f : m2));
@@ -453,7 +462,7 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
         };
         // that the buffers differ has to be said, else every read of LDS waits for the DMA
         auto step = [&](auto edge, auto steady, uint8_t * __restrict__ kw, uint8_t * __restrict__ vw, const uint8_t * __restrict__ kr,
-                        uint8_t * __restrict__ vr, const uint8_t * __restrict__ qlow, v16f & s, float & mx, int j) __attribute__((always_inline)) {
+                        uint8_t * __restrict__ vr, const uint8_t * __restrict__ qlow, float bottom, v16f & s, float & mx, int j) __attribute__((always_inline)) {
             constexpr bool EDGE = decltype(edge)::value;
             // fragments are read AHEAD steps before they are used
             constexpr int AHEAD = Z::QL ? 2 : 4;
@@ -477,6 +486,7 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
             if (EDGE || holes) {
                 mask(s, key, holes);
                 mx = largest(s);
+                if (sees(key, holes)) mx = fmaxf(mx, LEAST);
             }
             follow(mx);
             // the scores of the next tile, and between their MFMAs the weights of this one (E of a step)
@@ -522,7 +532,7 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
                 for (int i = 0; i < AHEAD; ++i) v_read(i);
             }
             // O takes them, and between the MFMAs the largest of the next scores are found
-            float top[2] = {-INFINITY, -INFINITY};
+            float top[2] = {bottom, bottom};
 #pragma unroll
             for (int i = 0; i < 2 * DT; ++i) {
                 if constexpr (LOW) {
@@ -563,7 +573,8 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
             v16f s = scores(kring, ql);
-            float mx = largest(s);
+            const float bottom = LEAST / fmaxf(c, 1.0f);   // (times c: finite)
+            float mx = fmaxf(largest(s), LEAST);
             // tiles that every row sees whole, then those at the edge
             const int plain = max(min(nt, (first_vis - k0) / 32), 0);
             // (steady: every load that a tile can start is there; R of them at a time, with the rings' places
@@ -580,7 +591,7 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
                 __builtin_amdgcn_s_barrier();              // the tiles are there, and all are done with the last ones
                 asm volatile("" ::: "memory");
                 step(edge, steady, kring + slot * Z::TILE, vring + before * Z::TILE, kring + after * Z::TILE, lds + slot * Z::TILE,
-                     ql, s, mx, j);
+                     ql, bottom, s, mx, j);
             };
             int j = 0;
             const int whole = min(plain, nt - R);
@@ -613,8 +624,15 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
                         int key, int holes) __attribute__((always_inline)) {
             if (key + 32 * Z::NW < k1) stage(key + 32 * Z::NW, false, next);
             v16f s = scores(cur, qlow);
-            if (key + 32 > least || holes) mask(s, key, holes);
-            follow(largest(s));
+            float mx;
+            if (key + 32 > least || holes) {
+                mask(s, key, holes);
+                mx = largest(s);
+                if (sees(key, holes)) mx = fmaxf(mx, LEAST);
+            } else {
+                mx = fmaxf(largest(s), LEAST);
+            }
+            follow(mx);
             weights(s);
             if (key + 32 > first_vis && nk > max(first_vis, key)) apart(s, cur + Z::TILE, key);
             values(s, cur);
@@ -642,7 +660,7 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
     if constexpr (!KEYS) {
         if (!live) return;
         const int64_t row = grow * a.n_head + head;
-        const float inv = parts ? 1.0f : l != 0.0f ? 1.0f / l : 0.0f;
+        const float inv = parts ? 1.0f : over(m, l);
         float * const po = a.part + ((int64_t)split * all_rows + row) * D;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
@@ -700,7 +718,7 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
                     *reinterpret_cast<float2 *>(a.part + (int64_t)a.n_split * all_rows * D +
                                                 2 * ((int64_t)split * all_rows + row)) = make_float2(mm, ll);
             } else {
-                const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;
+                const float inv = over(mm, ll);
 #pragma unroll
                 for (int j = 0; j < E; ++j) x[j] *= inv;
                 if constexpr (NT == 1)
@@ -790,7 +808,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int bm) {
             for (int j = 0; j < E; ++j) x[j] += sum[k][lane * E + j];
         }
     }
-    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+    const float inv = over(mm, l);
 #pragma unroll
     for (int j = 0; j < E; ++j) x[j] *= inv;
     store_row<TO>(reinterpret_cast<typename TO::elem *>(a.out) + (int64_t)tok * a.out_tok + (int64_t)head * D + lane * E, x);

@@ -115,6 +115,31 @@ def test_attn_query_elements_beside_a_large_one(n, kv, d, high):
         assert err <= 2.0 ** -18
 
 
+@pytest.mark.parametrize("t,io", [(F16, F16), (BF16, BF16), (F16, F32), (BF16, F32)])
+@pytest.mark.parametrize("n,kv,d", [(1, 50, 64), (1, 3000, 256), (40, 90, 128), (40, 700, 256)])
+def test_attn_scores_of_minus_infinity(n, kv, d, t, io):
+    """A key whose score is -inf has no weight, and where no other is seen the softmax is 0 / 0, not 0.  fp32 queries
+    meet a key's infinity with each of their terms, of which one is 0: NaN."""
+    g = gen(kv)
+    for which in ("all", "some", "first"):
+        case(f"-inf n={n} kv={kv} d={d} {t} {io} {which}")
+        q, k, v = torch.randn(n, 2, d, generator=g), torch.randn(kv, 1, d, generator=g), torch.randn(kv, 1, d, generator=g)
+        q[..., 3] = 300.0
+        k[..., 3] = 0.0                                     # (300 times -inf is -inf)
+        hit = slice(None) if which == "all" else slice(0, kv, 3) if which == "some" else slice(0, kv - n + 1)
+        k[hit, :, 3] = -float("inf")
+        for work in (True, False):
+            got, ref = attend(q, k, v, io, t, work)
+            # "first": the first token sees such keys only
+            assert bool(ref.isnan().all()) if which == "all" else bool(ref[0].isnan().all()) == (which == "first")
+            if io == F32:
+                assert bool(got.isnan().all())
+                continue
+            assert torch.equal(got.isnan(), ref.isnan())
+            fin = ~ref.isnan()
+            assert normwise(got[fin], ref[fin]) <= half_step(io)
+
+
 # -------------------------------------------------------------------- gdn
 def delta(q, k, v, g, beta, state, t, eps, work=True, scale=None):
     """One sequence; ((outputs, state), the same in 64 bits).  Heads as they come."""
