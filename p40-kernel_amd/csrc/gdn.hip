@@ -391,6 +391,8 @@ __global__ void __launch_bounds__(256) gdn_prep_kernel(GdnArgs a) {
             if (r < heads) {
                 const v4f hi = *reinterpret_cast<const v4f *>(&Gh[r][row]), lo = *reinterpret_cast<const v4f *>(&Gl[r][row]);
                 const v4f bi = *reinterpret_cast<const v4f *>(&bt[r][row]);
+                int under = row - l16;
+                asm("" : "+v"(under));                    // or 32 comparisons are kept for all heads, and spilled
 #pragma unroll
                 for (int n = 0; n < 4; ++n)
                     if (n <= (wave | 1)) {                // (block n = wave + 1 of even waves: the zeros beside the diagonal)
@@ -399,8 +401,8 @@ __global__ void __launch_bounds__(256) gdn_prep_kernel(GdnArgs a) {
 #pragma unroll
                         for (int i4 = 0; i4 < 4; ++i4) {
                             const float d = __builtin_amdgcn_exp2f((hi[i4] - hj) + (lo[i4] - lj)) * fj;
-                            mat[r][row + i4][j] = j <= row + i4 ? qk[n][i4] * (a.scale * fqi[i4]) * d : 0.0f;
-                            L[r][n][i4] = j < row + i4 ? kk[n][i4] * (bi[i4] * fki[i4]) * d : 0.0f;
+                            mat[r][row + i4][j] = 16 * n <= under + i4 ? qk[n][i4] * (a.scale * fqi[i4]) * d : 0.0f;
+                            L[r][n][i4] = 16 * n < under + i4 ? kk[n][i4] * (bi[i4] * fki[i4]) * d : 0.0f;
                         }
                     }
             }

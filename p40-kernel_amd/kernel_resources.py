@@ -22,11 +22,11 @@ LIB = os.path.join(HERE, "libbonsai_p40.so")
 LLVM = "/opt/rocm/llvm/bin"
 
 # the kernels of the hot path (decode GEMV family, prefill and small-batch
-# GEMMs, the FWHT / Q8_1 pre-passes, the repack and the PQ2_0 codec): a spill
-# or a scratch byte there is a regression.  The probes and the persistent
-# chain kernel are not on it.
+# GEMMs, the FWHT / Q8_1 pre-passes, the token mixers, the repack and the PQ2_0
+# codec): a spill or a scratch byte there is a regression.  The probes and the
+# persistent chain kernel are not on it.
 HOT_PATH = ("gemv_", "gemm_", "wide_x16", "rot_quant", "quant_kernel", "swiglu_rot_quant", "rmsnorm_kernel",
-            "repack_kernel", "quantize_pq2_0", "dequantize_pq2_0")
+            "repack_kernel", "quantize_pq2_0", "dequantize_pq2_0", "qk_norm_rope", "attn_", "gdn_")
 NOT_HOT = ("probe", "chain_kernel")
 
 
