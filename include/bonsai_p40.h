@@ -410,12 +410,13 @@ int bonsai_p40_chain_run(const void * plan, int n_steps, void * workspace, uint3
 // slots[t] = page * page_size + i.  A slot outside 0 .. n_pages * page_size - 1
 // (-1: padding) is not written.  Slots of one call have to differ: what two
 // tokens leave in one slot is a mix.  Where slots are not written, the pages
-// stay as they were.
+// stay as they were.  q_out and the pages overlap nothing that is read.
 // Errors: 1 if head_dim is not 64, 128 or 256, n_rot is not a multiple of 8 in
 // 0 .. head_dim, a type, page_size (1 .. 65536) or stride is not as stated (n_tok
 // > 1 with neither stride 1, q_out_tok < n_head * head_dim or q_out rows not
-// 16-byte aligned), n_head or n_kv_head is outside 1 .. 16384, a pointer is NULL
-// (pos and inv_freq may be where n_rot == 0) or misaligned; 0 (no-op) if n_tok <= 0.
+// 16-byte aligned), n_head or n_kv_head is outside 1 .. 16384, n_tok is 2^25 or more, n_pages
+// outside 0 .. 2^40, a pointer is NULL (pos and inv_freq may be where n_rot == 0) or
+// misaligned; 0 (no-op) if n_tok <= 0.
 typedef struct bonsai_p40_qk_norm_rope_args {
     const float * q, * k, * v;
     int64_t q_tok, q_head, q_el, k_tok, k_head, k_el, v_tok, v_head, v_el;
@@ -463,8 +464,8 @@ int bonsai_p40_qk_norm_rope(const bonsai_p40_qk_norm_rope_args * args, bonsai_st
 // Errors: 1 if head_dim is not 64, 128 or 256, n_head (up to 65536) is no multiple
 // of n_kv_head, io_type, kv_type, page_size (a power of two, 16 .. 65536) or a
 // stride is not as stated (rows of q and out are 16-byte aligned), scale is not
-// finite and > 0, max_pages * page_size >= 2^31 - 65536, a pointer is NULL or
-// misaligned, the workspace is too small, or there are 2^24 / n_head tokens and
+// finite and > 0, max_pages * page_size > 2^31 - 65536, n_pages is outside 0 .. 2^31 - 1,
+// a pointer is NULL or misaligned, the workspace is too small, or there are 2^24 / n_head tokens and
 // sequences or more; 0 (no-op) if n_tok <= 0 or n_seq <= 0.
 typedef struct bonsai_p40_attn_paged_args {
     const void * q;
@@ -524,7 +525,8 @@ int64_t bonsai_p40_attn_paged_workspace_bytes(const bonsai_p40_attn_paged_args *
 // stated (q_tok, k_tok, v_tok, out_tok and gate_tok at least a row; q, k and v rows
 // 16-byte aligned, v_tok up to 2^22), scale or l2_eps is not finite or l2_eps is negative, a
 // pointer is NULL or misaligned, the workspace is too small, or there are more
-// than 2^27 / n_v_head tokens or 2^20 / n_v_head sequences; 0 (no-op) if n_seq <= 0.
+// than 2^27 / n_v_head tokens or 2^40 states, or 2^20 / n_v_head sequences or more; 0 (no-op)
+// if n_seq <= 0.
 typedef struct bonsai_p40_gdn_args {
     const void * q, * k, * v;
     void * out;

@@ -31,7 +31,8 @@
 // fp32 queries and output (the activations' type) keep fp32 accuracy: Q and P
 // are split into 2 f16 terms (22 bits) or 3 bf16 terms (24 bits) and the products
 // summed in fp32.  16-bit ones round P once to the pages' type, as its relative
-// error is that of the output's own rounding.
+// error is that of the output's own rounding (norm of the error over that of the result,
+// scores of one size: bf16 1.7e-3 by the output alone, 2.3e-3 with P's; f16 2.1e-4, 2.9e-4).
 //   f16's smallest step is 2^-24, and a row may have one key of nearly all the weight
 // before thousands that share the rest.  So with f16 pages m is kept 11 below, and P
 // is 2^11 at the maximum, up to 2^15 as m follows with a lag of up to 4 (bf16, which

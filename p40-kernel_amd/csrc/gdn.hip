@@ -512,10 +512,11 @@ __device__ __forceinline__ float largest(const v4f (&x)[N]) {
 // 11000 clocks a chunk, the pair 6700, of which U is 2600.
 //   K, Q and K^T of a chunk follow one another through two buffers, each asked for
 // a phase ahead: with a third one PAIRS = 4 would not fit beside fp32's fragments,
-// and it gains nothing (2048 tokens of one sequence, both kernels, us: 150 against 153).
+// and PAIRS = 2 gained nothing by it (within 2 %).
 //   2 pairs or 4 (half the fragments' bytes through LDS, two waves to a SIMD):
-// gdn_wide.  MI355X, 48 value heads of 128 x 128, fp32, both kernels: 2048 tokens 116
-// us, 8 sequences of 2048 680 us, that is 1.6 TB/s of K, Q, V and outputs.
+// gdn_wide, which has the times.  MI355X, 48 value heads of 128 x 128, fp32, both kernels:
+// 2048 tokens of new inputs 134 us (116 to 126 where the caches hold them from the call
+// before), 8 sequences of 2048 690, that is 1.6 TB/s of K, Q, V and outputs.
 template <class T, int K, int PAIRS>
 __global__ void __launch_bounds__(128 * PAIRS) gdn_scan_kernel(GdnArgs a) {
     typedef typename T::elem elem;

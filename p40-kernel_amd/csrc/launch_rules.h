@@ -203,16 +203,26 @@ inline int rope_tile(bool columns, int64_t n_tok) { return n_tok <= 64 ? 4 : col
 // (32 rows, decode) or the rows (64 or 128), the number of row tiles that n_tok tokens
 // of n_seq sequences can have at most, and the keys of one workgroup: n_split
 // workgroups share a tile, the last of them takes what is left.
-//   The keys are split while one tile of 32 rows holds a sequence's: a second tile
-// reads K and V again.  Measured on MI355X (us, rows / keys split, 24 heads on 4 of
+//   The keys are split while one tile of 32 rows holds a sequence's, as the batch's
+// average has it (the host does not know each): a second tile reads K and V again.  Measured on MI355X (us, rows / keys split, 24 heads on 4 of
 // 256, fp32 queries, bf16 pages): 1 sequence, 16000 keys, 24 rows 34 / 31, 48 34 / 54,
 // 96 49 / 96; 8 of 2000, 24 39 / 41, 48 45 / 76; 32 of 4000, 24 143 / 137, 48 242 / 261, 96 300 / 395;
 // bf16 queries, 32 of 4000, 24 121 / 116, 48 115 / 191; 32 heads on 8 of 128, 16 of 2000,
-// 16 rows 62 / 47, 32 64 / 58, 64 53 / 99.
-//   Rows: key is the us of one key of a tile on one workgroup, part those of one more
-// part of every row, as fitted to 1 to 2048 tokens of 1000 to 60000 keys.  Up to 64
-// parts: with 16 at most, 8 tokens of 60000 keys took 228 us for 75 (fp32), 16
-// of 16000 74 for 49.
+// 16 rows 62 / 47, 32 64 / 58, 64 53 / 99.  Batches that are not alike, bf16, 24 heads of 256,
+// 31 single tokens and one chunk, 2000 keys each: chunk of 30 75 / 60 (keys are split),
+// 100 75 / 60 (keys), 300 75 / 102 (rows), 1000 118 / 188 (rows).
+//   Rows: key is the us of one key of a tile beside others', part those of one more
+// part of every row, as fitted to 1 to 2048 tokens of 1000 to 60000 keys.  One figure
+// serves all types: alone on a CU a key of heads of 256 takes 0.029 us with one term, 0.049
+// with two, 0.057 with three (tiles of 64 rows), but the number of parts follows from the
+// rounds of workgroups; with 1.3 to 3 times the figure for more terms it came out as good
+// within 2 %.  One sequence of 16 to 2048 tokens of 1024 to 60000 keys, time over that of
+// the best number from 1 to 64, on average and at worst: bf16 queries 3 % and 16 %
+// (heads of 256), 5 and 15 (128); fp32 queries on f16 pages 3 and 12, 6 and 22, on bf16
+// pages 8 and 29, 10 and 32 (128 tokens of 16000 keys, heads of 128: 12 parts 133 us, 8
+// 98, as three terms leave room for one workgroup a CU, and the tiles are counted with one
+// to spare).  Up to 64 parts: with 16 at most, 8 tokens of 60000 keys took 228 us for
+// 75 (fp32), 16 of 16000 74 for 49.
 struct AttnPlan {
     bool keys;
     int64_t tiles, chunk, n_split;
