@@ -5,7 +5,7 @@ Reference: 64 bits.  U = 2^-24 is a rounding of fp32."""
 import pytest
 
 import bonsai_p40 as B
-from test_gpu_mixers import BF16, F16, F32, U, case, gen, half_step, ints, normwise
+from test_gpu_mixers import BF16, F16, F32, U, case, gen, half_step, ints, normwise, run_attn
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -140,6 +140,55 @@ def test_attn_scores_of_minus_infinity(n, kv, d, t, io):
             assert normwise(got[fin], ref[fin]) <= half_step(io)
 
 
+@pytest.mark.parametrize("t", [F16, BF16])
+@pytest.mark.parametrize("n,kv,d", [(1, 4000, 256), (1, 3000, 64), (30, 3000, 128)])
+def test_attn_minus_infinity_in_whole_parts(n, kv, d, t):
+    """Workgroups and waves that see keys of -inf only, beside others: they count for nothing in the join."""
+    g = gen(kv + n)
+    for hit in (slice(0, kv // 2), slice(kv // 2, kv - n), slice(64, kv - n - 64)):
+        case(f"-inf part n={n} kv={kv} d={d} {t} {hit}")
+        q, k, v = torch.randn(n, 4, d, generator=g), torch.randn(kv, 2, d, generator=g), torch.randn(kv, 2, d, generator=g)
+        q[..., 3], k[..., 3] = 300.0, 0.0
+        k[hit, :, 3] = -float("inf")
+        for work in (True, False):
+            got, ref = attend(q, k, v, t, t, work)
+            assert normwise(got, ref) <= half_step(t)
+
+
+@pytest.mark.parametrize("io", [F16, F32])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_attn_what_is_not_seen_stays_out_of_f16(io, value):
+    """Keys and values of later tokens of the same chunk, whatever they hold, with the terms of f16 pages."""
+    for new, kv, heads, kvh, d in (([40], [40], 6, 1, 256), ([9], [50], 3, 1, 128), ([100, 30], [230, 30], 4, 1, 64)):
+        def both(q, k, v, table):
+            for s, (n, c) in enumerate(zip(new, kv)):
+                for j in (c - 1, c - n // 2):
+                    k[int(table[s, j // 16]), :, j % 16] = v[int(table[s, j // 16]), :, j % 16] = value
+        run_attn(new, kv, heads, kvh, d, 16, F16, io, edit=both)
+
+        def values_only(q, k, v, table):
+            for s, (n, c) in enumerate(zip(new, kv)):
+                v[int(table[s, (c - 2) // 16]), :, (c - 2) % 16, 3] = value
+        run_attn(new, kv, heads, kvh, d, 16, F16, io, edit=values_only)
+
+
+@pytest.mark.parametrize("io", [F16, F32])
+@pytest.mark.parametrize("n,kv", [(1, 2000), (40, 500)])
+def test_attn_large_values(n, kv, io):
+    """Values up to f16's largest, all of the weight on them or spread over all keys: sums stay inside fp32."""
+    for d in (64, 256):
+        for spread in (0.0, 1.0):
+            case(f"large values n={n} kv={kv} d={d} {io} spread={spread}")
+            g = gen(d)
+            q, k = torch.randn(n, 2, d, generator=g) * spread, torch.randn(kv, 1, d, generator=g)
+            v = torch.where(torch.rand(kv, 1, d, generator=g) < 0.5, -65504.0, 65504.0)
+            v[..., 0] = 65504.0
+            got, ref = attend(q, k, v, io, F16)
+            err = (got.double() - ref).abs().max()
+            # beside the mean of the magnitudes, 65504: 2^-18, or P's and the store's half steps
+            assert float(err) <= 65504 * (2.0 ** -18 if io == F32 else 2 * half_step(io))
+
+
 # -------------------------------------------------------------------- gdn
 def delta(q, k, v, g, beta, state, t, eps, work=True, scale=None):
     """One sequence; ((outputs, state), the same in 64 bits).  Heads as they come."""
@@ -239,6 +288,21 @@ def test_gdn_elements_of_a_row_beside_a_large_one(work, t):
         check_rows(out, ref, list(range(n)), 2.0 ** -18, t)
         assert all(normwise(S[h], final[h]) <= 2.0 ** -18 for h in range(2))
 
+
+@pytest.mark.parametrize("work", [True, False])
+def test_gdn_rows_of_the_state_beside_a_large_one(work):
+    """A state with one row 2^15 above the others, which no key or query meets: 2^-40 2^15 is below 2^-18."""
+    n, r = 100, gen(6)
+    case(f"gdn state range work={work}")
+    q, k = torch.randn(n, 2, 128, generator=r), torch.randn(n, 2, 128, generator=r)
+    v, state = torch.randn(n, 2, 64, generator=r), torch.randn(1, 2, 128, 64, generator=r)
+    q[..., 7], k[..., 7] = 0.0, 0.0
+    state[:, :, 7] *= 2.0 ** 15
+    g, beta = -0.01 * torch.rand(n, 2, generator=r), torch.sigmoid(torch.randn(n, 2, generator=r))
+    (out, S), (ref, final) = delta(q, k, v, g, beta, state, F32, 1e-6, work)
+    check_rows(out, ref, list(range(n)), 2.0 ** -18, F32)
+    rest = [i for i in range(128) if i != 7]
+    assert all(normwise(S[h][rest], final[h][rest]) <= 2.0 ** -18 for h in range(2))
 
 @pytest.mark.parametrize("work", [True, False])
 def test_gdn_large_and_small_rows(work):
