@@ -453,7 +453,9 @@ int bonsai_p40_qk_norm_rope(const bonsai_p40_qk_norm_rope_args * args, bonsai_st
 // statistics and all sums are fp32.  io_type kv_type rounds each softmax weight once to
 // it before the product with V (with f16 a weight below 2^-25 of its row's largest is
 // off by up to 2^-36 of that one); fp32 keeps 22 bits of it or more (with f16 pages one
-// below 2^-25 is off by up to 2^-47 of the largest).  A row all of whose seen scores are
+// below 2^-25 is off by up to 2^-47 of the largest).  A row whose largest scaled score is
+// beyond 7e5 in magnitude has its scores rounded to fp32 (f16: and weights below
+// 2^-14 off by up to 2^-25, fp32 rows 2^-36, of the largest).  A row all of whose seen scores are
 // -inf is NaN, as 0 / 0 is; with fp32 rows so is one that sees a key that is not finite.
 // max_kv: about the largest kv_len (0: unknown); it places the work, results hold for
 // any.  workspace: bonsai_p40_attn_paged_workspace_bytes bytes (of the same

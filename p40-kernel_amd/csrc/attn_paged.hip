@@ -323,12 +323,29 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
     auto sees = [&](int key0, int holes) __attribute__((always_inline)) {
         return (key0 < vis && !(holes & 1)) || (key0 + 16 < vis && !(holes & 2));
     };
-    // m follows UP below the running maximum with a lag, so that the sums are rescaled seldom.  It is -inf while
-    // the row has seen no key, and finite behind that, whatever the scores (LEAST): l = 0 is then 0 / 0
-    constexpr float LEAST = -3e38f;
-    auto follow = [&](float mx) __attribute__((always_inline)) {
-        if (__any(mx > m + (UP + LAG))) {
-            const float m2 = fmaxf(m, mx - UP), alpha = __builtin_amdgcn_exp2f(m - (m2 == -INFINITY ? 0.0f : m2));
+    // m follows UP below the running maximum with a lag, so that the sums are rescaled seldom: at a largest score above
+    // limit.  It is -inf while the row has seen no key, and finite behind that, whatever the scores (LEAST): l = 0 is then
+    // 0 / 0.  ref: what the weights subtract.
+    //   m is a product that was rounded, and one fma of a score less it is off by up to half its step: FAR from 0 that
+    // is p far from 1, or past f16's end.  There each tile's scores are rounded like m first, as those of a softmax of
+    // fp32 scores are, ref is 0, and P 1 at the maximum
+    constexpr float LEAST = -3e38f, FAR = 1048576.0f;
+    float limit = -INFINITY, ref = 0.0f;
+    auto follow = [&](v16f & s, float mx) __attribute__((always_inline)) {
+        if (__any(mx > limit)) {
+            const bool near = fabsf(fmaxf(m, mx)) < FAR;
+            const float m2 = fmaxf(m, near ? mx - UP : mx), base = m2 == -INFINITY ? 0.0f : m2;
+            if (!near) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    float x = s[i] * c;
+                    asm("" : "+v"(x));                     // (no fma)
+                    s[i] = (x - base) / c;
+                }
+            }
+            limit = near ? m2 + (UP + LAG) : -INFINITY;
+            ref = near ? m2 : 0.0f;
+            const float alpha = __builtin_amdgcn_exp2f(m - base);
             m = m2;
             l *= alpha;
 #pragma unroll
@@ -338,7 +355,6 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
         }
     };
     auto weights = [&](v16f & s) __attribute__((always_inline)) {
-        const float ref = m == -INFINITY ? 0.0f : m;
         float sum[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -489,10 +505,9 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
                 mx = largest(s);
                 if (sees(key, holes)) mx = fmaxf(mx, LEAST);
             }
-            follow(mx);
+            follow(s, mx);
             // the scores of the next tile, and between their MFMAs the weights of this one (E of a step)
             constexpr int E = 16 / QS > 0 ? 16 / QS : 1;
-            const float ref = m == -INFINITY ? 0.0f : m;
             float sum[2] = {0.0f, 0.0f};
             frag vf[AHEAD], pf[NT][2];
             // (heads of 256: one wave a SIMD, and room for two blocks' sums of the second term; else a block's go to O before the next)
@@ -633,7 +648,7 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
             } else {
                 mx = fmaxf(largest(s), LEAST);
             }
-            follow(mx);
+            follow(s, mx);
             weights(s);
             if (key + 32 > first_vis && nk > max(first_vis, key)) apart(s, cur + Z::TILE, key);
             values(s, cur);

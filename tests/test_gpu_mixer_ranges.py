@@ -189,6 +189,65 @@ def test_attn_large_values(n, kv, io):
             assert float(err) <= 65504 * (2.0 ** -18 if io == F32 else 2 * half_step(io))
 
 
+@pytest.mark.parametrize("t,io", [(F16, F16), (BF16, BF16), (F16, F32), (BF16, F32)])
+@pytest.mark.parametrize("n,kv,d", [(1, 60, 64), (1, 3000, 256), (1, 2000, 128), (40, 300, 64), (40, 700, 256), (50, 600, 128)])
+@pytest.mark.parametrize("high", [300.0, 3000.0, 60000.0])
+def test_attn_scores_of_any_size(n, kv, d, t, io, high):
+    """Queries and keys up to f16's largest: scores of up to 2^36, which fp32 holds to 2^12 of it.
+
+    The largest score of a row is far above the next (where it is not, by 2^-18 of the largest and 40, the row is
+    not looked at): its key has all the weight, and the row is that key's value."""
+    case(f"scores n={n} kv={kv} d={d} {t} io={io} high={high}")
+    g = gen(int(high) + d)
+    q, k = (torch.rand(n, 2, d, generator=g) * 2 - 1) * high, (torch.rand(kv, 1, d, generator=g) * 2 - 1) * high
+    v = torch.randn(kv, 1, d, generator=g)
+    for work in (True, False):
+        got, ref = attend(q, k, v, io, t, work)
+        for h in range(2):
+            x = (q[:, h].to(io).double() @ k[:, 0].to(t).double().t()) * d ** -0.5
+            x = x.masked_fill(torch.arange(kv)[None] > (kv - n + torch.arange(n))[:, None], -float("inf"))
+            top = x.topk(2, -1)
+            clear = top.values[:, 0] - top.values[:, 1] > 40 + 2.0 ** -18 * x.masked_fill(x.isinf(), 0.0).abs().amax(-1)
+            assert int(clear.sum()) >= (n + 1) // 2 or high < 1000
+            want = v[top.indices[:, 0], 0].to(t).double()
+            assert torch.equal(ref[clear, h], want[clear])
+            # V's own value times P over l: one weight, of which P has the half step of 16 bits and the store another, or
+            # 2^-22 (fp32), and l, 1 / l and the product 3 roundings
+            off = (got[clear, h].double() - want[clear]).abs()
+            step = 2 * half_step(io) if io != F32 else 2.0 ** -22
+            assert bool((off <= want[clear].abs() * (step + 8 * U)).all())
+            assert bool(torch.isfinite(got).all())
+
+
+@pytest.mark.parametrize("t,io", [(F16, F16), (BF16, BF16), (F16, F32), (BF16, F32)])
+@pytest.mark.parametrize("n,kv,d", [(1, 2000, 256), (1, 900, 64), (40, 600, 128), (40, 500, 256)])
+def test_attn_scores_far_from_the_others(n, kv, d, t, io):
+    """Keys whose scores are 2^22 and more below the others' count for nothing, wherever they come; one far above has
+    all the weight.  (Powers of two in one element, so that those scores are exact; the others' are sums in fp32 of
+    products of usual size.)"""
+    g = gen(kv + d)
+    for low in (slice(0, kv // 3), slice(kv // 4, kv // 2), slice(0, kv, 2)):
+        case(f"far below n={n} kv={kv} d={d} {t} io={io} {low}")
+        q, k, v = torch.randn(n, 2, d, generator=g), torch.randn(kv, 1, d, generator=g), torch.randn(kv, 1, d, generator=g)
+        q[..., 0], k[..., 0] = 4096.0, 0.0
+        k[low, :, 0] = -16384.0
+        k[kv - n, :, 0] = 0.0
+        for work in (True, False):
+            got, ref = attend(q, k, v, io, t, work)
+            assert normwise(got, ref) <= (2.0 ** -18 if io == F32 else half_step(io))
+    for at in (0, kv // 2, kv - n):
+        case(f"far above n={n} kv={kv} d={d} {t} io={io} at={at}")
+        q, k, v = torch.randn(n, 2, d, generator=g), torch.randn(kv, 1, d, generator=g), torch.randn(kv, 1, d, generator=g)
+        q[..., 0], k[..., 0] = 4096.0, 0.0
+        k[at, :, 0] = 16384.0
+        got, ref = attend(q, k, v, io, t)
+        off, want = (got.double() - ref).abs(), v[at, 0].to(t).double()
+        assert torch.equal(ref, want.expand_as(ref))
+        # as with scores of any size: P's step and the store's
+        step = 2 * half_step(io) if io != F32 else 2.0 ** -22
+        assert bool((off <= want.abs() * (step + 8 * U)).all())
+
+
 # -------------------------------------------------------------------- gdn
 def delta(q, k, v, g, beta, state, t, eps, work=True, scale=None):
     """One sequence; ((outputs, state), the same in 64 bits).  Heads as they come."""
