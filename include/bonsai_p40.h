@@ -389,11 +389,22 @@ int bonsai_p40_chain_run(const void * plan, int n_steps, void * workspace, uint3
 #define BONSAI_P40_F32 0
 #define BONSAI_P40_F16 1
 #define BONSAI_P40_BF16 2
+#define BONSAI_P40_Q8 3                 // pages only
 // Pages of a key/value cache: page p holds, for each of n_kv_head heads,
 // page_size (a power of two) rows of head_dim elements; element e of slot i of
 // head h at p * page_stride + (h * page_size + i) * head_dim + e (elements;
 // page_stride a multiple of 8, n_kv_head * page_size * head_dim at least).
 // 16-byte aligned; keys and values in buffers of their own.
+//   Q8 pages: a row is head_dim signed bytes n and one fp32 scale d, and stands for d * n
+// (rounded once to fp32).  The bytes of slot i of head h of page p are at p * page_stride
+// + (h * page_size + i) * head_dim, its scale, fp32, at p * page_stride + n_kv_head * page_size *
+// head_dim + 4 * (h * page_size + i): page_stride is in bytes, a multiple of 16 and
+// n_kv_head * page_size * (head_dim + 4) at least.  A page is one piece, to be copied as one.
+// A row x is written as d = max |x| / 127, n = x * (127 / max |x|) rounded to the nearest
+// whole number, ties to even, in fp32: d * n is off by 0.50002 d at most.  A row whose
+// largest magnitude is below 2^-112 is written as 0, and one that holds a value that is
+// not finite with d = NaN, so that all of it is.  What is read may hold any n in -128 .. 127;
+// keys and values that attention sees are to have |d| of 0 or 2^-120 to 2^120.
 
 // RMSNorm of every query and key head, position rotation, and the append of
 // keys and values to the pages, in one launch:
@@ -406,7 +417,7 @@ int bonsai_p40_chain_run(const void * plan, int n_steps, void * workspace, uint3
 // (q_el == 1: rows of a GEMV; a head's queries may be followed by its gates) or the
 // tokens are (q_tok == 1: the feature-major Y of bonsai_p40_gemm, q_el = n_tok).
 // q goes to q_out (q_type: fp32, f16 or bf16), token t at t * q_out_tok, heads
-// one after another; k and v, rounded to kv_type (f16 or bf16), go to slot
+// one after another; k and v, rounded to kv_type (f16, bf16 or Q8), go to slot
 // slots[t] = page * page_size + i.  A slot outside 0 .. n_pages * page_size - 1
 // (-1: padding) is not written.  Slots of one call have to differ: what two
 // tokens leave in one slot is a mix.  Where slots are not written, the pages
@@ -449,7 +460,7 @@ int bonsai_p40_qk_norm_rope(const bonsai_p40_qk_norm_rope_args * args, bonsai_st
 // and from starts[n_seq] on are not touched.  Keys and values that a token does
 // not see never reach its output, whatever they hold.
 // q and out: token t at t * q_tok and t * out_tok, heads one after another, of
-// io_type: kv_type, or fp32; out overlaps nothing that is read.  Scores, softmax
+// io_type: kv_type, or fp32 (Q8 pages: fp32, f16 or bf16); out overlaps nothing that is read.  Scores, softmax
 // statistics and all sums are fp32.  io_type kv_type rounds each softmax weight once to
 // it before the product with V (with f16 a weight below 2^-25 of its row's largest is
 // off by up to 2^-36 of that one); fp32 keeps 22 bits of it or more (with f16 pages one
@@ -457,6 +468,10 @@ int bonsai_p40_qk_norm_rope(const bonsai_p40_qk_norm_rope_args * args, bonsai_st
 // beyond 7e5 in magnitude has its scores rounded to fp32 (f16: and weights below
 // 2^-14 off by up to 2^-25, fp32 rows 2^-36, of the largest).  A row all of whose seen scores are
 // -inf is NaN, as 0 / 0 is; with fp32 rows so is one that sees a key that is not finite.
+//   Q8 pages: a row of q is taken as whole numbers, an element off by at most 1.01 x 2^-15
+// (fp32: 1.6 x 2^-23) of its largest one; a row with a value that is not finite gives NaN.  A weight times its value's
+// d is rounded once to f16 (fp32: to 22 bits); one below 2^-25 of the row's largest such
+// product, taken tile by tile of 32 keys, is off by up to 2^-36 (2^-47) of that.
 // max_kv: about the largest kv_len (0: unknown); it places the work, results hold for
 // any.  workspace: bonsai_p40_attn_paged_workspace_bytes bytes (of the same
 // args), 16-byte aligned, scratch for the call (stream-ordered; calls that may
@@ -465,7 +480,7 @@ int bonsai_p40_qk_norm_rope(const bonsai_p40_qk_norm_rope_args * args, bonsai_st
 // max_kv and on whether a workspace is given; the same call gives the same bytes.
 // Errors: 1 if head_dim is not 64, 128 or 256, n_head (up to 65536) is no multiple
 // of n_kv_head, io_type, kv_type, page_size (a power of two, 16 .. 65536) or a
-// stride is not as stated (rows of q and out are 16-byte aligned), scale is not
+// stride is not as stated (rows of q and out are 16-byte aligned), a Q8 page is 2 GiB or more, scale is not
 // finite and > 0, max_pages * page_size > 2^31 - 65536, n_pages is outside 0 .. 2^31 - 1,
 // a pointer is NULL or misaligned, the workspace is too small, or there are 2^24 / n_head tokens and
 // sequences or more; 0 (no-op) if n_tok <= 0 or n_seq <= 0.
@@ -492,6 +507,58 @@ int bonsai_p40_attn_paged(const bonsai_p40_attn_paged_args * args, bonsai_stream
 // The pointers of args are not looked at; 0 where the call needs none or args
 // are invalid.
 int64_t bonsai_p40_attn_paged_workspace_bytes(const bonsai_p40_attn_paged_args * args);
+
+// The same for a batch whose sequences, group by group, begin with the same keys (a
+// system prompt, a document, several samples of one prompt), which are read once for all
+// rows of the group: group g is sequences groups[g] .. groups[g + 1] - 1, and its first
+// shared[g] keys (cut to 0 .. max_pages * page_size) are those of table[groups[g]].  A token of its
+// sequence s sees all of them, and then keys shared[g] .. p_t - 1 of table[s], whose
+// places are the same as in attn_paged (key j: slot j % page_size of page table[s *
+// table_stride + j / page_size]): where the rows of a group have the same pages for the shared
+// keys, or copies of them, and shared[g] <= kv_len - n_new, the result is attn_paged's but for the last bits.
+// shared[g] need not end a page; what table[s] has before it is not read for s > groups[g],
+// except that the 16 keys that hold key shared[g] are.
+// groups, which does not fall (sequences that two groups claim are undefined), is cut to
+// 0 .. n_seq; a sequence of no group sees its own keys, from 0 on.  max_shared: about the largest of
+// shared (0: unknown); as max_kv it places the work.  groups and shared are device memory, as
+// the other lengths are.
+// The workspace (attn.workspace, bonsai_p40_attn_shared_workspace_bytes bytes) is
+// needed: the sums of the shared keys and of the own ones meet there.
+// Errors: 1 as attn_paged, and if n_group or max_shared is negative, groups, shared or the
+// workspace is NULL or misaligned, or there are 2^24 / n_head tokens and groups or more.  n_group == 0 is
+// attn_paged.
+typedef struct bonsai_p40_attn_shared_args {
+    bonsai_p40_attn_paged_args attn;
+    const int32_t * groups;             // n_group + 1
+    const int32_t * shared;             // n_group
+    int64_t max_shared;
+    int n_group;
+} bonsai_p40_attn_shared_args;
+int bonsai_p40_attn_shared(const bonsai_p40_attn_shared_args * args, bonsai_stream stream);
+// The pointers of args are not looked at; 0 where args are invalid.
+int64_t bonsai_p40_attn_shared_workspace_bytes(const bonsai_p40_attn_shared_args * args);
+
+// Rows read back from the pages of a cache, for a program that hands them on or
+// works on them itself: k_out and v_out, token t at t * k_tok and t * v_tok elements of
+// out_type (fp32, f16 or bf16), heads one after another, become the key and the value
+// of slot slots[t] (= page * page_size + i), rounded once to out_type (Q8: d * n to fp32
+// before).  Where a slot is outside 0 .. n_pages * page_size - 1 the rows stay as they were; the same
+// slot may be read twice.  The outputs overlap nothing that is read.
+// Errors: 1 if head_dim is not 64, 128 or 256, n_kv_head is outside 1 .. 16384, a type,
+// page_size (a power of two, 1 .. 65536) or stride is not as stated (k_tok and v_tok at least a row, rows
+// 16-byte aligned), n_pages is outside 0 .. 2^40, a pointer is NULL or misaligned, or there are
+// over 2^30 tokens or 2^34 elements of k; 0 (no-op) if n_tok <= 0 or n_pages == 0.
+typedef struct bonsai_p40_kv_read_args {
+    const void * k_pages, * v_pages;
+    int64_t n_pages, page_stride;
+    int page_size, n_kv_head, head_dim, kv_type;
+    const int64_t * slots;              // n_tok
+    int64_t n_tok;
+    void * k_out, * v_out;
+    int64_t k_tok, v_tok;
+    int out_type;
+} bonsai_p40_kv_read_args;
+int bonsai_p40_kv_read(const bonsai_p40_kv_read_args * args, bonsai_stream stream);
 
 // Gated delta rule over the new tokens of n_seq sequences (the linear-attention
 // layers), with a state S of k_dim x v_dim fp32 for each value head.  Token by

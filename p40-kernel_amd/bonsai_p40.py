@@ -59,6 +59,9 @@ SIGNATURES = {
     "bonsai_p40_qk_norm_rope": [_V, _V],
     "bonsai_p40_attn_paged": [_V, _V],
     "bonsai_p40_attn_paged_workspace_bytes": [_V],
+    "bonsai_p40_attn_shared": [_V, _V],
+    "bonsai_p40_attn_shared_workspace_bytes": [_V],
+    "bonsai_p40_kv_read": [_V, _V],
     "bonsai_p40_gdn": [_V, _V],
     "bonsai_p40_gdn_workspace_bytes": [_V],
     "bonsai_p40_chunk_dots": [_V, _V, _V, _I64, _I64, _V],
@@ -73,7 +76,8 @@ SIGNATURES = {
     "bonsai_p40_chain_run": [_V, C.c_int, _V, _V, _V],
 }
 RESTYPES = {"bonsai_p40_chain_plan_bytes": C.c_int64, "bonsai_p40_gemm_workspace_bytes": C.c_int64,
-            "bonsai_p40_attn_paged_workspace_bytes": C.c_int64, "bonsai_p40_gdn_workspace_bytes": C.c_int64}
+            "bonsai_p40_attn_paged_workspace_bytes": C.c_int64, "bonsai_p40_attn_shared_workspace_bytes": C.c_int64,
+            "bonsai_p40_gdn_workspace_bytes": C.c_int64}
 
 _lib = None
 
@@ -435,8 +439,7 @@ class Chain:
 
 
 # ------------------------------------------------------------ token mixers
-F32, F16, BF16 = 0, 1, 2
-
+F32, F16, BF16, Q8 = 0, 1, 2, 3
 
 _FORMATS = {_V: "P", _I64: "q", C.c_int: "i", C.c_float: "f"}
 
@@ -453,11 +456,16 @@ QkNormRopeArgs = _args_struct("QkNormRopeArgs", doc="bonsai_p40_qk_norm_rope_arg
     (C.c_int, "n_head n_kv_head head_dim n_rot interleaved"), (C.c_float, "eps"),
     (_V, "q_norm k_norm pos inv_freq slots q_out"), (_I64, "q_out_tok"), (C.c_int, "q_type kv_type"),
     (_V, "k_pages v_pages"), (_I64, "n_pages page_stride"), (C.c_int, "page_size")])
-AttnPagedArgs = _args_struct("AttnPagedArgs", doc="bonsai_p40_attn_paged_args of include/bonsai_p40.h.", spec=[
-    (_V, "q out"), (_I64, "q_tok out_tok n_tok"), (C.c_int, "n_seq n_head n_kv_head head_dim io_type kv_type"),
-    (C.c_float, "scale"), (_V, "k_pages v_pages"), (_I64, "n_pages page_stride"), (C.c_int, "page_size max_pages"),
-    (_V, "table"), (_I64, "table_stride"), (_V, "starts kv_len"), (_I64, "max_kv"), (_V, "workspace"),
-    (_I64, "workspace_bytes")])
+_PAGED = [(_V, "q out"), (_I64, "q_tok out_tok n_tok"), (C.c_int, "n_seq n_head n_kv_head head_dim io_type kv_type"),
+          (C.c_float, "scale"), (_V, "k_pages v_pages"), (_I64, "n_pages page_stride"), (C.c_int, "page_size max_pages"),
+          (_V, "table"), (_I64, "table_stride"), (_V, "starts kv_len"), (_I64, "max_kv"), (_V, "workspace"),
+          (_I64, "workspace_bytes")]
+AttnPagedArgs = _args_struct("AttnPagedArgs", doc="bonsai_p40_attn_paged_args of include/bonsai_p40.h.", spec=_PAGED)
+AttnSharedArgs = _args_struct("AttnSharedArgs", doc="bonsai_p40_attn_shared_args of include/bonsai_p40.h, the fields of attn in its place.",
+                              spec=_PAGED + [(_V, "groups shared"), (_I64, "max_shared"), (C.c_int, "n_group")])
+KvReadArgs = _args_struct("KvReadArgs", doc="bonsai_p40_kv_read_args of include/bonsai_p40.h.", spec=[
+    (_V, "k_pages v_pages"), (_I64, "n_pages page_stride"), (C.c_int, "page_size n_kv_head head_dim kv_type"), (_V, "slots"),
+    (_I64, "n_tok"), (_V, "k_out v_out"), (_I64, "k_tok v_tok"), (C.c_int, "out_type")])
 GdnArgs = _args_struct("GdnArgs", doc="bonsai_p40_gdn_args of include/bonsai_p40.h.", spec=[
     (_V, "q k v out"), (_I64, "q_tok k_tok v_tok out_tok"), (_V, "g beta"), (_I64, "gate_tok"),
     (_V, "state state_out"), (_I64, "n_states"), (_V, "slots starts"), (_I64, "n_tok"),
@@ -471,7 +479,7 @@ def _type(t) -> int:
     if not _TYPES:
         import torch
         _TYPES.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.int32: "int32",
-                       torch.int64: "int64", torch.float64: "float64"})
+                       torch.int64: "int64", torch.float64: "float64", torch.int8: "int8"})
     ty = _TYPES.get(t.dtype)
     if ty is None or ty.__class__ is str:
         raise ValueError(f"element type {t.dtype}: fp32, f16 or bf16 is wanted")
@@ -503,12 +511,34 @@ def _pages(k_pages, v_pages, dev: int):
     vt = v_pages.stride()
     if (len(st) != 4 or v_pages.shape != shape or v_pages.dtype is not k_pages.dtype
             or vt != st and any(a != b and m > 1 for a, b, m in zip(vt, st, shape)) or not dev == k_pages.get_device() == v_pages.get_device()):
-        raise ValueError("k_pages and v_pages: alike, (n_pages, n_kv_head, page_size, head_dim), beside q")
+        raise ValueError("k_pages and v_pages: alike, (n_pages, n_kv_head, page_size, head_dim), beside q or the outputs")
     n, h, p, d = shape
     page, head, row, el = st
     if (el != 1 and d != 1) or (row != d and p != 1) or (head != p * d and h != 1):
         raise ValueError("a page has to lie in one piece")
-    return n, h, p, d, page if n > 1 else h * p * d, _type(k_pages)
+    if _TYPES.get(k_pages.dtype) != "int8":
+        return n, h, p, d, page if n > 1 else h * p * d, _type(k_pages)
+    # 8 bits: the scales lie behind the rows of each page, outside the tensor that names these (a slice of its heads
+    # would put them elsewhere)
+    size = h * p * (d + 4)
+    if n <= 1:
+        page = size + -size % 16
+    if page != size + -size % 16 or any(t.storage_offset() + (n - 1) * page + size > t.untyped_storage().nbytes()
+                                        for t in (k_pages, v_pages) if n):
+        raise ValueError("8-bit pages follow each other, each with room for its scales, as q8_pages makes them")
+    return n, h, p, d, page, Q8
+
+
+def q8_pages(n_pages: int, n_kv_head: int, page_size: int, head_dim: int, device="cuda"):
+    """Zeroed 8-bit pages (of keys or of values): the whole numbers, int8 (n_pages,
+    n_kv_head, page_size, head_dim), which the calls take as k_pages or v_pages, and the
+    scales, fp32 (n_pages, n_kv_head, page_size), two views of one piece of memory in
+    which a page's scales follow its rows."""
+    import torch
+    rows, scales = n_kv_head * page_size * head_dim, 4 * n_kv_head * page_size
+    memory = torch.zeros((n_pages, rows + scales + -(rows + scales) % 16), dtype=torch.int8, device=device)
+    return (memory[:, :rows].unflatten(1, (n_kv_head, page_size, head_dim)),
+            memory[:, rows:rows + scales].view(torch.float32).unflatten(1, (n_kv_head, page_size)))
 
 
 def rope_inv_freq(n_rot: int, base: float, device="cuda"):
@@ -575,7 +605,7 @@ def qk_norm_rope(q, k, v, q_norm, k_norm, eps: float, pos, inv_freq, slots, k_pa
         _check("bonsai_p40_qk_norm_rope", rc)
 
 
-def _attn_args(q, k_pages, v_pages, table, starts, kv_len, out, workspace, max_kv, scale):
+def _attn_args(q, k_pages, v_pages, table, starts, kv_len, out, workspace, max_kv, scale, pack=None, *more):
     shape, entries, steps = q.shape, table.shape, table.stride()
     if len(shape) != 3 or len(steps) != 2:
         raise ValueError("q: (n_tok, heads, head_dim) and table: (n_seq, max_pages) are wanted")
@@ -592,11 +622,11 @@ def _attn_args(q, k_pages, v_pages, table, starts, kv_len, out, workspace, max_k
     if _TYPES.get(table.dtype) != "int32" or (col != 1 and cols > 1) or table.get_device() != dev:
         raise ValueError("table: int32 rows beside q are wanted")
     ws, ws_bytes = _scratch(workspace, dev)
-    return AttnPagedArgs.pack(
+    return (pack or AttnPagedArgs.pack)(
         q.data_ptr(), out.data_ptr(), _rows(q, "q", shape, dev), _rows(out, "out", shape, dev), n, n_seq, h, kv, d, io, kv_type,
         d ** -0.5 if scale is None else scale, k_pages.data_ptr(), v_pages.data_ptr(), pages, stride, page_size, cols,
         table.data_ptr(), row if n_seq > 1 else cols, _flat(starts, "starts", "int32", n_seq + 1, dev),
-        _flat(kv_len, "kv_len", "int32", n_seq, dev), max_kv, ws, ws_bytes)
+        _flat(kv_len, "kv_len", "int32", n_seq, dev), max_kv, ws, ws_bytes, *more)
 
 
 def attn_paged_workspace_bytes(q, k_pages, v_pages, table, starts, kv_len, out, max_kv: int = 0, scale=None) -> int:
@@ -614,6 +644,53 @@ def attn_paged(q, k_pages, v_pages, table, starts, kv_len, out, workspace=None, 
     rc = lib().bonsai_p40_attn_paged(a, _stream_of(q, stream))
     if rc:
         _check("bonsai_p40_attn_paged", rc)
+
+
+def _attn_shared_args(q, k_pages, v_pages, table, starts, kv_len, groups, shared, out, workspace, max_kv, max_shared, scale):
+    _type(q)
+    dev, n = q.get_device(), shared.numel()
+    return _attn_args(q, k_pages, v_pages, table, starts, kv_len, out, workspace, max_kv, scale, AttnSharedArgs.pack,
+                      _flat(groups, "groups", "int32", n + 1, dev), _flat(shared, "shared", "int32", n, dev), max_shared, n)
+
+
+def attn_shared_workspace_bytes(q, k_pages, v_pages, table, starts, kv_len, groups, shared, out, max_kv: int = 0,
+                                max_shared: int = 0, scale=None) -> int:
+    """bonsai_p40_attn_shared_workspace_bytes for these arguments of attn_shared."""
+    a = _attn_shared_args(q, k_pages, v_pages, table, starts, kv_len, groups, shared, out, None, max_kv, max_shared, scale)
+    return int(lib().bonsai_p40_attn_shared_workspace_bytes(a))
+
+
+def attn_shared(q, k_pages, v_pages, table, starts, kv_len, groups, shared, out, workspace, max_kv: int = 0,
+                max_shared: int = 0, scale=None, stream=None) -> None:
+    """attn_paged of a batch whose sequences groups[g] .. groups[g + 1] - 1 begin with
+    the same shared[g] keys, those of table[groups[g]], which are read once for all of them."""
+    a = _attn_shared_args(q, k_pages, v_pages, table, starts, kv_len, groups, shared, out, workspace, max_kv, max_shared, scale)
+    rc = lib().bonsai_p40_attn_shared(a, _stream_of(q, stream))
+    if rc:
+        _check("bonsai_p40_attn_shared", rc)
+
+
+def _kv_read_args(k_pages, v_pages, slots, k_out, v_out):
+    shape = k_out.shape
+    if len(shape) != 3 or v_out.dtype is not k_out.dtype:
+        raise ValueError("k_out and v_out: (n_tok, n_kv_head, head_dim) of one type are wanted")
+    n, kv, d = shape
+    out, dev = _type(k_out), k_out.get_device()
+    pages, page_kv, page_size, page_d, stride, kv_type = _pages(k_pages, v_pages, dev)
+    if page_kv != kv or page_d != d:
+        raise ValueError("the pages have other heads")
+    return KvReadArgs.pack(k_pages.data_ptr(), v_pages.data_ptr(), pages, stride, page_size, kv, d, kv_type,
+                           _flat(slots, "slots", "int64", n, dev), n, k_out.data_ptr(), v_out.data_ptr(),
+                           _rows(k_out, "k_out", shape, dev), _rows(v_out, "v_out", shape, dev), out)
+
+
+def kv_read(k_pages, v_pages, slots, k_out, v_out, stream=None) -> None:
+    """Rows slots of the pages (16-bit, or 8-bit as q8_pages makes them) into k_out and
+    v_out, (n_tok, n_kv_head, head_dim) fp32, f16 or bf16; rows of slots outside stay as they were."""
+    a = _kv_read_args(k_pages, v_pages, slots, k_out, v_out)
+    rc = lib().bonsai_p40_kv_read(a, _stream_of(k_out, stream))
+    if rc:
+        _check("bonsai_p40_kv_read", rc)
 
 
 def _gdn_args(q, k, v, g, beta, state, state_out, out, starts, workspace, max_new, slots, scale, l2_eps, tiled):

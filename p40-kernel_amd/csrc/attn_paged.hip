@@ -48,28 +48,13 @@
 #include "gemv_device.h"
 #include "host_state.h"
 #include "launch_rules.h"
-#include "mixer_device.h"
+#include "attn_device.h"
 
 #include <type_traits>
 
 using namespace mixer;
 
 namespace {
-
-struct AttnArgs {
-    const void * q;
-    void * out;
-    const uint8_t * k, * v;
-    const int32_t * table, * starts, * kv_len;
-    float * part;                       // [split][row][D] then [split][row] (m, l)
-    int64_t q_tok, out_tok;             // elements
-    int64_t page_bytes, head_bytes;
-    int64_t table_stride;
-    int n_tok, n_seq, n_head, n_kv, group;
-    int n_pages, page_log2, cap;        // cap: keys the table can name
-    int chunk, n_split, tiles;
-    float c;                            // scale * log2(e)
-};
 
 template <class T>
 __device__ __forceinline__ v16f mfma(typename T::frag a, typename T::frag b, v16f c);
@@ -88,9 +73,6 @@ __device__ __forceinline__ v2u read_tr(const uint8_t * at) {
     typedef __attribute__((address_space(3))) s4 lds_s4;
     return __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)at));
 }
-
-// 1 / l; 0 where no key was seen, NaN where the score of every key that was is -inf
-__device__ __forceinline__ float over(float m, float l) { return m == -INFINITY ? 0.0f : l != 0.0f ? 1.0f / l : NAN; }
 
 template <class T, int D, int NT, bool KEYS>
 struct Shape {
@@ -111,7 +93,7 @@ struct Shape {
     static constexpr int LDS = KEYS && JOIN > ALL ? JOIN : ALL;
 };
 
-template <class T, int D, int NT, bool KEYS>
+template <class T, int D, int NT, bool KEYS, bool SHARED>
 __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) attn_kernel(AttnArgs a) {
     typedef Shape<T, D, NT, KEYS> Z;
     typedef typename T::elem elem;
@@ -123,28 +105,22 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 31, half = lane >> 5;
-    // heads vary fastest: a head's tiles meet on the same XCDs, and then in their L2, as those that run at the
-    // same time have the same keys; the last tiles, which see the most, start first
-    const int kvh = blockIdx.x % a.n_kv, rest = blockIdx.x / a.n_kv;
-    const int split = rest / a.tiles, tile_no = a.tiles - 1 - rest % a.tiles;
+    const AttnPlace at = attn_place<SHARED>(&a);
+    const int kvh = at.kvh;
     // one sequence: its row of the table is known (and there is one, where there are pages), and the entries of a wave's first keys are asked for beside starts
     int early0 = -1, early1 = -1;
-    const bool early = KEYS && a.n_seq == 1 && a.cap > 0 && a.n_pages > 0;
+    const bool early = KEYS && !SHARED && a.n_seq == 1 && a.cap > 0 && a.n_pages > 0;
     if (early) {
-        const int key = split * a.chunk + 32 * wave, top = (a.cap >> a.page_log2) - 1;
+        const int key = at.split * a.chunk + 32 * wave, top = (a.cap >> a.page_log2) - 1;
         early0 = sload(a.table, min(key >> a.page_log2, top));
         early1 = sload(a.table, min((key + 16) >> a.page_log2, top));
     }
-    const Tile tl = find_tile<Z::BM>(a.starts, a.kv_len, a.n_seq, a.n_tok, a.group, tile_no);
-    if (tl.seq < 0) return;
-    const int rows = tl.count * a.group, row0 = tl.index * Z::BM;
-    const int kv = iclamp(tl.extra, 0, a.cap), before = kv - tl.count;
-    const int last = min(row0 + Z::BM, rows) - 1;
-    // (readfirstlane: the same in all lanes, which the compiler does not see through the division)
-    const int nk = a.n_pages > 0 ? __builtin_amdgcn_readfirstlane(iclamp(before + last / a.group + 1, 0, kv)) : 0;
-    const int k0 = split * a.chunk;
-    const int k1 = split == a.n_split - 1 ? nk : min(nk, k0 + a.chunk);
-    if (split > 0 && k0 >= nk) return;                     // the join counts the parts
+    AttnWork w;
+    if (!attn_work<Z::BM, SHARED>(a, at, w)) return;
+    const Tile & tl = w.tl;
+    const int kv = w.kv, before = w.before, nk = w.nk, k0 = w.k0, k1 = w.k1;
+    const int lo = SHARED ? w.lo : 0;                      // keys before it are not seen
+    const int rows = tl.count * a.group, row0 = tl.index * Z::BM, last = min(row0 + Z::BM, rows) - 1;
 
     // this lane's row
     const int wrow = row0 + (KEYS ? 0 : 32 * wave);
@@ -299,10 +275,22 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
     };
     // scores that are not seen to -inf
     auto mask = [&](v16f & s, int key0, int holes) __attribute__((always_inline)) {
+        if constexpr (SHARED) {
+            int from = lo - key0 - 4 * half, to = vis - key0 - 4 * half;
+            asm("" : "+v"(from));                          // (its part that all lanes share is not worth 16 scalars)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int j = 8 * (i / 4) + 4 * half + i % 4;
-            if (key0 + j >= vis || (holes >> (j >> 4) & 1)) s[i] = -INFINITY;
+            for (int g = 0; g < 2; ++g) {
+                const uint32_t count = holes >> g & 1 ? 0 : max(to - from, 0);   // places from .. from + count are seen
+#pragma unroll
+                for (int i = 8 * g; i < 8 * g + 8; ++i)
+                    if ((uint32_t)(8 * (i / 4) + i % 4 - from) >= count) s[i] = -INFINITY;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int j = 8 * (i / 4) + 4 * half + i % 4;
+                if (key0 + j >= vis || (holes >> (j >> 4) & 1)) s[i] = -INFINITY;
+            }
         }
     };
     // a row's largest score, in units of log2: half the keys are in lane ^ 32
@@ -321,7 +309,7 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
     };
     // whether the row sees a key of the sub-tile
     auto sees = [&](int key0, int holes) __attribute__((always_inline)) {
-        return (key0 < vis && !(holes & 1)) || (key0 + 16 < vis && !(holes & 2));
+        return (max(key0, lo) < (SHARED ? min(vis, key0 + 16) : vis) && !(holes & 1)) || (max(key0 + 16, lo) < vis && !(holes & 2));
     };
     // m follows UP below the running maximum with a lag, so that the sums are rescaled seldom: at a largest score above
     // limit.  It is -inf while the row has seen no key, and finite behind that, whatever the scores (LEAST): l = 0 is then
@@ -475,7 +463,9 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
             idk = own < 16 ? (ok0 ? raw0 : -1) : (ok1 ? raw1 : -1);
         };
         auto stage = [&](const uint8_t * base, int id, int t, uint8_t * to, bool is_v) __attribute__((always_inline)) {
-            stage_n(std::integral_constant<int, OWN>{}, base, id, k0 + 32 * t + own, own & 15, to + own * Z::RB, is_v);
+            int at = own;                                  // (SHARED: anew each time, as held for every slot it takes too many registers)
+            if (SHARED) asm volatile("" : "+s"(at));
+            stage_n(std::integral_constant<int, OWN>{}, base, id, k0 + 32 * t + at, at & 15, to + at * Z::RB, is_v);
         };
         // that the buffers differ has to be said, else every read of LDS waits for the DMA
         auto step = [&](auto edge, auto steady, uint8_t * __restrict__ kw, uint8_t * __restrict__ vw, const uint8_t * __restrict__ kr,
@@ -592,7 +582,7 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
             const float bottom = LEAST / fmaxf(c, 1.0f);   // (times c: finite)
             float mx = fmaxf(largest(s), LEAST);
             // tiles that every row sees whole, then those at the edge
-            const int plain = max(min(nt, (first_vis - k0) / 32), 0);
+            const int plain = SHARED && k0 < lo ? 0 : max(min(nt, (first_vis - k0) / 32), 0);
             // (steady: every load that a tile can start is there; R of them at a time, with the rings' places
             // known to the compiler)
             auto pass = [&](auto edge, auto steady, int slot, int j) __attribute__((always_inline)) {
@@ -601,6 +591,7 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
                 else pq2::wait_vmcnt<0>();
                 const int holes = hq >> (2 * R - 2) & 3, key = k0 + 32 * j + own;
                 const bool hole = holes >> (own >> 4) & 1;
+                if (SHARED && !steady && key < lo) zero_keys(vring + slot * Z::TILE + own * Z::RB, 0, min(lo - key, OWN));
                 if (hole || (!steady && key + OWN > nk))
                     zero_keys(vring + slot * Z::TILE + own * Z::RB, hole ? 0 : iclamp(nk - key, 0, OWN), OWN);
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -641,7 +632,7 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
             if (key + 32 * Z::NW < k1) stage(key + 32 * Z::NW, false, next);
             v16f s = scores(cur, qlow);
             float mx;
-            if (key + 32 > least || holes) {
+            if (key + 32 > least || holes || (SHARED && key < lo)) {
                 mask(s, key, holes);
                 mx = largest(s);
                 if (sees(key, holes)) mx = fmaxf(mx, LEAST);
@@ -661,6 +652,7 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
             const int holes = (id0 < 0 ? 1 : 0) | (id1 < 0 ? 2 : 0);
             uint8_t * const cur = mine + b * 2 * Z::TILE;
             pq2::wait_vmcnt<0>();
+            if (SHARED && key < lo) zero_keys(cur + Z::TILE, 0, min(lo - key, 32));
             if (holes || key + 32 > nk) {
                 zero_keys(cur + Z::TILE, holes & 1 ? 0 : iclamp(nk - key, 0, 16), 16);
                 zero_keys(cur + Z::TILE, holes & 2 ? 16 : iclamp(nk - key, 16, 32), 32);
@@ -671,13 +663,17 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
     }
     l += __shfl_xor(l, 32);
 
-    const bool parts = a.n_split > 1;
-    const int64_t all_rows = (int64_t)a.n_tok * a.n_head;
+    // (SHARED: the arguments of this end of the kernel are read again rather than held all along)
+    const auto z = args_of<SHARED>(a);
+    const int part = attn_part<SHARED>(z, SHARED ? attn_place<SHARED>(z) : at);
+    const int n_part = SHARED ? z->n_split1 + z->n_split : z->n_split;
+    const bool parts = SHARED || z->n_split > 1;
+    const int64_t all_rows = (int64_t)z->n_tok * z->n_head;
     if constexpr (!KEYS) {
         if (!live) return;
-        const int64_t row = grow * a.n_head + head;
+        const int64_t row = grow * z->n_head + head;
         const float inv = parts ? 1.0f : over(m, l);
-        float * const po = a.part + ((int64_t)split * all_rows + row) * D;
+        float * const po = z->part + ((int64_t)part * all_rows + row) * D;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -688,11 +684,11 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
                 const int at = 32 * d + 8 * g + 4 * half;
                 if (parts) store_row<F32>(po + at, x);
                 else if constexpr (NT == 1)
-                    store_row<T>(reinterpret_cast<elem *>(a.out) + grow * a.out_tok + (int64_t)head * D + at, x);
-                else store_row<F32>(reinterpret_cast<float *>(a.out) + grow * a.out_tok + (int64_t)head * D + at, x);
+                    store_row<T>(reinterpret_cast<elem *>(z->out) + grow * z->out_tok + (int64_t)head * D + at, x);
+                else store_row<F32>(reinterpret_cast<float *>(z->out) + grow * z->out_tok + (int64_t)head * D + at, x);
             }
         if (parts && half == 0)
-            *reinterpret_cast<float2 *>(a.part + (int64_t)a.n_split * all_rows * D + 2 * ((int64_t)split * all_rows + row)) =
+            *reinterpret_cast<float2 *>(z->part + (int64_t)n_part * all_rows * D + 2 * ((int64_t)part * all_rows + row)) =
                 make_float2(m, l);
     } else {
         // join the waves: [wave][row][D] and [wave][row] (m, l)
@@ -726,132 +722,55 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
 #pragma unroll
                 for (int j = 0; j < E; ++j) x[j] = fmaf(jo[(k * 32 + i) * Z::OROW + lane * E + j], w, x[j]);
             }
-            const int rr = row0 + i, t = rr / a.group, h = kvh * a.group + rr - t * a.group;
-            const int64_t g = tl.first + t, row = g * a.n_head + h;
+            const int rr = row0 + i, t = rr / z->group, h = kvh * z->group + rr - t * z->group;
+            const int64_t g = tl.first + t, row = g * z->n_head + h;
             if (parts) {
-                store_row<F32>(a.part + ((int64_t)split * all_rows + row) * D + lane * E, x);
+                store_row<F32>(z->part + ((int64_t)part * all_rows + row) * D + lane * E, x);
                 if (lane == 0)
-                    *reinterpret_cast<float2 *>(a.part + (int64_t)a.n_split * all_rows * D +
-                                                2 * ((int64_t)split * all_rows + row)) = make_float2(mm, ll);
+                    *reinterpret_cast<float2 *>(z->part + (int64_t)n_part * all_rows * D +
+                                                2 * ((int64_t)part * all_rows + row)) = make_float2(mm, ll);
             } else {
                 const float inv = over(mm, ll);
 #pragma unroll
                 for (int j = 0; j < E; ++j) x[j] *= inv;
                 if constexpr (NT == 1)
-                    store_row<T>(reinterpret_cast<elem *>(a.out) + g * a.out_tok + (int64_t)h * D + lane * E, x);
-                else store_row<F32>(reinterpret_cast<float *>(a.out) + g * a.out_tok + (int64_t)h * D + lane * E, x);
+                    store_row<T>(reinterpret_cast<elem *>(z->out) + g * z->out_tok + (int64_t)h * D + lane * E, x);
+                else store_row<F32>(reinterpret_cast<float *>(z->out) + g * z->out_tok + (int64_t)h * D + lane * E, x);
             }
         }
     }
 }
 
-// The parts of every row, by WR waves.  Their number follows from the keys the
-// row's tile saw, as in attn_kernel; the largest m is looked for among all that
-// there could be while the lengths are on their way.
-template <class TO, int D, int WR>
-__global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int bm) {
-    constexpr int E = D / 64, AHEAD = 8;
-    __shared__ float sum[4][D + 1];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave % WR;
-    const int64_t all_rows = (int64_t)a.n_tok * a.n_head, row = (int64_t)blockIdx.x * (4 / WR) + wave / WR;
-    if (row >= all_rows) return;
-    const int tok = (int)(row / a.n_head), head = (int)(row - (int64_t)tok * a.n_head);
-    const float2 * const ml = reinterpret_cast<const float2 *>(a.part + (int64_t)a.n_split * all_rows * D) + row;
-    float own = -INFINITY;
-    if (lane < a.n_split) own = ml[lane * all_rows].x;
-    // (4 waves: the first parts, too; those behind the last are not written, and not used)
-    float v[AHEAD][E];
-    float2 e[AHEAD];
-    auto load = [&](int i0, int n) __attribute__((always_inline)) {
-#pragma unroll
-        for (int k = 0; k < AHEAD; ++k) {
-            const int64_t i = min(i0 + k * WR, n - 1);
-            e[k] = ml[i * all_rows];
-            load_row<F32>(a.part + (i * all_rows + row) * D + lane * E, v[k]);
-        }
-    };
-    if (WR > 1) load(w, a.n_split);
-    // the sequence of this token
-    int seq = -1, first = 0, count = 0, kv = 0;
-    for (int s0 = 0; s0 < a.n_seq && seq < 0; s0 += 64) {
-        const int s = s0 + lane;
-        int b = 0, e = 0, len = 0;
-        if (s < a.n_seq) {
-            b = iclamp(a.starts[s], 0, a.n_tok);
-            e = iclamp(a.starts[s + 1], 0, a.n_tok);
-            len = iclamp(a.kv_len[s], 0, a.cap);
-        }
-        const uint64_t hit = __ballot(tok >= b && tok < e);
-        if (hit) {
-            const int k = __builtin_ctzll(hit);
-            seq = s0 + k;
-            first = __builtin_amdgcn_readlane(b, k);
-            count = __builtin_amdgcn_readlane(e, k) - first;
-            kv = __builtin_amdgcn_readlane(len, k);
-        }
-    }
-    if (seq < 0) return;                                   // a row behind the last sequence
-    const int r = (tok - first) * a.group + head % a.group;
-    const int last = min(r / bm * bm + bm, count * a.group) - 1;
-    const int nk = a.n_pages > 0 ? iclamp(kv - count + last / a.group + 1, 0, kv) : 0;
-    const int n = iclamp((nk + a.chunk - 1) / a.chunk, 1, a.n_split);
-    float mm = lane < n ? own : -INFINITY;
-    for (int i = 64 + lane; i < n; i += 64) mm = fmaxf(mm, ml[i * all_rows].x);
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) mm = fmaxf(mm, __shfl_xor(mm, d));
-    const float ref = mm == -INFINITY ? 0.0f : mm;
-    float x[E] = {}, l = 0.0f;
-    for (int i0 = w; i0 < n; i0 += WR * AHEAD) {
-        if (WR == 1 || i0 != w) load(i0, n);
-#pragma unroll
-        for (int k = 0; k < AHEAD; ++k)
-            if (i0 + k * WR < n) {
-                const float wt = __builtin_amdgcn_exp2f(e[k].x - ref);
-                l = fmaf(e[k].y, wt, l);
-#pragma unroll
-                for (int j = 0; j < E; ++j) x[j] = fmaf(v[k][j], wt, x[j]);
-            }
-    }
-    if constexpr (WR > 1) {
-#pragma unroll
-        for (int j = 0; j < E; ++j) sum[wave][lane * E + j] = x[j];
-        if (lane == 0) sum[wave][D] = l;
-        __syncthreads();                                   // (WR = 4: one row a workgroup, all waves are here)
-        if (w) return;
-        for (int k = 1; k < WR; ++k) {
-            l += sum[k][D];
-#pragma unroll
-            for (int j = 0; j < E; ++j) x[j] += sum[k][lane * E + j];
-        }
-    }
-    const float inv = over(mm, l);
-#pragma unroll
-    for (int j = 0; j < E; ++j) x[j] *= inv;
-    store_row<TO>(reinterpret_cast<typename TO::elem *>(a.out) + (int64_t)tok * a.out_tok + (int64_t)head * D + lane * E, x);
-}
-
-template <class T, int D, int NT, bool KEYS>
-int launch(AttnArgs & a, hipStream_t s) {
+// Shared prefixes: their phase and that of the own keys in one launch where both have this shape, then the join
+template <class T, int D, int NT, bool KEYS, bool SHARED>
+int launch(AttnArgs & a, bool first, bool own, hipStream_t s) {
     typedef Shape<T, D, NT, KEYS> Z;
-    const int64_t blocks = (int64_t)a.tiles * a.n_split * a.n_kv;
-    hipLaunchKernelGGL((attn_kernel<T, D, NT, KEYS>), dim3((unsigned)blocks), dim3(64 * Z::NW), 0, s, a);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || a.n_split == 1) return (int)e;
-    typedef typename std::conditional<NT == 1, T, F32>::type TO;
-    const int64_t rows = (int64_t)a.n_tok * a.n_head;
-    if (pq2::attn_join_wide(a.n_split))
-        hipLaunchKernelGGL((attn_join_kernel<TO, D, 4>), dim3((unsigned)rows), dim3(256), 0, s, a, (int)Z::BM);
-    else hipLaunchKernelGGL((attn_join_kernel<TO, D, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a, (int)Z::BM);
+    AttnArgs b = a;
+    b.blocks1 = first ? (unsigned)((int64_t)a.tiles1 * a.n_split1 * a.n_kv) : 0;
+    const int64_t blocks = b.blocks1 + (own ? (int64_t)a.tiles * a.n_split * a.n_kv : 0);
+    hipLaunchKernelGGL((attn_kernel<T, D, NT, KEYS, SHARED>), dim3((unsigned)blocks), dim3(64 * Z::NW), 0, s, b);
     return (int)hipGetLastError();
 }
+template <class T, int D, int NT, bool SHARED>
+int launch_k(const AttnLaunch & l, AttnArgs & a, hipStream_t s) {
+    int e = 0;
+    if (SHARED && l.keys1 != l.keys)
+        e = l.keys1 ? launch<T, D, NT, true, SHARED>(a, true, false, s) : launch<T, D, NT, false, SHARED>(a, true, false, s);
+    if (e) return e;
+    const bool both = SHARED && l.keys1 == l.keys;
+    e = l.keys ? launch<T, D, NT, true, SHARED>(a, both, true, s) : launch<T, D, NT, false, SHARED>(a, both, true, s);
+    if (e || !l.parts) return e;
+    typedef typename std::conditional<NT == 1, T, F32>::type TO;
+    return launch_join<TO, D, SHARED>(a, l.keys ? Shape<T, D, NT, true>::BM : Shape<T, D, NT, false>::BM, s);
+}
 template <class T, int D, int NT>
-int launch_k(bool keys, AttnArgs & a, hipStream_t s) {
-    return keys ? launch<T, D, NT, true>(a, s) : launch<T, D, NT, false>(a, s);
+int launch_s(const AttnLaunch & l, AttnArgs & a, hipStream_t s) {
+    return l.shared ? launch_k<T, D, NT, true>(l, a, s) : launch_k<T, D, NT, false>(l, a, s);
 }
 template <class T, int NT>
-int launch_d(int d, bool keys, AttnArgs & a, hipStream_t s) {
-    return d == 256 ? launch_k<T, 256, NT>(keys, a, s) : d == 128 ? launch_k<T, 128, NT>(keys, a, s)
-                                                                  : launch_k<T, 64, NT>(keys, a, s);
+int launch_d(const AttnLaunch & l, AttnArgs & a, hipStream_t s) {
+    return l.head_dim == 256 ? launch_s<T, 256, NT>(l, a, s) : l.head_dim == 128 ? launch_s<T, 128, NT>(l, a, s)
+                                                                                 : launch_s<T, 64, NT>(l, a, s);
 }
 
 // 1: invalid, 0: nothing to do, -1: to be run
@@ -860,10 +779,14 @@ int check(const bonsai_p40_attn_paged_args * p) {
     const int d = p->head_dim;
     if (d != 64 && d != 128 && d != 256) return 1;
     if (p->n_kv_head < 1 || p->n_head < 1 || p->n_head > 65536 || p->n_head % p->n_kv_head != 0) return 1;
-    if (!is_half(p->kv_type) || (p->io_type != BONSAI_P40_F32 && p->io_type != p->kv_type)) return 1;
+    if (p->kv_type == BONSAI_P40_Q8 ? !is_type(p->io_type)
+                                    : !is_half(p->kv_type) || (p->io_type != BONSAI_P40_F32 && p->io_type != p->kv_type))
+        return 1;
     if (!is_pow2(p->page_size) || p->page_size < 16 || p->page_size > 65536) return 1;
     if (p->n_pages < 0 || p->n_pages > 0x7fffffff) return 1;
-    if (p->page_stride < (int64_t)p->n_kv_head * p->page_size * d || p->page_stride % 8 != 0) return 1;
+    if (!page_stride_ok(p->kv_type, p->page_stride, p->n_kv_head, p->page_size, d)) return 1;
+    // (an 8-bit page is one buffer)
+    if (p->kv_type == BONSAI_P40_Q8 && (int64_t)p->n_kv_head * p->page_size * (d + 4) > 0x7fffffff) return 1;
     const int per16 = 16 / type_bytes(p->io_type);
     if (p->q_tok < (int64_t)p->n_head * d || p->q_tok % per16 != 0) return 1;
     if (p->out_tok < (int64_t)p->n_head * d || p->out_tok % per16 != 0) return 1;
@@ -875,42 +798,37 @@ int check(const bonsai_p40_attn_paged_args * p) {
     if ((p->n_tok + p->n_seq) * (int64_t)p->n_head >= 1 << 24) return 1;    // a grid has fewer than 2^32 threads
     return -1;
 }
+// ... of the pointers
+bool pointers_ok(const bonsai_p40_attn_paged_args * p) {
+    if (pq2host::any_null(p->q, p->out, p->starts, p->kv_len)) return false;
+    if (p->max_pages > 0 && p->n_pages > 0 && pq2host::any_null(p->k_pages, p->v_pages, p->table)) return false;
+    return aligned(p->q, 16) && aligned(p->out, 16) && aligned(p->k_pages, 16) && aligned(p->v_pages, 16) &&
+           aligned(p->workspace, 16) && aligned(p->table, 4) && aligned(p->starts, 4) && aligned(p->kv_len, 4);
+}
 
 struct Plan {
     bool keys;
     int tiles, chunk, n_split;
 };
-Plan plan_of(const bonsai_p40_attn_paged_args * p) {
+// n_seq sequences, or groups, of up to `most` keys
+Plan plan_of(const bonsai_p40_attn_paged_args * p, int n_seq, int64_t most) {
     const int group = p->n_head / p->n_kv_head;
-    const int64_t cap = (int64_t)p->max_pages * p->page_size;
-    const int64_t most = p->max_kv > 0 && p->max_kv < cap ? p->max_kv : cap;
     const int rows = p->head_dim == 256 && p->kv_type == BONSAI_P40_BF16 && p->io_type == BONSAI_P40_F32 ? 64 : 128;
-    const pq2::AttnPlan a = pq2::attn_plan(p->n_tok, p->n_seq, group, p->n_kv_head, p->head_dim, most, rows,
-                                           pq2host::device_info().cus);
+    const pq2::AttnPlan a = pq2::attn_plan(p->n_tok, n_seq, group, p->n_kv_head, p->head_dim, most, rows,
+                                           pq2host::device_info().cus, p->kv_type == BONSAI_P40_Q8);
     return {a.keys, (int)a.tiles, (int)a.chunk, (int)a.n_split};
 }
-int64_t part_bytes(const bonsai_p40_attn_paged_args * p, int n_split) {
-    return n_split <= 1 ? 0 : (int64_t)n_split * p->n_tok * p->n_head * (p->head_dim + 2) * 4;
+int64_t most_keys(const bonsai_p40_attn_paged_args * p) {
+    const int64_t cap = (int64_t)p->max_pages * p->page_size;
+    return p->max_kv > 0 && p->max_kv < cap ? p->max_kv : cap;
+}
+int64_t part_bytes(const bonsai_p40_attn_paged_args * p, int n_part) {
+    return n_part <= 1 ? 0 : (int64_t)n_part * p->n_tok * p->n_head * (p->head_dim + 2) * 4;
 }
 
-}  // namespace
-
-extern "C" int64_t bonsai_p40_attn_paged_workspace_bytes(const bonsai_p40_attn_paged_args * p) {
-    return check(p) == -1 ? part_bytes(p, plan_of(p).n_split) : 0;
-}
-
-extern "C" int bonsai_p40_attn_paged(const bonsai_p40_attn_paged_args * p, bonsai_stream stream) {
-    const int rc = check(p);
-    if (rc >= 0) return rc;
-    if (pq2host::any_null(p->q, p->out, p->starts, p->kv_len)) return 1;
-    if (p->max_pages > 0 && p->n_pages > 0 && pq2host::any_null(p->k_pages, p->v_pages, p->table)) return 1;
-    if (!aligned(p->q, 16) || !aligned(p->out, 16) || !aligned(p->k_pages, 16) || !aligned(p->v_pages, 16) ||
-        !aligned(p->workspace, 16) || !aligned(p->table, 4) || !aligned(p->starts, 4) || !aligned(p->kv_len, 4))
-        return 1;
-    Plan pl = plan_of(p);
-    if (p->workspace == nullptr) pl.n_split = 1;
-    else if (p->workspace_bytes < part_bytes(p, pl.n_split)) return 1;
-    AttnArgs a;
+void fill(AttnArgs & a, const bonsai_p40_attn_paged_args * p, const Plan & pl) {
+    const int el = p->kv_type == BONSAI_P40_Q8 ? 1 : 2;
+    a = AttnArgs{};
     a.q = p->q;
     a.out = p->out;
     a.k = reinterpret_cast<const uint8_t *>(p->k_pages);
@@ -921,8 +839,9 @@ extern "C" int bonsai_p40_attn_paged(const bonsai_p40_attn_paged_args * p, bonsa
     a.part = reinterpret_cast<float *>(p->workspace);
     a.q_tok = p->q_tok;
     a.out_tok = p->out_tok;
-    a.page_bytes = p->page_stride * 2;
-    a.head_bytes = (int64_t)p->page_size * p->head_dim * 2;
+    a.page_bytes = p->page_stride * el;
+    a.head_bytes = (int64_t)p->page_size * p->head_dim * el;
+    a.scales = p->n_kv_head * a.head_bytes;
     a.table_stride = p->table_stride;
     a.n_tok = (int)p->n_tok;
     a.n_seq = p->n_seq;
@@ -936,9 +855,73 @@ extern "C" int bonsai_p40_attn_paged(const bonsai_p40_attn_paged_args * p, bonsa
     a.n_split = pl.n_split;
     a.tiles = pl.tiles;
     a.c = p->scale * 1.4426950408889634f;
-    const hipStream_t s = (hipStream_t)stream;
+}
+int run(const bonsai_p40_attn_paged_args * p, AttnArgs & a, const AttnLaunch & l, hipStream_t s) {
+    if (p->kv_type == BONSAI_P40_Q8) return attn_q8_launch(a, l, s);
     const bool f32 = p->io_type == BONSAI_P40_F32;
-    if (p->kv_type == BONSAI_P40_F16)
-        return f32 ? launch_d<F16, 2>(p->head_dim, pl.keys, a, s) : launch_d<F16, 1>(p->head_dim, pl.keys, a, s);
-    return f32 ? launch_d<BF16, 3>(p->head_dim, pl.keys, a, s) : launch_d<BF16, 1>(p->head_dim, pl.keys, a, s);
+    if (p->kv_type == BONSAI_P40_F16) return f32 ? launch_d<F16, 2>(l, a, s) : launch_d<F16, 1>(l, a, s);
+    return f32 ? launch_d<BF16, 3>(l, a, s) : launch_d<BF16, 1>(l, a, s);
+}
+
+// ---- shared prefixes
+int check_shared(const bonsai_p40_attn_shared_args * p) {
+    if (!p || p->n_group < 0 || p->max_shared < 0) return 1;
+    const int rc = check(&p->attn);
+    return rc >= 0 ? rc : p->n_group > 0xffffff || (p->attn.n_tok + p->n_group) * (int64_t)p->attn.n_head >= 1 << 24 ? 1 : -1;
+}
+struct SharedPlan {
+    Plan first, own;
+};
+SharedPlan plan_of(const bonsai_p40_attn_shared_args * p) {
+    const int64_t cap = (int64_t)p->attn.max_pages * p->attn.page_size, all = most_keys(&p->attn);
+    const int64_t shared = p->max_shared > 0 && p->max_shared < cap ? p->max_shared : cap;
+    // (own keys begin anywhere in 16)
+    const int64_t own = p->max_shared > 0 && p->attn.max_kv > 0 && all > shared ? all - shared + 15 : all;
+    return {plan_of(&p->attn, p->n_group, shared), plan_of(&p->attn, p->attn.n_seq, own < cap ? own : cap)};
+}
+
+}  // namespace
+
+extern "C" int64_t bonsai_p40_attn_paged_workspace_bytes(const bonsai_p40_attn_paged_args * p) {
+    return check(p) == -1 ? part_bytes(p, plan_of(p, p->n_seq, most_keys(p)).n_split) : 0;
+}
+
+extern "C" int bonsai_p40_attn_paged(const bonsai_p40_attn_paged_args * p, bonsai_stream stream) {
+    const int rc = check(p);
+    if (rc >= 0) return rc;
+    if (!pointers_ok(p)) return 1;
+    Plan pl = plan_of(p, p->n_seq, most_keys(p));
+    if (p->workspace == nullptr) pl.n_split = 1;
+    else if (p->workspace_bytes < part_bytes(p, pl.n_split)) return 1;
+    AttnArgs a;
+    fill(a, p, pl);
+    const AttnLaunch l = {pl.keys, pl.keys, false, pl.n_split > 1, p->io_type, p->head_dim};
+    return run(p, a, l, (hipStream_t)stream);
+}
+
+extern "C" int64_t bonsai_p40_attn_shared_workspace_bytes(const bonsai_p40_attn_shared_args * p) {
+    if (check_shared(p) != -1) return 0;
+    if (p->n_group == 0) return bonsai_p40_attn_paged_workspace_bytes(&p->attn);
+    const SharedPlan pl = plan_of(p);
+    return part_bytes(&p->attn, pl.first.n_split + pl.own.n_split);
+}
+
+extern "C" int bonsai_p40_attn_shared(const bonsai_p40_attn_shared_args * p, bonsai_stream stream) {
+    const int rc = check_shared(p);
+    if (rc >= 0) return rc;
+    if (p->n_group == 0) return bonsai_p40_attn_paged(&p->attn, stream);
+    if (!pointers_ok(&p->attn) || pq2host::any_null(p->groups, p->shared, p->attn.workspace)) return 1;
+    if (!aligned(p->groups, 4) || !aligned(p->shared, 4)) return 1;
+    const SharedPlan pl = plan_of(p);
+    if (p->attn.workspace_bytes < part_bytes(&p->attn, pl.first.n_split + pl.own.n_split)) return 1;
+    AttnArgs a;
+    fill(a, &p->attn, pl.own);
+    a.groups = p->groups;
+    a.shared = p->shared;
+    a.n_group = p->n_group;
+    a.chunk1 = pl.first.chunk;
+    a.n_split1 = pl.first.n_split;
+    a.tiles1 = pl.first.tiles;
+    const AttnLaunch l = {pl.own.keys, pl.first.keys, true, true, p->attn.io_type, p->attn.head_dim};
+    return run(&p->attn, a, l, (hipStream_t)stream);
 }

@@ -228,10 +228,10 @@ struct AttnPlan {
     int64_t tiles, chunk, n_split;
 };
 inline AttnPlan attn_plan(int64_t n_tok, int64_t n_seq, int64_t group, int64_t n_kv, int64_t dim, int64_t max_kv, int64_t rows,
-                          int64_t cus) {
+                          int64_t cus, bool bytes = false) {
     AttnPlan p;
     p.keys = n_tok * group <= 32 * n_seq;
-    const int64_t bm = p.keys ? 32 : rows, step = p.keys && dim < 256 ? 128 : 64;
+    const int64_t bm = p.keys ? 32 : rows, step = p.keys && (bytes || dim < 256) ? 128 : 64;   // keys: 32 for each wave
     const int64_t some = n_seq < n_tok ? n_seq : n_tok;
     p.tiles = n_tok * group / bm + some;
     int64_t want = 1;

@@ -131,6 +131,10 @@ inline int type_bytes(int t) { return t == BONSAI_P40_F32 ? 4 : 2; }
 inline bool is_type(int t) { return t == BONSAI_P40_F32 || t == BONSAI_P40_F16 || t == BONSAI_P40_BF16; }
 inline bool is_half(int t) { return t == BONSAI_P40_F16 || t == BONSAI_P40_BF16; }
 inline bool is_pow2(int64_t v) { return v > 0 && (v & (v - 1)) == 0; }
+// page_stride (elements; bytes where they are of 8 bits, whose rows have an fp32 scale each) has room for a page
+inline bool page_stride_ok(int type, int64_t stride, int64_t n_kv, int64_t page, int64_t dim) {
+    return type == BONSAI_P40_Q8 ? stride >= n_kv * page * (dim + 4) && stride % 16 == 0 : stride >= n_kv * page * dim && stride % 8 == 0;
+}
 inline bool aligned(const void * p, unsigned a) { return ((uintptr_t)p & (a - 1)) == 0; }
 
 }  // namespace mixer

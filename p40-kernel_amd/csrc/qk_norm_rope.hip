@@ -21,9 +21,31 @@
 #include "mixer_device.h"
 #include "pq2_device.h"
 
+#include <type_traits>
+
 using namespace mixer;
 
 namespace {
+
+// Q8 pages: bytes, and a scale a row behind all of a page's
+struct Q8 {
+    typedef int8_t elem;
+};
+
+// the largest of 64 lanes, in all of them (0 is the identity)
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    auto step = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
+        v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
+    };
+    const std::integral_constant<int, 0xf> all;
+    step(std::integral_constant<int, pq2::DPP_QUAD_XOR1>{}, all);
+    step(std::integral_constant<int, pq2::DPP_QUAD_XOR2>{}, all);
+    step(std::integral_constant<int, pq2::DPP_ROW_HALF_MIRROR>{}, all);
+    step(std::integral_constant<int, pq2::DPP_ROW_MIRROR>{}, all);
+    step(std::integral_constant<int, pq2::DPP_ROW_BCAST15>{}, std::integral_constant<int, 0xa>{});
+    step(std::integral_constant<int, pq2::DPP_ROW_BCAST31>{}, std::integral_constant<int, 0xc>{});
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
 
 struct QkvArgs {
     const float * x[3];                 // q, k, v
@@ -162,8 +184,26 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkvArgs a) {
                                   (int64_t)row * D + lane * E, v[k]);
             } else {
                 const int64_t slot = a.slots[t0 + t];
-                if (slot >= 0 && slot < a.n_slots) {
-                    const int64_t page = slot >> a.page_log2, off = slot & ((1ll << a.page_log2) - 1);
+                if (slot < 0 || slot >= a.n_slots) continue;
+                const int64_t page = slot >> a.page_log2, off = slot & ((1ll << a.page_log2) - 1);
+                if constexpr (std::is_same<TC, Q8>::value) {
+                    // (as whole numbers magnitudes compare as they do as floats, and NaN is above infinity)
+                    uint32_t big = 0;
+#pragma unroll
+                    for (int j = 0; j < E; ++j) big = max(big, __builtin_bit_cast(uint32_t, v[k][j]) & 0x7fffffffu);
+                    big = wave_max(big);
+                    const float top = __builtin_bit_cast(float, big);
+                    const bool real = big < 0x7f800000u, some = real && top >= 0x1p-112f;
+                    const float d = some ? top / 127.0f : real ? 0.0f : NAN, r = some ? 127.0f / top : 0.0f;
+                    typedef int8_t bytes __attribute__((ext_vector_type(E)));
+                    bytes x;
+#pragma unroll
+                    for (int j = 0; j < E; ++j) x[j] = (int8_t)(int)rintf(some ? v[k][j] * r : 0.0f);
+                    int8_t * const at = reinterpret_cast<int8_t *>(a.pages[kind - 1]) + page * a.page_stride;
+                    *reinterpret_cast<bytes *>(at + (((int64_t)row << a.page_log2) + off) * D + lane * E) = x;
+                    if (lane == 0)
+                        reinterpret_cast<float *>(at + ((int64_t)a.n_kv << a.page_log2) * D)[((int64_t)row << a.page_log2) + off] = d;
+                } else {
                     store_row<TC>(reinterpret_cast<typename TC::elem *>(a.pages[kind - 1]) + page * a.page_stride +
                                       (((int64_t)row << a.page_log2) + off) * D + lane * E, v[k]);
                 }
@@ -179,6 +219,7 @@ void launch(const QkvArgs & a, dim3 grid, size_t bytes, hipStream_t s) {
 template <int D, class TQ>
 void launch_c(int kv, const QkvArgs & a, dim3 grid, size_t bytes, hipStream_t s) {
     if (kv == BONSAI_P40_F16) launch<D, TQ, F16>(a, grid, bytes, s);
+    else if (kv == BONSAI_P40_Q8) launch<D, TQ, Q8>(a, grid, bytes, s);
     else launch<D, TQ, BF16>(a, grid, bytes, s);
 }
 template <int D>
@@ -196,8 +237,8 @@ extern "C" int bonsai_p40_qk_norm_rope(const bonsai_p40_qk_norm_rope_args * p, b
     if (d != 64 && d != 128 && d != 256) return 1;
     if (p->n_head < 1 || p->n_kv_head < 1 || p->n_head > 16384 || p->n_kv_head > 16384) return 1;
     if (p->n_rot < 0 || p->n_rot > d || p->n_rot % 8 != 0) return 1;
-    if (!is_type(p->q_type) || !is_half(p->kv_type) || !is_pow2(p->page_size) || p->page_size > 65536) return 1;
-    if (p->n_pages < 0 || p->n_pages > (1ll << 40) || p->page_stride < (int64_t)p->n_kv_head * p->page_size * d || p->page_stride % 8 != 0) return 1;
+    if (!is_type(p->q_type) || (!is_half(p->kv_type) && p->kv_type != BONSAI_P40_Q8) || !is_pow2(p->page_size) || p->page_size > 65536) return 1;
+    if (p->n_pages < 0 || p->n_pages > (1ll << 40) || !page_stride_ok(p->kv_type, p->page_stride, p->n_kv_head, p->page_size, d)) return 1;
     if (p->q_out_tok < (int64_t)p->n_head * d || p->q_out_tok % (16 / type_bytes(p->q_type)) != 0) return 1;
     if (p->n_tok <= 0) return 0;
     if (p->n_tok > 0x7fffffff / 64) return 1;

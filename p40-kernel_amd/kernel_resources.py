@@ -26,7 +26,7 @@ LLVM = "/opt/rocm/llvm/bin"
 # codec): a spill or a scratch byte there is a regression.  The probes and the
 # persistent chain kernel are not on it.
 HOT_PATH = ("gemv_", "gemm_", "wide_x16", "rot_quant", "quant_kernel", "swiglu_rot_quant", "rmsnorm_kernel",
-            "repack_kernel", "quantize_pq2_0", "dequantize_pq2_0", "qk_norm_rope", "attn_", "gdn_")
+            "repack_kernel", "quantize_pq2_0", "dequantize_pq2_0", "qk_norm_rope", "attn_", "gdn_", "kv_read")
 NOT_HOT = ("probe", "chain_kernel")
 
 
