@@ -55,12 +55,17 @@ __device__ __forceinline__ auto args_of(const AttnArgs & a) {
 // 1 / l; 0 where no key was seen, NaN where the score of every key that was is -inf
 __device__ __forceinline__ float over(float m, float l) { return m == -INFINITY ? 0.0f : l != 0.0f ? 1.0f / l : NAN; }
 
-// The shared keys of sequence seq's group; -1: it is in none.  For whole waves.
-__device__ __forceinline__ int shared_of(const AttnArgs & a, int seq) {
-    if (a.n_group == 1) {
-        const int b = sload(a.groups, 0), e = sload(a.groups, 1), n = sload(a.shared, 0);
-        return seq >= b && seq < e ? iclamp(n, 0, a.cap) : -1;
-    }
+// The shared keys of sequence seq's group; -1: it is in none.  For whole waves.  only: the one group there is, asked
+// for beside what seq follows from
+struct OneGroup {
+    int first, next, keys;
+};
+__device__ __forceinline__ OneGroup one_group(const AttnArgs & a) {
+    if (a.n_group == 1) return OneGroup{sload(a.groups, 0), sload(a.groups, 1), sload(a.shared, 0)};
+    return OneGroup{0, 0, 0};
+}
+__device__ __forceinline__ int shared_of(const AttnArgs & a, const OneGroup & only, int seq) {
+    if (a.n_group == 1) return seq >= only.first && seq < only.next ? iclamp(only.keys, 0, a.cap) : -1;
     const int lane = threadIdx.x & 63;
     for (int g0 = 0; g0 < a.n_group; g0 += 64) {
         const int g = g0 + lane;
@@ -80,6 +85,12 @@ __device__ __forceinline__ int shared_of(const AttnArgs & a, int seq) {
 // 64 groups a step
 template <int BM>
 __device__ __forceinline__ Tile find_group_tile(const AttnArgs & a, int tile) {
+    if (a.n_group == 1) {               // no search
+        const int first = iclamp(sload(a.groups, 0), 0, a.n_seq), next = iclamp(sload(a.groups, 1), 0, a.n_seq), x = sload(a.shared, 0);
+        const int b = iclamp(sload(a.starts, first), 0, a.n_tok), n = max(iclamp(sload(a.starts, next), 0, a.n_tok) - b, 0);
+        const int tiles = (int)(((int64_t)n * a.group + BM - 1) / BM);
+        return Tile{tile < tiles ? first : -1, tile, b, n, x};
+    }
     const int lane = threadIdx.x & 63;
     int base = 0;
     for (int g0 = 0; g0 < a.n_group; g0 += 64) {
@@ -147,10 +158,12 @@ struct AttnWork {
 // false: there is nothing to do
 template <int BM, bool SHARED>
 __device__ __forceinline__ bool attn_work(const AttnArgs & a, const AttnPlace & p, AttnWork & w) {
+    OneGroup only = {0, 0, 0};
+    if (SHARED && !p.pre) only = one_group(a);
     w.tl = SHARED && p.pre ? find_group_tile<BM>(a, p.tile)
                            : find_tile<BM>(a.starts, a.kv_len, a.n_seq, a.n_tok, a.group, p.tile);
     if (w.tl.seq < 0) return false;
-    w.lo = SHARED && !p.pre ? max(shared_of(a, w.tl.seq), 0) : 0;
+    w.lo = SHARED && !p.pre ? max(shared_of(a, only, w.tl.seq), 0) : 0;
     const int rows = w.tl.count * a.group, last = min((w.tl.index + 1) * BM, rows) - 1;
     w.kv = iclamp(w.tl.extra, 0, a.cap);
     w.before = SHARED && p.pre ? w.kv : w.kv - w.tl.count;     // (pre: every row sees all of them)
@@ -198,18 +211,22 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int bm) {
     // (4 waves: the first parts, too; those behind the last are not written, and not used)
     float v[AHEAD][E];
     float2 e[AHEAD];
-    // shared prefixes: n1 parts of the prefix, the others behind the place of the last there could be
-    int n1 = 0;
-    auto load = [&](int i0, int n) __attribute__((always_inline)) {
-#pragma unroll
-        for (int k = 0; k < AHEAD; ++k) {
-            int64_t i = min(i0 + k * WR, n - 1);
-            if (SHARED && i >= n1) i += first_parts - n1;
-            e[k] = ml[i * all_rows];
-            load_row<F32>(a.part + (i * all_rows + row) * D + lane * E, v[k]);
-        }
+    // part i: the parts of a shared prefix, which are n1, come first, the others behind the place of the last there could be
+    auto load = [&](int k, int64_t i) __attribute__((always_inline)) {
+        e[k] = ml[i * all_rows];
+        load_row<F32>(a.part + (i * all_rows + row) * D + lane * E, v[k]);
     };
-    if (WR > 1 && !SHARED) load(w, a.n_split);
+    OneGroup only = {0, 0, 0};
+    constexpr int OWN = SHARED ? AHEAD - 1 : 0;            // SHARED: the last of the first loads is of the own keys' parts
+    if (SHARED) {
+        only = one_group(a);
+#pragma unroll
+        for (int k = 0; k < OWN; ++k) load(k, min(w + k * WR, first_parts - 1));
+        load(OWN, first_parts + min(w, a.n_split - 1));
+    } else if (WR > 1) {
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) load(k, min(w + k * WR, a.n_split - 1));
+    }
     // the sequence of this token
     int seq = -1, first = 0, count = 0, kv = 0;
     for (int s0 = 0; s0 < a.n_seq && seq < 0; s0 += 64) {
@@ -230,17 +247,17 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int bm) {
         }
     }
     if (seq < 0) return;                                   // a row behind the last sequence
-    int lo = 0;
+    int lo = 0, n1 = 0;
     if (SHARED) {
-        const int s = shared_of(a, seq);
+        const int s = shared_of(a, only, seq);
         lo = max(s, 0);
         if (s >= 0) n1 = attn_parts(a.n_pages > 0 ? s : 0, 0, a.chunk1, a.n_split1);
     }
     const int r = (tok - first) * a.group + head % a.group;
     const int last = min(r / bm * bm + bm, count * a.group) - 1;
     const int nk = a.n_pages > 0 ? iclamp(kv - count + last / a.group + 1, 0, kv) : 0;
-    const int n = n1 + attn_parts(nk, lo, a.chunk, a.n_split);
-    auto there = [&](int i) { return SHARED ? i < n1 || (i >= first_parts && i < first_parts + n - n1) : i < n; };
+    const int n = attn_parts(nk, lo, a.chunk, a.n_split);
+    auto there = [&](int i) { return SHARED ? i < n1 || (i >= first_parts && i < first_parts + n) : i < n; };
     float mm = there(lane) ? own : -INFINITY;
     for (int i = 64 + lane; i < (SHARED ? n_part : n); i += 64)
         if (!SHARED || there(i)) mm = fmaxf(mm, ml[i * all_rows].x);
@@ -248,16 +265,36 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int bm) {
     for (int d = 32; d > 0; d >>= 1) mm = fmaxf(mm, __shfl_xor(mm, d));
     const float ref = mm == -INFINITY ? 0.0f : mm;
     float x[E] = {}, l = 0.0f;
-    for (int i0 = w; i0 < n; i0 += WR * AHEAD) {
-        if (WR == 1 || SHARED || i0 != w) load(i0, n);
+    auto add = [&](int k) __attribute__((always_inline)) {
+        const float wt = __builtin_amdgcn_exp2f(e[k].x - ref);
+        l = fmaf(e[k].y, wt, l);
 #pragma unroll
-        for (int k = 0; k < AHEAD; ++k)
-            if (i0 + k * WR < n) {
-                const float wt = __builtin_amdgcn_exp2f(e[k].x - ref);
-                l = fmaf(e[k].y, wt, l);
+        for (int j = 0; j < E; ++j) x[j] = fmaf(v[k][j], wt, x[j]);
+    };
+    // parts base + from, from + WR, .. of base + count
+    auto rest = [&](int base, int from, int count) __attribute__((always_inline)) {
+        for (int i0 = from; i0 < count; i0 += WR * AHEAD) {
 #pragma unroll
-                for (int j = 0; j < E; ++j) x[j] = fmaf(v[k][j], wt, x[j]);
-            }
+            for (int k = 0; k < AHEAD; ++k) load(k, base + min(i0 + k * WR, count - 1));
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k)
+                if (i0 + k * WR < count) add(k);
+        }
+    };
+    if (SHARED) {
+#pragma unroll
+        for (int k = 0; k < OWN; ++k)
+            if (w + k * WR < n1) add(k);
+        if (w < n) add(OWN);
+        rest(0, w + OWN * WR, n1);
+        rest(first_parts, w + WR, n);
+    } else {
+        if (WR > 1) {
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k)
+                if (w + k * WR < n) add(k);
+        }
+        rest(0, WR > 1 ? w + WR * AHEAD : w, n);
     }
     if constexpr (WR > 1) {
 #pragma unroll

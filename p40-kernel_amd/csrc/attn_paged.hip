@@ -810,12 +810,16 @@ struct Plan {
     bool keys;
     int tiles, chunk, n_split;
 };
+enum Keys { ALL, SHARED_KEYS, OWN_KEYS };
 // n_seq sequences, or groups, of up to `most` keys
-Plan plan_of(const bonsai_p40_attn_paged_args * p, int n_seq, int64_t most) {
+Plan plan_of(const bonsai_p40_attn_paged_args * p, int n_seq, int64_t most, Keys which = ALL) {
     const int group = p->n_head / p->n_kv_head;
     const int rows = p->head_dim == 256 && p->kv_type == BONSAI_P40_BF16 && p->io_type == BONSAI_P40_F32 ? 64 : 128;
-    const pq2::AttnPlan a = pq2::attn_plan(p->n_tok, n_seq, group, p->n_kv_head, p->head_dim, most, rows,
-                                           pq2host::device_info().cus, p->kv_type == BONSAI_P40_Q8);
+    const int cus = pq2host::device_info().cus;
+    const bool bytes = p->kv_type == BONSAI_P40_Q8;
+    const pq2::AttnPlan a = which == OWN_KEYS
+        ? pq2::attn_own_plan(p->n_tok, n_seq, group, p->n_kv_head, p->head_dim, most, rows, cus, bytes)
+        : pq2::attn_plan(p->n_tok, n_seq, group, p->n_kv_head, p->head_dim, most, rows, cus, bytes, which == SHARED_KEYS);
     return {a.keys, (int)a.tiles, (int)a.chunk, (int)a.n_split};
 }
 int64_t most_keys(const bonsai_p40_attn_paged_args * p) {
@@ -877,7 +881,7 @@ SharedPlan plan_of(const bonsai_p40_attn_shared_args * p) {
     const int64_t shared = p->max_shared > 0 && p->max_shared < cap ? p->max_shared : cap;
     // (own keys begin anywhere in 16)
     const int64_t own = p->max_shared > 0 && p->attn.max_kv > 0 && all > shared ? all - shared + 15 : all;
-    return {plan_of(&p->attn, p->n_group, shared), plan_of(&p->attn, p->attn.n_seq, own < cap ? own : cap)};
+    return {plan_of(&p->attn, p->n_group, shared, SHARED_KEYS), plan_of(&p->attn, p->attn.n_seq, own < cap ? own : cap, OWN_KEYS)};
 }
 
 }  // namespace

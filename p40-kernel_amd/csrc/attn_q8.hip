@@ -43,6 +43,12 @@ __device__ __forceinline__ v2u read_tr8(const uint8_t * at) {
     typedef __attribute__((address_space(3))) i2 lds_i2;
     return __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2 *)at));
 }
+// 4 keys x 16 f16
+__device__ __forceinline__ v2u read_tr16(const uint8_t * at) {
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s4 lds_s4;
+    return __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)at));
+}
 // 8 signed bytes as f16
 __device__ __forceinline__ v8h unpack(v2u x) {
     const v2h off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
@@ -59,23 +65,26 @@ __device__ __forceinline__ v16f mfma(v8h a, v8h b, v16f c) { return __builtin_am
 
 template <int D, bool KEYS, bool WIDE>
 struct Shape {
-    static constexpr int NW = 4, BM = KEYS ? 32 : 32 * NW;
+    // (keys, heads of 256: two workgroups of 2 waves share a CU, so that one loads while the other begins or ends)
+    static constexpr int NW = KEYS && D == 256 ? 2 : 4, BM = KEYS ? 32 : 32 * NW;
     static constexpr int RB = D, TILE = 32 * RB;           // bytes of a key, of a tile of 32 keys
-    static constexpr int SC = 32 * 4;                      // of its scales
+    static constexpr int SC = (KEYS ? 2 : NW) * 256;       // of its scales: 256 for the keys of one DMA instruction
     static constexpr int R = 4;                            // rows: tiles of K, and of V, in LDS
     static constexpr int OROW = D + 4;                     // floats of a row in the join
     static constexpr int JOIN = NW * 32 * OROW * 4 + NW * 32 * 8;
     static constexpr int SLOTS = KEYS ? NW * 4 : 2 * R;    // keys: two buffers of K and V a wave
-    // fp32 rows of 256: the registers hold two digits of q, the lowest is in LDS
-    static constexpr bool QL = WIDE && D == 256 && !KEYS;
+    // heads of 256: the registers hold the other digits of q, the lowest is in LDS
+    static constexpr bool QL = D == 256 && !KEYS;
     static constexpr int QT = 32 * D;                      // bytes of a digit of 32 rows
-    static constexpr int MAIN = SLOTS * TILE, SCALED = MAIN + SLOTS * SC, ALL = SCALED + (QL ? NW * QT : 0);
+    // rows: two tiles of V in f16
+    static constexpr int MAIN = SLOTS * TILE, SCALED = MAIN + SLOTS * SC, WIDENED = SCALED + (QL ? NW * QT : 0);
+    static constexpr int ALL = WIDENED + (KEYS ? 0 : 2 * 2 * TILE);
     static constexpr int LDS = KEYS && JOIN > ALL ? JOIN : ALL;
 };
 
 // IO: type of queries and output
 template <class IO, int D, bool KEYS, bool SHARED>
-__global__ void __launch_bounds__(256) attn_q8_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(KEYS && D == 256 ? 128 : 256) attn_q8_kernel(AttnArgs a) {
     constexpr bool WIDE = std::is_same<IO, F32>::value;
     typedef Shape<D, KEYS, WIDE> Z;
     constexpr int NT = WIDE ? 3 : 2;                       // digits of q
@@ -137,14 +146,30 @@ __global__ void __launch_bounds__(256) attn_q8_kernel(AttnArgs a) {
     uint8_t * const ql = lds + Z::SCALED + wave * Z::QT + 16 * lane;
     float c = a.c;
     auto make_q = [&]() __attribute__((always_inline)) {
+        // the largest magnitude's bits: they compare as the magnitudes do, and NaN is above infinity
         uint32_t big = 0;
+        if constexpr (WIDE) {
 #pragma unroll
-        for (int s = 0; s < QS; ++s)
+            for (int s = 0; s < QS; ++s)
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const uint32_t x = __builtin_bit_cast(uint32_t, IO::to(qx[s][j])) & 0x7fffffffu;
-                big = x > big ? x : big;
+                for (int j = 0; j < 16; ++j) {
+                    const float f = qx[s][j];
+                    const uint32_t x = __builtin_bit_cast(uint32_t, f) & 0x7fffffffu;
+                    big = x > big ? x : big;
+                }
+        } else {
+            typedef unsigned short u16 __attribute__((ext_vector_type(16)));
+            typedef unsigned short u2 __attribute__((ext_vector_type(2)));
+            u2 top = {0, 0};
+#pragma unroll
+            for (int s = 0; s < QS; ++s) {
+                const u16 x = __builtin_bit_cast(u16, qx[s]) & (unsigned short)0x7fff;
+#pragma unroll
+                for (int j = 0; j < 16; j += 2) top = __builtin_elementwise_max(top, (u2){x[j], x[j + 1]});
             }
+            const unsigned short t = top[0] > top[1] ? top[0] : top[1];
+            big = __builtin_bit_cast(uint32_t, IO::to(__builtin_bit_cast(elem, t)));
+        }
         const uint32_t other = __shfl_xor(big, 32);
         big = other > big ? other : big;
         // times 2^k 127/128, so that the largest is 127/128 of 2^15 (2^23) at most: digits of -128 .. 127 hold it
@@ -159,16 +184,18 @@ __global__ void __launch_bounds__(256) attn_q8_kernel(AttnArgs a) {
                 uint32_t v[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    // the digits' bytes, 128 up, then without
-                    const int x = (int)rintf(IO::to(qx[s][j + i]) * up);
-                    v[i] = ((uint32_t)x + (NT == 3 ? 0x808080u : 0x8080u)) ^ (NT == 3 ? 0x808080u : 0x8080u);
+                    // the whole number, its digits' bytes 128 up (of 16 bits: behind the point of 1.5 x 2^23, whose own
+                    // low bits are 0)
+                    const float f = IO::to(qx[s][j + i]);
+                    if constexpr (NT == 3) v[i] = (uint32_t)(int)rintf(f * up) + 0x808080u;
+                    else v[i] = __builtin_bit_cast(uint32_t, fmaf(f, up, 12582912.0f)) + 0x8080u;
                 }
 #pragma unroll
                 for (int k = 0; k < NT; ++k) {
-                    // byte k of each
+                    // byte k of each, without the 128
                     const uint32_t p = __builtin_amdgcn_perm(v[1], v[0], 0x0c0c0400u + 0x0101u * k);
-                    const uint32_t q = __builtin_amdgcn_perm(v[3], v[2], 0x0c0c0400u + 0x0101u * k);
-                    qf[k][s][j / 4] = (int)(p | q << 16);
+                    const uint32_t q = __builtin_amdgcn_perm(v[3], v[2], 0x04000c0cu + 0x01010000u * k);
+                    qf[k][s][j / 4] = (int)((p | q) ^ 0x80808080u);
                 }
                 if (Z::QL && j == 12) *reinterpret_cast<v4i *>(ql + 1024 * s) = qf[0][s];
             }
@@ -176,36 +203,36 @@ __global__ void __launch_bounds__(256) attn_q8_kernel(AttnArgs a) {
 
     // ---- staging
     const int64_t trow = (int64_t)tl.seq * a.table_stride;
-    const int drow = lane / U, dunit = lane % U;
     auto swz_k = [](int key) { return (key / (16 / U)) & (U - 1); };
     auto swz_v = [](int key) {
         return U >= 16 ? 2 * (key & 3) | (key & 8) : U >= 8 ? (key & 2) | ((key >> 1) & 4) : (key >> 2) & 2;
     };
     // a page is one buffer: this head's rows are at head_at, their scales at scale_at
+    auto swz_w = [](int key) { return U >= 16 ? (key & 7) * 4 : U >= 8 ? (key & 3) * 4 : ((key >> 1) & 1) * 4; };   // (units of 8 f16)
     const int in_page = (1 << a.page_log2) - 1, range = (int)a.scales + (a.n_kv << a.page_log2) * 4;
     const int head_at = kvh * (int)a.head_bytes, scale_at = (int)a.scales + (kvh << a.page_log2) * 4;
     auto page = [&](const uint8_t * base, int id) __attribute__((always_inline)) {
-        return buffer_of(base + (int64_t)max(id, 0) * a.page_bytes, range);
+        return buffer_of(base + (int64_t)id * a.page_bytes, range);
     };
-    // N keys of one page from `key` on to dst; place: that of the first among 16, as far as the swizzle looks
-    auto stage_n = [&](auto count, __amdgpu_buffer_rsrc_t from, int key, int place, uint8_t * dst, bool is_v) __attribute__((always_inline)) {
-        constexpr int N = decltype(count)::value;
+    // N keys of one page from `key` on to dst; place: that of the first among 16, as far as the swizzle (of K: swz, or
+    // V's where the waves split the keys, or none) looks.  16 bytes a lane, or 4 where that is more than there are
+    auto stage_n = [&](auto count, __amdgpu_buffer_rsrc_t from, int key, int place, uint8_t * dst, bool swz) __attribute__((always_inline)) {
+        constexpr int N = decltype(count)::value, SIZE = N >= RPI ? 16 : 4, I = N * Z::RB / (64 * SIZE);
         const int first = head_at + (key & in_page) * Z::RB;
-        auto lane_off = [&](int i) __attribute__((always_inline)) {
-            const int kr = place + i * RPI + drow;
-            return drow * Z::RB + 16 * (dunit ^ (is_v ? swz_v(kr) : swz_k(kr)));
-        };
-        if constexpr (N >= RPI) {
 #pragma unroll
-            for (int i = 0; i < N / RPI; ++i) dma16(from, dst + i * 1024, lane_off(i), first + i * 1024);
-        } else {
-            if (lane < N * U) dma16(from, dst, lane_off(0), first);
+        for (int i = 0; i < I; ++i) {
+            // (the place of the lane's bytes in LDS, and theirs in the page, from a key that all lanes' begin at)
+            const int at = SIZE * lane, kr = at / Z::RB, whole = i * 64 * SIZE / Z::RB, sw = place + whole + kr;
+            const int off = kr * Z::RB + 16 * (at % Z::RB / 16 ^ (swz ? swz_k(sw) : KEYS ? swz_v(sw) : 0)) + at % 16;
+            if constexpr (SIZE == 16) dma16(from, dst + i * 1024, off, first + whole * Z::RB);
+            else dma4(from, dst + i * 256, off, first + whole * Z::RB);
         }
     };
-    // their scales
+    // Their scales, which a lane each brings.  The others ask for what is out of the buffer, for which nothing is read:
+    // were they masked, the compiler may put the DMA instructions behind it into both sides of the branch
     auto stage_scales = [&](auto count, __amdgpu_buffer_rsrc_t from, int key, uint8_t * dst) __attribute__((always_inline)) {
-        if (lane < decltype(count)::value)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_void *)dst, 4, 4 * lane, scale_at + 4 * (key & in_page), 0, 0);
+        const int off = lane < decltype(count)::value ? 4 * lane : 0x7fffff00;
+        dma4(from, dst, off, scale_at + 4 * (key & in_page));
     };
 
     // ---- one sub-tile of 32 keys
@@ -221,7 +248,7 @@ __global__ void __launch_bounds__(256) attn_q8_kernel(AttnArgs a) {
     };
     // the scales of this lane's 16 keys
     auto scales4 = [&](const uint8_t * sb, int i) __attribute__((always_inline)) {
-        return *reinterpret_cast<const v4f *>(sb + 32 * i + 16 * half);
+        return *reinterpret_cast<const v4f *>(sb + (KEYS ? 256 * (i / 2) + 32 * (i % 2) : 256 * i) + 16 * half);
     };
     auto scales = [&](const uint8_t * sb, v16f & x) __attribute__((always_inline)) {
 #pragma unroll
@@ -231,17 +258,18 @@ __global__ void __launch_bounds__(256) attn_q8_kernel(AttnArgs a) {
             for (int j = 0; j < 4; ++j) x[4 * i + j] = y[j];
         }
     };
-    // A sum of 256 products of digits is up to 2^22, 2^8 times that and another fit.  QL: the highest digit's sums are
+    // A sum of 256 products of digits is up to 2^22, 2^8 times that and another fit.  CHAIN: the highest digit's sums are
     // taken up 2^8 before the next digit's come into them, which saves the registers of one
-    constexpr int NA = Z::QL ? 2 : NT;
+    constexpr bool CHAIN = Z::QL && NT == 3;
+    constexpr int NA = CHAIN ? 2 : NT;
     auto whole = [&](const v16i (&x)[NA], int i) __attribute__((always_inline)) {
-        const float hi = (float)(Z::QL ? x[1][i] : (x[NA - 1][i] << 8) + x[NA - 2][i]);
+        const float hi = (float)(CHAIN ? x[1][i] : (x[NA - 1][i] << 8) + x[NA - 2][i]);
         return NT == 3 ? fmaf(hi, 256.0f, (float)x[0][i]) : hi;
     };
     // step t of the product of a tile of K: fragment kf, lowest digit lf where LDS holds it
-    constexpr int STEPS = Z::QL ? 2 * QS : QS;
+    constexpr int STEPS = CHAIN ? 2 * QS : QS;
     auto digits = [&](v16i (&x)[NA], v4i kf, v4i lf, int t) __attribute__((always_inline)) {
-        if constexpr (Z::QL) {
+        if constexpr (CHAIN) {
             if (t < QS) {
                 x[1] = __builtin_amdgcn_mfma_i32_32x32x32_i8(kf, qf[2][t], x[1], 0, 0, 0);
                 if (t == QS - 1) x[1] <<= 8;
@@ -251,16 +279,18 @@ __global__ void __launch_bounds__(256) attn_q8_kernel(AttnArgs a) {
             }
         } else {
 #pragma unroll
-            for (int k = NT - 1; k >= 0; --k) x[k] = __builtin_amdgcn_mfma_i32_32x32x32_i8(kf, qf[k][t], x[k], 0, 0, 0);
+            for (int k = NT - 1; k >= 0; --k)
+                x[k] = __builtin_amdgcn_mfma_i32_32x32x32_i8(kf, Z::QL && k == 0 ? lf : qf[k][t], x[k], 0, 0, 0);
         }
     };
+    auto low_at = [](int t) { return CHAIN ? t - QS : t; };   // the step of the lowest digit, from 0 on
     // the scores of a tile, in whole numbers, at once
     auto product = [&](v16i (&x)[NA], const uint8_t * kb, const uint8_t * qlow) __attribute__((always_inline)) {
 #pragma unroll
         for (int k = 0; k < NA; ++k) x[k] = v16i{};
 #pragma unroll
         for (int t = 0; t < STEPS; ++t)
-            digits(x, k_frag(kb, t % QS), Z::QL && t >= QS ? *reinterpret_cast<const v4i *>(qlow + 1024 * (t - QS)) : v4i{}, t);
+            digits(x, k_frag(kb, t % QS), Z::QL && low_at(t) >= 0 ? *reinterpret_cast<const v4i *>(qlow + 1024 * low_at(t)) : v4i{}, t);
     };
     auto over_halves = [&](float mx) __attribute__((always_inline)) {
         const uint32_t x = __builtin_bit_cast(uint32_t, mx);
@@ -277,11 +307,15 @@ __global__ void __launch_bounds__(256) attn_q8_kernel(AttnArgs a) {
         return over_halves(mx) * c;
     };
     // log2 of the largest of the scales
+    auto log_of = [&](float mx) __attribute__((always_inline)) {
+        constexpr float least = 0x1p-100f;
+        return __builtin_amdgcn_logf(fmaxf(over_halves(mx), least));
+    };
     auto log_scale = [&](const v16f & vs) __attribute__((always_inline)) {
         float mx = fabsf(vs[0]);
 #pragma unroll
         for (int i = 1; i < 16; ++i) mx = fmaxf(mx, fabsf(vs[i]));
-        return __builtin_amdgcn_logf(over_halves(mx));
+        return log_of(mx);
     };
     // what is not seen: scores -inf, scales 0; holes: bit g: the 16 keys from 16 g on are absent
     auto mask = [&](v16f & s, v16f & vs, int key0, int holes) __attribute__((always_inline)) {
@@ -313,16 +347,15 @@ __global__ void __launch_bounds__(256) attn_q8_kernel(AttnArgs a) {
     };
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[d] = v16f{};
-    // m and l as in attn_paged.hip; mo: the reference of o (at most 2^120 below m's), back: 2^(m - mo).  Far from 0 both
-    // follow every tile, and the tile's scores are rounded like m first
+    // limit, ref, FAR and LEAST as in attn_paged.hip, where m follows the scores; here it follows a tile's largest score
+    // and the log2 of its largest d together (b), so that p d, which becomes f16, is up to 2^(UP + LAG); o and l are both
+    // relative to it.  A d below 2^-100 counts as that here, as l has to stay finite
     constexpr float UP = 11.0f, LAG = 4.0f, LEAST = -3e38f, FAR = 1048576.0f, LOW_UP = 2048.0f;
-    float m = -INFINITY, l = 0.0f, mo = -INFINITY, limit = -INFINITY, limit_o = -INFINITY, ref = 0.0f, back = 0.0f;
-    auto follow = [&](v16f & s, float mx, float lv) __attribute__((always_inline)) {
-        if (__any(mx > limit || mx + lv > limit_o)) {
-            const bool near = fabsf(fmaxf(m, mx)) < FAR;
-            const float top = near ? mx - UP : mx;
-            const float m2 = fmaxf(m, top), base = m2 == -INFINITY ? 0.0f : m2;
-            const float mo2 = fmaxf(fmaxf(mo, top + lv), m2 - 120.0f), base_o = mo2 == -INFINITY ? 0.0f : mo2;
+    float m = -INFINITY, l = 0.0f, limit = -INFINITY, ref = 0.0f;
+    auto follow = [&](v16f & s, float b) __attribute__((always_inline)) {
+        if (__any(b > limit)) {
+            const bool near = fabsf(fmaxf(m, b)) < FAR;
+            const float m2 = fmaxf(m, near ? b - UP : b), base = m2 == -INFINITY ? 0.0f : m2;
             if (!near) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -332,13 +365,10 @@ __global__ void __launch_bounds__(256) attn_q8_kernel(AttnArgs a) {
                 }
             }
             limit = near ? m2 + (UP + LAG) : -INFINITY;
-            limit_o = near ? mo2 + (UP + LAG) : -INFINITY;
             ref = near ? m2 : 0.0f;
-            l *= __builtin_amdgcn_exp2f(m - base);
-            const float alpha = __builtin_amdgcn_exp2f(mo - base_o);
-            back = m2 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m2 - mo2);
+            const float alpha = __builtin_amdgcn_exp2f(m - base);
             m = m2;
-            mo = mo2;
+            l *= alpha;
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -350,7 +380,7 @@ __global__ void __launch_bounds__(256) attn_q8_kernel(AttnArgs a) {
     auto weight = [&](float s, float vs, v8h (&pf)[NP][2], int e, float & sum) __attribute__((always_inline)) {
         const float p = __builtin_amdgcn_exp2f(fmaf(s, c, -ref));
         sum += p;
-        float f = p * (vs * back);
+        float f = p * vs;
         if (NP == 2) asm("" : "+v"(f));                    // (both terms are of one f: not the product's f16 and then f's)
         const _Float16 x = (_Float16)f;
         pf[0][e / 8][e % 8] = x;
@@ -362,14 +392,18 @@ __global__ void __launch_bounds__(256) attn_q8_kernel(AttnArgs a) {
     };
 
     if constexpr (!KEYS) {
-        // as in attn_paged.hip: the scores of tile j + 1 beside the weights of tile j, K and V (and with K the scales
-        // of both) in rings of R tiles
-        constexpr int R = Z::R, OWN = 32 / Z::NW, PER = 2 * (OWN / RPI > 0 ? OWN / RPI : 1) + 2;   // keys, and DMA instructions, of a wave a tile
+        // As in attn_paged.hip: the scores of tile j + 1 beside the weights of tile j, K and V (and with K the scales
+        // of both) in rings of R tiles.  V's bytes become f16 in LDS once for the four waves, each of which takes the
+        // keys that it loaded itself, a tile ahead: as each wave would unpack all of a tile for itself it takes 120 more
+        // VALU instructions a tile, and these and the MFMAs of a wave do not run side by side
+        constexpr int R = Z::R, OWN = 32 / Z::NW, PER = 2 * (OWN >= RPI ? OWN / RPI : OWN * Z::RB / 256) + 2;   // keys, and DMA instructions, of a wave a tile
         const std::integral_constant<int, OWN> own_keys;
         const int own = wave * OWN, nt = (k1 - k0 + 31) / 32;
         uint8_t * const kring = lds, * const vring = lds + R * Z::TILE, * const ksring = lds + Z::MAIN, * const vsring = ksring + R * Z::SC;
+        uint8_t * const wide_v = lds + Z::WIDENED;
         uint32_t hq = 0;                                   // holes, 2 bits a tile, the latest taken lowest
-        int idk = -1, idv = -1;                            // pages of this wave's keys of the next tiles of K and of V
+        int id = 0;                                        // the page of this wave's keys of the next tile
+        const int second = own >= 16 ? -1 : 0;
         int raw0 = 0, raw1 = 0;
         const int top = max(nk - 1, 0) >> a.page_log2;
         const int32_t * const row = a.table + trow;
@@ -380,11 +414,10 @@ __global__ void __launch_bounds__(256) attn_q8_kernel(AttnArgs a) {
         };
         auto take = [&](int t) __attribute__((always_inline)) {
             const int key = k0 + 32 * t;
-            const bool ok0 = key < nk && (uint32_t)raw0 < (uint32_t)a.n_pages;
-            const bool ok1 = key + 16 < nk && (uint32_t)raw1 < (uint32_t)a.n_pages;
-            hq = hq << 2 | (ok0 ? 0 : 1) | (ok1 ? 0 : 2);
-            idv = idk;
-            idk = own < 16 ? (ok0 ? raw0 : -1) : (ok1 ? raw1 : -1);
+            const bool no0 = (key >= nk) | ((uint32_t)raw0 >= (uint32_t)a.n_pages);
+            const bool no1 = (key + 16 >= nk) | ((uint32_t)raw1 >= (uint32_t)a.n_pages);
+            hq = hq << 2 | (no0 ? 1 : 0) | (no1 ? 2 : 0);
+            id = (no0 ? 0 : raw0 & ~second) + (no1 ? 0 : raw1 & second);   // (no page: any, of which nothing is seen)
         };
         // (this wave's place in a tile is computed anew each time: held for every slot it would take 24 registers)
         auto place = [&]() __attribute__((always_inline)) {
@@ -392,38 +425,81 @@ __global__ void __launch_bounds__(256) attn_q8_kernel(AttnArgs a) {
             asm volatile("" : "+s"(x));
             return x;
         };
-        auto stage_v = [&](int t, uint8_t * to) __attribute__((always_inline)) {
-            const int own = place();
-            stage_n(own_keys, page(a.v, idv), k0 + 32 * t + own, own & 15, to + own * Z::RB, true);
+        auto stage_k = [&](int t, uint8_t * kt, uint8_t * ks) __attribute__((always_inline)) {
+            const int at = place(), key = k0 + 32 * t + at;
+            const auto from = page(a.k, id);
+            stage_n(own_keys, from, key, own & 15, kt + at * Z::RB, true);
+            stage_scales(own_keys, from, key, ks + at * (256 / OWN));
         };
-        auto stage_k = [&](int t, uint8_t * to, uint8_t * ks, uint8_t * vs) __attribute__((always_inline)) {
-            const int own = place(), key = k0 + 32 * t + own;
-            const auto from = page(a.k, idk);
-            stage_n(own_keys, from, key, own & 15, to + own * Z::RB, false);
-            stage_scales(own_keys, from, key, ks + 4 * own);
-            stage_scales(own_keys, page(a.v, idk), key, vs + 4 * own);
+        auto stage_v = [&](int t, uint8_t * vt, uint8_t * vs) __attribute__((always_inline)) {
+            const int at = place(), key = k0 + 32 * t + at;
+            const auto from = page(a.v, id);
+            stage_n(own_keys, from, key, 0, vt + at * Z::RB, false);
+            stage_scales(own_keys, from, key, vs + at * (256 / OWN));
+        };
+        // this wave's keys of a tile of V, a unit of 16 bytes a lane and step, to f16
+        constexpr int UNITS = OWN * U, WS = UNITS < 64 ? 1 : UNITS / 64;
+        const bool widens = UNITS >= 64 || lane < UNITS;
+        uint32_t wat[WS];
+#pragma unroll
+        for (int i = 0; i < WS; ++i) {
+            const int unit = lane + 64 * i, key = own + unit / U;
+            wat[i] = key * 2 * Z::RB + 16 * ((2 * (unit % U)) ^ swz_w(key));
+        }
+        auto bytes_of = [&](const uint8_t * from, int i) __attribute__((always_inline)) {
+            return *reinterpret_cast<const v4u *>(from + own * Z::RB + 1024 * i + 16 * lane);
+        };
+        // half h of unit i
+        auto widen = [&](v4u x, uint8_t * to, int i, int h) __attribute__((always_inline)) {
+            const v8h w = unpack((v2u){x[2 * h], x[2 * h + 1]});
+            if (widens) *reinterpret_cast<v8h *>(to + (wat[i] ^ (16 * h))) = w;
+        };
+        // V in f16: keys 16 g + 4 half + j % 4 + 8 (j / 4) of d = 32 d + lane % 32
+        const int wkey = 4 * half + (l16 >> 2), wcol = 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1);
+        const uint32_t fat = wkey * 2 * Z::RB + 16 * (wcol ^ swz_w(wkey)) + 8 * (l16 & 1);
+        auto w_frag = [&](const uint8_t * vb, int d, int g) __attribute__((always_inline)) {
+            const uint8_t * const at = vb + (fat ^ (64 * d)) + 16 * g * 2 * Z::RB;
+            const v2u x = read_tr16(at), y = read_tr16(at + 8 * 2 * Z::RB);
+            return __builtin_bit_cast(v8h, (v4u){x[0], x[1], y[0], y[1]});
         };
         v16f s, vs;                                        // the tile's scores, its scales of V
-        float mx, lv;
+        float mx, lv;                                      // their largest, log2 of the largest
         // that the buffers differ has to be said, else every read of LDS waits for the DMA
-        auto step = [&](auto edge, auto steady, uint8_t * __restrict__ kw, uint8_t * __restrict__ ksw, uint8_t * __restrict__ vsw,
-                        uint8_t * __restrict__ vw, const uint8_t * __restrict__ kr, const uint8_t * __restrict__ ksr,
-                        const uint8_t * __restrict__ vsr, const uint8_t * __restrict__ vr, const uint8_t * __restrict__ qlow, float bottom, int j) __attribute__((always_inline)) {
+        auto step = [&](auto edge, auto steady, uint8_t * __restrict__ kw, uint8_t * __restrict__ ksw, uint8_t * __restrict__ vw,
+                        uint8_t * __restrict__ vsw, const uint8_t * __restrict__ kr, const uint8_t * __restrict__ ksr,
+                        const uint8_t * __restrict__ v8r, const uint8_t * __restrict__ vsr, const uint8_t * __restrict__ vr,
+                        uint8_t * __restrict__ v16w, const uint8_t * __restrict__ qlow, float bottom, int j) __attribute__((always_inline)) {
             constexpr bool EDGE = decltype(edge)::value;
-            constexpr int KA = 2, VA = Z::QL ? 2 : 4;    // fragments are read so many steps before they are used
+            constexpr int KA = 2, VA = Z::QL && WIDE ? 2 : 4;   // fragments are read so many steps before they are used
             v4i kf[KA], lf[KA];
             auto k_read = [&](int i) __attribute__((always_inline)) {
                 kf[i % KA] = k_frag(kr, i % QS);
-                if (Z::QL && i >= QS) lf[i % KA] = *reinterpret_cast<const v4i *>(qlow + 1024 * (i - QS));
+                if (Z::QL && low_at(i) >= 0) lf[i % KA] = *reinterpret_cast<const v4i *>(qlow + 1024 * low_at(i));
             };
 #pragma unroll
             for (int i = 0; i < KA; ++i) k_read(i);
             __builtin_amdgcn_sched_barrier(0);
             take(j + R);
             ask(j + R + 1);
-            if (steady || j + R < nt) stage_k(j + R, kw, ksw, vsw);
-            if (steady || j + R - 1 < nt) stage_v(j + R - 1, vw);
-            if (!work) return;
+            v4u bytes[WS];
+            auto ask_bytes = [&]() __attribute__((always_inline)) {
+                asm volatile("");                          // (on either side of the branch, not before it)
+#pragma unroll
+                for (int i = 0; i < WS; ++i) bytes[i] = bytes_of(v8r, i);
+            };
+            if (!work) {
+                if (steady || j + R < nt) {
+                    stage_k(j + R, kw, ksw);
+                    stage_v(j + R, vw, vsw);
+                }
+                ask_bytes();
+#pragma unroll
+                for (int i = 0; i < 2 * WS; ++i) widen(bytes[i / 2], v16w, i / 2, i % 2);
+                return;
+            }
+            // (three digits and two terms leave registers for one unit at a time)
+            constexpr bool LATE = Z::QL && WIDE;
+            if (!LATE) ask_bytes();
             const int key = k0 + 32 * j, holes = hq >> (2 * R) & 3;
             if (EDGE || holes) {
                 mask(s, vs, key, holes);
@@ -431,11 +507,10 @@ __global__ void __launch_bounds__(256) attn_q8_kernel(AttnArgs a) {
                 lv = log_scale(vs);
                 if (sees(key, holes)) mx = fmaxf(mx, LEAST);
             }
-            follow(s, mx, lv);
+            follow(s, mx + lv);
             constexpr int E = 16 / STEPS;
             float sum[2] = {0.0f, 0.0f};
-            v2u vf[VA];
-            v8h pf[NP][2];
+            v8h vf[VA], pf[NP][2];
             v16i next[NA];
             v16f low;
             constexpr int KQ = Z::QL ? 2 : 4;              // scales of K in registers, 4 keys each
@@ -444,13 +519,18 @@ __global__ void __launch_bounds__(256) attn_q8_kernel(AttnArgs a) {
             for (int k = 0; k < NA; ++k) next[k] = v16i{};
             // a block's second term follows at once, where it has sums of its own
             auto v_read = [&](int i) __attribute__((always_inline)) {
-                vf[i % VA] = NP == 2 ? v_frag(vr, i / 2, i % 2) : v_frag(vr, i % DT, i / DT);
+                vf[i % VA] = NP == 2 ? w_frag(vr, i / 2, i % 2) : w_frag(vr, i % DT, i / DT);
             };
+#pragma unroll
+            for (int e = 0; e < E; ++e) weight(s[e], vs[e], pf, e, sum[e & 1]);
+            __builtin_amdgcn_sched_barrier(0);
             // lgkmcnt(0): with a scalar load under way the waits below could not count
             __builtin_amdgcn_s_waitcnt(0xC07F);
 #pragma unroll
             for (int i = 0; i < STEPS; ++i) {
                 digits(next, kf[i % KA], lf[i % KA], i);
+#pragma unroll
+                for (int e = (i + 1) * E; e < (i + 2) * E && e < 16; ++e) weight(s[e], vs[e], pf, e, sum[e & 1]);
                 if (i + KA < STEPS) k_read(i + KA);
                 // (the last steps ask for the first fragments of V)
                 constexpr int ASK = STEPS < VA ? STEPS : VA, EACH = VA / ASK;
@@ -458,8 +538,9 @@ __global__ void __launch_bounds__(256) attn_q8_kernel(AttnArgs a) {
 #pragma unroll
                     for (int x = 0; x < EACH; ++x) v_read((i - (STEPS - ASK)) * EACH + x);
                 }
-#pragma unroll
-                for (int e = i * E; e < (i + 1) * E; ++e) weight(s[e], vs[e], pf, e, sum[e & 1]);
+                // the loads of the tile R ahead, under the MFMAs
+                if (i == 0 && (steady || j + R < nt)) stage_k(j + R, kw, ksw);
+                if (i == STEPS / 2 && (steady || j + R < nt)) stage_v(j + R, vw, vsw);
                 __builtin_amdgcn_sched_barrier(0);
             }
             l += sum[0] + sum[1];
@@ -470,7 +551,7 @@ __global__ void __launch_bounds__(256) attn_q8_kernel(AttnArgs a) {
             float big[2] = {bottom, bottom}, lvs[2] = {0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < 2 * DT; ++i) {
-                const v8h vx = unpack(vf[i % VA]);
+                const v8h vx = vf[i % VA];
                 if constexpr (NP == 2) {
                     const int d = i / 2, g = i % 2;
                     if (g == 0) {
@@ -483,6 +564,10 @@ __global__ void __launch_bounds__(256) attn_q8_kernel(AttnArgs a) {
                     o[i % DT] = mfma(vx, pf[0][i / DT], o[i % DT]);
                 }
                 if (i + VA < 2 * DT) v_read(i + VA);
+                // V of the next tile becomes f16
+                constexpr int EVERY = 2 * DT / (2 * WS);
+                if (LATE && i % (2 * EVERY) == 0) bytes[0] = bytes_of(v8r, i / EVERY / 2);
+                if (i % EVERY == (LATE ? EVERY / 2 : 0)) widen(bytes[LATE ? 0 : i / EVERY / 2], v16w, i / EVERY / 2, i / EVERY % 2);
 #pragma unroll
                 for (int e = i * 8 / DT; e < (i + 1) * 8 / DT; ++e) {
                     s[e] = whole(next, e) * ks[e / 4 % KQ][e % 4];
@@ -494,7 +579,7 @@ __global__ void __launch_bounds__(256) attn_q8_kernel(AttnArgs a) {
             }
             if constexpr (NP == 2) add_low(low, o[DT - 1]);
             mx = over_halves(fmaxf(big[0], big[1])) * c;
-            lv = __builtin_amdgcn_logf(over_halves(fmaxf(lvs[0], lvs[1])));
+            lv = log_of(fmaxf(lvs[0], lvs[1]));
         };
         if (nt > 0) {
             ask(0);
@@ -502,13 +587,18 @@ __global__ void __launch_bounds__(256) attn_q8_kernel(AttnArgs a) {
             for (int t = 0; t < R; ++t) {
                 take(t);
                 ask(t + 1);
-                if (t < nt) stage_k(t, kring + t * Z::TILE, ksring + t * Z::SC, vsring + t * Z::SC);
-                if (t > 0 && t - 1 < nt) stage_v(t - 1, vring + (t - 1) * Z::TILE);
+                if (t < nt) {
+                    stage_k(t, kring + t * Z::TILE, ksring + t * Z::SC);
+                    stage_v(t, vring + t * Z::TILE, vsring + t * Z::SC);
+                }
             }
             make_q();
             clear();
             if (nt >= R) pq2::wait_vmcnt<(R - 1) * PER>();
             else pq2::wait_vmcnt<0>();
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int i = 0; i < 2 * WS; ++i) widen(bytes_of(vring, i / 2), wide_v, i / 2, i % 2);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
@@ -529,14 +619,15 @@ __global__ void __launch_bounds__(256) attn_q8_kernel(AttnArgs a) {
             // (steady: every load that a tile can start is there; R of them at a time, with the rings' places
             // known to the compiler)
             auto pass = [&](auto edge, auto steady, int slot, int j) __attribute__((always_inline)) {
-                const int after = slot + 1 == R ? 0 : slot + 1, behind = slot == 0 ? R - 1 : slot - 1;
+                const int after = slot + 1 == R ? 0 : slot + 1;
                 if (steady || j - 1 + R < nt) pq2::wait_vmcnt<(R - 2) * PER>();
                 else pq2::wait_vmcnt<0>();
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 __builtin_amdgcn_s_barrier();              // the tiles are there, and all are done with the last ones
                 asm volatile("" ::: "memory");
-                step(edge, steady, kring + slot * Z::TILE, ksring + slot * Z::SC, vsring + slot * Z::SC, vring + behind * Z::TILE,
-                     kring + after * Z::TILE, ksring + after * Z::SC, vsring + after * Z::SC, vring + slot * Z::TILE, ql, bottom, j);
+                step(edge, steady, kring + slot * Z::TILE, ksring + slot * Z::SC, vring + slot * Z::TILE, vsring + slot * Z::SC,
+                     kring + after * Z::TILE, ksring + after * Z::SC, vring + after * Z::TILE, vsring + after * Z::SC,
+                     wide_v + slot % 2 * 2 * Z::TILE, wide_v + (1 - slot % 2) * 2 * Z::TILE, ql, bottom, j);
             };
             int j = 0;
             const int all = min(plain, nt - R);
@@ -555,37 +646,55 @@ __global__ void __launch_bounds__(256) attn_q8_kernel(AttnArgs a) {
         }
     } else {
         uint8_t * const mine = lds + wave * 4 * Z::TILE, * const msc = lds + Z::MAIN + wave * 4 * Z::SC;
-        int id0 = -1, id1 = -1;
         auto page_of = [&](int key, bool have, int id) {
             if (key >= nk) return -1;
             if (!have) id = sload(a.table, trow + (key >> a.page_log2));
             return id >= 0 && id < a.n_pages ? id : -1;
         };
-        auto stage = [&](int key, bool have, uint8_t * to, uint8_t * sc) __attribute__((always_inline)) {
-            id0 = page_of(key, have, early0);
-            id1 = page_of(key + 16, have, early1);
-            const std::integral_constant<int, 16> half_tile;
-            const auto put = [&](const uint8_t * base, uint8_t * rows, uint8_t * sc, bool is_v) __attribute__((always_inline)) {
-                const auto p0 = page(base, id0), p1 = page(base, id1);
-                stage_n(half_tile, p0, key, 0, rows, is_v);
-                stage_n(half_tile, p1, key + 16, 0, rows + 16 * Z::RB, is_v);
-                stage_scales(half_tile, p0, key, sc);
-                stage_scales(half_tile, p1, key + 16, sc + 64);
-            };
-            put(a.k, to, sc, false);
-            put(a.v, to + Z::TILE, sc + Z::SC, true);
+        // K of tile t + 2 is asked for when the scores of tile t are made, V when its sums are, so that one to two tiles
+        // are under way: with both asked for at the start of tile t + 1, 32 sequences of up to 12000 keys took 102 us for 90
+        constexpr int HALF = 16 / RPI, NK = 2 * HALF + 4, NV = 2 * HALF;   // DMA instructions of a tile of K, of V
+        const std::integral_constant<int, 16> half_tile;
+        auto find = [&](int key, bool have, int (&to)[2]) __attribute__((always_inline)) {
+            to[0] = page_of(key, have, early0);
+            to[1] = page_of(key + 16, have, early1);
         };
-        auto step = [&](uint8_t * __restrict__ next, uint8_t * __restrict__ snext, const uint8_t * __restrict__ cur,
-                        const uint8_t * __restrict__ scur, int key, int holes) __attribute__((always_inline)) {
-            if (key + 32 * Z::NW < k1) stage(key + 32 * Z::NW, false, next, snext);
+        // (K brings the scales of both)
+        auto stage_k = [&](int key, const int (&from)[2], uint8_t * to, uint8_t * sc) __attribute__((always_inline)) {
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const auto kp = page(a.k, max(from[g], 0));
+                stage_n(half_tile, kp, key + 16 * g, 0, to + 16 * g * Z::RB, true);
+                stage_scales(half_tile, kp, key + 16 * g, sc + 256 * g);
+                stage_scales(half_tile, page(a.v, max(from[g], 0)), key + 16 * g, sc + Z::SC + 256 * g);
+            }
+        };
+        auto stage_v = [&](int key, const int (&from)[2], uint8_t * to) __attribute__((always_inline)) {
+#pragma unroll
+            for (int g = 0; g < 2; ++g) stage_n(half_tile, page(a.v, max(from[g], 0)), key + 16 * g, 0, to + 16 * g * Z::RB, false);
+        };
+        constexpr int STRIDE = 32 * Z::NW;
+        // kb, sc, vb: this tile's, which then take the one after the next's; ids: the pages of its halves, then of that one's
+        auto step = [&](uint8_t * kb, uint8_t * sc, uint8_t * vb, int (&ids)[2], int key) __attribute__((always_inline)) {
+            const bool next = key + STRIDE < k1, more = key + 2 * STRIDE < k1;
+            const int holes = (ids[0] < 0 ? 1 : 0) | (ids[1] < 0 ? 2 : 0);
+            // behind K: V, and K and V of the next tile
+            if (next) pq2::wait_vmcnt<NK + 2 * NV>();
+            else pq2::wait_vmcnt<NV>();
+            asm volatile("" ::: "memory");
             v16f s, ks, vs;
-            scales(scur, ks);
-            scales(scur + Z::SC, vs);
+            scales(sc, ks);
+            scales(sc + Z::SC, vs);
             {
                 v16i x[NA];
-                product(x, cur, nullptr);
+                product(x, kb, nullptr);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[i] = whole(x, i) * ks[i];
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // its reads are done
+            if (more) {
+                find(key + 2 * STRIDE, false, ids);
+                stage_k(key + 2 * STRIDE, ids, kb, sc);
             }
             float mx;
             if (key + 32 > least || holes || (SHARED && key < lo)) {
@@ -595,15 +704,20 @@ __global__ void __launch_bounds__(256) attn_q8_kernel(AttnArgs a) {
             } else {
                 mx = fmaxf(largest(s), LEAST);
             }
-            follow(s, mx, log_scale(vs));
+            follow(s, mx + log_scale(vs));
             v8h pf[NP][2];
             float sum[2] = {0.0f, 0.0f};
 #pragma unroll
             for (int e = 0; e < 16; ++e) weight(s[e], vs[e], pf, e, sum[e & 1]);
             l += sum[0] + sum[1];
+            // behind V: K and V of the next tile, K of the one after
+            if (more) pq2::wait_vmcnt<2 * NK + NV>();
+            else if (next) pq2::wait_vmcnt<NK + NV>();
+            else pq2::wait_vmcnt<0>();
+            asm volatile("" ::: "memory");
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                const v8h v0 = unpack(v_frag(cur + Z::TILE, d, 0)), v1 = unpack(v_frag(cur + Z::TILE, d, 1));
+                const v8h v0 = unpack(v_frag(vb, d, 0)), v1 = unpack(v_frag(vb, d, 1));
                 if constexpr (NP == 2) {
                     v16f low = mfma(v0, pf[1][0], v16f{});
                     low = mfma(v1, pf[1][1], low);
@@ -615,17 +729,31 @@ __global__ void __launch_bounds__(256) attn_q8_kernel(AttnArgs a) {
                     o[d] = mfma(v1, pf[0][1], o[d]);
                 }
             }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (more) stage_v(key + 2 * STRIDE, ids, vb);
         };
-        int key = k0 + 32 * wave, b = 0;
-        if (key < k1) stage(key, early, mine, msc);
+        int key = k0 + 32 * wave, ids[2] = {-1, -1}, next[2] = {-1, -1}, at = 0;
+        if (key < k1) {
+            find(key, early, ids);
+            stage_k(key, ids, mine, msc);
+            stage_v(key, ids, mine + Z::TILE);
+        }
+        if (key + STRIDE < k1) {
+            find(key + STRIDE, false, next);
+            stage_k(key + STRIDE, next, mine + 2 * Z::TILE, msc + 2 * Z::SC);
+            stage_v(key + STRIDE, next, mine + 3 * Z::TILE);
+        }
         make_q();
         clear();
 #pragma clang loop unroll(disable)
-        for (; key < k1; key += 32 * Z::NW, b ^= 1) {
-            const int holes = (id0 < 0 ? 1 : 0) | (id1 < 0 ? 2 : 0);
-            pq2::wait_vmcnt<0>();
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // also: the other buffer's reads are done
-            step(mine + (b ^ 1) * 2 * Z::TILE, msc + (b ^ 1) * 2 * Z::SC, mine + b * 2 * Z::TILE, msc + b * 2 * Z::SC, key, holes);
+        for (; key < k1; key += STRIDE, at ^= 1) {
+            step(mine + at * 2 * Z::TILE, msc + at * 2 * Z::SC, mine + at * 2 * Z::TILE + Z::TILE, ids, key);
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const int x = ids[g];
+                ids[g] = next[g];
+                next[g] = x;
+            }
         }
     }
     l += __shfl_xor(l, 32);
@@ -634,8 +762,6 @@ __global__ void __launch_bounds__(256) attn_q8_kernel(AttnArgs a) {
     LateArgs * const z = late_args();
     const int part = attn_part<SHARED>(z, attn_place<SHARED>(z));
 
-    // parts are relative to m + UP, so that their sums are those of weights up to 2^LAG
-    const float off = fabsf(m) < FAR ? UP : 0.0f;
     const int n_part = SHARED ? z->n_split1 + z->n_split : z->n_split;
     const bool parts = SHARED || z->n_split > 1;
     const int64_t all_rows = (int64_t)z->n_tok * z->n_head;
@@ -643,8 +769,7 @@ __global__ void __launch_bounds__(256) attn_q8_kernel(AttnArgs a) {
     if constexpr (!KEYS) {
         if (!live) return;
         const int64_t row = grow * z->n_head + head;
-        const float to_m = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mo - m - (parts ? off : 0.0f));
-        const float f = parts ? to_m : to_m * over(m, l);
+        const float f = parts ? 1.0f : over(m, l);
         float * const po = z->part + ((int64_t)part * all_rows + row) * D;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
@@ -659,7 +784,7 @@ __global__ void __launch_bounds__(256) attn_q8_kernel(AttnArgs a) {
             }
         if (parts && half == 0)
             *reinterpret_cast<float2 *>(pml + 2 * ((int64_t)part * all_rows + row)) =
-                make_float2(m + off, l * __builtin_amdgcn_exp2f(-off));
+                make_float2(m, l);
     } else {
         // join the waves: [wave][row][D] and [wave][row] (m, l)
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -668,14 +793,13 @@ __global__ void __launch_bounds__(256) attn_q8_kernel(AttnArgs a) {
         float * const jo = reinterpret_cast<float *>(lds);
         float2 * const ml = reinterpret_cast<float2 *>(lds + Z::NW * 32 * Z::OROW * 4);
         if (live) {
-            const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mo - m - off);
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
                 for (int g = 0; g < 4; ++g)
                     *reinterpret_cast<v4f *>(jo + (wave * 32 + n) * Z::OROW + 32 * d + 8 * g + 4 * half) =
-                        (v4f){o[d][4 * g] * f, o[d][4 * g + 1] * f, o[d][4 * g + 2] * f, o[d][4 * g + 3] * f};
-            if (half == 0) ml[wave * 32 + n] = make_float2(m + off, l * __builtin_amdgcn_exp2f(-off));
+                        (v4f){o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+            if (half == 0) ml[wave * 32 + n] = make_float2(m, l);
         }
         __syncthreads();
         constexpr int E = D / 64;
@@ -713,7 +837,7 @@ int launch(AttnArgs & a, bool first, bool own, hipStream_t s) {
     AttnArgs b = a;
     b.blocks1 = first ? (unsigned)((int64_t)a.tiles1 * a.n_split1 * a.n_kv) : 0;
     const int64_t blocks = b.blocks1 + (own ? (int64_t)a.tiles * a.n_split * a.n_kv : 0);
-    hipLaunchKernelGGL((attn_q8_kernel<IO, D, KEYS, SHARED>), dim3((unsigned)blocks), dim3(256), 0, s, b);
+    hipLaunchKernelGGL((attn_q8_kernel<IO, D, KEYS, SHARED>), dim3((unsigned)blocks), dim3(64 * Shape<D, KEYS, false>::NW), 0, s, b);
     return (int)hipGetLastError();
 }
 template <class IO, int D, bool SHARED>

@@ -223,26 +223,34 @@ inline int rope_tile(bool columns, int64_t n_tok) { return n_tok <= 64 ? 4 : col
 // 98, as three terms leave room for one workgroup a CU, and the tiles are counted with one
 // to spare).  Up to 64 parts: with 16 at most, 8 tokens of 60000 keys took 228 us for
 // 75 (fp32), 16 of 16000 74 for 49.
+//   bytes: 8-bit pages, of which two workgroups share a CU where heads of 256 split the keys.
+//   whole: one sequence has all of the tokens (a group's, whose shared keys these are), so that no tile is to spare.
 struct AttnPlan {
     bool keys;
     int64_t tiles, chunk, n_split;
 };
+inline void attn_split(AttnPlan & p, int64_t want, int64_t max_kv, int64_t step) {
+    if (want < 1) want = 1;
+    p.chunk = (max_kv + want * step - 1) / (want * step) * step;
+    if (p.chunk < step) p.chunk = step;
+    p.n_split = max_kv > p.chunk ? (max_kv + p.chunk - 1) / p.chunk : 1;
+}
 inline AttnPlan attn_plan(int64_t n_tok, int64_t n_seq, int64_t group, int64_t n_kv, int64_t dim, int64_t max_kv, int64_t rows,
-                          int64_t cus, bool bytes = false) {
+                          int64_t cus, bool bytes = false, bool whole = false) {
     AttnPlan p;
     p.keys = n_tok * group <= 32 * n_seq;
-    const int64_t bm = p.keys ? 32 : rows, step = p.keys && (bytes || dim < 256) ? 128 : 64;   // keys: 32 for each wave
+    const int64_t bm = p.keys ? 32 : rows, step = p.keys && dim < 256 ? 128 : 64;
     const int64_t some = n_seq < n_tok ? n_seq : n_tok;
-    p.tiles = n_tok * group / bm + some;
+    p.tiles = whole && n_seq == 1 ? ceil_div(n_tok * group, bm) : n_tok * group / bm + some;
     int64_t want = 1;
     if (p.keys) {
-        const int64_t slots = cus * (256 / dim);
+        const int64_t slots = cus * (bytes && dim == 256 ? 2 : 256 / dim);
         want = (some == 1 ? slots : 3 * slots) / (some * n_kv);
     } else {
         // rounds of workgroups times the keys of one, or the longest; a part of a row is written and read
         const int64_t slots = cus * (dim == 256 ? 1 : 2), blocks = p.tiles * n_kv;
         const double key = 0.022 * (double)dim / 256, part = (double)n_tok * group * n_kv * dim * 8 / 4.5e6;
-        const double longest = (double)max_kv, mean = longest - 0.5 * (double)(n_tok / some < max_kv ? n_tok / some : max_kv);
+        const double longest = (double)max_kv, mean = longest - (whole ? 0.0 : 0.5 * (double)(n_tok / some < max_kv ? n_tok / some : max_kv));
         double best = 0.0;
         for (int64_t n = 1; n <= 64 && blocks < 2 * slots; ++n) {
             const double rounds = (double)((blocks * n + slots - 1) / slots) * mean;
@@ -250,10 +258,24 @@ inline AttnPlan attn_plan(int64_t n_tok, int64_t n_seq, int64_t group, int64_t n
             if (n == 1 || us < best) best = us, want = n;
         }
     }
-    if (want < 1) want = 1;
-    p.chunk = (max_kv + want * step - 1) / (want * step) * step;
-    if (p.chunk < step) p.chunk = step;
-    p.n_split = max_kv > p.chunk ? (max_kv + p.chunk - 1) / p.chunk : 1;
+    attn_split(p, want, max_kv, step);
+    return p;
+}
+// The sequences' own keys behind shared prefixes: mostly few, so that what counts is how often a CU begins with
+// another workgroup (`begin` us), and how many steps (of 32 keys a wave, `step` us) the longest takes.
+inline AttnPlan attn_own_plan(int64_t n_tok, int64_t n_seq, int64_t group, int64_t n_kv, int64_t dim, int64_t max_kv, int64_t rows,
+                              int64_t cus, bool bytes) {
+    AttnPlan p = attn_plan(n_tok, n_seq, group, n_kv, dim, max_kv, rows, cus, bytes);
+    if (!p.keys) return p;
+    const int64_t some = n_seq < n_tok ? n_seq : n_tok, per = dim < 256 ? 128 : 64, slots = cus * (bytes && dim == 256 ? 2 : 256 / dim);
+    const double begin = 7.0, step = 2.0;
+    double best = 0.0;
+    int64_t want = 1;
+    for (int64_t n = 1; n <= 64; ++n) {
+        const double us = (double)ceil_div(some * n_kv * n, slots) * (begin + step * (double)ceil_div(ceil_div(max_kv, n), per));
+        if (n == 1 || us < best) best = us, want = n;
+    }
+    attn_split(p, want, max_kv, per);
     return p;
 }
 
