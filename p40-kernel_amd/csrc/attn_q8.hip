@@ -73,11 +73,12 @@ struct Shape {
     static constexpr int OROW = D + 4;                     // floats of a row in the join
     static constexpr int JOIN = NW * 32 * OROW * 4 + NW * 32 * 8;
     static constexpr int SLOTS = KEYS ? NW * 4 : 2 * R;    // keys: two buffers of K and V a wave
-    // heads of 256: the registers hold the other digits of q, the lowest is in LDS
-    static constexpr bool QL = D == 256 && !KEYS;
+    // heads of 256: the registers hold the other digits of q, the lowest is in LDS (keys: the waves' is the same, and
+    // all write it)
+    static constexpr bool QL = D == 256 && (WIDE || !KEYS);
     static constexpr int QT = 32 * D;                      // bytes of a digit of 32 rows
     // rows: two tiles of V in f16
-    static constexpr int MAIN = SLOTS * TILE, SCALED = MAIN + SLOTS * SC, WIDENED = SCALED + (QL ? NW * QT : 0);
+    static constexpr int MAIN = SLOTS * TILE, SCALED = MAIN + SLOTS * SC, WIDENED = SCALED + (QL ? (KEYS ? 1 : NW) * QT : 0);
     static constexpr int ALL = WIDENED + (KEYS ? 0 : 2 * 2 * TILE);
     static constexpr int LDS = KEYS && JOIN > ALL ? JOIN : ALL;
 };
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(KEYS && D == 256 ? 128 : 256) attn_q8_kernel(A
         }
     }
     v4i qf[NT][QS];
-    uint8_t * const ql = lds + Z::SCALED + wave * Z::QT + 16 * lane;
+    uint8_t * const ql = lds + Z::SCALED + (KEYS ? 0 : wave * Z::QT) + 16 * lane;
     float c = a.c;
     auto make_q = [&]() __attribute__((always_inline)) {
         // the largest magnitude's bits: they compare as the magnitudes do, and NaN is above infinity
@@ -237,8 +238,8 @@ __global__ void __launch_bounds__(KEYS && D == 256 ? 128 : 256) attn_q8_kernel(A
 
     // ---- one sub-tile of 32 keys
     const int l16 = lane & 15, vkey = 4 * half + ((l16 >> 1) & 3) + 8 * (l16 >> 3), vcol = (lane >> 4) & 1;
-    const uint32_t kat = n * Z::RB + 16 * (half ^ swz_k(n));
-    const uint32_t vat = vkey * Z::RB + 16 * (vcol ^ swz_v(vkey)) + 8 * (l16 & 1);
+    uint32_t kat = n * Z::RB + 16 * (half ^ swz_k(n));
+    uint32_t vat = vkey * Z::RB + 16 * (vcol ^ swz_v(vkey)) + 8 * (l16 & 1);
     auto k_frag = [&](const uint8_t * kb, int i) __attribute__((always_inline)) {
         return *reinterpret_cast<const v4i *>(kb + (kat ^ (32 * i)));
     };
@@ -289,8 +290,9 @@ __global__ void __launch_bounds__(KEYS && D == 256 ? 128 : 256) attn_q8_kernel(A
 #pragma unroll
         for (int k = 0; k < NA; ++k) x[k] = v16i{};
 #pragma unroll
-        for (int t = 0; t < STEPS; ++t)
+        for (int t = 0; t < STEPS; ++t) {
             digits(x, k_frag(kb, t % QS), Z::QL && low_at(t) >= 0 ? *reinterpret_cast<const v4i *>(qlow + 1024 * low_at(t)) : v4i{}, t);
+        }
     };
     auto over_halves = [&](float mx) __attribute__((always_inline)) {
         const uint32_t x = __builtin_bit_cast(uint32_t, mx);
@@ -338,7 +340,7 @@ __global__ void __launch_bounds__(KEYS && D == 256 ? 128 : 256) attn_q8_kernel(A
     };
     v16f o[DT];
     auto clear = [&]() __attribute__((always_inline)) {
-        asm volatile("" ::: "memory");                     // (not before the queries are digits, as registers go)
+        __builtin_amdgcn_sched_barrier(0);                 // (not before the queries are digits, as registers go)
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
             o[d] = v16f{};
@@ -677,17 +679,27 @@ __global__ void __launch_bounds__(KEYS && D == 256 ? 128 : 256) attn_q8_kernel(A
         // kb, sc, vb: this tile's, which then take the one after the next's; ids: the pages of its halves, then of that one's
         auto step = [&](uint8_t * kb, uint8_t * sc, uint8_t * vb, int (&ids)[2], int key) __attribute__((always_inline)) {
             const bool next = key + STRIDE < k1, more = key + 2 * STRIDE < k1;
+            // (fp32 rows of 256: the fragments' 16 addresses are made anew, as registers for them there are none)
+            if (Z::QL) asm volatile("" : "+v"(kat), "+v"(vat));
             const int holes = (ids[0] < 0 ? 1 : 0) | (ids[1] < 0 ? 2 : 0);
             // behind K: V, and K and V of the next tile
             if (next) pq2::wait_vmcnt<NK + 2 * NV>();
             else pq2::wait_vmcnt<NV>();
             asm volatile("" ::: "memory");
-            v16f s, ks, vs;
-            scales(sc, ks);
-            scales(sc + Z::SC, vs);
+            v16f s, vs;
             {
                 v16i x[NA];
-                product(x, kb, nullptr);
+                v16f ks;
+                auto get = [&]() __attribute__((always_inline)) {
+                    scales(sc, ks);
+                    scales(sc + Z::SC, vs);
+                };
+                if (!Z::QL) get();
+                product(x, kb, ql);
+                if (Z::QL) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    get();
+                }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[i] = whole(x, i) * ks[i];
             }
@@ -710,6 +722,7 @@ __global__ void __launch_bounds__(KEYS && D == 256 ? 128 : 256) attn_q8_kernel(A
 #pragma unroll
             for (int e = 0; e < 16; ++e) weight(s[e], vs[e], pf, e, sum[e & 1]);
             l += sum[0] + sum[1];
+            asm volatile("" : "+v"(l));                    // (here, not behind the product, up to which 16 weights would be kept)
             // behind V: K and V of the next tile, K of the one after
             if (more) pq2::wait_vmcnt<2 * NK + NV>();
             else if (next) pq2::wait_vmcnt<NK + NV>();
@@ -729,6 +742,7 @@ __global__ void __launch_bounds__(KEYS && D == 256 ? 128 : 256) attn_q8_kernel(A
                     o[d] = mfma(v1, pf[0][1], o[d]);
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             if (more) stage_v(key + 2 * STRIDE, ids, vb);
         };

@@ -7,6 +7,7 @@
 // output, a row's lanes are next to each other, and each lane has ROWS rows under way,
 // as a slot, a row and its scale are a chain of two loads.
 #include "host_state.h"
+#include "launch_rules.h"
 #include "mixer_device.h"
 
 #include <type_traits>
@@ -28,7 +29,8 @@ struct Q8 {
     typedef int8_t elem;
 };
 
-template <class TP, class TO, int D>
+// PAST: stores past the caches
+template <class TP, class TO, int D, bool PAST>
 __global__ void __launch_bounds__(256) kv_read_kernel(ReadArgs a) {
     constexpr int E = 16 / sizeof(typename TO::elem), L = D / E, ROWS = 4;   // elements of a lane, lanes of a row
     constexpr bool BYTES = std::is_same<TP, Q8>::value;
@@ -64,15 +66,23 @@ __global__ void __launch_bounds__(256) kv_read_kernel(ReadArgs a) {
             } else {
                 y[j] = TP::to(x[i][j]);
             }
-        store_row<TO>(reinterpret_cast<typename TO::elem *>(a.out[which]) + t * a.tok[which] + head * D + e, y);
+        typedef typename TO::elem row __attribute__((ext_vector_type(E)));
+        row z;
+#pragma unroll
+        for (int j = 0; j < E; ++j) z[j] = TO::from(y[j]);
+        row * const to = reinterpret_cast<row *>(reinterpret_cast<typename TO::elem *>(a.out[which]) + t * a.tok[which] + head * D + e);
+        if (PAST) __builtin_nontemporal_store(z, to);
+        else *to = z;
     }
 }
 
 template <class TP, class TO, int D>
 int launch(const ReadArgs & a, hipStream_t s) {
-    constexpr int per = 256 / (D * (int)sizeof(typename TO::elem) / 16) * 4;
-    hipLaunchKernelGGL((kv_read_kernel<TP, TO, D>), dim3((unsigned)((a.n_tok + per - 1) / per), (unsigned)(2 * a.n_kv)), dim3(256), 0,
-                       s, a);
+    constexpr int size = sizeof(typename TO::elem), per = 256 / (D * size / 16) * 4;
+    const dim3 grid((unsigned)((a.n_tok + per - 1) / per), (unsigned)(2 * a.n_kv));
+    if (pq2::read_streams(2 * (int64_t)a.n_tok * a.n_kv * D * size))
+        hipLaunchKernelGGL((kv_read_kernel<TP, TO, D, true>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((kv_read_kernel<TP, TO, D, false>), grid, dim3(256), 0, s, a);
     return (int)hipGetLastError();
 }
 template <class TP, class TO>

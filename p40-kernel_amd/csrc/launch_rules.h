@@ -262,7 +262,10 @@ inline AttnPlan attn_plan(int64_t n_tok, int64_t n_seq, int64_t group, int64_t n
     return p;
 }
 // The sequences' own keys behind shared prefixes: mostly few, so that what counts is how often a CU begins with
-// another workgroup (`begin` us), and how many steps (of 32 keys a wave, `step` us) the longest takes.
+// another workgroup (`begin` us), and how many steps (of 32 keys a wave, `step` us) the longest takes.  Measured on MI355X
+// (us of the kernel over the own keys, 24 heads of 256, split as attn_plan does / so): 64 sequences of up to 500, bf16, 3 / 1
+// parts 30.4 / 22.8; 32 of up to 1500, 8-bit pages, 6 / 4 36.6 / 23.2; 40 of up to 300 with 12 tokens, heads of 128, 1 part of
+// 128 keys each 32.2 / 19.5.  With 4 to 14 us to begin and 1.5 to 2 a step these three come out the same.
 inline AttnPlan attn_own_plan(int64_t n_tok, int64_t n_seq, int64_t group, int64_t n_kv, int64_t dim, int64_t max_kv, int64_t rows,
                               int64_t cus, bool bytes) {
     AttnPlan p = attn_plan(n_tok, n_seq, group, n_kv, dim, max_kv, rows, cus, bytes);
@@ -285,6 +288,12 @@ inline AttnPlan attn_own_plan(int64_t n_tok, int64_t n_seq, int64_t group, int64
 // parts) 14.2 / 14.4, 1000 (16) 16.0 / 14.8, 4000 (63) 23.5 / 16.9; 32 tokens of 60000 (32) 91.5 /
 // 89.2; 16 of 1000 (8) 24.9 / 25.3, 256 of 60000 (9) 454 / 458, of 16000 (4) 139 / 148.
 inline bool attn_join_wide(int64_t n_split) { return n_split > 8; }
+
+// Rows read back from a cache (kv_read.hip) are stored past the caches (true) where they are more than these hold for
+// what follows.  Measured on MI355X (us, rows of 8-bit pages to fp32, 4 heads of 256, through the caches / past them): 6000
+// rows (49 MB) 13.9 / 14.1, 12000 (98 MB) 29.6 / 25.1, 25000 60.4 / 49.2, 50001 128 / 118; to bf16, 12000 (49 MB) 13.2 / 13.1,
+// 50000 65.7 / 58.5.
+inline bool read_streams(int64_t out_bytes) { return out_bytes > 64 << 20; }
 
 // The gated delta rule (gdn.hip) in chunks of 64 tokens (true), or token by token:
 // a chunk takes the same time however few tokens it has, a token by itself about 1.1

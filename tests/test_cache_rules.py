@@ -1,0 +1,77 @@
+"""CPU: the rules that place the work over 8-bit pages and shared prefixes
+(csrc/launch_rules.h), compiled with g++, for a card of 256 CUs."""
+import ctypes
+import os
+import random
+import subprocess
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+CUS = 256
+I64 = ctypes.c_int64
+
+
+@pytest.fixture(scope="module")
+def rules(tmp_path_factory):
+    so = str(tmp_path_factory.mktemp("rules") / "cache_rules.so")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Wextra", "-Werror", "-shared", "-fPIC",
+                    os.path.join(ROOT, "tests", "host", "cache_rules.cpp"), "-o", so], check=True)
+    return ctypes.CDLL(so)
+
+
+def plan(rules, n_tok, n_seq, group, n_kv, dim, max_kv, rows=128, q8=False, whole=False):
+    out = (I64 * 4)()
+    rules.attn_plan(*map(I64, (n_tok, n_seq, group, n_kv, dim, max_kv, rows, CUS)), int(q8), int(whole), out)
+    return bool(out[0]), out[1], out[2], out[3]
+
+
+def own(rules, n_tok, n_seq, group, n_kv, dim, max_kv, rows=128, q8=False):
+    out = (I64 * 4)()
+    rules.attn_own_plan(*map(I64, (n_tok, n_seq, group, n_kv, dim, max_kv, rows, CUS)), int(q8), out)
+    return bool(out[0]), out[1], out[2], out[3]
+
+
+def test_plans_cover_the_work(rules):
+    """Every ragged set of sequences, or of groups, finds its row tiles, every key its part."""
+    rng = random.Random(7)
+    for _ in range(2000):
+        n_seq, n_kv, group = rng.choice((1, 2, 7, 64, 500)), rng.choice((1, 2, 8)), rng.choice((1, 4, 6, 16))
+        dim, rows, q8 = rng.choice((64, 128, 256)), rng.choice((64, 128)), rng.random() < 0.5
+        new = [rng.choice((0, 1, 1, 5, 33, 700)) for _ in range(n_seq)]
+        n_tok = max(sum(new), 1)
+        max_kv = rng.choice((1, 31, 32, 500, 4000, 131071, (1 << 31) - 1))
+        for keys, tiles, chunk, n_split in (plan(rules, n_tok, n_seq, group, n_kv, dim, max_kv, rows, q8, rng.random() < 0.5),
+                                            own(rules, n_tok, n_seq, group, n_kv, dim, max_kv, rows, q8)):
+            bm = 32 if keys else rows
+            assert tiles >= sum(-(-n * group // bm) for n in new)
+            assert chunk % 32 == 0 and chunk * n_split >= max_kv and (n_split == 1 or chunk * (n_split - 1) < max_kv)
+            assert 1 <= n_split <= 2048
+
+
+def test_16_bit_pages_keep_their_plan(rules):
+    """The plan without a prefix is that of 16-bit pages but where heads of 256 split the keys."""
+    for n_tok, n_seq, dim, kv in ((1, 1, 128, 4000), (32, 32, 64, 12000), (777, 1, 256, 16000), (300, 9, 128, 5000)):
+        assert plan(rules, n_tok, n_seq, 6, 4, dim, kv, q8=True) == plan(rules, n_tok, n_seq, 6, 4, dim, kv)
+    a, b = plan(rules, 32, 32, 6, 4, 256, 12000), plan(rules, 32, 32, 6, 4, 256, 12000, q8=True)
+    assert a[0] and b[0] and b[3] == 2 * a[3]               # two workgroups to a CU
+
+
+def test_one_group_has_no_tile_to_spare(rules):
+    keys, tiles, chunk, n_split = plan(rules, 64, 1, 6, 4, 256, 16000, whole=True)
+    assert not keys and tiles == 3 and CUS * 3 // 4 < 3 * 4 * n_split <= CUS
+    assert plan(rules, 64, 1, 6, 4, 256, 16000)[1] == 4
+    assert plan(rules, 64, 2, 6, 4, 256, 16000, whole=True)[1] == 5
+
+
+# timed with the parts of attn_plan and with these
+@pytest.mark.parametrize("n_tok,n_seq,group,n_kv,dim,keys,q8,parts", [
+    (64, 64, 6, 4, 256, 515, False, 1), (32, 32, 6, 4, 256, 1515, True, 4), (250, 40, 4, 8, 128, 315, False, 1),
+    (4, 4, 6, 4, 256, 35, False, 1)])
+def test_own_keys(rules, n_tok, n_seq, group, n_kv, dim, keys, q8, parts):
+    assert own(rules, n_tok, n_seq, group, n_kv, dim, keys, q8=q8)[::3] == (True, parts)
+
+
+@pytest.mark.parametrize("bytes_,past", [(0, 0), (49 << 20, 0), (64 << 20, 0), ((64 << 20) + 1, 1), (98 << 20, 1), (1 << 40, 1)])
+def test_rows_read_back(rules, bytes_, past):
+    assert rules.read_streams(I64(bytes_)) == past
