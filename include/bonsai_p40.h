@@ -404,7 +404,7 @@ int bonsai_p40_chain_run(const void * plan, int n_steps, void * workspace, uint3
 // whole number, ties to even, in fp32: d * n is off by 0.50002 d at most.  A row whose
 // largest magnitude is below 2^-112 is written as 0, and one that holds a value that is
 // not finite with d = NaN, so that all of it is.  What is read may hold any n in -128 .. 127;
-// keys and values that attention sees are to have |d| of 0 or 2^-120 to 2^120.
+// keys and values that attention sees are to have |d| of 0 or 2^-100 to 2^80.
 
 // RMSNorm of every query and key head, position rotation, and the append of
 // keys and values to the pages, in one launch:

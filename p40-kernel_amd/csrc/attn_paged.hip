@@ -27,6 +27,10 @@
 //     end: decode, bound by the stream of K and V.
 // Either splits the keys over workgroups where there are too few rows to fill the
 // card; attn_join_kernel adds the parts.
+//   SHARED: batches that share a prefix (attn_device.h).  A workgroup has rows of a whole group
+// and its shared keys, or a sequence's and its own, which need not begin with a tile: what is
+// before them is masked.  64 sequences behind 16000 keys, up to 500 each, bf16, 24 heads of 256:
+// 43 us for the prefix, 23 for the own keys, 10 to join (MI355X); attn_paged over the same tables reads the prefix 64 times.
 //
 // fp32 queries and output (the activations' type) keep fp32 accuracy: Q and P
 // are split into 2 f16 terms (22 bits) or 3 bf16 terms (24 bits) and the products

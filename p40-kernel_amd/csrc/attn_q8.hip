@@ -8,20 +8,26 @@
 // 16 bits (16-bit queries) or 24 (fp32), its largest element at 127/128 of their range,
 // as 2 or 3 digits of 8 bits with signs: a MFMA a digit, exact 32-bit sums, one
 // conversion at the end.  A MFMA of these does twice a f16 one's work in its time, so that
-// 2 digits cost what one f16 term does, 3 what 1.5 do, and no byte of K is unpacked.  an
+// 2 digits cost what one f16 term does, 3 what 1.5 do, and no byte of K is unpacked.  An
 // element of q is off by up to 2^-15 or 2^-23 of the row's largest.
 //   Values.  O = sum_j p_j d_j n_j: the scale goes into the weight, w_j = p_j d_j, and
-// V's bytes into f16, which holds them exactly: ds_read_b64_tr_b8 gives a lane the bytes
-// of 8 keys, one XOR, two permutations (1024 + 128 + n as f16 bits) and two packed
-// additions make 4 of them f16.  w is rounded to f16 once (16-bit output; error as in
-// attn_paged.hip), or is two terms of f16 whose second has sums of its own (fp32).
-//   f16's range is short for p_j d_j, so O has a reference of its own beside the
-// softmax's m: o = O 2^-mo, where mo follows the largest of (score + log2 of the tile's largest
-// d) of the tiles so far as m follows the scores, 11 below with a lag of 4: w is at most
-// 2^15, and a key whose p d is 2^-25 of its row's largest has all of f16's digits.  m and mo
-// move in one branch; O is scaled by mo's step alone, l by m's.
+// V's bytes become f16, which holds them exactly: one XOR, two permutations (1024 + 128 +
+// n as f16 bits) and two packed additions make 4 of them.  w is rounded to f16 once (16-bit
+// output; error as in attn_paged.hip), or is two terms of f16 whose second has sums of its
+// own (fp32).
+//   f16's range is short for p_j d_j.  So what m follows is a tile's largest score and the log2
+// of its largest d together: p is relative to that, which leaves w at most 2^15, and a key
+// whose p d is 2^-25 of its row's largest has all of f16's digits.  l and O have the same m.
 //   No value of V is NaN or infinite by itself, so a key that is not seen needs no
 // zeroed row: its weight is 0 and its d counts as 0.
+//   Keys (decode) is bound by the stream of the pages, half of 16-bit ones': 64 sequences of
+// 16384, bf16, 5.65 TB/s; 1 of 131071 66 us (16-bit pages 109), 32 of up to 12000 101 to 104
+// (154), where the batch's ragged parts leave CUs idle at the end (MI355X, heads of 256).
+//   Rows (prompts) is bound by instructions: a tile of 32 keys on 128 rows takes 1.38 us (16-bit
+// queries, heads of 256; 16-bit pages 1.15), 1024 clocks of it MFMA, and a wave's 270 VALU and 56
+// LDS instructions hardly run beside them; fp32 2.1 (1.97).  777 tokens of 16000 keys: 500 us with
+// each wave unpacking all of V for itself, 484 with each unpacking its own keys for all, 470 with
+// the loads and that under the products (16-bit pages 360).
 #include "attn_device.h"
 #include "gemv_device.h"
 #include "host_state.h"
@@ -396,8 +402,8 @@ __global__ void __launch_bounds__(KEYS && D == 256 ? 128 : 256) attn_q8_kernel(A
     if constexpr (!KEYS) {
         // As in attn_paged.hip: the scores of tile j + 1 beside the weights of tile j, K and V (and with K the scales
         // of both) in rings of R tiles.  V's bytes become f16 in LDS once for the four waves, each of which takes the
-        // keys that it loaded itself, a tile ahead: as each wave would unpack all of a tile for itself it takes 120 more
-        // VALU instructions a tile, and these and the MFMAs of a wave do not run side by side
+        // keys that it loaded itself, a tile ahead: where each wave unpacks all of a tile for itself it
+        // has that many more VALU instructions, and these and the MFMAs of a wave hardly run side by side
         constexpr int R = Z::R, OWN = 32 / Z::NW, PER = 2 * (OWN >= RPI ? OWN / RPI : OWN * Z::RB / 256) + 2;   // keys, and DMA instructions, of a wave a tile
         const std::integral_constant<int, OWN> own_keys;
         const int own = wave * OWN, nt = (k1 - k0 + 31) / 32;
@@ -654,7 +660,8 @@ __global__ void __launch_bounds__(KEYS && D == 256 ? 128 : 256) attn_q8_kernel(A
             return id >= 0 && id < a.n_pages ? id : -1;
         };
         // K of tile t + 2 is asked for when the scores of tile t are made, V when its sums are, so that one to two tiles
-        // are under way: with both asked for at the start of tile t + 1, 32 sequences of up to 12000 keys took 102 us for 90
+        // are under way (4 waves a workgroup: both asked for at the start of tile t + 1 measured the same, 32 sequences of
+        // up to 12000 keys 105 us; two workgroups a CU of 2 waves 101)
         constexpr int HALF = 16 / RPI, NK = 2 * HALF + 4, NV = 2 * HALF;   // DMA instructions of a tile of K, of V
         const std::integral_constant<int, 16> half_tile;
         auto find = [&](int key, bool have, int (&to)[2]) __attribute__((always_inline)) {

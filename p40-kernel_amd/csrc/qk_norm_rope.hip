@@ -16,6 +16,8 @@
 // (Padded rows would leave room for 3 workgroups a CU of 32 x 256, not 4: 30.1
 // us for 26.6, 2048 tokens of 24 + 4 + 4 heads, f16: 101 MB, 3.8 TB/s.)  All of a
 // tile's loads are asked for at once.
+//   Q8 pages: a row's largest magnitude by DPP over the wave that holds it, a byte an element and a scale a row:
+// 2048 tokens from columns, bf16 queries: 29.3 us, 97 MB.
 #include "host_state.h"
 #include "launch_rules.h"
 #include "mixer_device.h"

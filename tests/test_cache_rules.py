@@ -75,3 +75,16 @@ def test_own_keys(rules, n_tok, n_seq, group, n_kv, dim, keys, q8, parts):
 @pytest.mark.parametrize("bytes_,past", [(0, 0), (49 << 20, 0), (64 << 20, 0), ((64 << 20) + 1, 1), (98 << 20, 1), (1 << 40, 1)])
 def test_rows_read_back(rules, bytes_, past):
     assert rules.read_streams(I64(bytes_)) == past
+
+
+def test_the_cache_kernels_keep_to_registers():
+    import kernel_resources as kr
+    if not (os.path.exists(kr.LIB) and os.path.exists(os.path.join(kr.LLVM, "llvm-readelf"))):
+        pytest.skip("needs the built library and ROCm's llvm-readelf")
+    found = {}
+    for r in kr.kernel_resources():
+        found.setdefault(kr.family(r), []).append(r)
+    for f in ("attn_q8_kernel", "attn_kernel", "attn_join_kernel", "kv_read_kernel", "qk_norm_rope_kernel"):
+        assert f in found, f
+        assert all(kr.is_hot_path(r) for r in found[f]), f
+        assert not [r["name"] for r in found[f] if r["scratch"] or r["vgpr_spill"] or r["sgpr_spill"]], f
