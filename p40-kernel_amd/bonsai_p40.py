@@ -521,7 +521,7 @@ def _pages(k_pages, v_pages, dev: int):
     # 8 bits: the scales lie behind the rows of each page, outside the tensor that names these (a slice of its heads
     # would put them elsewhere)
     size = h * p * (d + 4)
-    if n <= 1:
+    if n == 0 or n == 1 and page == h * p * d:             # (views of one page may lose its stride; some of its heads keep all heads')
         page = size + -size % 16
     if page != size + -size % 16 or any(t.storage_offset() + (n - 1) * page + size > t.untyped_storage().nbytes()
                                         for t in (k_pages, v_pages) if n):
@@ -536,9 +536,11 @@ def q8_pages(n_pages: int, n_kv_head: int, page_size: int, head_dim: int, device
     which a page's scales follow its rows."""
     import torch
     rows, scales = n_kv_head * page_size * head_dim, 4 * n_kv_head * page_size
-    memory = torch.zeros((n_pages, rows + scales + -(rows + scales) % 16), dtype=torch.int8, device=device)
-    return (memory[:, :rows].unflatten(1, (n_kv_head, page_size, head_dim)),
-            memory[:, rows:rows + scales].view(torch.float32).unflatten(1, (n_kv_head, page_size)))
+    page = rows + scales + -(rows + scales) % 16
+    memory = torch.zeros((n_pages, page), dtype=torch.int8, device=device)
+    # (strided by hand, so that one page, too, has its stride: it tells all heads from some of them)
+    return (memory.as_strided((n_pages, n_kv_head, page_size, head_dim), (page, page_size * head_dim, head_dim, 1)),
+            memory.view(torch.float32).as_strided((n_pages, n_kv_head, page_size), (page // 4, page_size, 1), rows // 4))
 
 
 def rope_inv_freq(n_rot: int, base: float, device="cuda"):

@@ -186,3 +186,26 @@ def test_wrappers_refuse():
             back(**bad)
     with pytest.raises(ValueError):                       # tensors on the device are wanted
         B.kv_read(q8()[0], q8()[0], z(5, dtype=i64), z(5, 2, 64), z(5, 2, 64))
+
+
+@pytest.mark.parametrize("heads", [slice(0, 2), slice(2, 4), slice(1, 2)])
+def test_wrappers_refuse_the_heads_of_one_page(heads):
+    # the scales lie behind all heads' rows: where these begin does not follow from a slice of the heads
+    k, v = (B.q8_pages(1, 4, 16, 64, device="cpu")[0] for _ in range(2))
+    with pytest.raises(ValueError, match="8-bit pages"):
+        B._pages(k[:, heads], v[:, heads], -1)
+    assert B._pages(k, v, -1) == (1, 4, 16, 64, 16 * 4 * 68, B.Q8)
+
+
+def test_wrappers_take_one_page_of_a_view():
+    memory = torch.zeros(1, 4 * 16 * 68, dtype=i8)
+    k = memory[:, :4 * 16 * 64].unflatten(1, (4, 16, 64))
+    assert B._pages(k, k, -1) == (1, 4, 16, 64, 16 * 4 * 68, B.Q8)
+    with pytest.raises(ValueError, match="8-bit pages"):
+        B._pages(k[:, :2], k[:, :2], -1)
+
+
+def test_wrappers_take_one_page_of_many():
+    k, v = (B.q8_pages(5, 3, 8, 64, device="cpu")[0] for _ in range(2))
+    assert B._pages(k[2:3], v[4:], -1) == (1, 3, 8, 64, 3 * 8 * 68, B.Q8)
+    assert B._pages(k[:0], v[:0], -1)[0] == 0
