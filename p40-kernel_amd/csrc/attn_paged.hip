@@ -758,10 +758,11 @@ int launch(AttnArgs & a, bool first, bool own, hipStream_t s) {
 template <class T, int D, int NT, bool SHARED>
 int launch_k(const AttnLaunch & l, AttnArgs & a, hipStream_t s) {
     int e = 0;
-    if (SHARED && l.keys1 != l.keys)
+    const bool both = SHARED && l.keys1 == l.keys &&
+                      pq2::attn_one_launch((int64_t)a.tiles1 * a.n_split1 * a.n_kv, (int64_t)a.tiles * a.n_split * a.n_kv);
+    if (SHARED && !both)
         e = l.keys1 ? launch<T, D, NT, true, SHARED>(a, true, false, s) : launch<T, D, NT, false, SHARED>(a, true, false, s);
     if (e) return e;
-    const bool both = SHARED && l.keys1 == l.keys;
     e = l.keys ? launch<T, D, NT, true, SHARED>(a, both, true, s) : launch<T, D, NT, false, SHARED>(a, both, true, s);
     if (e || !l.parts) return e;
     typedef typename std::conditional<NT == 1, T, F32>::type TO;

@@ -864,10 +864,11 @@ int launch(AttnArgs & a, bool first, bool own, hipStream_t s) {
 template <class IO, int D, bool SHARED>
 int launch_k(const AttnLaunch & l, AttnArgs & a, hipStream_t s) {
     int e = 0;
-    if (SHARED && l.keys1 != l.keys)
+    const bool both = SHARED && l.keys1 == l.keys &&
+                      pq2::attn_one_launch((int64_t)a.tiles1 * a.n_split1 * a.n_kv, (int64_t)a.tiles * a.n_split * a.n_kv);
+    if (SHARED && !both)
         e = l.keys1 ? launch<IO, D, true, SHARED>(a, true, false, s) : launch<IO, D, false, SHARED>(a, true, false, s);
     if (e) return e;
-    const bool both = SHARED && l.keys1 == l.keys;
     e = l.keys ? launch<IO, D, true, SHARED>(a, both, true, s) : launch<IO, D, false, SHARED>(a, both, true, s);
     return e || !l.parts ? e : launch_join<IO, D, SHARED>(a, l.keys ? Shape<D, true, false>::BM : Shape<D, false, false>::BM, s);
 }

@@ -263,6 +263,8 @@ inline AttnPlan attn_plan(int64_t n_tok, int64_t n_seq, int64_t group, int64_t n
     attn_split(p, want, max_kv, step);
     return p;
 }
+// Whether both phases of shared prefixes, of so many workgroups of 256, are one launch where their kernel is the same
+inline bool attn_one_launch(int64_t first, int64_t own) { return first + own < 1 << 24; }
 // The sequences' own keys behind shared prefixes: mostly few, so that what counts is how often a CU begins with
 // another workgroup (`begin` us), and how many steps (of 32 keys a wave, `step` us) the longest takes.  Measured on MI355X
 // (us of the kernel over the own keys, 24 heads of 256, split as attn_plan does / so): 64 sequences of up to 500, bf16, 3 / 1
@@ -276,7 +278,8 @@ inline AttnPlan attn_own_plan(int64_t n_tok, int64_t n_seq, int64_t group, int64
     const double begin = 7.0, step = 2.0;
     double best = 0.0;
     int64_t want = 1;
-    for (int64_t n = 1; n <= 64; ++n) {
+    // (a batch that fills the card many times over is not split: a grid has fewer than 2^32 threads)
+    for (int64_t n = 1; n <= 64 && (n == 1 || some * n_kv * n <= 1 << 20); ++n) {
         const double us = (double)ceil_div(some * n_kv * n, slots) * (begin + step * (double)ceil_div(ceil_div(max_kv, n), per));
         if (n == 1 || us < best) best = us, want = n;
     }

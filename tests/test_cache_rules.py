@@ -88,3 +88,16 @@ def test_the_cache_kernels_keep_to_registers():
         assert f in found, f
         assert all(kr.is_hot_path(r) for r in found[f]), f
         assert not [r["name"] for r in found[f] if r["scratch"] or r["vgpr_spill"] or r["sgpr_spill"]], f
+
+
+@pytest.mark.parametrize("n_tok,n_seq,group,n_kv,dim,keys,q8", [
+    (131071, 131072, 1, 64, 64, 1224732915, False), (131071, 131072, 1, 64, 128, 742069199, True), (65535, 65536, 2, 64, 64, 542213998, True),
+    (8388607, 8388608, 1, 1, 256, 170, True), (1 << 20, 1 << 20, 8, 1, 256, (1 << 31) - 65536, False)])
+def test_grids_of_the_largest_batches(rules, n_tok, n_seq, group, n_kv, dim, keys, q8):
+    """Workgroups of 256 threads, fewer than 2^32 of these a grid."""
+    _, tiles, _, parts = own(rules, n_tok, n_seq, group, n_kv, dim, keys, q8=q8)
+    _, tiles1, _, parts1 = plan(rules, n_tok, n_seq, group, n_kv, dim, keys, q8=q8, whole=True)
+    first, second = tiles1 * parts1 * n_kv, tiles * parts * n_kv
+    assert 0 < first < 1 << 24 and 0 < second < 1 << 24
+    assert rules.attn_one_launch(I64(first), I64(second)) == (first + second < 1 << 24)
+    assert rules.attn_one_launch(I64(1), I64((1 << 24) - 2)) and not rules.attn_one_launch(I64(1), I64((1 << 24) - 1))
