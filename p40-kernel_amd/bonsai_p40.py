@@ -518,14 +518,19 @@ def _pages(k_pages, v_pages, dev: int):
         raise ValueError("a page has to lie in one piece")
     if _TYPES.get(k_pages.dtype) != "int8":
         return n, h, p, d, page if n > 1 else h * p * d, _type(k_pages)
-    # 8 bits: the scales lie behind the rows of each page, outside the tensor that names these (a slice of its heads
-    # would put them elsewhere)
+    # 8 bits: the scales lie behind the rows of each page, outside the tensor that names these, and a slice of its heads
+    # would put them elsewhere: so each tensor's page stride has to be that of its pages.  A view of one page may have
+    # lost it ([None] makes it the rows' alone); then its memory has to be this one page and no other
     size = h * p * (d + 4)
-    if n == 0 or n == 1 and page == h * p * d:             # (views of one page may lose its stride; some of its heads keep all heads')
-        page = size + -size % 16
-    if page != size + -size % 16 or any(t.storage_offset() + (n - 1) * page + size > t.untyped_storage().nbytes()
-                                        for t in (k_pages, v_pages) if n):
-        raise ValueError("8-bit pages follow each other, each with room for its scales, as q8_pages makes them")
+    page = size + -size % 16
+    for t in (k_pages, v_pages) if n else ():
+        at, there = t.storage_offset(), t.untyped_storage().nbytes()
+        if n == 1 and t.stride(0) == h * p * d:
+            fits = at == 0 and size <= there <= page
+        else:
+            fits = t.stride(0) == page and at + (n - 1) * page + size <= there
+        if not fits:
+            raise ValueError("8-bit pages follow each other, each with room for its scales, as q8_pages makes them")
     return n, h, p, d, page, Q8
 
 

@@ -209,3 +209,27 @@ def test_wrappers_take_one_page_of_many():
     k, v = (B.q8_pages(5, 3, 8, 64, device="cpu")[0] for _ in range(2))
     assert B._pages(k[2:3], v[4:], -1) == (1, 3, 8, 64, 3 * 8 * 68, B.Q8)
     assert B._pages(k[:0], v[:0], -1)[0] == 0
+
+
+def pages8(n, h, page=16, d=64):
+    return B.q8_pages(n, h, page, d, device="cpu")[0]
+
+
+@pytest.mark.parametrize("k,v", [
+    (pages8(1, 2), pages8(1, 4)[:, :2]), (pages8(1, 4)[:, :2], pages8(1, 2)), (pages8(1, 2), pages8(1, 4)[:, 2:]),     # the other has its own page
+    *((x, x) for x in (
+        pages8(1, 4)[0, :2][None], pages8(1, 4)[0, 2:][None], pages8(3, 4)[1, :2][None], pages8(3, 2)[0][None],        # one page's stride is lost
+        pages8(1, 4, 1)[0, 3:][None], torch.zeros(8, 2, 16, 64, dtype=i8)[0:1], torch.zeros(8, 2, 16, 64, dtype=i8)[7:])),   # no scales there
+    (pages8(1, 2), pages8(1, 4)[0, :2][None]), (pages8(1, 2), torch.zeros(8, 2, 16, 64, dtype=i8)[0:1])])
+def test_wrappers_refuse_one_page_whose_scales_are_elsewhere(k, v):
+    with pytest.raises(ValueError, match="8-bit pages"):
+        B._pages(k, v, -1)
+
+
+def test_wrappers_take_one_page_that_is_all_there_is():
+    """Its stride may be lost: memory of one page holds that page's scales."""
+    for shape in ((4, 16, 64), (1, 1, 64), (3, 1, 128)):
+        h, page, d = shape
+        k, v = pages8(1, *shape), pages8(1, *shape)[0][None]
+        want = (1, *shape, h * page * (d + 4) + -(h * page * (d + 4)) % 16, B.Q8)
+        assert B._pages(k, v, -1) == B._pages(v, k, -1) == B._pages(v, v, -1) == want
