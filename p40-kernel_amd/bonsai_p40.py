@@ -475,12 +475,16 @@ GdnArgs = _args_struct("GdnArgs", doc="bonsai_p40_gdn_args of include/bonsai_p40
 _TYPES = {}
 
 
-def _type(t) -> int:
+def _types() -> dict:
     if not _TYPES:
         import torch
         _TYPES.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.int32: "int32",
                        torch.int64: "int64", torch.float64: "float64", torch.int8: "int8"})
-    ty = _TYPES.get(t.dtype)
+    return _TYPES
+
+
+def _type(t) -> int:
+    ty = (_TYPES or _types()).get(t.dtype)
     if ty is None or ty.__class__ is str:
         raise ValueError(f"element type {t.dtype}: fp32, f16 or bf16 is wanted")
     return ty
@@ -516,7 +520,7 @@ def _pages(k_pages, v_pages, dev: int):
     page, head, row, el = st
     if (el != 1 and d != 1) or (row != d and p != 1) or (head != p * d and h != 1):
         raise ValueError("a page has to lie in one piece")
-    if _TYPES.get(k_pages.dtype) != "int8":
+    if (_TYPES or _types()).get(k_pages.dtype) != "int8":
         return n, h, p, d, page if n > 1 else h * p * d, _type(k_pages)
     # 8 bits: the scales lie behind the rows of each page, outside the tensor that names these, and a slice of its heads
     # would put them elsewhere: so each tensor's page stride has to be that of its pages.  A view of one page may have
