@@ -150,10 +150,15 @@ template <bool SHARED, class Args>
 __device__ __forceinline__ int attn_part(Args * a, const AttnPlace & p) {
     return SHARED && !p.pre ? a->n_split1 + p.split : p.split;
 }
+// Of kv keys, how many token tok sees.  (Without SHARED, where its own is one of them, nothing can overflow)
+template <bool SHARED>
+__device__ __forceinline__ int keys_seen(int before, int kv, int tok) {
+    return SHARED ? pq2::attn_seen(before, kv, tok) : iclamp(before + tok + 1, 0, kv);
+}
 struct AttnWork {
     Tile tl;
     int lo;
-    int kv, before, nk, k0, k1;         // keys k0 .. k1 of nk; a row sees those below before + its token + 1
+    int kv, before, nk, k0, k1;         // keys k0 .. k1 of nk; of kv a row sees keys_seen
 };
 // false: there is nothing to do
 template <int BM, bool SHARED>
@@ -168,7 +173,7 @@ __device__ __forceinline__ bool attn_work(const AttnArgs & a, const AttnPlace & 
     w.kv = iclamp(w.tl.extra, 0, a.cap);
     w.before = SHARED && p.pre ? w.kv : w.kv - w.tl.count;     // (pre: every row sees all of them)
     // (readfirstlane: the same in all lanes, which the compiler does not see through the division)
-    w.nk = a.n_pages > 0 ? __builtin_amdgcn_readfirstlane(iclamp(w.before + last / a.group + 1, 0, w.kv)) : 0;
+    w.nk = a.n_pages > 0 ? __builtin_amdgcn_readfirstlane(keys_seen<SHARED>(w.before, w.kv, last / a.group)) : 0;
     if (SHARED) {
         // (64 bits: where the host knows no lengths, the last part may begin anywhere)
         const int chunk = p.pre ? a.chunk1 : a.chunk, n_split = p.pre ? a.n_split1 : a.n_split;

@@ -131,14 +131,14 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
     const int r = wrow + n;
     const bool live = r < rows;
     const int tok = live ? r / a.group : 0, head = kvh * a.group + (live ? r - tok * a.group : 0);
-    const int vis = live ? iclamp(before + tok + 1, 0, kv) : 0;
+    const int vis = live ? keys_seen<SHARED>(before, kv, tok) : 0;
     const int64_t grow = (int64_t)(tl.first + tok);
     // the fewest keys any live row of the wave sees; 0 rows: nothing to do but stage
     const bool work = wrow < rows;
-    const int least = work ? __builtin_amdgcn_readfirstlane(iclamp(before + wrow / a.group + 1, 0, kv)) : 0;
+    const int least = work ? __builtin_amdgcn_readfirstlane(keys_seen<SHARED>(before, kv, wrow / a.group)) : 0;
 
     // the keys that all rows of the workgroup see
-    const int first_vis = __builtin_amdgcn_readfirstlane(iclamp(before + row0 / a.group + 1, 0, kv));
+    const int first_vis = __builtin_amdgcn_readfirstlane(keys_seen<SHARED>(before, kv, row0 / a.group));
 
     // Q^T, element j of half h: d = 16 step + 8 h + j (a lane without a row: the tile's first).  fp32 queries
     // are asked for here, and made into terms when the first tiles are on their way

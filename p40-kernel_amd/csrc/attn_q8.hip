@@ -124,12 +124,12 @@ __global__ void __launch_bounds__(KEYS && D == 256 ? 128 : 256) attn_q8_kernel(A
     const int r = wrow + n;
     const bool live = r < rows;
     const int tok = live ? r / a.group : 0, head = kvh * a.group + (live ? r - tok * a.group : 0);
-    const int vis = live ? iclamp(before + tok + 1, 0, kv) : 0;
+    const int vis = live ? keys_seen<SHARED>(before, kv, tok) : 0;
     const int64_t grow = (int64_t)(tl.first + tok);
     // the fewest keys any live row of the wave sees, and any of the workgroup; 0 rows: nothing to do but stage
     const bool work = wrow < rows;
-    const int least = work ? __builtin_amdgcn_readfirstlane(iclamp(before + wrow / a.group + 1, 0, kv)) : 0;
-    const int first_vis = __builtin_amdgcn_readfirstlane(iclamp(before + row0 / a.group + 1, 0, kv));
+    const int least = work ? __builtin_amdgcn_readfirstlane(keys_seen<SHARED>(before, kv, wrow / a.group)) : 0;
+    const int first_vis = __builtin_amdgcn_readfirstlane(keys_seen<SHARED>(before, kv, row0 / a.group));
 
     // Q^T, byte j of half h: d = 32 step + 16 h + j (a lane without a row: the tile's first), asked for here and
     // made into digits when the first tiles are on their way

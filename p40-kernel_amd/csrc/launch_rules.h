@@ -263,6 +263,12 @@ inline AttnPlan attn_plan(int64_t n_tok, int64_t n_seq, int64_t group, int64_t n
     attn_split(p, want, max_kv, step);
     return p;
 }
+// Of kv keys, how many token `tok` sees: its own is key before + tok.  The shared keys of a group, which all of its tokens
+// see, have before = kv, which no token's place is added to: kv may be 2^31 - 65536, and the tokens more than what is left.
+constexpr int attn_seen(int before, int kv, int tok) {
+    const int x = before + (tok + 1 < kv - before ? tok + 1 : kv - before);
+    return x < 0 ? 0 : x;
+}
 // Whether both phases of shared prefixes, of so many workgroups of 256, are one launch where their kernel is the same
 inline bool attn_one_launch(int64_t first, int64_t own) { return first + own < 1 << 24; }
 // The sequences' own keys behind shared prefixes: mostly few, so that what counts is how often a CU begins with

@@ -17,6 +17,7 @@ void attn_own_plan(int64_t n_tok, int64_t n_seq, int64_t group, int64_t n_kv, in
                    int bytes, int64_t * out) {
     put(pq2::attn_own_plan(n_tok, n_seq, group, n_kv, dim, max_kv, rows, cus, bytes != 0), out);
 }
+int attn_seen(int before, int kv, int tok) { return pq2::attn_seen(before, kv, tok); }
 int attn_one_launch(int64_t first, int64_t own) { return pq2::attn_one_launch(first, own); }
 int read_streams(int64_t bytes) { return pq2::read_streams(bytes); }
 }

@@ -101,3 +101,16 @@ def test_grids_of_the_largest_batches(rules, n_tok, n_seq, group, n_kv, dim, key
     assert 0 < first < 1 << 24 and 0 < second < 1 << 24
     assert rules.attn_one_launch(I64(first), I64(second)) == (first + second < 1 << 24)
     assert rules.attn_one_launch(I64(1), I64((1 << 24) - 2)) and not rules.attn_one_launch(I64(1), I64((1 << 24) - 1))
+
+
+def test_keys_a_token_sees(rules):
+    """Own keys: token t of n sees those up to its own, none where there are fewer keys than tokens behind it; shared
+    ones: every token all of them.  At lengths up to the longest there is, with the most tokens."""
+    rng = random.Random(3)
+    longest, most = (1 << 31) - 65536, (1 << 24) - 1
+    for kv in (0, 1, 2, 31, 40, 4000, 70000, longest - most - 1, longest - 65535, longest - 1, longest):
+        for n in (1, 2, 5, 33, 65535, 65536, 70000, most):
+            for t in {0, 1, n // 2, n - 2, n - 1, rng.randrange(n)}:
+                if 0 <= t < n:
+                    assert rules.attn_seen(kv - n, kv, t) == max(kv - n + t + 1, 0), (kv, n, t)
+                    assert rules.attn_seen(kv, kv, t) == kv, (kv, n, t)
