@@ -15,9 +15,12 @@
 // n as f16 bits) and two packed additions make 4 of them.  w is rounded to f16 once (16-bit
 // output; error as in attn_paged.hip), or is two terms of f16 whose second has sums of its
 // own (fp32).
-//   f16's range is short for p_j d_j.  So what m follows is a tile's largest score and the log2
-// of its largest d together: p is relative to that, which leaves w at most 2^15, and a key
-// whose p d is 2^-25 of its row's largest has all of f16's digits.  l and O have the same m.
+//   f16's range is short for p_j d_j.  So the weights are relative to what follows a tile's largest
+// score and the log2 of its largest d together, which leaves w at most 2^15, and a key
+// whose p d is 2^-25 of its row's largest has all of f16's digits.  That says nothing of l, in which a
+// key counts whatever its d: with 32 keys of d = 0 before 32 of d = 2^30 and equal scores, sums that shared that
+// reference lost the first ones.  So l has a reference 2^m of its own, the scores', and O's is 2^(m + g): 2^g takes a
+// tile's sum of weights over to l, and at the end O to m.
 //   No value of V is NaN or infinite by itself, so a key that is not seen needs no
 // zeroed row: its weight is 0 and its d counts as 0.
 //   Keys (decode) is bound by the stream of the pages, half of 16-bit ones': 64 sequences of
@@ -355,15 +358,22 @@ __global__ void __launch_bounds__(KEYS && D == 256 ? 128 : 256) attn_q8_kernel(A
     };
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[d] = v16f{};
-    // limit, ref, FAR and LEAST as in attn_paged.hip, where m follows the scores; here it follows a tile's largest score
-    // and the log2 of its largest d together (b), so that p d, which becomes f16, is up to 2^(UP + LAG); o and l are both
-    // relative to it.  A d below 2^-100 counts as that here, as l has to stay finite
-    constexpr float UP = 11.0f, LAG = 4.0f, LEAST = -3e38f, FAR = 1048576.0f, LOW_UP = 2048.0f;
-    float m = -INFINITY, l = 0.0f, limit = -INFINITY, ref = 0.0f;
-    auto follow = [&](v16f & s, float b) __attribute__((always_inline)) {
-        if (__any(b > limit)) {
-            const bool near = fabsf(fmaxf(m, b)) < FAR;
-            const float m2 = fmaxf(m, near ? b - UP : b), base = m2 == -INFINITY ? 0.0f : m2;
+    // limit, ref, FAR and LEAST as in attn_paged.hip, where m follows the scores.  Here l is relative to 2^m, m the largest
+    // score, whole, less a lag of up to LAG_L; O, and the weights that are made for it, to 2^(m + g), m + g following a tile's
+    // largest score and the log2 of its largest d together, so that p d, which becomes f16, is up to 2^(UP + LAG), and 2^UP for
+    // a key that has both (one of nearly all the weight is not rounded then).  g is in steps of 2^-16: m + g, and what these
+    // change by, are exact where scores are below 128 (log2), and 2^g takes a tile's sum of weights over to l.  A d below 2^-100
+    // counts as that: a weight is 2^115 at most, so that 16 of them add up, and with d up to 2^80 the smallest that fp32
+    // holds is 2^-57 of its row's largest; l is below 2^40, O at its end below 2^127, for 2^31 keys
+    constexpr float UP = 11.0f, LAG = 4.0f, LAG_L = 8.0f, LEAST = -3e38f, FAR = 1048576.0f, LOW_UP = 2048.0f;
+    float m = -INFINITY, l = 0.0f, limit = -INFINITY, ref = 0.0f, g = 0.0f;
+    // mx, lv: a tile's largest score, log2 of its largest d
+    auto follow = [&](v16f & s, float mx, float lv) __attribute__((always_inline)) {
+        if (__any(mx + lv > limit || mx - m > LAG_L)) {
+            const float m2 = fmaxf(m, floorf(mx));
+            const bool none = m2 == -INFINITY, near = fabsf(m2) < FAR;
+            const float base = none ? 0.0f : m2, fall = none ? 0.0f : m - base;
+            float g2 = fmaxf(g + fall, rintf((mx - base + lv) * 65536.0f) * (1.0f / 65536.0f) - UP);
             if (!near) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -372,11 +382,13 @@ __global__ void __launch_bounds__(KEYS && D == 256 ? 128 : 256) attn_q8_kernel(A
                     s[i] = (x - base) / c;
                 }
             }
-            limit = near ? m2 + (UP + LAG) : -INFINITY;
-            ref = near ? m2 : 0.0f;
-            const float alpha = __builtin_amdgcn_exp2f(m - base);
+            ref = near ? m2 + g2 : g2;
+            limit = near ? ref + (UP + LAG) : -INFINITY;
+            if (near) g2 = ref - m2;                       // (as that was rounded)
+            const float alpha = __builtin_amdgcn_exp2f(g + fall - g2);
             m = m2;
-            l *= alpha;
+            g = g2;
+            l *= __builtin_amdgcn_exp2f(fall);
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -448,9 +460,14 @@ __global__ void __launch_bounds__(KEYS && D == 256 ? 128 : 256) attn_q8_kernel(A
         // this wave's keys of a tile of V, a unit of 16 bytes a lane and step, to f16
         constexpr int UNITS = OWN * U, WS = UNITS < 64 ? 1 : UNITS / 64;
         const bool widens = UNITS >= 64 || lane < UNITS;
-        uint32_t wat[WS];
+        // (fp32 rows of 256: the address of unit lane + 64, which is 4 keys on, where the swizzle differs in one bit, is made
+        // from that of unit lane each time, as registers go: 777 tokens of 16000 keys up to 2 % faster than with two addresses.
+        // 16-bit rows have the registers: 478 us, 487 with one)
+        constexpr int WA = Z::QL && WIDE ? 1 : WS;
+        static_assert(WA == WS || (WS == 2 && U == 16), "");
+        uint32_t wat[WA];
 #pragma unroll
-        for (int i = 0; i < WS; ++i) {
+        for (int i = 0; i < WA; ++i) {
             const int unit = lane + 64 * i, key = own + unit / U;
             wat[i] = key * 2 * Z::RB + 16 * ((2 * (unit % U)) ^ swz_w(key));
         }
@@ -460,7 +477,8 @@ __global__ void __launch_bounds__(KEYS && D == 256 ? 128 : 256) attn_q8_kernel(A
         // half h of unit i
         auto widen = [&](v4u x, uint8_t * to, int i, int h) __attribute__((always_inline)) {
             const v8h w = unpack((v2u){x[2 * h], x[2 * h + 1]});
-            if (widens) *reinterpret_cast<v8h *>(to + (wat[i] ^ (16 * h))) = w;
+            const uint32_t at = i < WA ? wat[i < WA ? i : 0] ^ (16 * h) : (wat[0] ^ (16 * h + 256)) + 8 * Z::RB;
+            if (widens) *reinterpret_cast<v8h *>(to + at) = w;
         };
         // V in f16: keys 16 g + 4 half + j % 4 + 8 (j / 4) of d = 32 d + lane % 32
         const int wkey = 4 * half + (l16 >> 2), wcol = 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1);
@@ -515,7 +533,7 @@ __global__ void __launch_bounds__(KEYS && D == 256 ? 128 : 256) attn_q8_kernel(A
                 lv = log_scale(vs);
                 if (sees(key, holes)) mx = fmaxf(mx, LEAST);
             }
-            follow(s, mx + lv);
+            follow(s, mx, lv);
             constexpr int E = 16 / STEPS;
             float sum[2] = {0.0f, 0.0f};
             v8h vf[VA], pf[NP][2];
@@ -551,7 +569,7 @@ __global__ void __launch_bounds__(KEYS && D == 256 ? 128 : 256) attn_q8_kernel(A
                 if (i == STEPS / 2 && (steady || j + R < nt)) stage_v(j + R, vw, vsw);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            l += sum[0] + sum[1];
+            l = fmaf(sum[0] + sum[1], __builtin_amdgcn_exp2f(g), l);
 #pragma unroll
             for (int i = 0; i < KQ; ++i) ks[i] = scales4(ksr, i);
             scales(vsr, vs);
@@ -723,12 +741,12 @@ __global__ void __launch_bounds__(KEYS && D == 256 ? 128 : 256) attn_q8_kernel(A
             } else {
                 mx = fmaxf(largest(s), LEAST);
             }
-            follow(s, mx + log_scale(vs));
+            follow(s, mx, log_scale(vs));
             v8h pf[NP][2];
             float sum[2] = {0.0f, 0.0f};
 #pragma unroll
             for (int e = 0; e < 16; ++e) weight(s[e], vs[e], pf, e, sum[e & 1]);
-            l += sum[0] + sum[1];
+            l = fmaf(sum[0] + sum[1], __builtin_amdgcn_exp2f(g), l);
             asm volatile("" : "+v"(l));                    // (here, not behind the product, up to which 16 weights would be kept)
             // behind V: K and V of the next tile, K of the one after
             if (more) pq2::wait_vmcnt<2 * NK + NV>();
@@ -778,6 +796,13 @@ __global__ void __launch_bounds__(KEYS && D == 256 ? 128 : 256) attn_q8_kernel(A
         }
     }
     l += __shfl_xor(l, 32);
+    {
+        const float gain = __builtin_amdgcn_exp2f(g);      // O relative to 2^m, too
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] *= gain;
+    }
 
     // (arguments that only this end of the kernel needs, read again rather than held all along)
     LateArgs * const z = late_args();
