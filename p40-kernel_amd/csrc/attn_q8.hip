@@ -80,7 +80,7 @@ struct Shape {
     static constexpr int SC = (KEYS ? 2 : NW) * 256;       // of its scales: 256 for the keys of one DMA instruction
     static constexpr int R = 4;                            // rows: tiles of K, and of V, in LDS
     static constexpr int OROW = D + 4;                     // floats of a row in the join
-    static constexpr int JOIN = NW * 32 * OROW * 4 + NW * 32 * 8;
+    static constexpr int JOIN = NW * 32 * OROW * 4 + NW * 32 * 12;
     static constexpr int SLOTS = KEYS ? NW * 4 : 2 * R;    // keys: two buffers of K and V a wave
     // heads of 256: the registers hold the other digits of q, the lowest is in LDS (keys: the waves' is the same, and
     // all write it)
@@ -796,13 +796,12 @@ __global__ void __launch_bounds__(KEYS && D == 256 ? 128 : 256) attn_q8_kernel(A
         }
     }
     l += __shfl_xor(l, 32);
-    {
-        const float gain = __builtin_amdgcn_exp2f(g);      // O relative to 2^m, too
+    const float gain = __builtin_amdgcn_exp2f(g);          // takes O over to 2^m (keys: where the waves are joined)
+    if (!KEYS)
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[d][i] *= gain;
-    }
 
     // (arguments that only this end of the kernel needs, read again rather than held all along)
     LateArgs * const z = late_args();
@@ -820,11 +819,11 @@ __global__ void __launch_bounds__(KEYS && D == 256 ? 128 : 256) attn_q8_kernel(A
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
+            for (int q = 0; q < 4; ++q) {
                 float x[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) x[j] = o[d][4 * g + j] * f;
-                const int at = 32 * d + 8 * g + 4 * half;
+                for (int j = 0; j < 4; ++j) x[j] = o[d][4 * q + j] * f;
+                const int at = 32 * d + 8 * q + 4 * half;
                 if (parts) store_row<F32>(po + at, x);
                 else store_row<IO>(reinterpret_cast<elem *>(z->out) + grow * z->out_tok + (int64_t)head * D + at, x);
             }
@@ -832,20 +831,24 @@ __global__ void __launch_bounds__(KEYS && D == 256 ? 128 : 256) attn_q8_kernel(A
             *reinterpret_cast<float2 *>(pml + 2 * ((int64_t)part * all_rows + row)) =
                 make_float2(m, l);
     } else {
-        // join the waves: [wave][row][D] and [wave][row] (m, l)
+        // join the waves: [wave][row][D], [wave][row] (m, l) and [wave][row] 2^g
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         float * const jo = reinterpret_cast<float *>(lds);
         float2 * const ml = reinterpret_cast<float2 *>(lds + Z::NW * 32 * Z::OROW * 4);
+        float * const gains = reinterpret_cast<float *>(ml + Z::NW * 32);
         if (live) {
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
-                for (int g = 0; g < 4; ++g)
-                    *reinterpret_cast<v4f *>(jo + (wave * 32 + n) * Z::OROW + 32 * d + 8 * g + 4 * half) =
-                        (v4f){o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
-            if (half == 0) ml[wave * 32 + n] = make_float2(m, l);
+                for (int q = 0; q < 4; ++q)
+                    *reinterpret_cast<v4f *>(jo + (wave * 32 + n) * Z::OROW + 32 * d + 8 * q + 4 * half) =
+                        (v4f){o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]};
+            if (half == 0) {
+                ml[wave * 32 + n] = make_float2(m, l);
+                gains[wave * 32 + n] = gain;
+            }
         }
         __syncthreads();
         constexpr int E = D / 64;
@@ -858,10 +861,10 @@ __global__ void __launch_bounds__(KEYS && D == 256 ? 128 : 256) attn_q8_kernel(A
 #pragma unroll
             for (int k = 0; k < Z::NW; ++k) {
                 const float2 e = ml[k * 32 + i];
-                const float wt = __builtin_amdgcn_exp2f(e.x - to);
+                const float wt = __builtin_amdgcn_exp2f(e.x - to), wo = wt * gains[k * 32 + i];
                 ll = fmaf(e.y, wt, ll);
 #pragma unroll
-                for (int j = 0; j < E; ++j) x[j] = fmaf(jo[(k * 32 + i) * Z::OROW + lane * E + j], wt, x[j]);
+                for (int j = 0; j < E; ++j) x[j] = fmaf(jo[(k * 32 + i) * Z::OROW + lane * E + j], wo, x[j]);
             }
             const int rr = row0 + i, t = rr / z->group, h = kvh * z->group + rr - t * z->group;
             const int64_t g = tl.first + t, row = g * z->n_head + h;
