@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(D == 256 && (KEYS || NT == 3) ? 128 : 256) att
                 const int e = (int)((__builtin_bit_cast(uint32_t, big) >> 23) & 255);
                 if (e > 14 && e < 255) {
                     up = __builtin_bit_cast(float, (uint32_t)(268 - e) << 23);
-                    c *= __builtin_bit_cast(float, (uint32_t)(e - 14) << 23);
+                    c = fmaxf(c * __builtin_bit_cast(float, (uint32_t)(e - 14) << 23), 0x1p-149f);   // (0 times -inf is none)
                 }
             }
 #pragma unroll

@@ -186,7 +186,8 @@ __global__ void __launch_bounds__(KEYS && D == 256 ? 128 : 256) attn_q8_kernel(A
         constexpr int TOP = NT == 3 ? 22 : 14;
         const int e = max((int)(big >> 23), TOP + 1);
         const float up = __builtin_bit_cast(float, (uint32_t)(254 + TOP - min(e, 254)) << 23) * (127.0f / 128.0f);
-        c = big >= 0x7f800000u ? NAN : c * __builtin_bit_cast(float, (uint32_t)(min(e, 254) - TOP) << 23) * (128.0f / 127.0f);
+        // (the factor of a row next to 0 may come out as 0, which times a score of -inf is none)
+        c = big >= 0x7f800000u ? NAN : fmaxf(c * __builtin_bit_cast(float, (uint32_t)(min(e, 254) - TOP) << 23) * (128.0f / 127.0f), 0x1p-148f);
 #pragma unroll
         for (int s = 0; s < QS; ++s)
 #pragma unroll

@@ -5,7 +5,7 @@ Reference: 64 bits; U = 2^-24 is a rounding of fp32."""
 import pytest
 
 import bonsai_p40 as B
-from test_gpu_mixers import BF16, F16, F32, U, case, gen, half_step, ints, normwise
+from test_gpu_mixers import BF16, F16, F32, NAN, U, case, gen, half_step, ints, normwise
 from test_gpu_q8_cache import pages_of
 
 torch = pytest.importorskip("torch")
@@ -31,23 +31,24 @@ def paged(codes, scales, page):
     return pages_of(pc, ps)[0], perm.int()
 
 
-def check(got, ref, mag, top, io, keys, split):
+def check(got, ref, mag, top, io, keys, split, least=0.0):
     """q is whole.  A score of up to top is rounded 16 times (and its query's one element is off by 1.01 x 2^-15 or 1.6 x
     2^-23 of itself, as the header has it); a weight is rounded once to f16 (fp32: to 22 bits), or is off by 2^-36
     (2^-47) of the largest.  The sums over keys add a rounding a tile of 32, each U of a sum that is at most the whole:
-    keys / 32 U in one part, where all may go the same way as the terms are alike."""
+    keys / 32 U in one part, where all may go the same way as the terms are alike.  least: more that a weight may be off
+    by, of the largest, so that a sum of n of them is by that times n values."""
     assert torch.equal(torch.isfinite(got.double()), torch.isfinite(ref))
     e, p, tiny = (1.6 * 2.0 ** -23, 2.0 ** -22, 2.0 ** -47) if io == F32 else (1.01 * 2.0 ** -15, 2.0 ** -11, 2.0 ** -36)
     sums = (keys / 32 + 24) * U
-    lim = mag * (2 * (e + 16 * U) * top + p + 2 * sums) + keys * tiny * mag.amax(-1, keepdim=True) * 4
+    lim = mag * (2 * (e + 16 * U) * top + p + 2 * sums) + keys * max(tiny, least) * mag.amax(-1, keepdim=True) * 4
     lim = lim + half_step(io) * (ref.abs() + lim) + torch.finfo(io).tiny
     err = (got.double() - ref).abs()
     assert bool((err <= lim).all()), float((err - lim).max())
     rel = normwise(got, ref)
-    assert rel <= (half_step(io) if io != F32 else 2.0 ** -18) + (0.0 if split else sums), rel
+    assert rel <= (half_step(io) if io != F32 else 2.0 ** -18) + (0.0 if split else sums) + least * keys ** 0.5, rel
 
 
-def attend(n, heads, d, score, vd, io, work, what, scale=1.0, seed=0, groups=None):
+def attend(n, heads, d, score, vd, io, work, what, scale=1.0, seed=0, groups=None, tiny=0.0):
     """The last n tokens of one sequence whose key j has the score score[j] and values of scale vd[j]; groups: the keys
     that are the prefix of n sequences of one token each, of which the first has all the others."""
     kv = score.numel()
@@ -80,7 +81,7 @@ def attend(n, heads, d, score, vd, io, work, what, scale=1.0, seed=0, groups=Non
     p = torch.softmax(x.masked_fill(late, -INF), -1)
     v = vc[:, 0].double() * vs.double()
     ref, mag = p @ v, p @ v.abs()
-    check(out.cpu(), ref[:, None].expand(n, heads, d), mag[:, None].expand(n, heads, d), float(x.abs().max()), io, kv, work)
+    check(out.cpu(), ref[:, None].expand(n, heads, d), mag[:, None].expand(n, heads, d), float(x.abs().max()), io, kv, work, tiny)
 
 
 LOG2 = 0.6931471805599453
@@ -169,3 +170,29 @@ def test_scales_far_apart_in_16_bits(d):
             # f16 holds the results of scales up to 2^8
             attend(n, 2, d, torch.randn(kv, generator=gen(kv)), 2.0 ** torch.linspace(-20, 8, kv), F16, True, "2^-20 .. 2^8")
             attend(n, 2, d, torch.randn(kv, generator=gen(kv)), 2.0 ** torch.linspace(8, -20, kv), F16, True, "2^8 .. 2^-20")
+
+
+@pytest.mark.parametrize("kind", ["q8", F16, BF16])
+@pytest.mark.parametrize("value", [0.0, 2.0 ** -112, 2.0 ** -140])
+def test_scores_whose_factor_is_next_to_nothing(kind, value):
+    """Queries of (next to) nothing and a scale of 1e-9 or less: every score is 0, and each token's result the mean of
+    the values it sees."""
+    d, kv = 64, 100
+    g = gen(3)
+    codes = torch.randint(-127, 128, (kv, 1, d), generator=g, dtype=torch.int8)
+    one = torch.full((kv, 1), 2.0 ** -6)
+    if kind == "q8":
+        (kp, perm), (vp, _) = paged(codes, one, 16), paged(codes.flip(0), one, 16)
+    else:
+        perm = torch.arange(7, dtype=torch.int32)
+        kp, vp = ((torch.cat([x, torch.zeros(12, 1, d)]).view(7, 16, 1, d).transpose(1, 2) * 2.0 ** -6).to(kind).cuda() for x in (codes, codes.flip(0)))
+    v = codes.flip(0)[:, 0].double() * 2.0 ** -6
+    for n in (1, 40):
+        for scale in (1e-9, 1e-30, 1e-45):
+            case(f"tiny scores {kind} value={value} n={n} scale={scale}")
+            out = torch.zeros(n, 2, d, device="cuda")
+            B.attn_paged(torch.full((n, 2, d), value, device="cuda"), kp, vp, perm.cuda()[None], ints([0, n]), ints([kv]), out, scale=scale)
+            torch.cuda.synchronize()
+            ref = torch.stack([v[:kv - n + t + 1].mean(0) for t in range(n)])[:, None].expand(n, 2, d)
+            # weights of 22 bits or more, alike; sums of 100 terms
+            assert bool(((out.cpu().double() - ref).abs() <= (2.0 ** -21 + 16 * U) * v.abs().max()).all()), (n, scale)
