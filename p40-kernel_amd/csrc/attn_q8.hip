@@ -155,6 +155,9 @@ __global__ void __launch_bounds__(KEYS && D == 256 ? 128 : 256) attn_q8_kernel(A
     v4i qf[NT][QS];
     uint8_t * const ql = lds + Z::SCALED + (KEYS ? 0 : wave * Z::QT) + 16 * lane;
     float c = a.c;
+    // the factor of a row with a value that is not finite, which no other has: its sums mean nothing, and are NaN at the end
+    // where it has seen a key
+    constexpr float NOT_FINITE = 0x1p-149f;
     auto make_q = [&]() __attribute__((always_inline)) {
         // the largest magnitude's bits: they compare as the magnitudes do, and NaN is above infinity
         uint32_t big = 0;
@@ -187,7 +190,7 @@ __global__ void __launch_bounds__(KEYS && D == 256 ? 128 : 256) attn_q8_kernel(A
         const int e = max((int)(big >> 23), TOP + 1);
         const float up = __builtin_bit_cast(float, (uint32_t)(254 + TOP - min(e, 254)) << 23) * (127.0f / 128.0f);
         // (the factor of a row next to 0 may come out as 0, which times a score of -inf is none)
-        c = big >= 0x7f800000u ? NAN : fmaxf(c * __builtin_bit_cast(float, (uint32_t)(min(e, 254) - TOP) << 23) * (128.0f / 127.0f), 0x1p-148f);
+        c = big >= 0x7f800000u ? NOT_FINITE : fmaxf(c * __builtin_bit_cast(float, (uint32_t)(min(e, 254) - TOP) << 23) * (128.0f / 127.0f), 0x1p-148f);
 #pragma unroll
         for (int s = 0; s < QS; ++s)
 #pragma unroll
@@ -796,6 +799,7 @@ __global__ void __launch_bounds__(KEYS && D == 256 ? 128 : 256) attn_q8_kernel(A
             }
         }
     }
+    if (c == NOT_FINITE && m > -INFINITY) l = NAN;
     l += __shfl_xor(l, 32);
     const float gain = __builtin_amdgcn_exp2f(g);          // takes O over to 2^m (keys: where the waves are joined)
     if (!KEYS)

@@ -196,3 +196,27 @@ def test_scores_whose_factor_is_next_to_nothing(kind, value):
             ref = torch.stack([v[:kv - n + t + 1].mean(0) for t in range(n)])[:, None].expand(n, 2, d)
             # weights of 22 bits or more, alike; sums of 100 terms
             assert bool(((out.cpu().double() - ref).abs() <= (2.0 ** -21 + 16 * U) * v.abs().max()).all()), (n, scale)
+
+
+@pytest.mark.parametrize("io", [BF16, F16, F32])
+@pytest.mark.parametrize("d", [64, 256])
+def test_queries_of_nan_that_see_no_key(io, d):
+    """0, as of any query without keys: whole sequences, a chunk's first tokens beside others that see some, pages that
+    are none; those that see a key are NaN."""
+    case(f"q8 ranges queries of NaN without keys io={io} d={d}")
+    pages = pages_of(torch.ones(9, 1, 16, d, dtype=torch.int8), torch.ones(9, 1, 16))[0]
+    for starts, lens, table, seen in (
+            ([0, 1, 2], [0, 5], [[0, 1, 2], [3, 4, 5]], [0, 1]),
+            ([0, 40, 41], [3, 0], [[0, 1, 2], [3, 4, 5]], [0] * 37 + [1] * 3 + [0]),
+            ([0, 70, 75], [48, 2], [[-1, -1, 7], [-1, 9, 8]], [0] * 54 + [1] * 16 + [0] * 5),
+            ([0, 1, 2], [300, 300], [[-1] * 19, [-1] * 9 + [3] + [-1] * 9], [0, 1])):
+        n = starts[-1]
+        q = torch.full((n, 2, d), NAN, dtype=io)
+        out = torch.full((n, 2, d), 7.0, dtype=io, device="cuda")
+        for work in (True, False):
+            args = [q.cuda(), pages, pages, ints(table), ints(starts), ints(lens), out.fill_(7.0)]
+            ws = torch.full((B.attn_paged_workspace_bytes(*args) + 16,), 255, dtype=torch.uint8, device="cuda") if work else None
+            B.attn_paged(*args, ws)
+            torch.cuda.synchronize()
+            some = torch.tensor(seen, dtype=torch.bool)
+            assert bool(out.cpu()[some].isnan().all()) and bool((out.cpu()[~some] == 0).all()), (starts, lens, work)
