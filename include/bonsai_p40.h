@@ -403,8 +403,9 @@ int bonsai_p40_chain_run(const void * plan, int n_steps, void * workspace, uint3
 // A row x is written as d = max |x| / 127, n = x * (127 / max |x|) rounded to the nearest
 // whole number, ties to even, in fp32: d * n is off by 0.50002 d at most.  A row whose
 // largest magnitude is below 2^-112 is written as 0, and one that holds a value that is
-// not finite with d = NaN, so that all of it is.  What is read may hold any n in -128 .. 127;
-// keys and values that attention sees are to have |d| of 0 or 2^-100 to 2^80.
+// not finite with d = NaN, so that all of it is (one that holds the largest fp32 number reads back as
+// infinity there: 127 d is beyond it).  What is read may hold any n in -128 .. 127; keys and
+// values that attention sees are to have |d| of 2^80 at most, as rows up to 2^87 have.
 
 // RMSNorm of every query and key head, position rotation, and the append of
 // keys and values to the pages, in one launch:
@@ -471,7 +472,8 @@ int bonsai_p40_qk_norm_rope(const bonsai_p40_qk_norm_rope_args * args, bonsai_st
 //   Q8 pages: a row of q is taken as whole numbers, an element off by at most 1.01 x 2^-15
 // (fp32: 1.6 x 2^-23) of its largest one; a row with a value that is not finite gives NaN.  A weight times its value's
 // d is rounded once to f16 (fp32: to 22 bits); one below 2^-25 of the row's largest such
-// product, taken tile by tile of 32 keys, is off by up to 2^-36 (2^-47) of that.
+// product, taken tile by tile of 32 keys, is off by up to 2^-36 (2^-47) of that, and any by 2^-136 / D
+// (2^-147 / D) of it where the largest d that the row sees, D, is below 2^-100.
 // max_kv: about the largest kv_len (0: unknown); it places the work, results hold for
 // any.  workspace: bonsai_p40_attn_paged_workspace_bytes bytes (of the same
 // args), 16-byte aligned, scratch for the call (stream-ordered; calls that may

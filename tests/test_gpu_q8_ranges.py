@@ -220,3 +220,14 @@ def test_queries_of_nan_that_see_no_key(io, d):
             torch.cuda.synchronize()
             some = torch.tensor(seen, dtype=torch.bool)
             assert bool(out.cpu()[some].isnan().all()) and bool((out.cpu()[~some] == 0).all()), (starts, lens, work)
+
+
+@pytest.mark.parametrize("n,heads,d", SHAPES)
+def test_values_as_small_as_the_append_writes(n, heads, d):
+    """Scales of 2^-119, those of rows of 2^-112, alone and beside others: a weight is off by up to 2^-17 (fp32 rows
+    2^-28) of the largest where all that a row sees are below 2^-100."""
+    score = torch.randn(200, generator=gen(n))
+    for low, high in ((-119, -119), (-119, -101), (-119, 0)):
+        vd = 2.0 ** torch.round(low + (high - low) * torch.rand(200, generator=gen(1)))
+        for io in (BF16, F32):
+            attend(n, heads, d, score, vd, io, True, f"2^{low} .. 2^{high}", tiny=2.0 ** (-28 if io == F32 else -17) if high < -100 else 0.0)
