@@ -522,8 +522,10 @@ int64_t bonsai_p40_attn_paged_workspace_bytes(const bonsai_p40_attn_paged_args *
 // except that the 16 keys that hold key shared[g] are.
 // groups, which does not fall (sequences that two groups claim are undefined), is cut to
 // 0 .. n_seq; a sequence of no group sees its own keys, from 0 on.  max_shared: about the largest of
-// shared (0: unknown); as max_kv it places the work.  groups and shared are device memory, as
-// the other lengths are.
+// shared (0: unknown); as max_kv it places the work: that of the own keys for max_kv - max_shared of
+// them, or max_kv where max_shared is 0.  Where a sequence has more, as it is of no group or behind a short prefix, give
+// max_shared and the most own keys together as max_kv, though no sequence be so long.  groups and
+// shared are device memory, as the other lengths are.
 // The workspace (attn.workspace, bonsai_p40_attn_shared_workspace_bytes bytes) is
 // needed: the sums of the shared keys and of the own ones meet there.
 // Errors: 1 as attn_paged, and if n_group or max_shared is negative, groups, shared or the

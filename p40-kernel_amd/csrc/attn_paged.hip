@@ -882,10 +882,11 @@ struct SharedPlan {
     Plan first, own;
 };
 SharedPlan plan_of(const bonsai_p40_attn_shared_args * p) {
-    const int64_t cap = (int64_t)p->attn.max_pages * p->attn.page_size, all = most_keys(&p->attn);
+    const int64_t cap = (int64_t)p->attn.max_pages * p->attn.page_size;
     const int64_t shared = p->max_shared > 0 && p->max_shared < cap ? p->max_shared : cap;
-    // (own keys begin anywhere in 16)
-    const int64_t own = p->max_shared > 0 && p->attn.max_kv > 0 && all > shared ? all - shared + 15 : all;
+    // (own keys begin anywhere in 16; max_kv is not cut: a sequence of no group may have more of them than are left of the
+    // table behind the longest prefix)
+    const int64_t own = p->max_shared > 0 && p->attn.max_kv > shared ? p->attn.max_kv - shared + 15 : most_keys(&p->attn);
     return {plan_of(&p->attn, p->n_group, shared, SHARED_KEYS), plan_of(&p->attn, p->attn.n_seq, own < cap ? own : cap, OWN_KEYS)};
 }
 

@@ -233,3 +233,15 @@ def test_wrappers_take_one_page_that_is_all_there_is():
         k, v = pages8(1, *shape), pages8(1, *shape)[0][None]
         want = (1, *shape, h * page * (d + 4) + -(h * page * (d + 4)) % 16, B.Q8)
         assert B._pages(k, v, -1) == B._pages(v, k, -1) == B._pages(v, v, -1) == want
+
+
+def test_workspace_bytes_of_a_long_sequence_outside_the_groups():
+    """The hints can say that own keys are many, though the table has room for no sequence of a prefix and so many."""
+    def parts(max_kv, max_shared):
+        a = make(B.AttnSharedArgs, {**SHARED, "max_pages": 1024, "table_stride": 1024, "max_kv": max_kv, "max_shared": max_shared})
+        return B.lib().bonsai_p40_attn_shared_workspace_bytes(C.byref(a)) // (3 * 8 * 130 * 4)
+    cap = 1024 * 16
+    prefix = parts(cap, 16000) - parts(400, 16)             # (the parts of 16000 keys less those of 16, which are one)
+    own = parts(16000 + 16000, 16000) - prefix - 1
+    assert parts(cap, 16000) - prefix - 1 < own <= parts(16016, 16) - 1
+    assert parts(1 << 40, 16000) >= parts(32000, 16000)
