@@ -272,10 +272,16 @@ constexpr int attn_seen(int before, int kv, int tok) {
 // Whether both phases of shared prefixes, of so many workgroups of 256, are one launch where their kernel is the same
 inline bool attn_one_launch(int64_t first, int64_t own) { return first + own < 1 << 24; }
 // The sequences' own keys behind shared prefixes: mostly few, so that what counts is how often a CU begins with
-// another workgroup (`begin` us), and how many steps (of 32 keys a wave, `step` us) the longest takes.  Measured on MI355X
-// (us of the kernel over the own keys, 24 heads of 256, split as attn_plan does / so): 64 sequences of up to 500, bf16, 3 / 1
-// parts 30.4 / 22.8; 32 of up to 1500, 8-bit pages, 6 / 4 36.6 / 23.2; 40 of up to 300 with 12 tokens, heads of 128, 1 part of
-// 128 keys each 32.2 / 19.5.  With 4 to 14 us to begin and 1.5 to 2 a step these three come out the same.
+// another workgroup (`begin` us), and how many steps (of 32 keys a wave, `step` us) the longest takes.  182 batches of 6 to
+// 300 sequences of 90 to 12000 own keys, equal and ragged (bf16 with heads of 64, 128, 256, 8-bit pages 256; MI355X), each timed
+// with 1 to 32 parts: the rule is within 4 % of the best number of parts in the mean, and no constants of 2 to 30 us to
+// begin and 1 to 3 a step are better by 0.2 %.  Where it changes its mind, us by parts: 20 sequences, bf16, heads of 256,
+// 400 keys 1 / 2 / 3 / 7: 37.0 / 32.5 / 33.9 / 40.4; 50 of 1200, 8-bit pages 1 / 2 / 3 / 7: 72 / 58 / 67 / 73.  It is furthest off where
+// 6 sequences of 1200 keys, heads of 128, take 10 parts, 20.9, 12.8 with 4, and 20 of 12000, equal, 3, 273, 187 with 2.
+//   A part is 32 steps at most: the lengths are not known, and one sequence of many own keys among others of few is as slow as its
+// longest part.  64 sequences behind 16000 keys, of 500 own keys but one of 16000, where the hints say so: 425
+// us with one part, 132 so (8-bit pages 309, 139).  On the 182 batches that costs nothing (3.7 % above the best, 3.9 without; 16
+// steps 3.9, 64 3.9).
 inline AttnPlan attn_own_plan(int64_t n_tok, int64_t n_seq, int64_t group, int64_t n_kv, int64_t dim, int64_t max_kv, int64_t rows,
                               int64_t cus, bool bytes) {
     AttnPlan p = attn_plan(n_tok, n_seq, group, n_kv, dim, max_kv, rows, cus, bytes);
@@ -283,11 +289,12 @@ inline AttnPlan attn_own_plan(int64_t n_tok, int64_t n_seq, int64_t group, int64
     const int64_t some = n_seq < n_tok ? n_seq : n_tok, per = dim < 256 ? 128 : 64, slots = cus * (bytes && dim == 256 ? 2 : 256 / dim);
     const double begin = 7.0, step = 2.0;
     double best = 0.0;
-    int64_t want = 1;
+    int64_t want = 1, longest = 0;
     // (a batch that fills the card many times over is not split: a grid has fewer than 2^32 threads)
-    for (int64_t n = 1; n <= 64 && (n == 1 || some * n_kv * n <= 1 << 20); ++n) {
-        const double us = (double)ceil_div(some * n_kv * n, slots) * (begin + step * (double)ceil_div(ceil_div(max_kv, n), per));
-        if (n == 1 || us < best) best = us, want = n;
+    for (int64_t n = 1; n <= 64 && (n == 1 || p.tiles * n_kv * n <= 1 << 20); ++n) {
+        const int64_t steps = ceil_div(ceil_div(max_kv, n), per);
+        const double us = (double)ceil_div(some * n_kv * n, slots) * (begin + step * (double)steps);
+        if (n == 1 || longest > 32 || us < best) best = us, want = n, longest = steps;
     }
     attn_split(p, want, max_kv, per);
     return p;

@@ -114,3 +114,22 @@ def test_keys_a_token_sees(rules):
                 if 0 <= t < n:
                     assert rules.attn_seen(kv - n, kv, t) == max(kv - n + t + 1, 0), (kv, n, t)
                     assert rules.attn_seen(kv, kv, t) == kv, (kv, n, t)
+
+
+def test_own_keys_in_parts_of_32_steps_at_most(rules):
+    """Up to 64 parts, unless the batch fills the card many times over."""
+    for n_seq in (1, 6, 64, 300, 1000):
+        for dim, q8 in ((64, False), (128, True), (256, False), (256, True)):
+            for keys in (515, 2048, 4096, 4097, 16015, 60000, 131071):
+                _, tiles, chunk, parts = own(rules, n_seq, n_seq, 6, 4, dim, keys, q8=q8)
+                assert chunk <= 32 * (64 if dim == 256 else 128) or parts >= 60, (n_seq, dim, keys, chunk, parts)
+
+
+@pytest.mark.parametrize("n_tok,n_seq,group,n_kv", [((1 << 14) - 1, 1 << 19, 1024, 1), (16383, 1 << 23, 16, 64), (255, 1 << 21, 65536, 1), (1, 1 << 23, 1, 1),
+                                                    ((1 << 23) - 1, 1 << 20, 1, 1)])
+def test_grids_of_batches_with_more_rows_than_tokens(rules, n_tok, n_seq, group, n_kv):
+    for dim in (64, 128, 256):
+        for keys in (1, 4000, 1 << 20, (1 << 31) - 65536):
+            for q8 in (False, True):
+                _, tiles, _, parts = own(rules, n_tok, n_seq, group, n_kv, dim, keys, q8=q8)
+                assert 0 < tiles * parts * n_kv < 1 << 24, (dim, keys, q8, tiles, parts)
