@@ -228,3 +228,24 @@ def test_no_groups_is_attn_paged():
     B.attn_paged(*args, a)
     B.attn_shared(*args, ints([0]), torch.zeros(0, dtype=torch.int32, device="cuda"), b, None)
     assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("heads,kvh", [(24, 4), (6, 1)])
+@pytest.mark.parametrize("t,io", [("q8", F32), ("q8", BF16), (F16, F32), (BF16, BF16)])
+def test_samples_of_a_long_prompt(t, io, heads, kvh):
+    """Two samples of a prompt of 16000 keys: more parts than a wave has lanes."""
+    part = 2 * heads * 258 * 4
+    got = run_shared([1, 1], [40, 125], [0, 2], [16000], heads, kvh, 256, 64, t, io)
+    q = torch.zeros(2, heads, 256, dtype=io, device="cuda")
+    pages = B.q8_pages(1, kvh, 64, 256)[0] if t == "q8" else torch.zeros(1, kvh, 64, 256, dtype=t, device="cuda")
+    table = torch.zeros(2, 252, dtype=torch.int32, device="cuda")
+    args = [q, pages, pages, table, ints([0, 1, 2]), ints([1, 1]), ints([0, 2]), ints([16000]), got.cuda()]
+    assert B.attn_shared_workspace_bytes(*args, max_kv=16125, max_shared=16000) // part > 64
+
+
+@pytest.mark.parametrize("t,io", [("q8", BF16), (F16, F16), (F16, F32)])
+def test_one_long_sequence_outside_the_groups(t, io):
+    """Short own keys behind a prefix, and many of a sequence of no group, or of one behind a short prefix, whatever the hints."""
+    for hints in (True, (700 + 3000, 700), (0, 0), (3100, 0), (1, 3000)):
+        run_shared([1] * 5, [9, 20, 3, 15, 3000], [0, 4], [700], 4, 2, 64, 16, t, io, hints=hints)
+        run_shared([1, 2, 1, 40], [9, 20, 1500, 60], [0, 2, 3], [700, 10], 6, 2, 256, 16, t, io, hints=hints)
