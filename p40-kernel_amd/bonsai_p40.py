@@ -534,7 +534,7 @@ def _pages(k_pages, v_pages, dev: int):
         else:
             fits = t.stride(0) == page and at + (n - 1) * page + size <= there
         if not fits:
-            raise ValueError("8-bit pages follow each other, each with room for its scales, as q8_pages makes them")
+            raise ValueError("8-bit pages follow each other, each with room for its scales, as q8_pages makes them ([i:i + 1] of these is one page)")
     return n, h, p, d, page, Q8
 
 
@@ -674,7 +674,8 @@ def attn_shared_workspace_bytes(q, k_pages, v_pages, table, starts, kv_len, grou
 def attn_shared(q, k_pages, v_pages, table, starts, kv_len, groups, shared, out, workspace, max_kv: int = 0,
                 max_shared: int = 0, scale=None, stream=None) -> None:
     """attn_paged of a batch whose sequences groups[g] .. groups[g + 1] - 1 begin with
-    the same shared[g] keys, those of table[groups[g]], which are read once for all of them."""
+    the same shared[g] keys, those of table[groups[g]], which are read once for all of them.
+    max_kv, max_shared: the longest prefix and the most own keys of a sequence together, and that prefix."""
     a = _attn_shared_args(q, k_pages, v_pages, table, starts, kv_len, groups, shared, out, workspace, max_kv, max_shared, scale)
     rc = lib().bonsai_p40_attn_shared(a, _stream_of(q, stream))
     if rc:

@@ -24,13 +24,13 @@
 //   No value of V is NaN or infinite by itself, so a key that is not seen needs no
 // zeroed row: its weight is 0 and its d counts as 0.
 //   Keys (decode) is bound by the stream of the pages, half of 16-bit ones': 64 sequences of
-// 16384, bf16, 5.65 TB/s; 1 of 131071 66 us (16-bit pages 109), 32 of up to 12000 101 to 104
+// 16384, bf16, 5.64 TB/s; 1 of 131071 66 us (16-bit pages 109), 32 of up to 12000 103 to 104
 // (154), where the batch's ragged parts leave CUs idle at the end (MI355X, heads of 256).
 //   Rows (prompts) is bound by instructions: a tile of 32 keys on 128 rows takes 1.38 us (16-bit
 // queries, heads of 256; 16-bit pages 1.15), 1024 clocks of it MFMA, and a wave's 270 VALU and 56
 // LDS instructions hardly run beside them; fp32 2.1 (1.97).  777 tokens of 16000 keys: 500 us with
-// each wave unpacking all of V for itself, 484 with each unpacking its own keys for all, 470 with
-// the loads and that under the products (16-bit pages 360).
+// each wave unpacking all of V for itself, 484 with each unpacking its own keys for all, 475 with
+// the loads and that under the products (16-bit pages 362); fp32 rows 700.
 #include "attn_device.h"
 #include "gemv_device.h"
 #include "host_state.h"
