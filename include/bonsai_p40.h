@@ -470,7 +470,8 @@ int bonsai_p40_qk_norm_rope(const bonsai_p40_qk_norm_rope_args * args, bonsai_st
 // 2^-14 off by up to 2^-25, fp32 rows 2^-36, of the largest).  A row all of whose seen scores are
 // -inf is NaN, as 0 / 0 is; with fp32 rows so is one that sees a key that is not finite.
 //   Q8 pages: a row of q is taken as whole numbers, an element off by at most 1.01 x 2^-15
-// (fp32: 1.6 x 2^-23) of its largest one; a row with a value that is not finite gives NaN.  A weight times its value's
+// (fp32: 1.6 x 2^-23) of its largest one, if that is 2^-104 or more (else of 2^-104); a row with a value that is not
+// finite gives NaN where it sees a key.  A weight times its value's
 // d is rounded once to f16 (fp32: to 22 bits); one below 2^-25 of the row's largest such
 // product, taken tile by tile of 32 keys, is off by up to 2^-36 (2^-47) of that, and any by 2^-136 / D
 // (2^-147 / D) of it where the largest d that the row sees, D, is below 2^-100.

@@ -135,14 +135,15 @@ template <bool SHARED, class Args>
 __device__ __forceinline__ AttnPlace attn_place(Args * a) {
     AttnPlace p;
     p.pre = SHARED && blockIdx.x < a->blocks1;
-    const int block = SHARED && !p.pre ? blockIdx.x - a->blocks1 : blockIdx.x;
-    const int tiles = SHARED && p.pre ? a->tiles1 : a->tiles;
+    // (unsigned: these divisions are ahead of the first load)
+    const unsigned block = SHARED && !p.pre ? blockIdx.x - a->blocks1 : blockIdx.x, n_kv = a->n_kv;
+    const unsigned tiles = SHARED && p.pre ? a->tiles1 : a->tiles;
     // heads vary fastest: a head's tiles meet on the same XCDs, and then in their L2, as those that run at the
     // same time have the same keys; the last tiles, which see the most, start first
-    p.kvh = block % a->n_kv;
-    const int rest = block / a->n_kv;
-    p.split = rest / tiles;
-    p.tile = tiles - 1 - rest % tiles;
+    p.kvh = (int)(block % n_kv);
+    const unsigned rest = block / n_kv;
+    p.split = (int)(rest / tiles);
+    p.tile = (int)(tiles - 1 - rest % tiles);
     return p;
 }
 // its place among the parts of a row
